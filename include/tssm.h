@@ -42,6 +42,10 @@ extern "C" {
 #define TSSM_DISC_EULER 0 /* Bbar = dt * B           (multihead_ssm_kernel.py:73) */
 #define TSSM_DISC_ZOH 1   /* Bbar = expm1(dt a)/a * B (discretize_kernel.py:50-54) */
 
+/* activations of tssm_group_norm_act_fwd/bwd */
+#define TSSM_ACT_NONE 0
+#define TSSM_ACT_SILU 1 /* x / (1 + exp(-x)) */
+
 int tssm_abi_version(void);
 const char* tssm_strerror(int status);
 
@@ -563,6 +567,62 @@ int tssm_mean_pool_logit(int dtype, const void* h, const void* W, const void* bi
  * mask [B,T]).  mask_code: 0 f32, 1 bf16, 2 f16, 3 int32, 4 uint8/bool. */
 int tssm_masked_fill_zero(int dtype, int mask_code, const void* x, const void* mask, void* out,
                           int64_t n, int64_t H, void* stream);
+
+/* ------------------------------------------------------------------ gated delta rule
+ * A state S [K, V] per (batch, value head) whose every step corrects what the
+ * state holds for its key (no reference counterpart):
+ *   u_t = beta_t (v_t - exp(g_t) S_{t-1}^T k_t),
+ *   S_t = exp(g_t) S_{t-1} + k_t u_t^T,   o_t = scale S_t^T q_t.
+ * q, k [B,L,Hk,K], v, o [B,L,Hv,V] of `dtype` with strides (b, l, h) and unit
+ * innermost stride; Hv a multiple of Hk (value head h reads key head
+ * h / (Hv / Hk)); g (log decay, <= 0), beta f32 [B,L,Hv] with strides (b, l, h).
+ * h0/h_last f32 contiguous [B,Hv,K,V] or NULL (h0 NULL: zero; they may be the
+ * same buffer).  K <= 128.  State, sums and products that reach the state are
+ * fp32 whatever the dtype.  Workspace: tssm_gated_delta_workspace_bytes()
+ * bytes, 256-byte aligned, raw fp32 (not look-back words), no clearing. */
+int64_t tssm_gated_delta_workspace_bytes(int64_t nbatch, int64_t L, int64_t Hk, int64_t Hv,
+                                         int64_t K, int64_t V);
+int tssm_gated_delta_forward(int dtype, const void* q, const void* k, const void* v,
+                             const float* g, const float* beta, const float* h0, void* o,
+                             float* h_last, int64_t nbatch, int64_t L, int64_t Hk, int64_t Hv,
+                             int64_t K, int64_t V, int64_t sq_b, int64_t sq_l, int64_t sq_h,
+                             int64_t sk_b, int64_t sk_l, int64_t sk_h, int64_t sv_b,
+                             int64_t sv_l, int64_t sv_h, int64_t sg_b, int64_t sg_l,
+                             int64_t sg_h, int64_t sbe_b, int64_t sbe_l, int64_t sbe_h,
+                             int64_t so_b, int64_t so_l, int64_t so_h, float scale,
+                             void* workspace, int64_t workspace_bytes, void* stream);
+
+/* One step of S streams, state f32 contiguous [S,Hv,K,V] updated in place:
+ * q, k [S,Hk,K], v, o [S,Hv,V], g, beta [S,Hv], strides (s, h). */
+int tssm_gated_delta_step(int dtype, const void* q, const void* k, const void* v, const float* g,
+                          const float* beta, float* state, void* o, int64_t S, int64_t Hk,
+                          int64_t Hv, int64_t K, int64_t V, int64_t sq_s, int64_t sq_h,
+                          int64_t sk_s, int64_t sk_h, int64_t sv_s, int64_t sv_h, int64_t sg_s,
+                          int64_t sg_h, int64_t sbe_s, int64_t sbe_h, int64_t so_s, int64_t so_h,
+                          float scale, void* stream);
+
+/* ------------------------------------------------------------------ group norm, activation
+ * x [N,S,C], C = G Cg, unit channel stride, strides (n, s); mean and variance
+ * over each group's S x Cg elements (S = 1: per row).  xhat = (x - mean) rstd,
+ * z = xhat w + b (w, b f32 [C] or NULL), y = act(z), or z act(gate) where gate
+ * [N,S,C] is given.  mean, rstd f32 [N,G] are written where not NULL (both or
+ * neither) and read by the backward, which writes dx, dgate (NULL without a
+ * gate) of `dtype` and dw, db f32 [C], summed in a fixed order.  No reference
+ * counterpart.  Workspace: tssm_group_norm_workspace_bytes() bytes, 256-byte
+ * aligned, no clearing. */
+int64_t tssm_group_norm_workspace_bytes(int64_t N, int64_t S, int64_t G, int64_t Cg);
+int tssm_group_norm_act_fwd(int dtype, int act, const void* x, const float* w, const float* b,
+                            const void* gate, void* y, float* mean, float* rstd, int64_t N,
+                            int64_t S, int64_t G, int64_t Cg, int64_t sx_n, int64_t sx_s,
+                            int64_t sgt_n, int64_t sgt_s, int64_t sy_n, int64_t sy_s, float eps,
+                            void* workspace, int64_t workspace_bytes, void* stream);
+int tssm_group_norm_act_bwd(int dtype, int act, const void* dy, const void* x, const float* mean,
+                            const float* rstd, const float* w, const float* b, const void* gate,
+                            void* dx, float* dw, float* db, void* dgate, int64_t N, int64_t S,
+                            int64_t G, int64_t Cg, int64_t sdy_n, int64_t sdy_s, int64_t sx_n,
+                            int64_t sx_s, int64_t sgt_n, int64_t sgt_s, int64_t sdx_n,
+                            int64_t sdx_s, int64_t sdg_n, int64_t sdg_s, void* workspace,
+                            int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,283 @@
+"""GPU parity of the gated delta rule against its float64 definition.
+
+Tolerances, normwise.  fp32 outputs (states, and everything with fp32 inputs):
+1e-5 -- sums of at most 128 products carry about sqrt(128) 2^-24 = 7e-7, a
+chunk has five of them in a row, and beta (1 - |k|^2 beta) keeps older errors
+from growing.  16-bit outputs: twice the rounding of the largest value, 2^-8
+for bfloat16 and 2^-11 for float16.
+"""
+import numpy as np
+import pytest
+import torch
+
+from helpers import assert_close, np64
+from oracle import mixer_oracle as M
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+TOL = {F32: 1e-5, BF16: 2.0 ** -8, F16: 2.0 ** -11}
+
+
+def inputs(dev, B, L, Hk, Hv, K, V, dtype, seed=0, h0=False, rate=1.0):
+    """Unit keys with a shared direction, decays of irregular gaps."""
+    r = torch.Generator().manual_seed(seed)
+
+    def unit(t):
+        return t / t.norm(dim=-1, keepdim=True)
+
+    d = dict(q=unit(torch.randn(B, L, Hk, K, generator=r)).to(dtype),
+             k=unit(torch.randn(B, L, Hk, K, generator=r)
+                    + 0.5 * torch.randn(Hk, K, generator=r)).to(dtype),
+             v=torch.randn(B, L, Hv, V, generator=r).to(dtype),
+             g=-torch.empty(B, L, Hv).exponential_(10.0, generator=r) * rate,
+             beta=torch.sigmoid(torch.randn(B, L, Hv, generator=r)))
+    d["h0"] = torch.randn(B, Hv, K, V, generator=r) if h0 else None
+    return {n: t if t is None else t.to(dev) for n, t in d.items()}
+
+
+def run(d, **kw):
+    from tssm import gated_delta_forward
+    return gated_delta_forward(d["q"], d["k"], d["v"], d["g"], d["beta"], h0=d["h0"],
+                               return_state=True, **kw)
+
+
+def oracle(d, **kw):
+    c = {n: None if t is None else np64(t) for n, t in d.items()}
+    return M.delta_forward(**c, **kw)
+
+
+SIZES = [  # B, L, Hk, Hv, K, V
+    (1, 1, 1, 1, 1, 1),
+    (2, 5, 2, 4, 64, 64),
+    (1, 31, 1, 1, 16, 16),
+    (2, 32, 3, 3, 32, 48),
+    (1, 33, 2, 6, 40, 72),
+    (3, 64, 1, 2, 128, 128),
+    (1, 100, 2, 2, 7, 33),       # no vector access
+    (2, 257, 2, 2, 96, 20),
+    (1, 1000, 2, 4, 64, 64),
+    (1, 130, 1, 1, 100, 300),
+]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("B,L,Hk,Hv,K,V", SIZES)
+def test_forward(dev, dtype, B, L, Hk, Hv, K, V):
+    d = inputs(dev, B, L, Hk, Hv, K, V, dtype, seed=L + K, h0=L % 2 == 1)
+    o, S = run(d)
+    o_ref, S_ref = oracle(d)
+    assert_close(o, o_ref, TOL[dtype], "o")
+    assert_close(S, S_ref, TOL[F32], "state")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_forward_strides(dev, dtype):
+    """q, k and v as slices of one projection, heads before steps, a shared g."""
+    B, L, H, K, V = 2, 77, 3, 32, 32
+    d = inputs(dev, B, L, H, H, K, V, dtype, seed=5, h0=True)
+    packed = torch.zeros(B, L, H * (2 * K + V) + 3, device=dev, dtype=dtype)
+    o_ref, S_ref = oracle(d)
+    for name, at in (("q", 0), ("k", H * K), ("v", 2 * H * K)):
+        view = packed[..., at + 1:at + 1 + H * K].view(B, L, H, K)
+        view.copy_(d[name])
+        d[name] = view
+    d["beta"] = d["beta"].transpose(1, 2).contiguous().transpose(1, 2)
+    out = torch.empty(B, H, L, V, device=dev, dtype=dtype).transpose(1, 2)
+    o, S = run(d, out=out)
+    assert o is out
+    assert_close(o, o_ref, TOL[dtype], "o")
+    assert_close(S, S_ref, TOL[F32], "state")
+    d["g"] = d["g"][:, :1, :1].expand(B, L, H)     # one decay for all steps and heads
+    o, S = run(d)
+    o_ref, S_ref = oracle(d)
+    assert_close(o, o_ref, TOL[dtype], "o")
+    assert_close(S, S_ref, TOL[F32], "state")
+
+
+@pytest.mark.parametrize("L", [0, 1])
+def test_empty(dev, L):
+    d = inputs(dev, 2, L, 2, 2, 32, 32, F32, h0=True)
+    o, S = run(d)
+    assert o.shape == (2, L, 2, 32)
+    if L == 0:
+        assert torch.equal(S, d["h0"])
+        d["h0"] = None
+        assert not run(d)[1].any()
+    none = {n: None if t is None else t[:0] for n, t in d.items()}
+    o, S = run(none)
+    assert o.shape[0] == 0 and S.shape[0] == 0
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_extreme_decay(dev, dtype):
+    """No decay at all, complete resets (g = -inf and the lowest value) among
+    slow steps, and steps whose beta is 0 or 1."""
+    d = inputs(dev, 2, 150, 2, 2, 64, 64, dtype, seed=8, h0=True, rate=0.05)
+    d["g"][:, ::7] = 0.0
+    d["g"][0, 40] = -float("inf")
+    d["g"][1, 41] = torch.finfo(F32).min
+    d["g"][1, 90:100] = -300.0
+    d["beta"][:, 10:20] = 0.0
+    d["beta"][:, 20:30] = 1.0
+    o, S = run(d)
+    o_ref, S_ref = oracle(d)
+    assert_close(o, o_ref, TOL[dtype], "o")
+    assert_close(S, S_ref, TOL[F32], "state")
+    # the steps after a reset alone, so that larger earlier outputs hide nothing
+    assert_close(o[0, 40:48], o_ref[0, 40:48], TOL[dtype], "o after a reset")
+
+
+def test_correlated_keys(dev):
+    """One key for all steps: products of the chunk's triangular matrix grow
+    like binomials, its inverse does not."""
+    d = inputs(dev, 1, 200, 1, 1, 64, 32, F32, seed=9)
+    d["k"] = d["k"][:, :1].expand_as(d["k"])
+    d["beta"] = torch.ones_like(d["beta"])
+    d["g"] = torch.zeros_like(d["g"])
+    o, S = run(d)
+    o_ref, S_ref = oracle(d)
+    assert_close(o, o_ref, TOL[F32], "o")
+    assert_close(S, S_ref, TOL[F32], "state")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("name", ["v", "k", "q", "beta"])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_not_finite(dev, dtype, name, value):
+    """A value that is not finite at one step leaves every earlier output, and
+    (in v) every other column, as it was."""
+    B, L, H, K, V, t0 = 1, 150, 2, 64, 64, 75
+    d = inputs(dev, B, L, H, H, K, V, dtype, seed=11, h0=True)
+    o_ref, S_ref = oracle(d)
+    if name == "beta":
+        d["beta"][0, t0, 1] = value
+    else:
+        d[name][0, t0, 1, 5] = value
+    o, S = run(d)
+    assert_close(o[:, :t0], o_ref[:, :t0], TOL[dtype], "earlier steps")
+    assert_close(o[:, :, 0], o_ref[:, :, 0], TOL[dtype], "the other head")
+    assert not torch.isfinite(o[0, t0, 1]).all()
+    if name == "v":
+        keep = [c for c in range(V) if c != 5]
+        assert_close(o[:, :, 1, keep], o_ref[:, :, 1, keep], TOL[dtype], "other columns")
+        assert_close(S[:, 1][..., keep], S_ref[:, 1][..., keep], TOL[F32], "state")
+    if name == "q":
+        assert_close(o[:, t0 + 1:], o_ref[:, t0 + 1:], TOL[dtype], "later steps")
+        assert_close(S, S_ref, TOL[F32], "state")
+
+
+def test_chained_calls(dev):
+    """A sequence in three calls, the state handed on, against one call."""
+    d = inputs(dev, 2, 300, 2, 4, 64, 64, BF16, seed=12)
+    o, S = run(d)
+    parts, h = [], None
+    for lo, hi in ((0, 7), (7, 168), (168, 300)):
+        p = {n: d[n][:, lo:hi] for n in ("q", "k", "v", "g", "beta")}
+        op, h = run(dict(p, h0=h))
+        parts.append(op)
+    assert_close(torch.cat(parts, 1), np64(o), TOL[BF16], "o")
+    assert_close(h, np64(S), TOL[F32], "state")
+
+
+def test_repeat_and_stream(dev):
+    """The same bits on a repeated call, and on another stream than the
+    tensors' own."""
+    d = inputs(dev, 2, 500, 2, 2, 64, 64, BF16, seed=13)
+    o, S = run(d)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        o2, S2 = run(d)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert torch.equal(o, o2) and torch.equal(S, S2)
+
+
+# ------------------------------------------------------------------ decode
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("S,Hk,Hv,K,V", [(1, 1, 1, 1, 1), (1, 8, 16, 128, 128), (7, 2, 2, 64, 64),
+                                         (33, 1, 3, 40, 72), (5, 2, 2, 7, 33),
+                                         (300, 4, 4, 128, 64), (3, 2, 2, 16, 300)])
+def test_step(dev, dtype, S, Hk, Hv, K, V):
+    from tssm import gated_delta_step
+    d = inputs(dev, 4, S, Hk, Hv, K, V, dtype, seed=S + V)
+    state = torch.randn(S, Hv, K, V, device=dev)
+    ref = np64(state)
+    for t in range(4):
+        x = {n: d[n][t] for n in ("q", "k", "v", "g", "beta")}
+        o_ref, ref = M.delta_forward(**{n: np64(a)[:, None] for n, a in x.items()}, h0=ref)
+        o = gated_delta_step(**x, state=state)
+        assert_close(o, o_ref[:, 0], TOL[dtype], f"o, step {t}")
+        assert_close(state, ref, TOL[F32], f"state, step {t}")
+
+
+def test_step_continues_forward(dev):
+    """Prefill, then decode from its state, against one longer prefill."""
+    from tssm import gated_delta_step
+    d = inputs(dev, 2, 70, 2, 4, 64, 32, BF16, seed=15)
+    o, S = run(d)
+    _, state = run({n: None if t is None else t[:, :64] for n, t in d.items()})
+    for t in range(64, 70):
+        x = {n: d[n][:, t] for n in ("q", "k", "v", "g", "beta")}
+        assert_close(gated_delta_step(**x, state=state), np64(o[:, t]), TOL[BF16], f"step {t}")
+    assert_close(state, np64(S), TOL[F32], "state")
+
+
+def test_step_graph(dev):
+    """A captured step replayed with eager work between the replays."""
+    from tssm import gated_delta_step
+    d = inputs(dev, 4, 9, 2, 2, 64, 64, BF16, seed=16)
+    x = {n: d[n][0].clone() for n in ("q", "k", "v", "g", "beta")}
+    state = torch.randn(9, 2, 64, 64, device=dev)
+    eager, out = state.clone(), torch.empty_like(x["v"])
+    gated_delta_step(**x, state=state.clone(), out=out)      # loads the kernel
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        gated_delta_step(**x, state=state, out=out)
+    for t in range(4):
+        for n in x:
+            x[n].copy_(d[n][t])
+        graph.replay()
+        torch.cuda.synchronize()
+        ref = gated_delta_step(**x, state=eager)
+        assert torch.equal(out, ref) and torch.equal(state, eager), f"replay {t}"
+
+
+# ------------------------------------------------------------------ refusals
+def test_refusals(dev):
+    from tssm import gated_delta_forward, gated_delta_step
+    d = inputs(dev, 2, 6, 2, 4, 16, 8, BF16, h0=True)
+
+    def call(**kw):
+        a = dict(d, **kw)
+        return gated_delta_forward(a["q"], a["k"], a["v"], a["g"], a["beta"], h0=a["h0"],
+                                   out=a.get("out"))
+
+    for bad, match in [
+        (dict(k=d["k"][:, :5]), "k must be"),
+        (dict(q=d["q"][0]), "expected q"),
+        (dict(v=d["v"][:, :, :3]), "multiple"),
+        (dict(v=d["v"][:, :5]), "v must be"),
+        (dict(g=d["g"][:, :, :2]), "g must be"),
+        (dict(beta=d["beta"][0]), "beta must be"),
+        (dict(h0=d["h0"][:, :2]), "h0 must be"),
+        (dict(out=torch.empty(2, 6, 4, 9, device=dev, dtype=BF16)), "out must be"),
+        (dict(q=d["q"].cpu()), "HIP device"),
+        (dict(v=d["v"].transpose(2, 3).contiguous().transpose(2, 3)), "contiguous"),
+        (dict(q=torch.zeros(2, 6, 2, 129, device=dev, dtype=BF16)), "at most 128"),
+    ]:
+        with pytest.raises(ValueError, match=match):
+            call(**bad)
+    for bad, match in [(dict(k=d["k"].float()), "k must be"), (dict(v=d["v"].half()), "v must be"),
+                       (dict(q=d["q"].double()), "unsupported dtype"),
+                       (dict(g=d["g"].long()), "float tensor"), (dict(q=None), "torch.Tensor")]:
+        with pytest.raises(TypeError, match=match):
+            call(**bad)
+    x = {n: d[n][:, 0] for n in ("q", "k", "v", "g", "beta")}
+    with pytest.raises(ValueError, match="contiguous"):
+        gated_delta_step(**x, state=d["h0"].transpose(2, 3).contiguous().transpose(2, 3))
+    with pytest.raises(TypeError, match="state must be"):
+        gated_delta_step(**x, state=d["h0"].bfloat16())
+    with pytest.raises(ValueError, match="state must be"):
+        gated_delta_step(**x, state=d["h0"][:1])

@@ -1,0 +1,27 @@
+// Shared argument block of the gated delta rule's kernels (delta.hip and
+// its translation units).  Per batch b, value head h (key head h / per):
+//   u_t = beta_t (v_t - e^{g_t} S_{t-1}^T k_t),  S_t = e^{g_t} S_{t-1} + k_t u_t^T,
+//   o_t = scale S_t^T q_t,   S [K, V] fp32.
+#pragma once
+
+#include <type_traits>
+
+#include "common.h"
+
+namespace tssm {
+
+struct DeltaArgs {
+  const void *q, *k, *v;
+  const float *g, *beta, *h0;
+  void* o;
+  float* h_last;
+  int64_t B, L, Hk, Hv, K, V;
+  int64_t q_b, q_l, q_h, k_b, k_l, k_h, v_b, v_l, v_h;
+  int64_t g_b, g_l, g_h, be_b, be_l, be_h, o_b, o_l, o_h;
+  float scale;
+};
+
+// delta_seq.hip: one step after another, the state in registers.
+int delta_seq_launch(int dtype, const DeltaArgs& a, hipStream_t s);
+
+}  // namespace tssm

@@ -1,0 +1,130 @@
+"""Gated delta rule: a state S [K, V] per value head whose every step corrects
+what the state already holds for its key (no reference counterpart).
+
+    u_t = beta_t (v_t - exp(g_t) S_{t-1}^T k_t)
+    S_t = exp(g_t) S_{t-1} + k_t u_t^T
+    o_t = scale S_t^T q_t
+
+``gated_delta_forward``   whole sequences (prefill, training), any length
+``gated_delta_backward``  every gradient of it
+``gated_delta_step``      one step of many streams, the state in place (decode)
+
+q and k have Hk heads, v, g and beta Hv, a multiple of Hk: value head h reads
+key head h // (Hv // Hk).  The state and every sum that reaches it are fp32;
+keys of unit length and beta in [0, 1] keep the recurrence contracting, which
+is the caller's business: nothing is normalised here.  ``g`` (log decay) and
+``beta`` are read as float32.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib, workspace
+from .launch import as_f32, dcode, need_gpu, ptr, stream_handle
+
+
+def _check(t, what, shape, dtype, device):
+    need_gpu(t, what)
+    if t.shape != shape:
+        raise ValueError(f"{what} must be {list(shape)}, got {list(t.shape)}")
+    if t.dtype != dtype:
+        raise TypeError(f"{what} must be {dtype}, got {t.dtype}")
+    if t.get_device() != device:
+        raise ValueError(f"{what} must be on device {device}")
+
+
+def _rows(t, what):
+    """Strides of every dimension but the innermost, which must be contiguous."""
+    s = t.stride()
+    if s[-1] != 1 and t.shape[-1] != 1:
+        raise ValueError(f"{what}: innermost dimension must be contiguous")
+    return s[:-1]
+
+
+def _operands(q, k, v, g, beta, lead):
+    """Checks q, k, v, g, beta with ``lead`` leading dimensions; returns (sizes,
+    dtype code, g, beta, scale of None)."""
+    for t, w in ((q, "q"), (k, "k"), (v, "v"), (g, "g"), (beta, "beta")):
+        need_gpu(t, w)
+    if q.dim() != lead + 2 or v.dim() != lead + 2:
+        names = "[B, L, Hk, K] and v [B, L, Hv, V]" if lead == 2 else "[S, Hk, K] and v [S, Hv, V]"
+        raise ValueError(f"expected q, k {names}")
+    rows, (Hk, K), (Hv, V), dev = q.shape[:lead], q.shape[lead:], v.shape[lead:], q.get_device()
+    if Hk == 0 or Hv == 0 or K == 0 or V == 0 or Hv % Hk:
+        raise ValueError(f"v's heads must be a multiple of q's, all sizes positive: Hk = {Hk}, "
+                         f"Hv = {Hv}, K = {K}, V = {V}")
+    if K > 128:
+        raise ValueError(f"K = {K}: the key dimension may be at most 128")
+    code = dcode(q, "q")
+    _check(k, "k", q.shape, q.dtype, dev)
+    _check(v, "v", rows + (Hv, V), q.dtype, dev)
+    g, beta = as_f32(g, "g"), as_f32(beta, "beta")
+    _check(g, "g", rows + (Hv,), torch.float32, dev)
+    _check(beta, "beta", rows + (Hv,), torch.float32, dev)
+    return (*rows, Hk, Hv, K, V), code, g, beta
+
+
+def _state(t, what, shape, device):
+    if t is None:
+        return None
+    need_gpu(t, what)
+    t = as_f32(t, what).contiguous()
+    _check(t, what, shape, torch.float32, device)
+    return t
+
+
+def gated_delta_forward(q, k, v, g, beta, *, scale=None, h0=None, return_state=False, out=None):
+    """Gated delta rule over whole sequences.
+
+    q, k   [B, L, Hk, K]  float32 / bfloat16 / float16, K <= 128
+    v      [B, L, Hv, V]  dtype of q, Hv a multiple of Hk
+    g      [B, L, Hv]     log decay of each step (<= 0)
+    beta   [B, L, Hv]     step size
+    scale  of q; None: K ** -0.5
+    h0     [B, Hv, K, V] float32 or None (zero initial state)
+
+    Returns o [B, L, Hv, V] (dtype of v; ``out`` if given) and, with
+    ``return_state``, the final state [B, Hv, K, V] float32, which continues
+    the sequence as the next call's ``h0`` or in ``gated_delta_step``.  An
+    input that is not finite at some step changes no earlier output, and no
+    other column of v.
+    """
+    (B, L, Hk, Hv, K, V), code, g, beta = _operands(q, k, v, g, beta, 2)
+    h0 = _state(h0, "h0", (B, Hv, K, V), q.get_device())
+    o = torch.empty(v.shape, device=v.device, dtype=v.dtype) if out is None else out
+    _check(o, "out", v.shape, v.dtype, q.get_device())
+    h_last = torch.empty(B, Hv, K, V, device=v.device, dtype=torch.float32) \
+        if return_state else None
+    if B:
+        stream = stream_handle(q)
+        ws = workspace.get(q.device, stream, _lib.lib().tssm_gated_delta_workspace_bytes(
+            B, L, Hk, Hv, K, V), workspace.SSD)
+        _lib.call("tssm_gated_delta_forward", code, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                  g.data_ptr(), beta.data_ptr(), ptr(h0), o.data_ptr(), ptr(h_last), B, L, Hk,
+                  Hv, K, V, *_rows(q, "q"), *_rows(k, "k"), *_rows(v, "v"), *g.stride(),
+                  *beta.stride(), *_rows(o, "out"), K ** -0.5 if scale is None else float(scale),
+                  ws.data_ptr(), ws.numel(), stream)
+    return (o, h_last) if return_state else o
+
+
+def gated_delta_step(q, k, v, g, beta, state, *, scale=None, out=None):
+    """One step of S streams, the state updated in place.
+
+    q, k [S, Hk, K], v [S, Hv, V] of one dtype (float32 / bfloat16 / float16),
+    g, beta [S, Hv], state [S, Hv, K, V] float32 contiguous.  Returns o
+    [S, Hv, V] (dtype of v; ``out`` if given).  The same step as
+    ``gated_delta_forward`` with L = 1.
+    """
+    (S, Hk, Hv, K, V), code, g, beta = _operands(q, k, v, g, beta, 1)
+    _check(state, "state", (S, Hv, K, V), torch.float32, q.get_device())
+    if not state.is_contiguous():
+        raise ValueError("state must be contiguous")
+    o = torch.empty(v.shape, device=v.device, dtype=v.dtype) if out is None else out
+    _check(o, "out", v.shape, v.dtype, q.get_device())
+    if S:
+        _lib.call("tssm_gated_delta_step", code, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                  g.data_ptr(), beta.data_ptr(), state.data_ptr(), o.data_ptr(), S, Hk, Hv, K, V,
+                  *_rows(q, "q"), *_rows(k, "k"), *_rows(v, "v"), *g.stride(), *beta.stride(),
+                  *_rows(o, "out"), K ** -0.5 if scale is None else float(scale),
+                  stream_handle(q))
+    return o
