@@ -9,6 +9,18 @@ bool sizes_ok(int64_t B, int64_t L, int64_t Hk, int64_t Hv, int64_t K, int64_t V
   return B >= 0 && L >= 0 && Hk > 0 && Hv > 0 && Hv % Hk == 0 && K > 0 && V > 0;
 }
 
+// Shorter sequences go step by step.
+constexpr int64_t kSeqMost = 16;
+
+int64_t chunk_heads(int64_t B, int64_t L, int64_t Hv) { return B * Hv * cdiv64(L, 32); }
+
+// q's and k's rows are whole 16-byte accesses.
+bool vec_rows(int dtype, const DeltaArgs& a) {
+  const int64_t E = dtype == TSSM_F32 ? 4 : 2;
+  return a.K % 8 == 0 && aligned(a.q, 16) && aligned(a.k, 16) &&
+         (a.q_b | a.q_l | a.q_h | a.k_b | a.k_l | a.k_h) * E % 16 == 0;
+}
+
 }  // namespace
 }  // namespace tssm
 
@@ -29,9 +41,14 @@ extern "C" int tssm_gated_delta_forward(
   const DeltaArgs a = {q, k, v, g, beta, h0, o, h_last, nbatch, L, Hk, Hv, K, V,
                        sq_b, sq_l, sq_h, sk_b, sk_l, sk_h, sv_b, sv_l, sv_h,
                        sg_b, sg_l, sg_h, sbe_b, sbe_l, sbe_h, so_b, so_l, so_h, scale};
-  (void)workspace;
-  (void)workspace_bytes;
-  return delta_seq_launch(dtype, a, as_stream(stream));
+  if (L <= kSeqMost) return delta_seq_launch(dtype, a, as_stream(stream));
+  const int64_t units = chunk_heads(nbatch, L, Hv);
+  TSSM_CHECK(units <= 0x7fffffff, TSSM_ERR_UNSUPPORTED);
+  TSSM_CHECK(workspace && workspace_bytes >= units * delta_chunk_ws_bytes(dtype) &&
+                 aligned(workspace, 256), TSSM_ERR_WORKSPACE);
+  const bool vec = vec_rows(dtype, a);
+  const int rc = delta_prep_launch(dtype, a, vec, workspace, as_stream(stream));
+  return rc ? rc : delta_walk_launch(dtype, a, vec, workspace, as_stream(stream));
 }
 
 extern "C" int tssm_gated_delta_step(int dtype, const void* q, const void* k, const void* v,
@@ -56,5 +73,6 @@ extern "C" int64_t tssm_gated_delta_workspace_bytes(int64_t nbatch, int64_t L, i
                                                     int64_t Hv, int64_t K, int64_t V) {
   if (!sizes_ok(nbatch, L, Hk, Hv, K, V)) return TSSM_ERR_SHAPE;
   if (K > 128) return TSSM_ERR_UNSUPPORTED;
-  return 256;
+  if (L <= kSeqMost) return 256;
+  return chunk_heads(nbatch, L, Hv) * delta_chunk_ws_bytes(TSSM_F32) + 256;
 }

@@ -1,0 +1,201 @@
+// Gated delta rule, preparing pass: per chunk of 32 steps and value head, what
+// the walks need of the keys, queries, decays and step sizes alone.
+//
+// With G the running sums of g within the chunk and D[t][i] = e^(G_t - G_i):
+//   A[t][i] = beta_t D[t][i] k_t.k_i (i < t),   T = (I + A)^-1,
+//   P[t][i] = scale D[t][i] q_t.k_i (i <= t).
+// One wave per chunk and head.  The Gram products run on the matrix cores (3
+// of the 4 tiles of 16 x 16).  T's diagonal blocks come from forward
+// substitution (a lane per column: stable where keys repeat, unlike products
+// of powers of A), the block below from -T22 A21 T11 in fp32.  G is summed in
+// 64 bits: its differences are what counts, and a reset may put -6400 before a
+// slow step; a decay below e^-200 is 0 in fp32 either way.
+#include "delta_dev.h"
+
+namespace tssm {
+namespace {
+
+constexpr int kLd = 36;  // floats of a row of A, T or P in LDS
+
+__device__ inline void wave_order() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// Row lane / 2, columns 16 (lane & 1) .. + 15 of an fp32 matrix into planes.
+template <int NP>
+__device__ inline void put_planes(const float* m, uint16_t (*out)[kC][kC], int lane) {
+  const int r = lane >> 1, c = 16 * (lane & 1);
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    float v[8];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const float4 f = *reinterpret_cast<const float4*>(m + r * kLd + c + 8 * x + 4 * q);
+      v[4 * q] = f.x; v[4 * q + 1] = f.y; v[4 * q + 2] = f.z; v[4 * q + 3] = f.w;
+    }
+    u32x4 p[NP];
+    split8<NP>(v, p);
+#pragma unroll
+    for (int n = 0; n < NP; ++n) *reinterpret_cast<u32x4*>(&out[n][r][c + 8 * x]) = p[n];
+  }
+}
+
+template <typename T, int KP, bool VEC, int NPP>
+__global__ __launch_bounds__(256) void delta_prep_kernel(DeltaArgs a, ChunkWs<NPP>* ws,
+                                                         int64_t nch, int64_t units) {
+  constexpr int NP = Piece<T, VEC>::NP;
+  __shared__ __attribute__((aligned(16))) float mat[4][3][kC * kLd];
+  __shared__ double sums[4][kC];
+  __shared__ float bet[4][kC];
+  const int lane = threadIdx.x & 63, j = lane >> 4, c = lane & 15;
+  const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int64_t unit = (int64_t)blockIdx.x * 4 + wv;
+  if (unit >= units) return;
+  // units run over the value heads of one chunk first: a group shares its keys
+  const int64_t bn = unit / a.Hv, h = unit - bn * a.Hv, b = bn / nch, n = bn - b * nch;
+  const int64_t hk = h / (a.Hv / a.Hk), t0 = n * kC;
+  const int rows = a.L - t0 < kC ? (int)(a.L - t0) : kC;
+  ChunkWs<NPP>& out = ws[(b * a.Hv + h) * nch + n];
+  float *mA = mat[wv][0], *mT = mat[wv][1], *mP = mat[wv][2];
+
+  // running sums of g, per step
+  const int t = lane & 31;
+  const bool on = t < rows;
+  const int64_t tt = t0 + (on ? t : 0);
+  const float g0 = a.g[b * a.g_b + tt * a.g_l + h * a.g_h];
+  const float b0 = a.beta[b * a.be_b + tt * a.be_l + h * a.be_h];
+  const float g = on ? (g0 < -200.0f ? -200.0f : g0) : 0.0f, beta = on ? b0 : 0.0f;
+  double G = g;
+#pragma unroll
+  for (int s = 1; s < 32; s *= 2) {
+    const double up = __shfl_up(G, s, 32);
+    if (t >= s) G += up;
+  }
+  const double Gl = __shfl(G, 31, 32);
+  if (lane < kC) {
+    sums[wv][t] = G;
+    bet[wv][t] = beta;
+    out.fac[0][t] = exp_acc((float)G);
+    out.fac[1][t] = beta;
+    out.fac[2][t] = exp_acc((float)(Gl - G));
+    out.fac[3][t] = on ? g0 : 0.0f;
+  }
+
+  // Gram products: tiles (0,0), (1,0), (1,1)
+  const T* kb = reinterpret_cast<const T*>(a.k) + b * a.k_b + t0 * a.k_l + hk * a.k_h;
+  const T* qb = reinterpret_cast<const T*>(a.q) + b * a.q_b + t0 * a.q_l + hk * a.q_h;
+  f32x4 kk[3] = {zero4(), zero4(), zero4()}, qk[3] = {zero4(), zero4(), zero4()};
+  Piece<T, VEC> pk[2], pq[2];
+#pragma unroll
+  for (int s = 0; s < KP / 32; ++s) {
+    const int col = 32 * s + 8 * j, clim = (int)a.K - col;
+    u32x4 fk[2][NP], fq[2][NP];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int r = 16 * x + c, lim = r < rows ? clim : 0;
+      const int64_t kr = (r < rows ? r : 0) * a.k_l + (clim > 0 ? col : 0);
+      const int64_t qr = (r < rows ? r : 0) * a.q_l + (clim > 0 ? col : 0);
+      pk[x].load(kb + kr, lim);
+      pq[x].load(qb + qr, lim);
+      pk[x].planes(lim, fk[x]);
+      pq[x].planes(lim, fq[x]);
+    }
+#pragma unroll
+    for (int x = 0; x < 3; ++x) {
+      const int ro = x > 0, co = x > 1;
+      kk[x] = mfma_planes<NP, NP, 3>(fk[ro], fk[co], kk[x]);
+      qk[x] = mfma_planes<NP, NP, 3>(fq[ro], fk[co], qk[x]);
+    }
+  }
+  wave_order();
+#pragma unroll
+  for (int x = 0; x < 3; ++x) {
+    const int i = 16 * (x > 1) + c;
+    const double Gi = sums[wv][i];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int row = 16 * (x > 0) + 4 * j + r;
+      const float d = exp_acc((float)(sums[wv][row] - Gi));
+      mA[row * kLd + i] = i < row ? bet[wv][row] * d * kk[x][r] : 0.0f;
+      mP[row * kLd + i] = i <= row ? a.scale * d * qk[x][r] : 0.0f;
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {  // the blocks above the diagonal
+    mT[(4 * j + r) * kLd + 16 + c] = 0.0f;
+    mP[(4 * j + r) * kLd + 16 + c] = 0.0f;
+  }
+  wave_order();
+  // diagonal blocks: lane (d, c) solves for column c of block d
+  {
+    const int d = (lane >> 4) & 1;
+    const float* A = mA + 16 * d * kLd + 16 * d;
+    float X[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float row[16];
+#pragma unroll
+      for (int q = 0; q < (i + 3) / 4; ++q) {
+        const float4 f = *reinterpret_cast<const float4*>(A + i * kLd + 4 * q);
+        row[4 * q] = f.x; row[4 * q + 1] = f.y; row[4 * q + 2] = f.z; row[4 * q + 3] = f.w;
+      }
+      float s0 = i == c ? 1.0f : 0.0f, s1 = 0.0f;
+#pragma unroll
+      for (int m = 0; m < i; ++m) {
+        if (m & 1) s1 = __builtin_fmaf(-row[m], X[m], s1);
+        else s0 = __builtin_fmaf(-row[m], X[m], s0);
+      }
+      X[i] = s0 + s1;
+    }
+    if (lane < kC) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mT[(16 * d + i) * kLd + 16 * d + c] = X[i];
+    }
+  }
+  wave_order();
+  {
+    f32x4 x = zero4(), y = zero4();
+#pragma unroll
+    for (int m = 0; m < 4; ++m)
+      x = __builtin_amdgcn_mfma_f32_16x16x4f32(mA[(16 + c) * kLd + 4 * m + j],
+                                               mT[(4 * m + j) * kLd + c], x, 0, 0, 0);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      y = __builtin_amdgcn_mfma_f32_16x16x4f32(mT[(16 + c) * kLd + 16 + 4 * j + r], x[r], y, 0, 0,
+                                               0);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) mT[(16 + 4 * j + r) * kLd + c] = -y[r];
+  }
+  wave_order();
+  put_planes<3>(mT, out.T, lane);
+  put_planes<NPP>(mP, out.P, lane);
+}
+
+template <typename T, int KP, bool VEC, int NPP>
+void launch(const DeltaArgs& a, void* ws, hipStream_t s) {
+  const int64_t nch = cdiv64(a.L, kC), units = a.B * a.Hv * nch;
+  delta_prep_kernel<T, KP, VEC, NPP><<<(unsigned)cdiv64(units, 4), 256, 0, s>>>(
+      a, reinterpret_cast<ChunkWs<NPP>*>(ws), nch, units);
+}
+
+template <typename T, int NPP>
+void prep(const DeltaArgs& a, bool vec, void* ws, hipStream_t s) {
+  if (a.K <= 32) vec ? launch<T, 32, true, NPP>(a, ws, s) : launch<T, 32, false, NPP>(a, ws, s);
+  else if (a.K <= 64) vec ? launch<T, 64, true, NPP>(a, ws, s) : launch<T, 64, false, NPP>(a, ws, s);
+  else vec ? launch<T, 128, true, NPP>(a, ws, s) : launch<T, 128, false, NPP>(a, ws, s);
+}
+
+}  // namespace
+
+int delta_prep_launch(int dtype, const DeltaArgs& a, bool vec, void* ws, hipStream_t s) {
+  switch (dtype) {
+    case TSSM_F32: prep<float, 3>(a, vec, ws, s); break;
+    case TSSM_BF16: prep<bf16_t, 2>(a, vec, ws, s); break;
+    default: prep<f16_t, 3>(a, vec, ws, s); break;
+  }
+  return launch_status();
+}
+
+}  // namespace tssm
