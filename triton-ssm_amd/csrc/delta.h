@@ -25,9 +25,9 @@ struct DeltaArgs {
 int delta_seq_launch(int dtype, const DeltaArgs& a, hipStream_t s);
 
 // Chunked form: delta_prep.hip (per chunk, in parallel) into the workspace,
-// then delta_walk.hip.  vec: q and k rows are whole 16-byte accesses.
+// then delta_walk.hip.  vec: the rows of q, k and v are whole 16-byte accesses.
 int delta_prep_launch(int dtype, const DeltaArgs& a, bool vec, void* ws, hipStream_t s);
 int delta_walk_launch(int dtype, const DeltaArgs& a, bool vec, const void* ws, hipStream_t s);
-int64_t delta_chunk_ws_bytes(int dtype);  // of one chunk of one value head
+int64_t delta_chunk_ws_bytes();  // of one chunk of one value head
 
 }  // namespace tssm

@@ -14,11 +14,20 @@ constexpr int64_t kSeqMost = 16;
 
 int64_t chunk_heads(int64_t B, int64_t L, int64_t Hv) { return B * Hv * cdiv64(L, 32); }
 
-// q's and k's rows are whole 16-byte accesses.
+// The rows of q, k and v are whole 16-byte accesses.
 bool vec_rows(int dtype, const DeltaArgs& a) {
   const int64_t E = dtype == TSSM_F32 ? 4 : 2;
-  return a.K % 8 == 0 && aligned(a.q, 16) && aligned(a.k, 16) &&
-         (a.q_b | a.q_l | a.q_h | a.k_b | a.k_l | a.k_h) * E % 16 == 0;
+  return a.K % 8 == 0 && a.V % 8 == 0 && aligned(a.q, 16) && aligned(a.k, 16) &&
+         aligned(a.v, 16) &&
+         (a.q_b | a.q_l | a.q_h | a.k_b | a.k_l | a.k_h | a.v_b | a.v_l | a.v_h) * E % 16 == 0;
+}
+
+// What the chunked kernels' buffer accesses ask for: the rows of q, k, v and o
+// do not overlap, and a chunk's lie within 31 bits of its first.
+bool chunk_rows(int dtype, const DeltaArgs& a) {
+  const int64_t most = (INT64_C(1) << 31) / (33 * (dtype == TSSM_F32 ? 4 : 2));
+  const auto fit = [&](int64_t stride, int64_t cols) { return stride >= cols && stride < most; };
+  return fit(a.q_l, a.K) && fit(a.k_l, a.K) && fit(a.v_l, a.V) && fit(a.o_l, a.V);
 }
 
 }  // namespace
@@ -41,10 +50,10 @@ extern "C" int tssm_gated_delta_forward(
   const DeltaArgs a = {q, k, v, g, beta, h0, o, h_last, nbatch, L, Hk, Hv, K, V,
                        sq_b, sq_l, sq_h, sk_b, sk_l, sk_h, sv_b, sv_l, sv_h,
                        sg_b, sg_l, sg_h, sbe_b, sbe_l, sbe_h, so_b, so_l, so_h, scale};
-  if (L <= kSeqMost) return delta_seq_launch(dtype, a, as_stream(stream));
+  if (L <= kSeqMost || !chunk_rows(dtype, a)) return delta_seq_launch(dtype, a, as_stream(stream));
   const int64_t units = chunk_heads(nbatch, L, Hv);
   TSSM_CHECK(units <= 0x7fffffff, TSSM_ERR_UNSUPPORTED);
-  TSSM_CHECK(workspace && workspace_bytes >= units * delta_chunk_ws_bytes(dtype) &&
+  TSSM_CHECK(workspace && workspace_bytes >= units * delta_chunk_ws_bytes() &&
                  aligned(workspace, 256), TSSM_ERR_WORKSPACE);
   const bool vec = vec_rows(dtype, a);
   const int rc = delta_prep_launch(dtype, a, vec, workspace, as_stream(stream));
@@ -74,5 +83,5 @@ extern "C" int64_t tssm_gated_delta_workspace_bytes(int64_t nbatch, int64_t L, i
   if (!sizes_ok(nbatch, L, Hk, Hv, K, V)) return TSSM_ERR_SHAPE;
   if (K > 128) return TSSM_ERR_UNSUPPORTED;
   if (L <= kSeqMost) return 256;
-  return chunk_heads(nbatch, L, Hv) * delta_chunk_ws_bytes(TSSM_F32) + 256;
+  return chunk_heads(nbatch, L, Hv) * delta_chunk_ws_bytes() + 256;
 }

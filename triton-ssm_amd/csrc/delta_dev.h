@@ -35,6 +35,19 @@ __device__ inline f32x4 mfma32(u32x4 a, u32x4 b, f32x4 c) {
 }
 __device__ inline f32x4 zero4() { return f32x4{0.0f, 0.0f, 0.0f, 0.0f}; }
 
+// What the bf16 values in w leave of (a, b): one v_dot2c each, which takes the
+// plane as it is packed; every intermediate is exact.  The constants (-1 in
+// one half) come through asm: folded as literals they reach the instruction
+// in the wrong half.
+__device__ inline void take_plane(uint32_t w, float& a, float& b) {
+  uint32_t lo, hi;
+  asm("s_mov_b32 %0, 0xbf80" : "=s"(lo));
+  asm("s_mov_b32 %0, 0xbf800000" : "=s"(hi));
+  const hw_bf16x2 p = __builtin_bit_cast(hw_bf16x2, w);
+  a = __builtin_amdgcn_fdot2_f32_bf16(p, __builtin_bit_cast(hw_bf16x2, lo), a, false);
+  b = __builtin_amdgcn_fdot2_f32_bf16(p, __builtin_bit_cast(hw_bf16x2, hi), b, false);
+}
+
 // The first NP planes of 8 values, as operands.
 template <int NP>
 __device__ inline void split8(const float* x, u32x4* p) {
@@ -45,10 +58,7 @@ __device__ inline void split8(const float* x, u32x4* p) {
     for (int n = 0; n < NP; ++n) {
       const uint32_t w = pk_bf16(a, b);
       p[n][i] = w;
-      if (n + 1 < NP) {
-        a -= __uint_as_float(w << 16);
-        b -= __uint_as_float(w & 0xffff0000u);
-      }
+      if (n + 1 < NP) take_plane(w, a, b);
     }
   }
 }
@@ -88,6 +98,15 @@ struct Piece {
     for (int i = 0; i < kW; ++i)
       w[i] = reinterpret_cast<const word*>(p)[VEC || i < lim ? i : 0];
   }
+  // through a buffer descriptor, whose end bounds the access
+  __device__ inline void load(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+#pragma unroll
+    for (int i = 0; i < kW; ++i) {
+      if constexpr (VEC) w[i] = __builtin_amdgcn_raw_buffer_load_b128(r, off + 16 * i, 0, 0);
+      else if constexpr (sizeof(T) == 4) w[i] = __builtin_amdgcn_raw_buffer_load_b32(r, off + 4 * i, 0, 0);
+      else w[i] = __builtin_amdgcn_raw_buffer_load_b16(r, off + 2 * i, 0, 0);
+    }
+  }
   __device__ inline void planes(int lim, u32x4* out) const {
     if constexpr (NP == 1 && VEC) {
       out[0] = lim > 0 ? w[0] : u32x4{0, 0, 0, 0};
@@ -99,6 +118,60 @@ struct Piece {
     }
   }
 };
+
+// The rows of a tensor for one batch and head, chunk by chunk: a buffer
+// descriptor of the chunk at hand, whose end is its last row's, so that rows
+// past the sequence read zero and drop stores.  (Rows must not overlap, and
+// their offsets within a chunk take 31 bits: delta.hip sees to it.)  next()
+// stays at the last chunk once there: loads ahead of it read that one again.
+struct ChunkRows {
+  const char* p;
+  int64_t step;      // bytes of 32 rows
+  int row, full, end, left;  // bytes of a row, a full chunk, the last chunk; chunks after this one
+  template <typename T>
+  __device__ inline void init(const T* base, int64_t stride, int cols, int64_t L, int nch) {
+    p = reinterpret_cast<const char*>(base);
+    row = (int)(stride * (int64_t)sizeof(T));
+    step = stride * (int64_t)sizeof(T) * kC;
+    full = (kC - 1) * row + cols * (int)sizeof(T);
+    end = (int)(L - 1 - (int64_t)(nch - 1) * kC) * row + cols * (int)sizeof(T);
+    left = nch - 1;
+  }
+  __device__ inline __amdgpu_buffer_rsrc_t at() const {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), (short)0,
+                                             left > 0 ? full : end, 0x00020000);
+  }
+  __device__ inline void next() {
+    p += left > 0 ? step : 0;
+    left -= left > 0 ? 1 : 0;
+  }
+};
+constexpr uint32_t kPast = 0x7ffffff0u;  // an offset past every descriptor's end
+
+template <typename T>
+__device__ inline T buf_elem(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+  if constexpr (sizeof(T) == 4)
+    return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0));
+  else
+    return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b16(r, off, 0, 0));
+}
+template <typename T>
+__device__ inline void buf_put(__amdgpu_buffer_rsrc_t r, uint32_t off, float x) {
+  T y;
+  stf(&y, x);
+  if constexpr (sizeof(T) == 4)
+    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, y), r, off, 0, 0);
+  else
+    __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, y), r, off, 0, 0);
+}
+
+// A workgroup's waves meet; what they wrote to LDS is there for all.  (Global
+// loads and stores stay in flight, unlike with __syncthreads.)
+__device__ inline void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
 
 // LDS reads of A operands.
 __device__ inline u32x4 lds16(const uint16_t* p) { return *reinterpret_cast<const u32x4*>(p); }
@@ -118,12 +191,13 @@ __device__ inline u32x4 lds_col(const uint16_t* m, int ld, int col, int lane) {
 }
 
 // What the preparing pass leaves for each chunk and value head, in the
-// workspace.  Rows past the sequence's end count as k = q = 0, g = beta = 0.
-template <int NPP>
+// workspace.  Steps past the sequence's end count as k = q = 0, g = beta = 0.
+// With G the sums of g within the chunk:
+//   fac: e^{G_t}, beta_t, e^{G_last - G_t}, g_t, and G_t log2(e) in two parts
+enum { kEg, kBeta, kEnd, kG, kGhi, kGlo, kFac = 8 };
 struct ChunkWs {
   uint16_t T[3][kC][kC];    // planes of (I + A)^-1
-  uint16_t P[NPP][kC][kC];  // planes of scale (Q K^T) o D
-  float fac[4][kC];         // e^{G_t}, beta_t, e^{G_last - G_t}, g_t
+  float fac[kFac][kC];
 };
 
 }  // namespace

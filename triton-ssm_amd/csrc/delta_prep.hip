@@ -1,10 +1,9 @@
 // Gated delta rule, preparing pass: per chunk of 32 steps and value head, what
-// the walks need of the keys, queries, decays and step sizes alone.
+// the walks need of the keys, decays and step sizes alone.
 //
-// With G the running sums of g within the chunk and D[t][i] = e^(G_t - G_i):
-//   A[t][i] = beta_t D[t][i] k_t.k_i (i < t),   T = (I + A)^-1,
-//   P[t][i] = scale D[t][i] q_t.k_i (i <= t).
-// One wave per chunk and head.  The Gram products run on the matrix cores (3
+// With G the running sums of g within the chunk:
+//   A[t][i] = beta_t e^(G_t - G_i) k_t.k_i (i < t),   T = (I + A)^-1.
+// One wave per chunk and head.  The Gram product runs on the matrix cores (3
 // of the 4 tiles of 16 x 16).  T's diagonal blocks come from forward
 // substitution (a lane per column: stable where keys repeat, unlike products
 // of powers of A), the block below from -T22 A21 T11 in fp32.  G is summed in
@@ -15,7 +14,7 @@
 namespace tssm {
 namespace {
 
-constexpr int kLd = 36;  // floats of a row of A, T or P in LDS
+constexpr int kLd = 36;  // floats of a row of A or T in LDS
 
 __device__ inline void wave_order() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -42,11 +41,11 @@ __device__ inline void put_planes(const float* m, uint16_t (*out)[kC][kC], int l
   }
 }
 
-template <typename T, int KP, bool VEC, int NPP>
-__global__ __launch_bounds__(256) void delta_prep_kernel(DeltaArgs a, ChunkWs<NPP>* ws,
-                                                         int64_t nch, int64_t units) {
+template <typename T, int KP, bool VEC>
+__global__ __launch_bounds__(256) void delta_prep_kernel(DeltaArgs a, ChunkWs* ws, int64_t nch,
+                                                         int64_t units) {
   constexpr int NP = Piece<T, VEC>::NP;
-  __shared__ __attribute__((aligned(16))) float mat[4][3][kC * kLd];
+  __shared__ __attribute__((aligned(16))) float mat[4][2][kC * kLd];
   __shared__ double sums[4][kC];
   __shared__ float bet[4][kC];
   const int lane = threadIdx.x & 63, j = lane >> 4, c = lane & 15;
@@ -57,8 +56,8 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(DeltaArgs a, ChunkWs<NP
   const int64_t bn = unit / a.Hv, h = unit - bn * a.Hv, b = bn / nch, n = bn - b * nch;
   const int64_t hk = h / (a.Hv / a.Hk), t0 = n * kC;
   const int rows = a.L - t0 < kC ? (int)(a.L - t0) : kC;
-  ChunkWs<NPP>& out = ws[(b * a.Hv + h) * nch + n];
-  float *mA = mat[wv][0], *mT = mat[wv][1], *mP = mat[wv][2];
+  ChunkWs& out = ws[(b * a.Hv + h) * nch + n];
+  float *mA = mat[wv][0], *mT = mat[wv][1];
 
   // running sums of g, per step
   const int t = lane & 31;
@@ -77,36 +76,34 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(DeltaArgs a, ChunkWs<NP
   if (lane < kC) {
     sums[wv][t] = G;
     bet[wv][t] = beta;
-    out.fac[0][t] = exp_acc((float)G);
-    out.fac[1][t] = beta;
-    out.fac[2][t] = exp_acc((float)(Gl - G));
-    out.fac[3][t] = on ? g0 : 0.0f;
+    out.fac[kEg][t] = exp_acc((float)G);
+    out.fac[kBeta][t] = beta;
+    out.fac[kEnd][t] = exp_acc((float)(Gl - G));
+    out.fac[kG][t] = on ? g0 : 0.0f;
+    const double G2 = G * 1.4426950408889634074;
+    out.fac[kGhi][t] = (float)G2;
+    out.fac[kGlo][t] = (float)(G2 - (double)(float)G2);
   }
 
-  // Gram products: tiles (0,0), (1,0), (1,1)
+  // Gram product: tiles (0,0), (1,0), (1,1)
   const T* kb = reinterpret_cast<const T*>(a.k) + b * a.k_b + t0 * a.k_l + hk * a.k_h;
-  const T* qb = reinterpret_cast<const T*>(a.q) + b * a.q_b + t0 * a.q_l + hk * a.q_h;
-  f32x4 kk[3] = {zero4(), zero4(), zero4()}, qk[3] = {zero4(), zero4(), zero4()};
-  Piece<T, VEC> pk[2], pq[2];
+  f32x4 kk[3] = {zero4(), zero4(), zero4()};
+  Piece<T, VEC> pk[2];
 #pragma unroll
   for (int s = 0; s < KP / 32; ++s) {
     const int col = 32 * s + 8 * j, clim = (int)a.K - col;
-    u32x4 fk[2][NP], fq[2][NP];
+    u32x4 fk[2][NP];
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       const int r = 16 * x + c, lim = r < rows ? clim : 0;
       const int64_t kr = (r < rows ? r : 0) * a.k_l + (clim > 0 ? col : 0);
-      const int64_t qr = (r < rows ? r : 0) * a.q_l + (clim > 0 ? col : 0);
       pk[x].load(kb + kr, lim);
-      pq[x].load(qb + qr, lim);
       pk[x].planes(lim, fk[x]);
-      pq[x].planes(lim, fq[x]);
     }
 #pragma unroll
     for (int x = 0; x < 3; ++x) {
       const int ro = x > 0, co = x > 1;
       kk[x] = mfma_planes<NP, NP, 3>(fk[ro], fk[co], kk[x]);
-      qk[x] = mfma_planes<NP, NP, 3>(fq[ro], fk[co], qk[x]);
     }
   }
   wave_order();
@@ -119,14 +116,10 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(DeltaArgs a, ChunkWs<NP
       const int row = 16 * (x > 0) + 4 * j + r;
       const float d = exp_acc((float)(sums[wv][row] - Gi));
       mA[row * kLd + i] = i < row ? bet[wv][row] * d * kk[x][r] : 0.0f;
-      mP[row * kLd + i] = i <= row ? a.scale * d * qk[x][r] : 0.0f;
     }
   }
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {  // the blocks above the diagonal
-    mT[(4 * j + r) * kLd + 16 + c] = 0.0f;
-    mP[(4 * j + r) * kLd + 16 + c] = 0.0f;
-  }
+  for (int r = 0; r < 4; ++r) mT[(4 * j + r) * kLd + 16 + c] = 0.0f;  // above the diagonal
   wave_order();
   // diagonal blocks: lane (d, c) solves for column c of block d
   {
@@ -170,30 +163,31 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(DeltaArgs a, ChunkWs<NP
   }
   wave_order();
   put_planes<3>(mT, out.T, lane);
-  put_planes<NPP>(mP, out.P, lane);
 }
 
-template <typename T, int KP, bool VEC, int NPP>
-void launch(const DeltaArgs& a, void* ws, hipStream_t s) {
+template <typename T, int KP>
+void launch(const DeltaArgs& a, bool vec, ChunkWs* ws, hipStream_t s) {
   const int64_t nch = cdiv64(a.L, kC), units = a.B * a.Hv * nch;
-  delta_prep_kernel<T, KP, VEC, NPP><<<(unsigned)cdiv64(units, 4), 256, 0, s>>>(
-      a, reinterpret_cast<ChunkWs<NPP>*>(ws), nch, units);
+  const unsigned wgs = (unsigned)cdiv64(units, 4);
+  if (vec) delta_prep_kernel<T, KP, true><<<wgs, 256, 0, s>>>(a, ws, nch, units);
+  else delta_prep_kernel<T, KP, false><<<wgs, 256, 0, s>>>(a, ws, nch, units);
 }
 
-template <typename T, int NPP>
-void prep(const DeltaArgs& a, bool vec, void* ws, hipStream_t s) {
-  if (a.K <= 32) vec ? launch<T, 32, true, NPP>(a, ws, s) : launch<T, 32, false, NPP>(a, ws, s);
-  else if (a.K <= 64) vec ? launch<T, 64, true, NPP>(a, ws, s) : launch<T, 64, false, NPP>(a, ws, s);
-  else vec ? launch<T, 128, true, NPP>(a, ws, s) : launch<T, 128, false, NPP>(a, ws, s);
+template <typename T>
+void prep(const DeltaArgs& a, bool vec, ChunkWs* ws, hipStream_t s) {
+  if (a.K <= 32) launch<T, 32>(a, vec, ws, s);
+  else if (a.K <= 64) launch<T, 64>(a, vec, ws, s);
+  else launch<T, 128>(a, vec, ws, s);
 }
 
 }  // namespace
 
-int delta_prep_launch(int dtype, const DeltaArgs& a, bool vec, void* ws, hipStream_t s) {
+int delta_prep_launch(int dtype, const DeltaArgs& a, bool vec, void* workspace, hipStream_t s) {
+  ChunkWs* ws = reinterpret_cast<ChunkWs*>(workspace);
   switch (dtype) {
-    case TSSM_F32: prep<float, 3>(a, vec, ws, s); break;
-    case TSSM_BF16: prep<bf16_t, 2>(a, vec, ws, s); break;
-    default: prep<f16_t, 3>(a, vec, ws, s); break;
+    case TSSM_F32: prep<float>(a, vec, ws, s); break;
+    case TSSM_BF16: prep<bf16_t>(a, vec, ws, s); break;
+    default: prep<f16_t>(a, vec, ws, s); break;
   }
   return launch_status();
 }

@@ -64,6 +64,12 @@ def _operands(q, k, v, g, beta, lead):
     return (*rows, Hk, Hv, K, V), code, g, beta
 
 
+def _steps(t):
+    """t [B, L, H, N], copied where its steps overlap in memory (as expanded
+    ones do): the chunked kernels take steps that lie one after the other."""
+    return t.contiguous() if t.shape[1] > 1 and t.stride(1) < t.shape[3] else t
+
+
 def _state(t, what, shape, device):
     if t is None:
         return None
@@ -90,6 +96,7 @@ def gated_delta_forward(q, k, v, g, beta, *, scale=None, h0=None, return_state=F
     other column of v.
     """
     (B, L, Hk, Hv, K, V), code, g, beta = _operands(q, k, v, g, beta, 2)
+    q, k, v = _steps(q), _steps(k), _steps(v)
     h0 = _state(h0, "h0", (B, Hv, K, V), q.get_device())
     o = torch.empty(v.shape, device=v.device, dtype=v.dtype) if out is None else out
     _check(o, "out", v.shape, v.dtype, q.get_device())
