@@ -202,7 +202,7 @@ def test_repeat_and_stream(dev):
 def test_step(dev, dtype, S, Hk, Hv, K, V):
     from tssm import gated_delta_step
     d = inputs(dev, 4, S, Hk, Hv, K, V, dtype, seed=S + V)
-    state = torch.randn(S, Hv, K, V, device=dev)
+    state = torch.randn(S, Hv, K, V, generator=torch.Generator().manual_seed(S)).to(dev)
     ref = np64(state)
     for t in range(4):
         x = {n: d[n][t] for n in ("q", "k", "v", "g", "beta")}
@@ -229,7 +229,7 @@ def test_step_graph(dev):
     from tssm import gated_delta_step
     d = inputs(dev, 4, 9, 2, 2, 64, 64, BF16, seed=16)
     x = {n: d[n][0].clone() for n in ("q", "k", "v", "g", "beta")}
-    state = torch.randn(9, 2, 64, 64, device=dev)
+    state = torch.randn(9, 2, 64, 64, generator=torch.Generator().manual_seed(16)).to(dev)
     eager, out = state.clone(), torch.empty_like(x["v"])
     gated_delta_step(**x, state=state.clone(), out=out)      # loads the kernel
     graph = torch.cuda.CUDAGraph()

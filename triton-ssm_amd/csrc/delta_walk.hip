@@ -410,9 +410,8 @@ __device__ inline void helper(const DeltaArgs& a, typename Walk<T, KP, VEC, NCW>
 }
 
 template <typename T, int KP, bool VEC, int NCW>
-__global__ __launch_bounds__(64 * (NCW + 2),
-                                  Walk<T, KP, VEC, NCW>::kWaves) void delta_walk_kernel(DeltaArgs a, const ChunkWs* ws,
-                                                                    int nch, uint32_t nvb) {
+__global__ __launch_bounds__(64 * (NCW + 2), (Walk<T, KP, VEC, NCW>::kWaves)) void
+    delta_walk_kernel(DeltaArgs a, const ChunkWs* ws, int nch, uint32_t nvb) {
   typedef Walk<T, KP, VEC, NCW> W;
   extern __shared__ __attribute__((aligned(16))) char raw[];
   typename W::Lds& lds = *reinterpret_cast<typename W::Lds*>(raw);
