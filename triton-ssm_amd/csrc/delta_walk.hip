@@ -9,11 +9,11 @@
 // operand in place (delta_dev.h).
 //
 // The chain S -> R -> U -> S' sets the time, one chunk after the other, so it
-// has waves of its own: a workgroup is NCW of them and two helpers, each on a
-// SIMD of its own.  The helpers bring K, Q, V and T into LDS two chunks ahead
-// and form the outputs of the chunk before from the planes of S and U that the
-// chain waves leave in LDS, one helper the even and one the odd half-rows of
-// tiles.  One barrier a chunk.
+// has waves of its own.  A workgroup is NCW of them, two output waves and two
+// loaders, on the four SIMDs of a CU.  The loaders bring K, Q, V and T into LDS
+// two chunks ahead.  The output waves form the outputs of the chunk before from
+// the planes of S and U that the chain waves leave in LDS, one wave rows
+// 8 j + r, one rows 8 j + 4 + r.  One barrier a chunk.
 //
 // A chunk whose U is not finite is done again step by step from S: zero
 // weights would otherwise carry a later step's NaN to earlier outputs.
@@ -26,7 +26,8 @@ template <typename T, int KP, bool VEC, int NCW>
 struct Walk {
   static constexpr int NP = Piece<T, VEC>::NP;  // planes of the inputs
   static constexpr int NO = NP == 1 ? 2 : 3;    // of S, P and U in the outputs' products
-  static constexpr int NS = KP / 32, NT = 128;  // threads of the helpers
+  static constexpr int NS = KP / 32, NT = 128;  // threads of the loaders
+  static constexpr int kThreads = 64 * (NCW + 4);
   static constexpr int kLd = KP + 8;            // bf16 elements of a row of K or Q in LDS
   static constexpr int kNk = kC * KP / 8 / NT;  // 8-element pieces of K a thread brings
   static constexpr int kTp = 3 * kC * kC / 8;   // 16-byte pieces of T
@@ -34,6 +35,7 @@ struct Walk {
   static constexpr int kVld = NP == 1 ? 16 * NCW + 8 : 16 * NCW + 4;  // elements of V's row
   // 256 registers where they suffice: with more to give out the compiler puts
   // products into accumulation registers and copies them back
+  static constexpr bool kEarly = NP * KP <= 128;  // registers for K^T's operands too
   static constexpr int kWaves = VEC && NP * KP < 384 ? 2 : 1;
   typedef std::conditional_t<NP == 1, uint16_t, float> vlds_t;
   struct Operands {  // of one chunk
@@ -75,10 +77,21 @@ __device__ inline void chain(const DeltaArgs& a, typename W::Lds& lds, int64_t b
       const float x = a.h0 ? a.h0[sbase + (int64_t)(k < K ? k : 0) * a.V] : 0.0f;
       S[i][r] = on && k < K ? x : 0.0f;
     }
+  __builtin_amdgcn_s_setprio(3);  // before the loader on the same SIMD
   lds_barrier();
   for (int n = 0; n < nch; ++n) {
     const typename W::Operands& B = lds.op[n & 1];
     typename W::Left& left = lds.left[n & 1][wv];
+    // every operand but V's decays is asked for here: read where they are
+    // used, each product would wait for LDS
+    u32x4 fk[NS][2][NP], ft[2][3], fc[NP][2 * NS];
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+          fk[s][x][p] = lds16(&B.K[p][(ar + 4 * x) * W::kLd + 32 * s + 8 * j]);
     float v[8], eg[8], be[8], en[8];
     if constexpr (NP == 1) {
       const uint16_t* p = B.V + (8 * j + (c >> 2)) * W::kVld + 16 * wv + 4 * (c & 3);
@@ -103,35 +116,38 @@ __device__ inline void chain(const DeltaArgs& a, typename W::Lds& lds, int64_t b
           *reinterpret_cast<const float4*>(&B.fac[kEnd][8 * j + 4 * q]);
     }
     const float last = B.fac[kEg][kC - 1];
+#pragma unroll
+    for (int p = 0; p < 3; ++p)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) ft[x][p] = lds16(&B.M[p][(ar + 4 * x) * kTld + 8 * j]);
+    if constexpr (W::kEarly) {
+#pragma unroll
+      for (int p = 0; p < NP; ++p)
+#pragma unroll
+        for (int i = 0; i < 2 * NS; ++i)
+          fc[p][i] = lds_col(B.K[p], W::kLd, 32 * (i >> 1) + 4 * (i & 1), lane);
+    }
+    __builtin_amdgcn_sched_barrier(0);
     f32x4 ks[2] = {zero4(), zero4()};
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
-      u32x4 sp[3], f[2][NP];
+      u32x4 sp[3];
       split_tiles<3>(S[2 * s], S[2 * s + 1], sp);
 #pragma unroll
       for (int p = 0; p < W::NO; ++p) left.S[s][p][lane] = sp[p];
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int p = 0; p < NP; ++p)
-          f[x][p] = lds16(&B.K[p][(ar + 4 * x) * W::kLd + 32 * s + 8 * j]);
 #pragma unroll
       for (int p = 0; p < NP; ++p)
 #pragma unroll
         for (int q = 0; q + p < 3; ++q)
 #pragma unroll
-          for (int x = 0; x < 2; ++x) ks[x] = mfma32(f[x][p], sp[q], ks[x]);
+          for (int x = 0; x < 2; ++x) ks[x] = mfma32(fk[s][x][p], sp[q], ks[x]);
     }
     f32x4 R[2], U[2] = {zero4(), zero4()};
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       R[e >> 2][e & 3] = be[e] * __builtin_fmaf(-eg[e], ks[e >> 2][e & 3], v[e]);
-    u32x4 rp[3], ft[2][3];
+    u32x4 rp[3];
     split_tiles<3>(R[0], R[1], rp);
-#pragma unroll
-    for (int x = 0; x < 2; ++x)
-#pragma unroll
-      for (int p = 0; p < 3; ++p) ft[x][p] = lds16(&B.M[p][(ar + 4 * x) * kTld + 8 * j]);
 #pragma unroll
     for (int p = 0; p < 3; ++p)
 #pragma unroll
@@ -156,14 +172,15 @@ __device__ inline void chain(const DeltaArgs& a, typename W::Lds& lds, int64_t b
       for (int r = 0; r < 4; ++r) N[i][r] = S[i][r] * last;
 #pragma unroll
     for (int p = 0; p < NP; ++p) {
-      u32x4 f[2 * NS];
+      if constexpr (!W::kEarly) {
 #pragma unroll
-      for (int i = 0; i < 2 * NS; ++i)
-        f[i] = lds_col(B.K[p], W::kLd, 32 * (i >> 1) + 4 * (i & 1), lane);
+        for (int i = 0; i < 2 * NS; ++i)
+          fc[p][i] = lds_col(B.K[p], W::kLd, 32 * (i >> 1) + 4 * (i & 1), lane);
+      }
 #pragma unroll
       for (int q = 0; q + p < 3; ++q)
 #pragma unroll
-        for (int i = 0; i < 2 * NS; ++i) N[i] = mfma32(f[i], ep[q], N[i]);
+        for (int i = 0; i < 2 * NS; ++i) N[i] = mfma32(fc[p][i], ep[q], N[i]);
     }
     const bool slow = __ballot(!(big < __builtin_inff())) != 0;
     if (lane == 0) left.slow = slow;
@@ -220,22 +237,20 @@ __device__ inline void chain(const DeltaArgs& a, typename W::Lds& lds, int64_t b
     }
 }
 
-// The operands' way to LDS, and the outputs of rows 8 j + 4 y + r.
+// The operands' way to LDS.
 template <typename T, int KP, bool VEC, int NCW>
-__device__ inline void helper(const DeltaArgs& a, typename Walk<T, KP, VEC, NCW>::Lds& lds,
-                              const ChunkWs* ws, int64_t bh, int64_t v0, int y, int nch) {
+__device__ inline void bring(const DeltaArgs& a, typename Walk<T, KP, VEC, NCW>::Lds& lds,
+                              const ChunkWs* ws, int64_t bh, int64_t v0, int nch) {
   typedef Walk<T, KP, VEC, NCW> W;
-  constexpr int NP = W::NP, NO = W::NO, NS = W::NS, NT = W::NT, kE = (int)sizeof(T);
-  const int id = threadIdx.x - 64 * NCW, lane = id & 63, j = lane >> 4, c = lane & 15;
-  const int ar = 8 * (c >> 2) + (c & 3);
+  constexpr int NP = W::NP, NT = W::NT, kE = (int)sizeof(T);
+  const int id = threadIdx.x - 64 * (NCW + 2);
   const int64_t b = bh / a.Hv, h = bh - b * a.Hv, hk = h / (a.Hv / a.Hk);
   const int nv = a.V - v0 < 16 * NCW ? (int)(a.V - v0) : 16 * NCW, K = (int)a.K;
-  ChunkRows rk, rq, rv, ro;
+  ChunkRows rk, rq, rv;
   rk.init(reinterpret_cast<const T*>(a.k) + b * a.k_b + hk * a.k_h, a.k_l, K, a.L, nch);
   rq.init(reinterpret_cast<const T*>(a.q) + b * a.q_b + hk * a.q_h, a.q_l, K, a.L, nch);
   rv.init(reinterpret_cast<const T*>(a.v) + b * a.v_b + h * a.v_h + v0, a.v_l, nv, a.L, nch);
-  ro.init(reinterpret_cast<T*>(a.o) + b * a.o_b + h * a.o_h + v0, a.o_l, nv, a.L, nch);
-  uint32_t ok[W::kNk], oq[W::kNk], oo[NCW][4];
+  uint32_t ok[W::kNk], oq[W::kNk];
 #pragma unroll
   for (int i = 0; i < W::kNk; ++i) {
     const int r = (id + NT * i) / (KP / 8), col = (id + NT * i) % (KP / 8) * 8;
@@ -244,11 +259,6 @@ __device__ inline void helper(const DeltaArgs& a, typename Walk<T, KP, VEC, NCW>
   }
   const int vr = id / W::kVp, vcol = id % W::kVp * 8;   // this thread's piece of V
   const uint32_t ov = vr < kC && vcol < nv ? vr * rv.row + vcol * kE : kPast;
-#pragma unroll
-  for (int g = 0; g < NCW; ++g)
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-      oo[g][r] = 16 * g + c < nv ? (8 * j + 4 * y + r) * ro.row + (16 * g + c) * kE : kPast;
 
   // as they lie in memory: a conversion on the way would wait for the load
   struct Regs {
@@ -313,6 +323,42 @@ __device__ inline void helper(const DeltaArgs& a, typename Walk<T, KP, VEC, NCW>
   };
   static_assert(W::kTp == 3 * NT && kFac * kC == 2 * NT, "pieces of a chunk");
 
+  Regs g0, g1;
+  load(g0);
+  load(g1);
+  store(g0, 0);
+  lds_barrier();
+  // the chain waves are in chunk n; nx holds chunk n + 1, g takes n + 2
+  auto turn = [&](int n, Regs& g, Regs& nx) {
+    load(g);
+    store(nx, n + 1);
+    lds_barrier();
+  };
+  for (int n = 0; n < nch; n += 2) {
+    turn(n, g0, g1);
+    if (n + 1 < nch) turn(n + 1, g1, g0);
+  }
+}
+
+// The outputs of rows 8 j + 4 y + r, one chunk behind the chain waves.
+template <typename T, int KP, bool VEC, int NCW>
+__device__ inline void outputs(const DeltaArgs& a, typename Walk<T, KP, VEC, NCW>::Lds& lds,
+                               int64_t bh, int64_t v0, int y, int nch) {
+  typedef Walk<T, KP, VEC, NCW> W;
+  constexpr int NP = W::NP, NO = W::NO, NS = W::NS, kE = (int)sizeof(T);
+  const int lane = threadIdx.x & 63, j = lane >> 4, c = lane & 15;
+  const int ar = 8 * (c >> 2) + (c & 3);
+  const int64_t b = bh / a.Hv, h = bh - b * a.Hv;
+  const int nv = a.V - v0 < 16 * NCW ? (int)(a.V - v0) : 16 * NCW;
+  ChunkRows ro;
+  ro.init(reinterpret_cast<T*>(a.o) + b * a.o_b + h * a.o_h + v0, a.o_l, nv, a.L, nch);
+  uint32_t oo[NCW][4];
+#pragma unroll
+  for (int g = 0; g < NCW; ++g)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      oo[g][r] = 16 * g + c < nv ? (8 * j + 4 * y + r) * ro.row + (16 * g + c) * kE : kPast;
+
   // what the outputs of a chunk need besides S and U: read while the chunk is
   // in LDS, used when the chain waves are past it
   u32x4 fq[NS][NP], fp[NO];
@@ -352,7 +398,7 @@ __device__ inline void helper(const DeltaArgs& a, typename Walk<T, KP, VEC, NCW>
     *reinterpret_cast<float4*>(eg) =
         *reinterpret_cast<const float4*>(&B.fac[kEg][8 * j + 4 * y]);
   };
-  auto outputs = [&](int n) {
+  auto put = [&](int n) {
     const auto dst = ro.at();
     ro.next();
     f32x4 o[NCW];
@@ -388,29 +434,17 @@ __device__ inline void helper(const DeltaArgs& a, typename Walk<T, KP, VEC, NCW>
       for (int r = 0; r < 4; ++r) buf_put<T>(dst, oo[g][r], a.scale * o[g][r]);
   };
 
-  Regs g0, g1;
-  load(g0);
-  load(g1);
-  store(g0, 0);
   lds_barrier();
-  // the chain waves are in chunk n; nx holds chunk n + 1, g takes n + 2
-  auto turn = [&](int n, Regs& g, Regs& nx) {
-    load(g);
-    if (n > 0) outputs(n - 1);
+  for (int n = 0; n < nch; ++n) {
+    if (n > 0) put(n - 1);
     weights(n);
-    store(nx, n + 1);
     lds_barrier();
-  };
-  turn(0, g0, g1);
-  for (int n = 1; n < nch; n += 2) {
-    turn(n, g1, g0);
-    if (n + 1 < nch) turn(n + 1, g0, g1);
   }
-  outputs(nch - 1);
+  put(nch - 1);
 }
 
 template <typename T, int KP, bool VEC, int NCW>
-__global__ __launch_bounds__(64 * (NCW + 2), (Walk<T, KP, VEC, NCW>::kWaves)) void
+__global__ __launch_bounds__((Walk<T, KP, VEC, NCW>::kThreads), (Walk<T, KP, VEC, NCW>::kWaves)) void
     delta_walk_kernel(DeltaArgs a, const ChunkWs* ws, int nch, uint32_t nvb) {
   typedef Walk<T, KP, VEC, NCW> W;
   extern __shared__ __attribute__((aligned(16))) char raw[];
@@ -422,8 +456,10 @@ __global__ __launch_bounds__(64 * (NCW + 2), (Walk<T, KP, VEC, NCW>::kWaves)) vo
   if (bh >= heads) return;
   if (wv < NCW)
     chain<W, NCW>(a, lds, bh, v0 + 16 * wv + (threadIdx.x & 15), wv, nch);
+  else if (wv < NCW + 2)
+    outputs<T, KP, VEC, NCW>(a, lds, bh, v0, wv - NCW, nch);
   else
-    helper<T, KP, VEC, NCW>(a, lds, ws + bh * (int64_t)nch, bh, v0, wv - NCW, nch);
+    bring<T, KP, VEC, NCW>(a, lds, ws + bh * (int64_t)nch, bh, v0, nch);
 }
 
 template <typename T, int KP, bool VEC, int NCW>
@@ -439,7 +475,7 @@ int launch(const DeltaArgs& a, const ChunkWs* ws, hipStream_t s) {
                                              hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != hipSuccess) return (int)e;
   }
-  f<<<(unsigned)wgs, 64 * (NCW + 2), bytes, s>>>(a, ws, (int)cdiv64(a.L, kC), (uint32_t)nvb);
+  f<<<(unsigned)wgs, W::kThreads, bytes, s>>>(a, ws, (int)cdiv64(a.L, kC), (uint32_t)nvb);
   return launch_status();
 }
 
