@@ -95,6 +95,21 @@ def test_forward_strides(dev, dtype):
     assert_close(S, S_ref, TOL[F32], "state")
 
 
+@pytest.mark.parametrize("dtype,B,L,Hk,Hv,K,V,rate,h0", [
+    (BF16, 1, 8200, 1, 2, 64, 64, 0.02, True),    # segments, slow decay across them
+    (F32, 1, 5001, 1, 1, 40, 72, 0.05, False),
+    (F16, 2, 3000, 1, 1, 128, 30, 0.02, True),
+    (BF16, 1, 4096, 2, 2, 16, 16, 0.0, True),     # no decay
+])
+def test_segments(dev, dtype, B, L, Hk, Hv, K, V, rate, h0):
+    """Long sequences over few heads are walked in segments."""
+    d = inputs(dev, B, L, Hk, Hv, K, V, dtype, seed=L, h0=h0, rate=rate)
+    o, S = run(d)
+    o_ref, S_ref = oracle(d)
+    assert_close(o, o_ref, TOL[dtype], "o")
+    assert_close(S, S_ref, TOL[F32], "state")
+
+
 @pytest.mark.parametrize("L", [0, 1])
 def test_empty(dev, L):
     d = inputs(dev, 2, L, 2, 2, 32, 32, F32, h0=True)

@@ -24,10 +24,26 @@ struct DeltaArgs {
 // delta_seq.hip: one step after another, the state in registers.
 int delta_seq_launch(int dtype, const DeltaArgs& a, hipStream_t s);
 
-// Chunked form: delta_prep.hip (per chunk, in parallel) into the workspace,
-// then delta_walk.hip.  vec: the rows of q, k and v are whole 16-byte accesses.
-int delta_prep_launch(int dtype, const DeltaArgs& a, bool vec, void* ws, hipStream_t s);
-int delta_walk_launch(int dtype, const DeltaArgs& a, bool vec, const void* ws, hipStream_t s);
+// Chunked form.  Workspace of one call: what the preparing pass leaves of each
+// chunk and, for sequences walked in segments, the segments' transfer
+// matrices and entry states; for the gradients also the states before the
+// chunks, and the gradients of the states after them.
+struct DeltaPlan {
+  void* chunks;
+  float *transfer, *entry;     // nseg > 1
+  float *states;               // gradients only
+  int nch, per, nseg;          // chunks, chunks of a segment, segments
+  int64_t bytes;
+};
+
+// vec: the rows of q, k and v are whole 16-byte accesses.
+int delta_prep_launch(int dtype, const DeltaArgs& a, bool vec, void* chunks, hipStream_t s);
+int delta_walk_launch(int dtype, const DeltaArgs& a, bool vec, const DeltaPlan& p, hipStream_t s);
+// The segments' transfer matrices, then their entry states.
+int delta_transfer_launch(int dtype, const DeltaArgs& a, bool vec, const DeltaPlan& p,
+                          hipStream_t s);
+int delta_states_launch(int dtype, const DeltaArgs& a, bool vec, const DeltaPlan& p,
+                        hipStream_t s);
 int64_t delta_chunk_ws_bytes();  // of one chunk of one value head
 
 }  // namespace tssm

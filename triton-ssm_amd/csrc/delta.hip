@@ -12,7 +12,50 @@ bool sizes_ok(int64_t B, int64_t L, int64_t Hk, int64_t Hv, int64_t K, int64_t V
 // Shorter sequences go step by step.
 constexpr int64_t kSeqMost = 16;
 
-int64_t chunk_heads(int64_t B, int64_t L, int64_t Hv) { return B * Hv * cdiv64(L, 32); }
+// How many segments a sequence of nch chunks is walked in, by the times that the
+// walks take (in tenths of a chunk's time of one workgroup on each CU, a
+// microsecond): the outputs' walk fills a CU with one workgroup of 32 columns;
+// the walk from zero over V + KP columns, which s > 1 segments add, takes 1.5
+// and 2 times as long a chunk with two and four workgroups on a CU; joining
+// takes half a chunk's time a segment.  B = 1, L = 65536, H = 8, K = V = 64,
+// bf16: 1780 us in one segment; with 8, 16, 32 and 64: 513, 375, 332 and 406.
+int64_t segments(int64_t heads, int64_t nch, int64_t KP, int64_t V) {
+  const int64_t out = heads * cdiv64(V, 32), all = heads * (cdiv64(V, 32) + KP / 32);
+  int64_t best = 1, least = nch * 10 * cdiv64(out, 256);
+  for (int64_t s = 2; s <= 512 && s <= nch / 4; s = s < 8 ? s + 1 : s + s / 8) {
+    const int64_t per = cdiv64(nch, s), w = (s - 1) * all;
+    const int64_t zero = w <= 256 ? 10 : (w <= 512 ? 15 : 20 * cdiv64(w, 1024));
+    const int64_t cost = per * (zero + 10 * cdiv64(cdiv64(nch, per) * out, 256)) + 5 * s;
+    if (cost < least) {
+      best = s;
+      least = cost;
+    }
+  }
+  return best;
+}
+
+// The chunked form's plan over a workspace at base (which may be null: sizes).
+DeltaPlan delta_plan(char* base, int64_t B, int64_t L, int64_t Hv, int64_t K, int64_t V) {
+  DeltaPlan p = {};
+  const int64_t nch = cdiv64(L, 32), heads = B * Hv, KP = K <= 32 ? 32 : (K <= 64 ? 64 : 128);
+  const int64_t Vp = cdiv64(V, 16) * 16;
+  int64_t at = 0;
+  const auto take = [&](int64_t bytes) {
+    char* q = base + at;
+    at += cdiv64(bytes, 256) * 256;
+    return q;
+  };
+  p.nch = (int)nch;
+  p.per = (int)cdiv64(nch, segments(heads, nch, KP, V));
+  p.nseg = (int)cdiv64(nch, p.per);
+  p.chunks = take(heads * nch * delta_chunk_ws_bytes());
+  if (p.nseg > 1) {
+    p.transfer = reinterpret_cast<float*>(take(heads * p.nseg * (Vp + KP) * KP * 4));
+    p.entry = reinterpret_cast<float*>(take(heads * p.nseg * Vp * KP * 4));
+  }
+  p.bytes = at;
+  return p;
+}
 
 // The rows of q, k and v are whole 16-byte accesses.
 bool vec_rows(int dtype, const DeltaArgs& a) {
@@ -51,13 +94,15 @@ extern "C" int tssm_gated_delta_forward(
                        sq_b, sq_l, sq_h, sk_b, sk_l, sk_h, sv_b, sv_l, sv_h,
                        sg_b, sg_l, sg_h, sbe_b, sbe_l, sbe_h, so_b, so_l, so_h, scale};
   if (L <= kSeqMost || !chunk_rows(dtype, a)) return delta_seq_launch(dtype, a, as_stream(stream));
-  const int64_t units = chunk_heads(nbatch, L, Hv);
-  TSSM_CHECK(units <= 0x7fffffff, TSSM_ERR_UNSUPPORTED);
-  TSSM_CHECK(workspace && workspace_bytes >= units * delta_chunk_ws_bytes() &&
-                 aligned(workspace, 256), TSSM_ERR_WORKSPACE);
+  TSSM_CHECK(nbatch * Hv <= 0x7fffffff / cdiv64(L, 32), TSSM_ERR_UNSUPPORTED);
+  const DeltaPlan p = delta_plan(reinterpret_cast<char*>(workspace), nbatch, L, Hv, K, V);
+  TSSM_CHECK(workspace && workspace_bytes >= p.bytes && aligned(workspace, 256),
+             TSSM_ERR_WORKSPACE);
   const bool vec = vec_rows(dtype, a);
-  const int rc = delta_prep_launch(dtype, a, vec, workspace, as_stream(stream));
-  return rc ? rc : delta_walk_launch(dtype, a, vec, workspace, as_stream(stream));
+  hipStream_t st = as_stream(stream);
+  int rc = delta_prep_launch(dtype, a, vec, p.chunks, st);
+  if (!rc && p.nseg > 1) rc = delta_transfer_launch(dtype, a, vec, p, st);
+  return rc ? rc : delta_walk_launch(dtype, a, vec, p, st);
 }
 
 extern "C" int tssm_gated_delta_step(int dtype, const void* q, const void* k, const void* v,
@@ -82,6 +127,6 @@ extern "C" int64_t tssm_gated_delta_workspace_bytes(int64_t nbatch, int64_t L, i
                                                     int64_t Hv, int64_t K, int64_t V) {
   if (!sizes_ok(nbatch, L, Hk, Hv, K, V)) return TSSM_ERR_SHAPE;
   if (K > 128) return TSSM_ERR_UNSUPPORTED;
-  if (L <= kSeqMost) return 256;
-  return chunk_heads(nbatch, L, Hv) * delta_chunk_ws_bytes() + 256;
+  if (L <= kSeqMost || nbatch == 0) return 256;
+  return delta_plan(nullptr, nbatch, L, Hv, K, V).bytes;
 }

@@ -119,31 +119,28 @@ struct Piece {
   }
 };
 
-// The rows of a tensor for one batch and head, chunk by chunk: a buffer
-// descriptor of the chunk at hand, whose end is its last row's, so that rows
-// past the sequence read zero and drop stores.  (Rows must not overlap, and
-// their offsets within a chunk take 31 bits: delta.hip sees to it.)  next()
-// stays at the last chunk once there: loads ahead of it read that one again.
+// The rows of a tensor for one batch and head: at(n) is a buffer descriptor of
+// chunk n whose end is the chunk's last row's, so that rows past the sequence
+// read zero and drop stores.  (Rows must not overlap, and their offsets within
+// a chunk take 31 bits: delta.hip sees to it.)  A chunk outside the sequence
+// is taken for the nearest one in it: loads ahead need no branch.
 struct ChunkRows {
   const char* p;
-  int64_t step;      // bytes of 32 rows
-  int row, full, end, left;  // bytes of a row, a full chunk, the last chunk; chunks after this one
+  int64_t step;             // bytes of 32 rows
+  int row, full, end, last; // bytes of a row, a full chunk, the last chunk; its number
   template <typename T>
-  __device__ inline void init(const T* base, int64_t stride, int cols, int64_t L, int nch) {
+  __device__ inline void init(const T* base, int64_t stride, int cols, int64_t L) {
     p = reinterpret_cast<const char*>(base);
     row = (int)(stride * (int64_t)sizeof(T));
     step = stride * (int64_t)sizeof(T) * kC;
+    last = (int)((L - 1) / kC);
     full = (kC - 1) * row + cols * (int)sizeof(T);
-    end = (int)(L - 1 - (int64_t)(nch - 1) * kC) * row + cols * (int)sizeof(T);
-    left = nch - 1;
+    end = (int)((L - 1) % kC) * row + cols * (int)sizeof(T);
   }
-  __device__ inline __amdgpu_buffer_rsrc_t at() const {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), (short)0,
-                                             left > 0 ? full : end, 0x00020000);
-  }
-  __device__ inline void next() {
-    p += left > 0 ? step : 0;
-    left -= left > 0 ? 1 : 0;
+  __device__ inline __amdgpu_buffer_rsrc_t at(int n) const {
+    const int m = n < 0 ? 0 : (n < last ? n : last);
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p + m * step), (short)0,
+                                             m < last ? full : end, 0x00020000);
   }
 };
 constexpr uint32_t kPast = 0x7ffffff0u;  // an offset past every descriptor's end
@@ -173,6 +170,10 @@ __device__ inline void lds_barrier() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
+__device__ inline __amdgpu_buffer_rsrc_t rsrc_of(const void* p, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, bytes, 0x00020000);
+}
+
 // LDS reads of A operands.
 __device__ inline u32x4 lds16(const uint16_t* p) { return *reinterpret_cast<const u32x4*>(p); }
 // Four elements of column lane % 16 from the rows that the quads of each
@@ -199,6 +200,54 @@ struct ChunkWs {
   uint16_t T[3][kC][kC];    // planes of (I + A)^-1
   float fac[kFac][kC];
 };
+
+__device__ inline const ChunkWs* chunk_at(const ChunkWs* ws, int n, int nch) {
+  return ws + (n < 0 ? 0 : (n < nch ? n : nch - 1));
+}
+
+// The state (or its gradient) of one value head in the workspace: [Vp][KP]
+// fp32, column by column, Vp = V rounded up to 16, zero past K and V.  A lane's
+// rows 8 j .. 8 j + 7 of 32 are 32 bytes.
+template <int NS>
+__device__ inline void put_cols(float* m, const f32x4 (&S)[2 * NS], int64_t col, int j) {
+  float* p = m + col * 32 * NS + 8 * j;
+#pragma unroll
+  for (int i = 0; i < 2 * NS; ++i)
+    *reinterpret_cast<f32x4*>(p + 32 * (i >> 1) + 4 * (i & 1)) = S[i];
+}
+template <int NS>
+__device__ inline void get_cols(const float* m, f32x4 (&S)[2 * NS], int64_t col, int j) {
+  const float* p = m + col * 32 * NS + 8 * j;
+#pragma unroll
+  for (int i = 0; i < 2 * NS; ++i)
+    S[i] = *reinterpret_cast<const f32x4*>(p + 32 * (i >> 1) + 4 * (i & 1));
+}
+// The same from and to a caller's [K][V] state.
+template <int NS>
+__device__ inline void get_state(const float* m, f32x4 (&S)[2 * NS], int64_t col, int64_t V, int K,
+                                 int j) {
+  const bool on = m && col < V;
+#pragma unroll
+  for (int i = 0; i < 2 * NS; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int k = 32 * (i >> 1) + 8 * j + 4 * (i & 1) + r;
+      const float x = m ? m[(int64_t)(k < K ? k : 0) * V + (on ? col : 0)] : 0.0f;
+      S[i][r] = on && k < K ? x : 0.0f;
+    }
+}
+template <int NS>
+__device__ inline void put_state(float* m, const f32x4 (&S)[2 * NS], int64_t col, int64_t V, int K,
+                                 int j) {
+  if (!m || col >= V) return;
+#pragma unroll
+  for (int i = 0; i < 2 * NS; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int k = 32 * (i >> 1) + 8 * j + 4 * (i & 1) + r;
+      if (k < K) m[(int64_t)k * V + col] = S[i][r];
+    }
+}
 
 }  // namespace
 }  // namespace tssm
