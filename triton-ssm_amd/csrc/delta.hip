@@ -17,7 +17,7 @@ constexpr int64_t kSeqMost = 16;
 // microsecond): the outputs' walk fills a CU with one workgroup of 32 columns;
 // the walk from zero over V + KP columns, which s > 1 segments add, takes 1.5
 // and 2 times as long a chunk with two and four workgroups on a CU; joining
-// takes half a chunk's time a segment.  B = 1, L = 65536, H = 8, K = V = 64,
+// takes a chunk's time a segment, the two launches more twelve.  B = 1, L = 65536, H = 8, K = V = 64,
 // bf16: 1780 us in one segment; with 8, 16, 32 and 64: 513, 375, 332 and 406.
 int64_t segments(int64_t heads, int64_t nch, int64_t KP, int64_t V) {
   const int64_t out = heads * cdiv64(V, 32), all = heads * (cdiv64(V, 32) + KP / 32);
@@ -25,7 +25,7 @@ int64_t segments(int64_t heads, int64_t nch, int64_t KP, int64_t V) {
   for (int64_t s = 2; s <= 512 && s <= nch / 4; s = s < 8 ? s + 1 : s + s / 8) {
     const int64_t per = cdiv64(nch, s), w = (s - 1) * all;
     const int64_t zero = w <= 256 ? 10 : (w <= 512 ? 15 : 20 * cdiv64(w, 1024));
-    const int64_t cost = per * (zero + 10 * cdiv64(cdiv64(nch, per) * out, 256)) + 5 * s;
+    const int64_t cost = per * (zero + 10 * cdiv64(cdiv64(nch, per) * out, 256)) + 10 * s + 120;
     if (cost < least) {
       best = s;
       least = cost;
