@@ -592,6 +592,29 @@ int tssm_gated_delta_forward(int dtype, const void* q, const void* k, const void
                              int64_t so_b, int64_t so_l, int64_t so_h, float scale,
                              void* workspace, int64_t workspace_bytes, void* stream);
 
+/* Gradients of the forward for dout [B,L,Hv,V] (strides sd) and dh_last f32
+ * [B,Hv,K,V] or NULL (zero): dq, dk [B,L,Hk,K] (summed over the value heads
+ * that share a key head, in order), dv [B,L,Hv,V] of `dtype`, dg, dbeta f32
+ * [B,L,Hv], all contiguous, dh0 f32 [B,Hv,K,V] or NULL.  The rows of q, k, v
+ * and dout must not overlap (L > 1).  The states are formed again from the
+ * inputs and kept in the workspace
+ * (tssm_gated_delta_backward_workspace_bytes() bytes, else as the forward's):
+ * 8 K V bytes for every 32 steps of a value head.  With L = 0 nothing is
+ * written (dh0 would be dh_last). */
+int64_t tssm_gated_delta_backward_workspace_bytes(int64_t nbatch, int64_t L, int64_t Hk,
+                                                  int64_t Hv, int64_t K, int64_t V);
+int tssm_gated_delta_backward(int dtype, const void* q, const void* k, const void* v,
+                              const float* g, const float* beta, const float* h0,
+                              const void* dout, const float* dh_last, void* dq, void* dk,
+                              void* dv, float* dg, float* dbeta, float* dh0, int64_t nbatch,
+                              int64_t L, int64_t Hk, int64_t Hv, int64_t K, int64_t V,
+                              int64_t sq_b, int64_t sq_l, int64_t sq_h, int64_t sk_b,
+                              int64_t sk_l, int64_t sk_h, int64_t sv_b, int64_t sv_l,
+                              int64_t sv_h, int64_t sg_b, int64_t sg_l, int64_t sg_h,
+                              int64_t sbe_b, int64_t sbe_l, int64_t sbe_h, int64_t sd_b,
+                              int64_t sd_l, int64_t sd_h, float scale, void* workspace,
+                              int64_t workspace_bytes, void* stream);
+
 /* One step of S streams, state f32 contiguous [S,Hv,K,V] updated in place:
  * q, k [S,Hk,K], v, o [S,Hv,V], g, beta [S,Hv], strides (s, h). */
 int tssm_gated_delta_step(int dtype, const void* q, const void* k, const void* v, const float* g,

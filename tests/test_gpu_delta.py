@@ -209,6 +209,107 @@ def test_repeat_and_stream(dev):
     assert torch.equal(o, o2) and torch.equal(S, S2)
 
 
+# ------------------------------------------------------------------ gradients
+NAMES = ("dq", "dk", "dv", "dg", "dbeta", "dh0")
+
+
+def gradients(d, do, dh=None, **kw):
+    from tssm import gated_delta_backward
+    return gated_delta_backward(d["q"], d["k"], d["v"], d["g"], d["beta"], do, h0=d["h0"],
+                                dh_last=dh, **kw)
+
+
+def check_gradients(dev, d, dtype, seed, dh=True, **kw):
+    r = torch.Generator().manual_seed(seed)
+    B, L, Hv, V = d["v"].shape
+    K = d["q"].shape[-1]
+    do = torch.randn(B, L, Hv, V, generator=r).to(dtype).to(dev)
+    dh = torch.randn(B, Hv, K, V, generator=r).to(dev) if dh else None
+    got = gradients(d, do, dh, **kw)
+    ref = M.delta_backward(**{n: None if t is None else np64(t) for n, t in d.items()},
+                           do=np64(do), dh_last=None if dh is None else np64(dh), **kw)
+    for name, x, y in zip(NAMES, got, ref):
+        if name == "dh0" and d["h0"] is None:
+            assert x is None
+        else:
+            assert_close(x, y, TOL[dtype] if name in ("dq", "dk", "dv") else TOL[F32], name)
+    return do, dh, got
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("B,L,Hk,Hv,K,V", SIZES)
+def test_backward(dev, dtype, B, L, Hk, Hv, K, V):
+    d = inputs(dev, B, L, Hk, Hv, K, V, dtype, seed=L + K, h0=L % 2 == 1)
+    check_gradients(dev, d, dtype, seed=V, dh=L % 2 == 1)
+
+
+@pytest.mark.parametrize("dtype,B,L,Hk,Hv,K,V,rate", [
+    (BF16, 1, 6000, 1, 2, 64, 64, 0.05), (F32, 1, 3001, 1, 1, 40, 72, 0.05),
+    (F16, 1, 2500, 1, 1, 128, 30, 0.02)])
+def test_backward_segments(dev, dtype, B, L, Hk, Hv, K, V, rate):
+    d = inputs(dev, B, L, Hk, Hv, K, V, dtype, seed=L, h0=True, rate=rate)
+    check_gradients(dev, d, dtype, seed=1)
+
+
+def test_backward_scale_and_strides(dev):
+    B, L, H, K, V = 2, 77, 3, 32, 32
+    d = inputs(dev, B, L, H, H, K, V, BF16, seed=5, h0=True)
+    packed = torch.zeros(B, L, H * (2 * K + V) + 3, device=dev, dtype=BF16)
+    for name, at in (("q", 0), ("k", H * K), ("v", 2 * H * K)):
+        view = packed[..., at + 1:at + 1 + H * K].view(B, L, H, K)
+        view.copy_(d[name])
+        d[name] = view
+    d["g"] = d["g"][:, :1, :1].expand(B, L, H)
+    do, dh, got = check_gradients(dev, d, BF16, seed=3, scale=0.7)
+    one = do[:, :1].expand_as(do)              # a gradient shared by all steps
+    again = gradients(d, one, dh, scale=0.7)
+    assert all(torch.equal(x, y) for x, y in zip(again, gradients(d, one.contiguous(), dh,
+                                                                  scale=0.7)))
+
+
+def test_backward_resets(dev):
+    d = inputs(dev, 2, 150, 2, 2, 64, 64, F32, seed=8, h0=True, rate=0.05)
+    d["g"][:, ::7] = 0.0
+    d["g"][1, 90:100] = -300.0
+    d["beta"][:, 10:20] = 0.0
+    check_gradients(dev, d, F32, seed=2)
+    d["g"][0, 40] = -float("inf")
+    do = torch.ones_like(d["v"])
+    assert all(torch.isfinite(x).all() for x in gradients(d, do))
+
+
+def test_backward_against_differences(dev):
+    """Directional differences of the forward in fp32: the change of
+    sum(o do) + sum(S dh) along a random direction.  Step 1e-2 of O(1) inputs:
+    third-order truncation 1e-4 of the directional derivative's scale, rounding
+    of a sum of 4e3 terms 1e-6 / 1e-2 of it."""
+    r = torch.Generator().manual_seed(4)
+    d = inputs(dev, 1, 70, 1, 2, 32, 32, F32, seed=4, h0=True)
+    do = torch.randn(1, 70, 2, 32, generator=r).to(dev)
+    dh = torch.randn(1, 2, 32, 32, generator=r).to(dev)
+    got = dict(zip(("q", "k", "v", "g", "beta", "h0"), gradients(d, do, dh)))
+    for name in got:
+        way = torch.randn(d[name].shape, generator=r).to(dev)
+        way = way / way.norm()
+        loss = []
+        for e in (1e-2, -1e-2):
+            o, S = run(dict(d, **{name: d[name] + e * way}))
+            loss.append(float((o.double() * do.double()).sum() + (S.double() * dh.double()).sum()))
+        want = (loss[0] - loss[1]) / 2e-2
+        have = float((got[name].double() * way.double()).sum())
+        assert abs(have - want) <= 1e-3 * float(got[name].norm()), (name, have, want)
+
+
+def test_backward_repeat_and_empty(dev):
+    d = inputs(dev, 2, 200, 2, 4, 64, 64, BF16, seed=13, h0=True)
+    do, dh, got = check_gradients(dev, d, BF16, seed=6)
+    assert all(torch.equal(x, y) for x, y in zip(got, gradients(d, do, dh)))
+    none = {n: t[:, :0] if n != "h0" else t for n, t in d.items()}
+    got = gradients(none, do[:, :0], dh)
+    assert torch.equal(got[5], dh) and got[0].shape == (2, 0, 2, 64)
+    assert not gradients(none, do[:, :0])[5].any()
+
+
 # ------------------------------------------------------------------ decode
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("S,Hk,Hv,K,V", [(1, 1, 1, 1, 1), (1, 8, 16, 128, 128), (7, 2, 2, 64, 64),
@@ -289,6 +390,12 @@ def test_refusals(dev):
                        (dict(g=d["g"].long()), "float tensor"), (dict(q=None), "torch.Tensor")]:
         with pytest.raises(TypeError, match=match):
             call(**bad)
+    for do, err in ((d["v"][:1], ValueError), (d["v"].float(), TypeError),
+                    (d["v"].cpu(), ValueError)):
+        with pytest.raises(err, match="do"):
+            gradients(d, do)
+    with pytest.raises(ValueError, match="dh_last must be"):
+        gradients(d, d["v"], d["h0"][..., :4])
     x = {n: d[n][:, 0] for n in ("q", "k", "v", "g", "beta")}
     with pytest.raises(ValueError, match="contiguous"):
         gated_delta_step(**x, state=d["h0"].transpose(2, 3).contiguous().transpose(2, 3))

@@ -54,3 +54,22 @@ def test_group_norm_status():
     assert bwd(ws=None) == -5 and bwd(nbytes=8) == -5 and bwd(G=-1) == -2
     assert L.tssm_group_norm_workspace_bytes(32768, 1, 16, 64) > 0
     assert L.tssm_group_norm_workspace_bytes(1, 1, 0, 64) < 0
+
+
+def test_delta_backward_status():
+    L = _lib.lib()
+
+    def back(dtype=1, q=P, dg=P, B=2, n=40, Hk=2, Hv=4, K=64, V=64, sq=512, sv=256, ws=P,
+             nbytes=1 << 40):
+        s = [0, sq, 64, 0, sq, 64, 0, sv, 64, 0, 4, 1, 0, 4, 1, 0, sv, 64]
+        return L.tssm_gated_delta_backward(dtype, q, P, P, P, P, None, P, None, P, P, P, dg, P,
+                                           None, B, n, Hk, Hv, K, V, *s, 0.125, ws, nbytes, None)
+
+    assert back(dtype=5) == -4 and back(q=None) == -1 and back(dg=None) == -1
+    assert back(Hv=3) == -2 and back(K=129) == -6
+    assert back(sq=8) == -3 and back(sv=0) == -3        # rows that overlap
+    assert back(ws=None) == -5 and back(nbytes=1 << 10) == -5 and back(ws=P + 8) == -5
+    assert back(B=0) == 0 and back(n=0) == 0
+    f = L.tssm_gated_delta_backward_workspace_bytes
+    assert f(2, 40, 2, 4, 64, 64) > L.tssm_gated_delta_workspace_bytes(2, 40, 2, 4, 64, 64)
+    assert f(1, 4, 2, 3, 8, 8) == -2 and f(1, 4, 1, 1, 129, 8) == -6

@@ -31,7 +31,8 @@ int delta_seq_launch(int dtype, const DeltaArgs& a, hipStream_t s);
 struct DeltaPlan {
   void* chunks;
   float *transfer, *entry;     // nseg > 1
-  float *states;               // gradients only
+  float *states, *grads;       // gradients only: of the state before, the gradient after each chunk
+  float *back, *gentry;        // gradients only, nseg > 1: like transfer's N and entry
   int nch, per, nseg;          // chunks, chunks of a segment, segments
   int64_t bytes;
 };
@@ -44,6 +45,18 @@ int delta_transfer_launch(int dtype, const DeltaArgs& a, bool vec, const DeltaPl
                           hipStream_t s);
 int delta_states_launch(int dtype, const DeltaArgs& a, bool vec, const DeltaPlan& p,
                         hipStream_t s);
+// The way back (a.v: dO, a.h0: dh_last, a.h_last: dh0), and its segments' joining.
+int delta_back_launch(int dtype, const DeltaArgs& a, bool vec, const DeltaPlan& p, hipStream_t s);
+int delta_fold_back(const DeltaArgs& a, const DeltaPlan& p, hipStream_t s);
+// Gradients of the inputs; outputs contiguous, dO with strides.
+struct DeltaGrads {
+  const void* dout;
+  int64_t d_b, d_l, d_h;
+  void *dq, *dk, *dv;
+  float *dg, *dbeta;
+};
+int delta_grads_launch(int dtype, const DeltaArgs& a, const DeltaGrads& d, bool vec,
+                       const DeltaPlan& p, hipStream_t s);
 int64_t delta_chunk_ws_bytes();  // of one chunk of one value head
 
 }  // namespace tssm

@@ -35,7 +35,8 @@ int64_t segments(int64_t heads, int64_t nch, int64_t KP, int64_t V) {
 }
 
 // The chunked form's plan over a workspace at base (which may be null: sizes).
-DeltaPlan delta_plan(char* base, int64_t B, int64_t L, int64_t Hv, int64_t K, int64_t V) {
+DeltaPlan delta_plan(char* base, int64_t B, int64_t L, int64_t Hv, int64_t K, int64_t V,
+                     bool gradients) {
   DeltaPlan p = {};
   const int64_t nch = cdiv64(L, 32), heads = B * Hv, KP = K <= 32 ? 32 : (K <= 64 ? 64 : 128);
   const int64_t Vp = cdiv64(V, 16) * 16;
@@ -53,6 +54,14 @@ DeltaPlan delta_plan(char* base, int64_t B, int64_t L, int64_t Hv, int64_t K, in
     p.transfer = reinterpret_cast<float*>(take(heads * p.nseg * (Vp + KP) * KP * 4));
     p.entry = reinterpret_cast<float*>(take(heads * p.nseg * Vp * KP * 4));
   }
+  if (gradients) {
+    if (p.nseg > 1) {
+      p.back = reinterpret_cast<float*>(take(heads * p.nseg * Vp * KP * 4));
+      p.gentry = reinterpret_cast<float*>(take(heads * p.nseg * Vp * KP * 4));
+    }
+    p.states = reinterpret_cast<float*>(take(heads * nch * Vp * KP * 4));
+    p.grads = reinterpret_cast<float*>(take(heads * nch * Vp * KP * 4));
+  }
   p.bytes = at;
   return p;
 }
@@ -65,12 +74,16 @@ bool vec_rows(int dtype, const DeltaArgs& a) {
          (a.q_b | a.q_l | a.q_h | a.k_b | a.k_l | a.k_h | a.v_b | a.v_l | a.v_h) * E % 16 == 0;
 }
 
+bool fits(int dtype, int64_t stride, int64_t cols) {
+  const int64_t most = (INT64_C(1) << 31) / (33 * (dtype == TSSM_F32 ? 4 : 2));
+  return stride >= cols && stride < most;
+}
+
 // What the chunked kernels' buffer accesses ask for: the rows of q, k, v and o
 // do not overlap, and a chunk's lie within 31 bits of its first.
 bool chunk_rows(int dtype, const DeltaArgs& a) {
-  const int64_t most = (INT64_C(1) << 31) / (33 * (dtype == TSSM_F32 ? 4 : 2));
-  const auto fit = [&](int64_t stride, int64_t cols) { return stride >= cols && stride < most; };
-  return fit(a.q_l, a.K) && fit(a.k_l, a.K) && fit(a.v_l, a.V) && fit(a.o_l, a.V);
+  return fits(dtype, a.q_l, a.K) && fits(dtype, a.k_l, a.K) && fits(dtype, a.v_l, a.V) &&
+         fits(dtype, a.o_l, a.V);
 }
 
 }  // namespace
@@ -95,7 +108,7 @@ extern "C" int tssm_gated_delta_forward(
                        sg_b, sg_l, sg_h, sbe_b, sbe_l, sbe_h, so_b, so_l, so_h, scale};
   if (L <= kSeqMost || !chunk_rows(dtype, a)) return delta_seq_launch(dtype, a, as_stream(stream));
   TSSM_CHECK(nbatch * Hv <= 0x7fffffff / cdiv64(L, 32), TSSM_ERR_UNSUPPORTED);
-  const DeltaPlan p = delta_plan(reinterpret_cast<char*>(workspace), nbatch, L, Hv, K, V);
+  const DeltaPlan p = delta_plan(reinterpret_cast<char*>(workspace), nbatch, L, Hv, K, V, false);
   TSSM_CHECK(workspace && workspace_bytes >= p.bytes && aligned(workspace, 256),
              TSSM_ERR_WORKSPACE);
   const bool vec = vec_rows(dtype, a);
@@ -128,5 +141,51 @@ extern "C" int64_t tssm_gated_delta_workspace_bytes(int64_t nbatch, int64_t L, i
   if (!sizes_ok(nbatch, L, Hk, Hv, K, V)) return TSSM_ERR_SHAPE;
   if (K > 128) return TSSM_ERR_UNSUPPORTED;
   if (L <= kSeqMost || nbatch == 0) return 256;
-  return delta_plan(nullptr, nbatch, L, Hv, K, V).bytes;
+  return delta_plan(nullptr, nbatch, L, Hv, K, V, false).bytes;
+}
+
+extern "C" int64_t tssm_gated_delta_backward_workspace_bytes(int64_t nbatch, int64_t L, int64_t Hk,
+                                                             int64_t Hv, int64_t K, int64_t V) {
+  if (!sizes_ok(nbatch, L, Hk, Hv, K, V)) return TSSM_ERR_SHAPE;
+  if (K > 128) return TSSM_ERR_UNSUPPORTED;
+  if (L == 0 || nbatch == 0) return 256;
+  return delta_plan(nullptr, nbatch, L, Hv, K, V, true).bytes;
+}
+
+extern "C" int tssm_gated_delta_backward(
+    int dtype, const void* q, const void* k, const void* v, const float* g, const float* beta,
+    const float* h0, const void* dout, const float* dh_last, void* dq, void* dk, void* dv,
+    float* dg, float* dbeta, float* dh0, int64_t nbatch, int64_t L, int64_t Hk, int64_t Hv,
+    int64_t K, int64_t V, int64_t sq_b, int64_t sq_l, int64_t sq_h, int64_t sk_b, int64_t sk_l,
+    int64_t sk_h, int64_t sv_b, int64_t sv_l, int64_t sv_h, int64_t sg_b, int64_t sg_l,
+    int64_t sg_h, int64_t sbe_b, int64_t sbe_l, int64_t sbe_h, int64_t sd_b, int64_t sd_l,
+    int64_t sd_h, float scale, void* workspace, int64_t workspace_bytes, void* stream) {
+  TSSM_CHECK(dtype >= TSSM_F32 && dtype <= TSSM_F16, TSSM_ERR_DTYPE);
+  TSSM_CHECK(sizes_ok(nbatch, L, Hk, Hv, K, V), TSSM_ERR_SHAPE);
+  TSSM_CHECK(K <= 128, TSSM_ERR_UNSUPPORTED);
+  if (nbatch == 0 || L == 0) return TSSM_OK;
+  TSSM_CHECK(q && k && v && g && beta && dout && dq && dk && dv && dg && dbeta, TSSM_ERR_NULL);
+  TSSM_CHECK(nbatch * Hv <= 0x7fffffff / cdiv64(L, 32), TSSM_ERR_UNSUPPORTED);
+  DeltaArgs a = {q, k, v, g, beta, h0, nullptr, nullptr, nbatch, L, Hk, Hv, K, V,
+                 sq_b, sq_l, sq_h, sk_b, sk_l, sk_h, sv_b, sv_l, sv_h,
+                 sg_b, sg_l, sg_h, sbe_b, sbe_l, sbe_h, V, V, V, scale};
+  TSSM_CHECK((chunk_rows(dtype, a) && fits(dtype, sd_l, V)) || L == 1, TSSM_ERR_STRIDE);
+  const DeltaPlan p = delta_plan(reinterpret_cast<char*>(workspace), nbatch, L, Hv, K, V, true);
+  TSSM_CHECK(workspace && workspace_bytes >= p.bytes && aligned(workspace, 256),
+             TSSM_ERR_WORKSPACE);
+  DeltaArgs way = a;  // the way back reads dO where the walk reads v
+  way.v = dout;
+  way.v_b = sd_b;
+  way.v_l = sd_l;
+  way.v_h = sd_h;
+  way.h0 = dh_last;
+  way.h_last = dh0;
+  const DeltaGrads d = {dout, sd_b, sd_l, sd_h, dq, dk, dv, dg, dbeta};
+  const bool vec = vec_rows(dtype, a) && vec_rows(dtype, way);
+  hipStream_t st = as_stream(stream);
+  int rc = delta_prep_launch(dtype, a, vec, p.chunks, st);
+  if (!rc && p.nseg > 1) rc = delta_transfer_launch(dtype, a, vec, p, st);
+  if (!rc) rc = delta_states_launch(dtype, a, vec, p, st);
+  if (!rc) rc = delta_back_launch(dtype, way, vec, p, st);
+  return rc ? rc : delta_grads_launch(dtype, a, d, vec, p, st);
 }

@@ -97,12 +97,20 @@ int delta_transfer_launch(int dtype, const DeltaArgs& a, bool vec, const DeltaPl
   g.nch = p.nch;
   g.per = p.per;
   g.nseg = p.nseg;
+  // the last one's is for the way back
+  g.walked = p.back ? p.nseg : p.nseg - 1;
   g.states = p.transfer;
   const int rc = walk_mode<kTransfer>(dtype, g, vec, s);
   if (rc) return rc;
   const FoldArgs f = {a.h0, p.transfer, nullptr, p.entry, a.B * a.Hv, a.V, (int)a.K, p.nseg,
                       (int)cdiv64(a.V, 16)};
   return fold<false>(f, s);
+}
+
+int delta_fold_back(const DeltaArgs& a, const DeltaPlan& p, hipStream_t s) {
+  const FoldArgs f = {a.h0, p.transfer, p.back, p.gentry, a.B * a.Hv, a.V, (int)a.K, p.nseg,
+                      (int)cdiv64(a.V, 16)};
+  return fold<true>(f, s);
 }
 
 int delta_states_launch(int dtype, const DeltaArgs& a, bool vec, const DeltaPlan& p,
@@ -112,7 +120,7 @@ int delta_states_launch(int dtype, const DeltaArgs& a, bool vec, const DeltaPlan
   g.ws = reinterpret_cast<const ChunkWs*>(p.chunks);
   g.nch = p.nch;
   g.per = p.per;
-  g.nseg = p.nseg;
+  g.nseg = g.walked = p.nseg;
   g.entry = p.entry;
   g.states = p.states;
   return walk_mode<kStates>(dtype, g, vec, s);

@@ -38,6 +38,7 @@ struct WalkArgs {
   DeltaArgs a;
   const ChunkWs* ws;
   int nch, per, nseg;
+  int walked;          // the first segments that are walked
   uint32_t nvb;        // workgroups of a head and segment
   const float* entry;  // [bh][nseg][Vp][KP]
   float* states;       // kStates: [bh][nch][Vp][KP]; kTransfer: [bh][nseg][Vp + KP][KP]
@@ -485,7 +486,7 @@ __global__ __launch_bounds__((Walk<T, KP, VEC, NCW, MODE>::kThreads),
   typename W::Lds& lds = *reinterpret_cast<typename W::Lds*>(raw);
   const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   // workgroups of one head and segment on one XCD: they share its keys and queries
-  const int64_t runs = g.a.B * g.a.Hv * (MODE == kTransfer ? g.nseg - 1 : g.nseg);
+  const int64_t runs = g.a.B * g.a.Hv * g.walked;
   const int64_t run = (int64_t)(blockIdx.x / (8 * g.nvb)) * 8 + (blockIdx.x & 7);
   if (run >= runs) return;
   const int64_t bh = run % (g.a.B * g.a.Hv);
@@ -505,7 +506,7 @@ int walk_launch(WalkArgs& g, hipStream_t s) {
   typedef Walk<T, KP, VEC, NCW, MODE> W;
   const int64_t cols = MODE == kTransfer ? (g.a.V + 15) / 16 * 16 + KP : g.a.V;
   g.nvb = (uint32_t)cdiv64(cols, 16 * NCW);
-  const int64_t runs = g.a.B * g.a.Hv * (MODE == kTransfer ? g.nseg - 1 : g.nseg);
+  const int64_t runs = g.a.B * g.a.Hv * g.walked;
   const int64_t wgs = cdiv64(runs, 8) * 8 * g.nvb;
   if (wgs > 0x7fffffff) return TSSM_ERR_UNSUPPORTED;
   constexpr int bytes = (int)sizeof(typename W::Lds);

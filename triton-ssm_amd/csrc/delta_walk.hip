@@ -9,7 +9,7 @@ int delta_walk_launch(int dtype, const DeltaArgs& a, bool vec, const DeltaPlan& 
   g.ws = reinterpret_cast<const ChunkWs*>(p.chunks);
   g.nch = p.nch;
   g.per = p.per;
-  g.nseg = p.nseg;
+  g.nseg = g.walked = p.nseg;
   g.entry = p.entry;
   return walk_mode<kOutputs>(dtype, g, vec, s);
 }

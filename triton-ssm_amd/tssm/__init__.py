@@ -13,7 +13,7 @@ with an activation (``groupnorm``) and the seeded synthetic workloads
 from . import _lib, launch, workspace  # noqa: F401
 from ._lib import TssmError  # noqa: F401
 from .corrected import streaming_interp_step_corrected, time_aware_interp_corrected  # noqa: F401
-from .delta import gated_delta_forward, gated_delta_step  # noqa: F401
+from .delta import gated_delta_backward, gated_delta_forward, gated_delta_step  # noqa: F401
 from .fused import (fused_interp_ssm_forward, multihead_ssm_forward,  # noqa: F401
                     selective_scan_forward, ssd_scan_forward, ssd_stream_step)
 from .groupnorm import group_norm_act_backward, group_norm_act_forward  # noqa: F401
@@ -21,5 +21,6 @@ from .workspace import check  # noqa: F401
 
 __all__ = ["multihead_ssm_forward", "selective_scan_forward", "ssd_scan_forward",
            "ssd_stream_step", "fused_interp_ssm_forward", "time_aware_interp_corrected",
-           "streaming_interp_step_corrected", "gated_delta_forward", "gated_delta_step",
-           "group_norm_act_forward", "group_norm_act_backward", "check", "TssmError"]
+           "streaming_interp_step_corrected", "gated_delta_forward", "gated_delta_backward",
+           "gated_delta_step", "group_norm_act_forward", "group_norm_act_backward", "check",
+           "TssmError"]

@@ -114,6 +114,43 @@ def gated_delta_forward(q, k, v, g, beta, *, scale=None, h0=None, return_state=F
     return (o, h_last) if return_state else o
 
 
+def gated_delta_backward(q, k, v, g, beta, do, *, scale=None, h0=None, dh_last=None):
+    """Gradients of ``gated_delta_forward`` for its inputs and do [B, L, Hv, V]
+    (dtype of v), the gradient of o, and dh_last [B, Hv, K, V] float32 or None,
+    that of the final state.
+
+    Returns (dq, dk, dv, dg, dbeta, dh0): dq, dk and dv of q's dtype, dg, dbeta
+    and dh0 float32 (dh0 is None without h0).  dq and dk are summed over the
+    value heads that share a key head; repeated calls give identical bits.  The
+    states are formed again from the inputs: nothing but the inputs needs to be
+    kept between the passes.  An input or gradient that is not finite makes its
+    chunk of 32 steps, and what depends on it, not finite.
+    """
+    (B, L, Hk, Hv, K, V), code, g, beta = _operands(q, k, v, g, beta, 2)
+    dev = q.get_device()
+    _check(do, "do", v.shape, v.dtype, dev)
+    q, k, v, do = _steps(q), _steps(k), _steps(v), _steps(do)
+    h0, dh_last = _state(h0, "h0", (B, Hv, K, V), dev), \
+        _state(dh_last, "dh_last", (B, Hv, K, V), dev)
+    dq = torch.empty(B, L, Hk, K, device=q.device, dtype=q.dtype)
+    dk, dv = torch.empty_like(dq), torch.empty(B, L, Hv, V, device=q.device, dtype=q.dtype)
+    dg, dbeta = torch.empty(2, B, L, Hv, device=q.device, dtype=torch.float32)
+    dh0 = None if h0 is None else torch.empty(B, Hv, K, V, device=q.device, dtype=torch.float32)
+    if B and L:
+        stream = stream_handle(q)
+        ws = workspace.get(q.device, stream, _lib.lib().tssm_gated_delta_backward_workspace_bytes(
+            B, L, Hk, Hv, K, V), workspace.SSD)
+        _lib.call("tssm_gated_delta_backward", code, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                  g.data_ptr(), beta.data_ptr(), ptr(h0), do.data_ptr(), ptr(dh_last),
+                  dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dg.data_ptr(), dbeta.data_ptr(),
+                  ptr(dh0), B, L, Hk, Hv, K, V, *_rows(q, "q"), *_rows(k, "k"), *_rows(v, "v"),
+                  *g.stride(), *beta.stride(), *_rows(do, "do"),
+                  K ** -0.5 if scale is None else float(scale), ws.data_ptr(), ws.numel(), stream)
+    elif dh0 is not None:
+        dh0.zero_() if dh_last is None else dh0.copy_(dh_last)
+    return dq, dk, dv, dg, dbeta, dh0
+
+
 def gated_delta_step(q, k, v, g, beta, state, *, scale=None, out=None):
     """One step of S streams, the state updated in place.
 
