@@ -628,18 +628,19 @@ int tssm_gated_delta_step(int dtype, const void* q, const void* k, const void* v
  * x [N,S,C], C = G Cg, unit channel stride, strides (n, s); mean and variance
  * over each group's S x Cg elements (S = 1: per row).  xhat = (x - mean) rstd,
  * z = xhat w + b (w, b f32 [C] or NULL), y = act(z), or z act(gate) where gate
- * [N,S,C] is given.  mean, rstd f32 [N,G] are written where not NULL (both or
- * neither) and read by the backward, which writes dx, dgate (NULL without a
+ * [N,S,C] is given.  mean (64 bits: groups whose values almost agree need it)
+ * and rstd f32 [N,G] are written where not NULL (both or neither) and read by
+ * the backward, which writes dx, dgate (NULL without a
  * gate) of `dtype` and dw, db f32 [C], summed in a fixed order.  No reference
  * counterpart.  Workspace: tssm_group_norm_workspace_bytes() bytes, 256-byte
  * aligned, no clearing. */
 int64_t tssm_group_norm_workspace_bytes(int64_t N, int64_t S, int64_t G, int64_t Cg);
 int tssm_group_norm_act_fwd(int dtype, int act, const void* x, const float* w, const float* b,
-                            const void* gate, void* y, float* mean, float* rstd, int64_t N,
+                            const void* gate, void* y, double* mean, float* rstd, int64_t N,
                             int64_t S, int64_t G, int64_t Cg, int64_t sx_n, int64_t sx_s,
                             int64_t sgt_n, int64_t sgt_s, int64_t sy_n, int64_t sy_s, float eps,
                             void* workspace, int64_t workspace_bytes, void* stream);
-int tssm_group_norm_act_bwd(int dtype, int act, const void* dy, const void* x, const float* mean,
+int tssm_group_norm_act_bwd(int dtype, int act, const void* dy, const void* x, const double* mean,
                             const float* rstd, const float* w, const float* b, const void* gate,
                             void* dx, float* dw, float* db, void* dgate, int64_t N, int64_t S,
                             int64_t G, int64_t Cg, int64_t sdy_n, int64_t sdy_s, int64_t sx_n,

@@ -187,3 +187,13 @@ def test_refusals(dev):
         group_norm_act_backward(dy, x, mean[:2], rstd, 4, w, b, gate)
     with pytest.raises(ValueError, match="dy"):
         group_norm_act_backward(dy[:1], x, mean, rstd, 4, w, b, gate)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("N,S,G,C", [
+    (3, 1, 1, 4099),      # rows past a wave's registers
+    (2, 3, 3, 12297),     # series past a workgroup's row
+    (2, 40, 1, 8192), (1, 70, 2, 2050), (2, 9, 513, 1026),
+])
+def test_wide(dev, dtype, N, S, G, C):
+    check(inputs(dev, N, S, C, dtype, True, seed=C), G, "silu", dtype)

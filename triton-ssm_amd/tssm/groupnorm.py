@@ -7,7 +7,7 @@ reference counterpart; the reference's own norm is ``layernorm_kernel``).
 
 x is [N, C] (statistics per row, as after a multi-head mixer) or [N, ..., C],
 where the middle dimensions are positions that share their statistics.  Sums
-and statistics are fp32 (fixed order: repeated runs give identical bits);
+and statistics are fp32, the mean 64 bits (fixed order: repeated runs give identical bits);
 ``weight`` and ``bias`` are read as float32 and their gradients are float32.
 """
 from __future__ import annotations
@@ -89,14 +89,16 @@ def group_norm_act_forward(x, groups, weight=None, bias=None, gate=None, *, act=
     to the gate that multiplies it.  weight, bias [C] or None.
 
     Returns y (dtype of x; ``out`` if given) and, with ``return_stats``, mean
-    and rstd [N, groups] float32, which the backward needs.
+    (float64: groups whose values almost agree need it) and rstd (float32)
+    [N, groups], which the backward needs.
     """
     code, act_, N, S, G, Cg, sx, sg, w, b = _operands(x, groups, weight, bias, gate, act)
     y = torch.empty(x.shape, device=x.device, dtype=x.dtype) if out is None else out
     sy = _same(y, "out", x)
     mean = rstd = None
     if return_stats:
-        mean, rstd = torch.empty(2, N, G, device=x.device, dtype=torch.float32)
+        mean = torch.empty(N, G, device=x.device, dtype=torch.float64)
+        rstd = torch.empty(N, G, device=x.device, dtype=torch.float32)
     if N * S:
         ws, stream = _ws(x, N, S, G, Cg)
         _lib.call("tssm_group_norm_act_fwd", code, act_, x.data_ptr(), ptr(w), ptr(b), ptr(gate),
@@ -114,10 +116,10 @@ def group_norm_act_backward(dy, x, mean, rstd, groups, weight=None, bias=None, g
     """
     code, act_, N, S, G, Cg, sx, sg, w, b = _operands(x, groups, weight, bias, gate, act)
     sdy = _same(dy, "dy", x)
-    for t, what in ((mean, "mean"), (rstd, "rstd")):
+    for t, what, dtype in ((mean, "mean", torch.float64), (rstd, "rstd", torch.float32)):
         need_gpu(t, what)
-        if t.shape != (N, G) or t.dtype != torch.float32 or not t.is_contiguous():
-            raise ValueError(f"{what} must be contiguous float32 [{N}, {G}]")
+        if t.shape != (N, G) or t.dtype != dtype or not t.is_contiguous():
+            raise ValueError(f"{what} must be contiguous {dtype} [{N}, {G}]")
     dx = torch.empty(x.shape, device=x.device, dtype=x.dtype)
     dgate = torch.empty(x.shape, device=x.device, dtype=x.dtype) if gate is not None else None
     dw, db = torch.empty(2, G * Cg, device=x.device, dtype=torch.float32)
