@@ -191,6 +191,14 @@ __device__ inline u32x4 lds_col(const uint16_t* m, int ld, int col, int lane) {
   return u32x4{a[0], a[1], b[0], b[1]};
 }
 
+// The same for the 16 columns from col on.
+__device__ inline u32x4 lds_col16(const uint16_t* m, int ld, int col, int lane) {
+  const int j = lane >> 4, i = lane & 15;
+  const uint16_t* p = m + (8 * j + (i >> 2)) * ld + col + 4 * (i & 3);
+  const u32x2v a = lds_tr(p), b = lds_tr(p + 4 * ld);
+  return u32x4{a[0], a[1], b[0], b[1]};
+}
+
 // What the preparing pass leaves for each chunk and value head, in the
 // workspace.  Steps past the sequence's end count as k = q = 0, g = beta = 0.
 // With G the sums of g within the chunk:

@@ -10,15 +10,16 @@
 //   dQ = e^G X1 + M K,
 //   dK = M^T Q + (E + E^T) K + e^(G_last - G) X2 - beta e^G X3,
 //   dbeta = sum_v dR Y + sum_i dA D kk,
-//   dG_t = e^G q.X1 - beta e^G k.X3 - b_t + sum_i F[t][i] - sum_i F[i][t],
-//     F = dP P + dA A,  b_t = e^(G_last - G_t) k.X2,
+//   dG_t = e^G sum_v (scale dO (Q S) - beta dR (K S)) - b_t
+//          + sum_i F[t][i] - sum_i F[i][t],
+//     F = dP P + dA A,  b_t = e^(G_last - G_t) sum_v U (K G'),
 //   dG_last += sum_t b_t + e^(G_last) <S, G'>,   dg_t = sum of dG from t on.
 // A workgroup of four waves takes one chunk of one key head and goes through
 // its value heads (whose gradients of q and k add up in registers, in order),
 // and through V in slices of 64 columns: first column by column as the walks
 // do (U, dR), then the sums over v, whose results are the tiles of 32 x K and
-// 32 x 32 a wave keeps.  All products that reach dg and dbeta take three
-// planes.
+// 32 x 32 a wave keeps.  Products that reach dg and dbeta take three planes, X1
+// to X3, M and E as many as dq and dk need (two for bf16).
 #include "delta_dev.h"
 
 namespace tssm {
@@ -38,9 +39,10 @@ struct GradArgs {
 template <typename T, int KP, bool VEC>
 struct Grad {
   static constexpr int NP = Piece<T, VEC>::NP;
-  static constexpr int NO = NP == 1 ? 2 : 3;  // planes of M and E: they reach dq and dk only
+  static constexpr int NO = NP == 1 ? 2 : 3;  // planes where dq and dk alone are reached
   static constexpr int NS = KP / 32, NK = NS < 2 ? 1 : NS / 2;  // tiles of 16 keys a wave keeps
   static constexpr int kLd = KP + 8, kVld = 64 + 8;
+  // two workgroups a CU where LDS holds both
   static constexpr int kWaves = NP * KP <= 64 ? 2 : 1;
   struct Lds {
     uint16_t K[NP][kC * kLd], Q[NP][kC * kLd];
@@ -55,7 +57,9 @@ struct Grad {
       } m;
     };
     float fac[kFac][kC];
-    float row[4][5][kC];  // a wave's sums for each step: F, dA D kk, dR Y, q.X1 and k.X3, k.X2
+    // a wave's sums for each step: F, dA D kk, dR Y, e^G (scale dO (Q S) - beta dR (K S)),
+    // e^(G_last - G) U (K G')
+    float row[4][5][kC];
     float col[4][kC];     // and of F over t
     float dot[4];
   };
@@ -76,44 +80,38 @@ __device__ inline void put4(uint16_t (*m)[kC * kTld], int at, const f32x4& x) {
   }
 }
 
-template <typename T, int KP, bool VEC>
+// ONE: one value head to a key head, and V in one slice.
+template <typename T, int KP, bool VEC, bool ONE>
 __global__ __launch_bounds__(256, (Grad<T, KP, VEC>::kWaves)) void delta_grads_kernel(GradArgs g) {
   typedef Grad<T, KP, VEC> W;
   constexpr int NP = W::NP, NO = W::NO, NS = W::NS, NK = W::NK;
+  constexpr int kNk = (kC * KP / 8 + 255) / 256;  // pieces of K a thread brings
   extern __shared__ __attribute__((aligned(16))) char raw[];
   typename W::Lds& lds = *reinterpret_cast<typename W::Lds*>(raw);
   const DeltaArgs& a = g.a;
   const int tid = threadIdx.x, lane = tid & 63, j = lane >> 4, c = lane & 15;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6), tx = w >> 1, ty = w & 1;
-  const int ar = 8 * (c >> 2) + (c & 3);
-  const int K = (int)a.K, per = (int)(a.Hv / a.Hk);
+  const int K = (int)a.K, per = ONE ? 1 : (int)(a.Hv / a.Hk);
   const int64_t Vp = (a.V + 15) / 16 * 16;
-  // the chunks of one head follow each other; heads go round the XCDs
+  // the chunks of one head follow each other
   const int64_t n = blockIdx.x % g.nch, bk = blockIdx.x / g.nch, b = bk / a.Hk, hk = bk - b * a.Hk;
   const int64_t t0 = n * kC;
   const int rows = a.L - t0 < kC ? (int)(a.L - t0) : kC;
 
-  {  // K and Q
+  // K and Q on their way; they go to LDS with the first head's operands
+  Piece<T, VEC> pk[kNk], pq[kNk];
+  {
     const T* kp = reinterpret_cast<const T*>(a.k) + b * a.k_b + hk * a.k_h + t0 * a.k_l;
     const T* qp = reinterpret_cast<const T*>(a.q) + b * a.q_b + hk * a.q_h + t0 * a.q_l;
 #pragma unroll
-    for (int i = 0; i < (kC * KP / 8 + 255) / 256; ++i) {
+    for (int i = 0; i < kNk; ++i) {
       const int id = tid + 256 * i, r = id / (KP / 8), col = id % (KP / 8) * 8;
-      if (kC * KP / 8 % 256 && r >= kC) continue;
       const int lim = r < rows ? K - col : 0;
-      Piece<T, VEC> x, y;
-      x.load(kp + (r < rows ? r : 0) * a.k_l + (col < K ? col : 0), lim);
-      y.load(qp + (r < rows ? r : 0) * a.q_l + (col < K ? col : 0), lim);
-      u32x4 p[NP];
-      x.planes(lim, p);
-#pragma unroll
-      for (int m = 0; m < NP; ++m) *reinterpret_cast<u32x4*>(&lds.K[m][r * W::kLd + col]) = p[m];
-      y.planes(lim, p);
-#pragma unroll
-      for (int m = 0; m < NP; ++m) *reinterpret_cast<u32x4*>(&lds.Q[m][r * W::kLd + col]) = p[m];
+      pk[i].load(kp + (r < rows ? r : 0) * a.k_l + (col < K ? col : 0), lim);
+      pq[i].load(qp + (r < rows ? r : 0) * a.q_l + (col < K ? col : 0), lim);
     }
   }
-  f32x4 aq[NK][2], ak[NK][2];  // dQ and dK, rows 8 j + 4 x + r, keys 32 s + 4 h + ar of tile (s, h)
+  f32x4 aq[NK][2], ak[NK][2];  // dQ and dK, rows 8 j + 4 x + r, keys 16 (w + 4 m) + c
 #pragma unroll
   for (int m = 0; m < NK; ++m)
 #pragma unroll
@@ -121,23 +119,90 @@ __global__ __launch_bounds__(256, (Grad<T, KP, VEC>::kWaves)) void delta_grads_k
 
   for (int hh = 0; hh < per; ++hh) {
     const int64_t h = hk * per + hh, bh = b * a.Hv + h, unit = bh * g.nch + n;
-    const ChunkWs& cw = g.ws[unit];
-    __syncthreads();
-    for (int i = tid; i < 3 * kC * 4; i += 256)
-      *reinterpret_cast<u32x4*>(&lds.Tm[i / 128][i % 128 / 4 * kTld + i % 4 * 8]) =
-          *reinterpret_cast<const u32x4*>(&cw.T[i / 128][i % 128 / 4][i % 4 * 8]);
-    (&lds.fac[0][0])[tid] = (&cw.fac[0][0])[tid];
-    __syncthreads();
-    float eg[8], be[8], en[8];
+    // the thread's place anew for each head: addresses that follow from it
+    // would otherwise be kept in registers across the loop, more than there are
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    const int lane = tid & 63, j = lane >> 4, c = lane & 15, ar = 8 * (c >> 2) + (c & 3);
+    const int ti = ar + 4 * ty;  // the column i of this wave's 32 x 32 tile
+    const T* vp = reinterpret_cast<const T*>(a.v) + b * a.v_b + h * a.v_h + t0 * a.v_l;
+    const T* dp = reinterpret_cast<const T*>(g.dout) + b * g.d_b + h * g.d_h + t0 * g.d_l;
+    T* dvp = reinterpret_cast<T*>(g.dv) + ((b * a.L + t0) * a.Hv + h) * a.V;
+    // S and G' through descriptors that end with them: columns past Vp read zero
+    const auto Sp = rsrc_of(g.states + unit * Vp * KP, (int)(Vp * KP * 4));
+    const auto Gp = rsrc_of(g.grads + unit * Vp * KP, (int)(Vp * KP * 4));
+    // a slice of V and dO, and this wave's columns of S and G', on their way
+    Piece<T, VEC> pv, pd;
+    f32x4 S[2 * NS], G[2 * NS];
+    const int sr = tid / 8, scol = tid % 8 * 8;  // this thread's piece of a slice
+    auto slice = [&](int64_t v0) {
+      const int64_t left = a.V - v0 - scol;
+      const int lim = sr < rows ? (left < 0 ? 0 : (left < 8 ? (int)left : 8)) : 0;
+      pv.load(vp + (sr < rows ? sr : 0) * a.v_l + (left > 0 ? v0 + scol : 0), lim);
+      pd.load(dp + (sr < rows ? sr : 0) * g.d_l + (left > 0 ? v0 + scol : 0), lim);
+      const uint32_t at = ((uint32_t)(v0 + 16 * w + c) * KP + 8 * j) * 4;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      eg[e] = lds.fac[kEg][8 * j + e];
-      be[e] = lds.fac[kBeta][8 * j + e];
-      en[e] = lds.fac[kEnd][8 * j + e];
+      for (int i = 0; i < 2 * NS; ++i) {
+        const int k = (32 * (i >> 1) + 4 * (i & 1)) * 4;
+        S[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(Sp, at + k, 0, 0));
+        G[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(Gp, at + k, 0, 0));
+      }
+    };
+    auto put_slice = [&](int64_t v0) {
+      const int64_t left = a.V - v0 - scol;
+      const int lim = sr < rows ? (left < 0 ? 0 : (left < 8 ? (int)left : 8)) : 0;
+      u32x4 p[NP];
+      pv.planes(lim, p);
+#pragma unroll
+      for (int m = 0; m < NP; ++m)
+        *reinterpret_cast<u32x4*>(&lds.V[m][sr * W::kVld + scol]) = p[m];
+      pd.planes(lim, p);
+#pragma unroll
+      for (int m = 0; m < NP; ++m)
+        *reinterpret_cast<u32x4*>(&lds.D[m][sr * W::kVld + scol]) = p[m];
+    };
+    {
+      const u32x4* tp = reinterpret_cast<const u32x4*>(g.ws + unit);
+      u32x4 t[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) t[i] = tp[tid + 256 * i < 384 ? tid + 256 * i : 0];
+      const float f = (&g.ws[unit].fac[0][0])[tid];
+      slice(0);
+      __syncthreads();
+      if (hh == 0) {
+#pragma unroll
+        for (int i = 0; i < kNk; ++i) {
+          const int id = tid + 256 * i, r = id / (KP / 8), col = id % (KP / 8) * 8;
+          if (kC * KP / 8 % 256 && r >= kC) continue;
+          const int lim = r < rows ? K - col : 0;
+          u32x4 p[NP];
+          pk[i].planes(lim, p);
+#pragma unroll
+          for (int m = 0; m < NP; ++m)
+            *reinterpret_cast<u32x4*>(&lds.K[m][r * W::kLd + col]) = p[m];
+          pq[i].planes(lim, p);
+#pragma unroll
+          for (int m = 0; m < NP; ++m)
+            *reinterpret_cast<u32x4*>(&lds.Q[m][r * W::kLd + col]) = p[m];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int id = tid + 256 * i;
+        if (id < 384)
+          *reinterpret_cast<u32x4*>(&lds.Tm[id / 128][id % 128 / 4 * kTld + id % 4 * 8]) = t[i];
+      }
+      (&lds.fac[0][0])[tid] = f;
+      put_slice(0);
+      __syncthreads();
     }
-    // this wave's tile of D, P and D kk: rows t = 8 j + 4 tx + r, column i = ar + 4 ty
+    auto fac8 = [&](int which, float* x) {  // of rows 8 j + e
+      *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(&lds.fac[which][8 * j]);
+      *reinterpret_cast<float4*>(x + 4) =
+          *reinterpret_cast<const float4*>(&lds.fac[which][8 * j + 4]);
+    };
+    // this wave's tile of D, P and D kk: rows t = 8 j + 4 tx + r, column ti
     f32x4 dd, pp = zero4(), dkk = zero4();
-    const int ti = ar + 4 * ty;
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
       u32x4 fk[NP], fa[NP];
@@ -155,74 +220,78 @@ __global__ __launch_bounds__(256, (Grad<T, KP, VEC>::kWaves)) void delta_grads_k
     }
     {
       const float hi = lds.fac[kGhi][ti], lo = lds.fac[kGlo][ti];
+      const float4 h4 = *reinterpret_cast<const float4*>(&lds.fac[kGhi][8 * j + 4 * tx]);
+      const float4 l4 = *reinterpret_cast<const float4*>(&lds.fac[kGlo][8 * j + 4 * tx]);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int t = 8 * j + 4 * tx + r;
-        const float d = exp2_fast((lds.fac[kGhi][t] - hi) + (lds.fac[kGlo][t] - lo));
+        const float d = exp2_fast(((&h4.x)[r] - hi) + ((&l4.x)[r] - lo));
         dd[r] = ti <= t ? d : 0.0f;
         pp[r] = ti <= t ? d * pp[r] : 0.0f;
         dkk[r] = ti < t ? d * dkk[r] : 0.0f;
       }
       put4<3>(lds.PT, ti * kTld + 8 * j + 4 * tx, pp);
     }
+    __syncthreads();
     f32x4 X1[NK][2], X2[NK][2], X3[NK][2], dP = zero4(), dA = zero4();
-    float db[8], ss = 0.0f;
+    float ss = 0.0f;
 #pragma unroll
     for (int m = 0; m < NK; ++m)
 #pragma unroll
       for (int x = 0; x < 2; ++x) X1[m][x] = X2[m][x] = X3[m][x] = zero4();
-#pragma unroll
-    for (int e = 0; e < 8; ++e) db[e] = 0.0f;
-
-    const T* vp = reinterpret_cast<const T*>(a.v) + b * a.v_b + h * a.v_h + t0 * a.v_l;
-    const T* dp = reinterpret_cast<const T*>(g.dout) + b * g.d_b + h * g.d_h + t0 * g.d_l;
-    T* dvp = reinterpret_cast<T*>(g.dv) + ((b * a.L + t0) * a.Hv + h) * a.V;
-    const float* Sp = g.states + unit * Vp * KP;
-    const float* Gp = g.grads + unit * Vp * KP;
-    for (int64_t v0 = 0; v0 < a.V; v0 += 64) {
-      {
-        const int r = tid / 8, col = tid % 8 * 8;
-        const int64_t left = a.V - v0 - col;
-        const int lim = r < rows ? (left < 0 ? 0 : (left < 8 ? (int)left : 8)) : 0;
-        Piece<T, VEC> x, y;
-        x.load(vp + (r < rows ? r : 0) * a.v_l + (left > 0 ? v0 + col : 0), lim);
-        y.load(dp + (r < rows ? r : 0) * g.d_l + (left > 0 ? v0 + col : 0), lim);
-        u32x4 p[NP];
-        x.planes(lim, p);
-#pragma unroll
-        for (int m = 0; m < NP; ++m) *reinterpret_cast<u32x4*>(&lds.V[m][r * W::kVld + col]) = p[m];
-        y.planes(lim, p);
-#pragma unroll
-        for (int m = 0; m < NP; ++m) *reinterpret_cast<u32x4*>(&lds.D[m][r * W::kVld + col]) = p[m];
+    for (int64_t v0 = 0; v0 < (ONE ? 1 : a.V); v0 += 64) {
+      if (v0) {
+        put_slice(v0);
+        __syncthreads();
       }
-      __syncthreads();
       const int64_t vc = v0 + 16 * w + c;
-      if (v0 + 16 * w < Vp) {
-        f32x4 ks[2] = {zero4(), zero4()}, kg[2] = {zero4(), zero4()};
+      const bool act = v0 + 16 * w < Vp;
+      f32x4 ks[2] = {zero4(), zero4()}, kg[2] = {zero4(), zero4()}, qs[2] = {zero4(), zero4()};
+      if (act) {
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
-          f32x4 S[2], G[2];
           u32x4 sp[3], gp[3];
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            S[x] = *reinterpret_cast<const f32x4*>(Sp + vc * KP + 32 * s + 8 * j + 4 * x);
-            G[x] = *reinterpret_cast<const f32x4*>(Gp + vc * KP + 32 * s + 8 * j + 4 * x);
+          for (int x = 0; x < 2; ++x)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) ss = __builtin_fmaf(S[x][r], G[x][r], ss);
-          }
-          split_tiles<3>(S[0], S[1], sp);
-          split_tiles<3>(G[0], G[1], gp);
+            for (int r = 0; r < 4; ++r) ss = __builtin_fmaf(S[2 * s + x][r], G[2 * s + x][r], ss);
+          split_tiles<3>(S[2 * s], S[2 * s + 1], sp);
+          split_tiles<3>(G[2 * s], G[2 * s + 1], gp);
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            u32x4 f[NP];
+            u32x4 f[NP], q[NP];
 #pragma unroll
-            for (int p = 0; p < NP; ++p)
+            for (int p = 0; p < NP; ++p) {
               f[p] = lds16(&lds.K[p][(ar + 4 * x) * W::kLd + 32 * s + 8 * j]);
+              q[p] = lds16(&lds.Q[p][(ar + 4 * x) * W::kLd + 32 * s + 8 * j]);
+            }
             ks[x] = mfma_planes<NP, 3, 3>(f, sp, ks[x]);
             kg[x] = mfma_planes<NP, 3, 3>(f, gp, kg[x]);
+            qs[x] = mfma_planes<NP, 3, 3>(q, sp, qs[x]);
           }
         }
-        float v[8];
+      }
+      // the sums over v want S and G' the other way round: on their way now
+      float s8[2][NK][8], g8[2][NK][8];
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int m = 0; m < NK; ++m) {
+          const int tile = w + 4 * m < 2 * NS ? w + 4 * m : 0;
+          const uint32_t at = ((uint32_t)(v0 + 32 * q + 8 * j) * KP + 16 * tile + c) * 4;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            s8[q][m][e] = __uint_as_float(
+                __builtin_amdgcn_raw_buffer_load_b32(Sp, at + e * KP * 4, 0, 0));
+            g8[q][m][e] = __uint_as_float(
+                __builtin_amdgcn_raw_buffer_load_b32(Gp, at + e * KP * 4, 0, 0));
+          }
+        }
+      if (act) {
+        float v[8], d[8], x8[8];
+        // per row 8 j + e, over this slice's columns: dR Y,
+        // e^G (scale dO (Q S) - beta dR (K S)), e^(G_last - G) U (K G')
+        float db[8], s1[8], s2[8];
         u32x4 dop[NP], pl[3];
 #pragma unroll
         for (int p = 0; p < NP; ++p) {
@@ -234,15 +303,22 @@ __global__ __launch_bounds__(256, (Grad<T, KP, VEC>::kWaves)) void delta_grads_k
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const uint32_t x = e & 1 ? u[e >> 1] & 0xffff0000u : u[e >> 1] << 16;
+            const uint32_t y = e & 1 ? dop[p][e >> 1] & 0xffff0000u : dop[p][e >> 1] << 16;
             v[e] = p == 0 ? __uint_as_float(x) : v[e] + __uint_as_float(x);
+            d[e] = p == 0 ? __uint_as_float(y) : d[e] + __uint_as_float(y);
           }
         }
         f32x4 R[2], U[2] = {zero4(), zero4()}, Z[2] = {zero4(), zero4()};
+        fac8(kEg, x8);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          v[e] = __builtin_fmaf(-eg[e], ks[e >> 2][e & 3], v[e]);  // Y
-          R[e >> 2][e & 3] = be[e] * v[e];
+          v[e] = __builtin_fmaf(-x8[e], ks[e >> 2][e & 3], v[e]);  // Y
+          s1[e] = x8[e] * a.scale * d[e] * qs[e >> 2][e & 3];
+          ks[e >> 2][e & 3] *= x8[e];  // e^G K S
         }
+        fac8(kBeta, x8);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) R[e >> 2][e & 3] = x8[e] * v[e];
         split_tiles<3>(R[0], R[1], pl);
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
@@ -258,9 +334,12 @@ __global__ __launch_bounds__(256, (Grad<T, KP, VEC>::kWaves)) void delta_grads_k
 #pragma unroll
         for (int p = 0; p < 3; ++p)
           *reinterpret_cast<u32x4*>(&lds.c.U[p][(16 * w + c) * kTld + 8 * j]) = pl[p];
+        fac8(kEnd, x8);
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          Z[e >> 2][e & 3] = __builtin_fmaf(en[e], kg[e >> 2][e & 3], a.scale * Z[e >> 2][e & 3]);
+        for (int e = 0; e < 8; ++e) {
+          s2[e] = x8[e] * U[e >> 2][e & 3] * kg[e >> 2][e & 3];
+          Z[e >> 2][e & 3] = __builtin_fmaf(x8[e], kg[e >> 2][e & 3], a.scale * Z[e >> 2][e & 3]);
+        }
         split_tiles<3>(Z[0], Z[1], pl);
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
@@ -273,13 +352,39 @@ __global__ __launch_bounds__(256, (Grad<T, KP, VEC>::kWaves)) void delta_grads_k
 #pragma unroll
         for (int p = 0; p < 3; ++p)
           *reinterpret_cast<u32x4*>(&lds.c.R[p][(16 * w + c) * kTld + 8 * j]) = pl[p];
+        fac8(kBeta, x8);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float r = R[e >> 2][e & 3];
-          db[e] = __builtin_fmaf(r, v[e], db[e]);
-          if (8 * j + e < rows && vc < a.V) stf(dvp + (8 * j + e) * a.Hv * a.V + vc, be[e] * r);
+          db[e] = r * v[e];
+          s1[e] = __builtin_fmaf(-x8[e] * r, ks[e >> 2][e & 3], s1[e]);
+          // one plane: dV through LDS where this wave's V was; otherwise as it is
+          if constexpr (NP == 1) lds.V[0][(8 * j + e) * W::kVld + 16 * w + c] = f32_to_bf16_bits(x8[e] * r);
+          else if (8 * j + e < rows && vc < a.V) stf(dvp + (8 * j + e) * a.Hv * a.V + vc, x8[e] * r);
+        }
+        const auto add = [&](float* row, const float* x, int e0) {
+          float4 q = v0 ? *reinterpret_cast<const float4*>(row + e0) : make_float4(0, 0, 0, 0);
+          q.x += x[e0]; q.y += x[e0 + 1]; q.z += x[e0 + 2]; q.w += x[e0 + 3];
+          *reinterpret_cast<float4*>(row + e0) = q;
+        };
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          db[e] = group_sum<16>(db[e]);
+          s1[e] = group_sum<16>(s1[e]);
+          s2[e] = group_sum<16>(s2[e]);
+        }
+        if (c == 0) {
+#pragma unroll
+          for (int q = 0; q < 8; q += 4) {
+            add(&lds.row[w][2][8 * j], db, q);
+            add(&lds.row[w][3][8 * j], s1, q);
+            add(&lds.row[w][4][8 * j], s2, q);
+          }
         }
       } else {
+        if (v0 == 0) {
+          for (int i = lane; i < 3 * kC; i += 64) lds.row[w][2 + i / kC][i % kC] = 0.0f;
+        }
 #pragma unroll
         for (int p = 0; p < 3; ++p) {
           *reinterpret_cast<u32x4*>(&lds.c.U[p][(16 * w + c) * kTld + 8 * j]) = u32x4{0, 0, 0, 0};
@@ -287,52 +392,60 @@ __global__ __launch_bounds__(256, (Grad<T, KP, VEC>::kWaves)) void delta_grads_k
         }
       }
       __syncthreads();
+      if constexpr (NP == 1) {
+        const int64_t left = a.V - v0 - scol;
+        T* p = dvp + sr * a.Hv * a.V + v0 + scol;
+        const T* q = reinterpret_cast<const T*>(&lds.V[0][sr * W::kVld + scol]);
+        if (sr < rows) {
+          if (VEC) {
+            if (left > 0) *reinterpret_cast<u32x4*>(p) = *reinterpret_cast<const u32x4*>(q);
+          } else {
+            for (int e = 0; e < 8 && e < left; ++e) p[e] = q[e];
+          }
+        }
+      }
+      const bool more = !ONE && v0 + 64 < a.V;
+      if (more) slice(v0 + 64);
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         if (v0 + 32 * q >= Vp) continue;
-        u32x4 fd[2][NP], fu[2][3], fr[2][3];
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
+        __builtin_amdgcn_sched_barrier(0);  // one half's operands in registers at a time
+        const auto rows_d = [&](int x, u32x4* f) {
 #pragma unroll
           for (int p = 0; p < NP; ++p)
-            fd[x][p] = lds16(&lds.D[p][(ar + 4 * x) * W::kVld + 32 * q + 8 * j]);
+            f[p] = lds16(&lds.D[p][(ar + 4 * x) * W::kVld + 32 * q + 8 * j]);
+        };
+        const auto rows_of = [&](const uint16_t (&m)[3][64 * kTld], int x, u32x4* f, int np) {
 #pragma unroll
-          for (int p = 0; p < 3; ++p) {
-            fu[x][p] = lds_col(&lds.c.U[p][32 * q * kTld], kTld, 4 * x, lane);
-            fr[x][p] = lds_col(&lds.c.R[p][32 * q * kTld], kTld, 4 * x, lane);
-          }
+          for (int p = 0; p < 3; ++p)
+            if (p < np) f[p] = lds_col(&m[p][32 * q * kTld], kTld, 4 * x, lane);
+        };
+        {
+          u32x4 da[NP], ra[3], ub[3];
+          rows_d(tx, da);
+          rows_of(lds.c.U, ty, ub, 3);
+          rows_of(lds.c.R, tx, ra, 3);
+          dP = mfma_planes<NP, 3, 3>(da, ub, dP);
+          dA = mfma_planes<3, 3, 3>(ra, ub, dA);
         }
-        // (uniform selections: a register array has no runtime index)
-        u32x4 da[NP], ra[3], ub[3];
-#pragma unroll
-        for (int p = 0; p < NP; ++p) da[p] = tx ? fd[1][p] : fd[0][p];
-#pragma unroll
-        for (int p = 0; p < 3; ++p) {
-          ra[p] = tx ? fr[1][p] : fr[0][p];
-          ub[p] = ty ? fu[1][p] : fu[0][p];
-        }
-        dP = mfma_planes<NP, 3, 3>(da, ub, dP);
-        dA = mfma_planes<3, 3, 3>(ra, ub, dA);
+        u32x4 sp[NK][NO], gp[NK][NO];
 #pragma unroll
         for (int m = 0; m < NK; ++m) {
-          const int tile = w + 4 * m;
-          if (tile >= 2 * NS) continue;
-          const int key = 32 * (tile >> 1) + 4 * (tile & 1) + ar;
-          float s8[8], g8[8];
-          u32x4 sp[3], gp[3];
+          split8<NO>(s8[q][m], sp[m]);
+          split8<NO>(g8[q][m], gp[m]);
+        }
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int64_t r = v0 + 32 * q + 8 * j + e, rr = r < Vp ? r : Vp - 1;
-            s8[e] = Sp[rr * KP + key];
-            g8[e] = Gp[rr * KP + key];
-          }
-          split8<3>(s8, sp);
-          split8<3>(g8, gp);
+        for (int x = 0; x < 2; ++x) {
+          u32x4 fd[NP], fu[3], fr[3];
+          rows_d(x, fd);
+          rows_of(lds.c.U, x, fu, NO);
+          rows_of(lds.c.R, x, fr, NO);
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            X1[m][x] = mfma_planes<NP, 3, 3>(fd[x], sp, X1[m][x]);
-            X2[m][x] = mfma_planes<3, 3, 3>(fu[x], gp, X2[m][x]);
-            X3[m][x] = mfma_planes<3, 3, 3>(fr[x], sp, X3[m][x]);
+          for (int m = 0; m < NK; ++m) {
+            if (w + 4 * m >= 2 * NS) continue;
+            X1[m][x] = mfma_planes<NP, NO, NO>(fd, sp[m], X1[m][x]);
+            X2[m][x] = mfma_planes<NO, NO, NO>(fu, gp[m], X2[m][x]);
+            X3[m][x] = mfma_planes<NO, NO, NO>(fr, sp[m], X3[m][x]);
           }
         }
       }
@@ -342,60 +455,34 @@ __global__ __launch_bounds__(256, (Grad<T, KP, VEC>::kWaves)) void delta_grads_k
     // the 32 x 32 tiles: M, E and the sums of F
     {
       f32x4 M, E;
-      float fcol = 0.0f;
+      float fcol = 0.0f, frow[4], kb[4];
+      const float4 b4 = *reinterpret_cast<const float4*>(&lds.fac[kBeta][8 * j + 4 * tx]);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int t = 8 * j + 4 * tx + r;
-        const float bt = lds.fac[kBeta][t];
-        const float p = a.scale * dP[r], q = -dA[r];
+        const float bt = (&b4.x)[r], p = a.scale * dP[r], q = -dA[r];
         M[r] = p * dd[r];
-        E[r] = ti < t ? q * dd[r] * bt : 0.0f;
+        E[r] = ti < 8 * j + 4 * tx + r ? q * dd[r] * bt : 0.0f;
         const float f = __builtin_fmaf(p, pp[r], q * bt * dkk[r]);
         fcol += f;
-        const float frow = group_sum<16>(f), kb = group_sum<16>(q * dkk[r]);
-        if (c == 0) {
-          lds.row[w][0][t] = frow;
-          lds.row[w][1][t] = kb;
-        }
+        frow[r] = group_sum<16>(f);
+        kb[r] = group_sum<16>(q * dkk[r]);
       }
       fcol += __shfl_xor(fcol, 16);
       fcol += __shfl_xor(fcol, 32);
       if (j == 0) lds.col[w][ti] = fcol;
+      if (c == 0) {
+        *reinterpret_cast<float4*>(&lds.row[w][0][8 * j + 4 * tx]) =
+            make_float4(frow[0], frow[1], frow[2], frow[3]);
+        *reinterpret_cast<float4*>(&lds.row[w][1][8 * j + 4 * tx]) =
+            make_float4(kb[0], kb[1], kb[2], kb[3]);
+      }
       put4<NO>(lds.m.M, ti * kTld + 8 * j + 4 * tx, M);
       put4<NO>(lds.m.E, ti * kTld + 8 * j + 4 * tx, E);
-    }
-    // products with q and k over the keys, step by step
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int t = 8 * j + e;
-      float s1 = 0.0f, s2 = 0.0f;
-#pragma unroll
-      for (int m = 0; m < NK; ++m) {
-        const int tile = w + 4 * m;
-        if (tile >= 2 * NS) continue;
-        const int at = t * W::kLd + 32 * (tile >> 1) + 4 * (tile & 1) + ar;
-        float kv = 0.0f, qv = 0.0f;
-#pragma unroll
-        for (int p = NP - 1; p >= 0; --p) {
-          kv += bf16_bits_to_f32(lds.K[p][at]);
-          qv += bf16_bits_to_f32(lds.Q[p][at]);
-        }
-        s1 += a.scale * qv * X1[m][e >> 2][e & 3] - be[e] * kv * X3[m][e >> 2][e & 3];
-        s2 = __builtin_fmaf(kv, X2[m][e >> 2][e & 3], s2);
-      }
-      s1 = group_sum<16>(s1);
-      s2 = group_sum<16>(s2);
-      const float s3 = group_sum<16>(db[e]);
-      if (c == 0) {
-        lds.row[w][2][t] = s3;
-        lds.row[w][3][t] = eg[e] * s1;
-        lds.row[w][4][t] = en[e] * s2;
-      }
     }
     ss = group_sum<64>(ss);
     if (lane == 0) lds.dot[w] = ss;
     __syncthreads();
-    if (w == 0) {
+    if (w == (int)(n & 3)) {  // (the waves' turn about)
       const int t = lane & 31, x = t >> 2 & 1;  // the tiles of row t: waves 2 x, 2 x + 1
       const auto sum4 = [&](int i) {
         return (lds.row[0][i][t] + lds.row[1][i][t]) + (lds.row[2][i][t] + lds.row[3][i][t]);
@@ -404,33 +491,36 @@ __global__ __launch_bounds__(256, (Grad<T, KP, VEC>::kWaves)) void delta_grads_k
       const float kb = lds.row[2 * x][1][t] + lds.row[2 * x + 1][1][t];
       const float fc = lds.col[x][t] + lds.col[2 + x][t];  // column t: waves x and 2 + x
       const float bt = sum4(4);
-      double G = (double)(f - fc) + (double)(sum4(3) - bt), B = bt;
+      double G_ = (double)(f - fc) + (double)(sum4(3) - bt), B = bt;
 #pragma unroll
       for (int s = 1; s < 32; s *= 2) B += __shfl_xor(B, s, 32);
       if (t == 31)
-        G += B + (double)lds.fac[kEg][31] *
-                     (double)((lds.dot[0] + lds.dot[1]) + (lds.dot[2] + lds.dot[3]));
+        G_ += B + (double)lds.fac[kEg][31] *
+                      (double)((lds.dot[0] + lds.dot[1]) + (lds.dot[2] + lds.dot[3]));
 #pragma unroll
       for (int s = 1; s < 32; s *= 2) {
-        const double y = __shfl_down(G, s, 32);
-        if (t + s < 32) G += y;
+        const double y = __shfl_down(G_, s, 32);
+        if (t + s < 32) G_ += y;
       }
       if (lane < rows) {
         const int64_t at = (b * a.L + t0 + t) * a.Hv + h;
-        g.dg[at] = (float)G;
+        g.dg[at] = (float)G_;
         g.dbeta[at] = sum4(2) + kb;
       }
     }
+    float be[8], eg[8], en[8];
+    fac8(kBeta, be);
+    fac8(kEg, eg);
+    fac8(kEnd, en);
 #pragma unroll
     for (int m = 0; m < NK; ++m) {
       const int tile = w + 4 * m;
       if (tile >= 2 * NS) continue;
-      const int at = 32 * (tile >> 1) + 4 * (tile & 1);
       u32x4 kc[NP], qc[NP];
 #pragma unroll
       for (int p = 0; p < NP; ++p) {
-        kc[p] = lds_col(lds.K[p], W::kLd, at, lane);
-        qc[p] = lds_col(lds.Q[p], W::kLd, at, lane);
+        kc[p] = lds_col16(lds.K[p], W::kLd, 16 * tile, lane);
+        qc[p] = lds_col16(lds.Q[p], W::kLd, 16 * tile, lane);
       }
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
@@ -458,16 +548,41 @@ __global__ __launch_bounds__(256, (Grad<T, KP, VEC>::kWaves)) void delta_grads_k
   }
   T* dqp = reinterpret_cast<T*>(g.dq) + ((b * a.L + t0) * a.Hk + hk) * K;
   T* dkp = reinterpret_cast<T*>(g.dk) + ((b * a.L + t0) * a.Hk + hk) * K;
+  // one plane: through LDS, where Q and K were, for whole accesses
+  if constexpr (NP == 1) __syncthreads();
 #pragma unroll
   for (int m = 0; m < NK; ++m) {
-    const int tile = w + 4 * m, key = 32 * (tile >> 1) + 4 * (tile & 1) + ar;
-    if (tile >= 2 * NS || key >= K) continue;
+    const int tile = w + 4 * m, key = 16 * tile + c;
+    if (tile >= 2 * NS) continue;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int t = 8 * j + e;
-      if (t < rows) {
+      if constexpr (NP == 1) {
+        lds.Q[0][t * W::kLd + key] = f32_to_bf16_bits(aq[m][e >> 2][e & 3]);
+        lds.K[0][t * W::kLd + key] = f32_to_bf16_bits(ak[m][e >> 2][e & 3]);
+      } else if (t < rows && key < K) {
         stf(dqp + t * a.Hk * K + key, aq[m][e >> 2][e & 3]);
         stf(dkp + t * a.Hk * K + key, ak[m][e >> 2][e & 3]);
+      }
+    }
+  }
+  if constexpr (NP == 1) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kNk; ++i) {
+      const int id = tid + 256 * i, r = id / (KP / 8), col = id % (KP / 8) * 8;
+      if (r >= rows || col >= K) continue;
+      const T* q = reinterpret_cast<const T*>(&lds.Q[0][r * W::kLd + col]);
+      const T* k = reinterpret_cast<const T*>(&lds.K[0][r * W::kLd + col]);
+      const int64_t at = r * a.Hk * K + col;
+      if (VEC) {
+        *reinterpret_cast<u32x4*>(dqp + at) = *reinterpret_cast<const u32x4*>(q);
+        *reinterpret_cast<u32x4*>(dkp + at) = *reinterpret_cast<const u32x4*>(k);
+      } else {
+        for (int e = 0; e < 8 && col + e < K; ++e) {
+          dqp[at + e] = q[e];
+          dkp[at + e] = k[e];
+        }
       }
     }
   }
@@ -486,8 +601,16 @@ int grads_launch(const GradArgs& g, bool vec, hipStream_t s) {
     return launch_status();
   };
   static_assert(sizeof(typename Grad<T, KP, true>::Lds) <= 160 * 1024, "LDS of a CU");
-  return vec ? go(delta_grads_kernel<T, KP, true>, (int)sizeof(typename Grad<T, KP, true>::Lds))
-             : go(delta_grads_kernel<T, KP, false>, (int)sizeof(typename Grad<T, KP, false>::Lds));
+  const int bytes = (int)sizeof(typename Grad<T, KP, true>::Lds);
+  // without the loops over heads and slices 256 registers hold everything (88
+  // bytes a lane spilled with them: 232 us against 171 at B=4 L=4096 H=16 K=V=64)
+  if constexpr (Grad<T, KP, true>::kWaves == 2) {
+    if (g.a.Hv == g.a.Hk && g.a.V <= 64)
+      return vec ? go(delta_grads_kernel<T, KP, true, true>, bytes)
+                 : go(delta_grads_kernel<T, KP, false, true>, bytes);
+  }
+  return vec ? go(delta_grads_kernel<T, KP, true, false>, bytes)
+             : go(delta_grads_kernel<T, KP, false, false>, bytes);
 }
 
 template <typename T>
