@@ -43,11 +43,12 @@ int delta_walk_launch(int dtype, const DeltaArgs& a, bool vec, const DeltaPlan& 
 // The segments' transfer matrices, then their entry states.
 int delta_transfer_launch(int dtype, const DeltaArgs& a, bool vec, const DeltaPlan& p,
                           hipStream_t s);
-int delta_states_launch(int dtype, const DeltaArgs& a, bool vec, const DeltaPlan& p,
-                        hipStream_t s);
-// The way back (a.v: dO, a.h0: dh_last, a.h_last: dh0), and its segments' joining.
-int delta_back_launch(int dtype, const DeltaArgs& a, bool vec, const DeltaPlan& p, hipStream_t s);
+int delta_fold(const DeltaArgs& a, const DeltaPlan& p, hipStream_t s);
 int delta_fold_back(const DeltaArgs& a, const DeltaPlan& p, hipStream_t s);
+// The states before the chunks and the gradients of those after them (way.v:
+// dO, way.h0: dh_last, way.h_last: dh0), segments included.
+int delta_both_launch(int dtype, const DeltaArgs& a, const DeltaArgs& way, bool vec,
+                      const DeltaPlan& p, hipStream_t s);
 // Gradients of the inputs; outputs contiguous, dO with strides.
 struct DeltaGrads {
   const void* dout;

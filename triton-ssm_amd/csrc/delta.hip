@@ -185,8 +185,6 @@ extern "C" int tssm_gated_delta_backward(
   const bool vec = vec_rows(dtype, a) && vec_rows(dtype, way);
   hipStream_t st = as_stream(stream);
   int rc = delta_prep_launch(dtype, a, vec, p.chunks, st);
-  if (!rc && p.nseg > 1) rc = delta_transfer_launch(dtype, a, vec, p, st);
-  if (!rc) rc = delta_states_launch(dtype, a, vec, p, st);
-  if (!rc) rc = delta_back_launch(dtype, way, vec, p, st);
+  if (!rc) rc = delta_both_launch(dtype, a, way, vec, p, st);
   return rc ? rc : delta_grads_launch(dtype, a, d, vec, p, st);
 }

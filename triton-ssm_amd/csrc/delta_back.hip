@@ -10,6 +10,8 @@
 // dO) are formed by two helper waves a chunk ahead, and two loaders bring K, Q,
 // dO and T.  The gradient after every chunk goes to the workspace, where the
 // gradients of the inputs are formed from it in parallel (delta_grads.hip).
+// The walk that leaves the states needs nothing of this one: both go in one
+// launch, each workgroup of one or the other.
 // Two barriers a chunk: before the first the loaders put the next chunk into
 // LDS while the chain waves multiply K G', after it the helpers work on that
 // chunk.
@@ -352,19 +354,17 @@ __device__ inline void back_bring(const BackArgs& g, typename Back<T, KP, VEC, N
 }
 
 template <typename T, int KP, bool VEC, int NCW, bool ZERO>
-__global__ __launch_bounds__((Back<T, KP, VEC, NCW>::kThreads),
-                             (Back<T, KP, VEC, NCW>::kWaves)) void delta_back_kernel(BackArgs g) {
+__device__ inline void back_body(const BackArgs& g, char* raw, uint32_t block) {
   typedef Back<T, KP, VEC, NCW> W;
-  extern __shared__ __attribute__((aligned(16))) char raw[];
   typename W::Lds& lds = *reinterpret_cast<typename W::Lds*>(raw);
   const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int64_t heads = g.a.B * g.a.Hv, runs = heads * (ZERO ? g.nseg - 1 : g.nseg);
-  const int64_t run = (int64_t)(blockIdx.x / (8 * g.nvb)) * 8 + (blockIdx.x & 7);
+  const int64_t run = (int64_t)(block / (8 * g.nvb)) * 8 + (block & 7);
   if (run >= runs) return;
   const int64_t bh = run % heads;
   const int seg = (int)(run / heads) + (ZERO ? 1 : 0);
   const int n0 = seg * g.per, n1 = n0 + g.per < g.nch ? n0 + g.per : g.nch;
-  const int64_t v0 = (int64_t)(blockIdx.x / 8 % g.nvb) * 16 * NCW;
+  const int64_t v0 = (int64_t)(block / 8 % g.nvb) * 16 * NCW;
   if (wv < NCW)
     back_chain<W, NCW, ZERO>(g, lds, bh, seg, v0 + 16 * wv + (threadIdx.x & 15), wv, n0, n1);
   else if (wv < NCW + 2)
@@ -373,63 +373,100 @@ __global__ __launch_bounds__((Back<T, KP, VEC, NCW>::kThreads),
     back_bring<T, KP, VEC, NCW>(g, lds, bh, v0, n0, n1);
 }
 
+// The first nback workgroups walk back, the others there.  (Waves that one of
+// the two has no use for end at once: barriers count the others.)
 template <typename T, int KP, bool VEC, int NCW, bool ZERO>
-int back_launch(BackArgs& g, hipStream_t s) {
-  typedef Back<T, KP, VEC, NCW> W;
+struct Both {
+  static constexpr int MODE = ZERO ? kTransfer : kStates;
+  typedef Back<T, KP, VEC, NCW> B;
+  typedef Walk<T, KP, VEC, 2, MODE> F;
+  static constexpr int kThreads = B::kThreads > F::kThreads ? B::kThreads : F::kThreads;
+  static constexpr int kBytes = sizeof(typename B::Lds) > sizeof(typename F::Lds)
+                                    ? (int)sizeof(typename B::Lds) : (int)sizeof(typename F::Lds);
+};
+template <typename T, int KP, bool VEC, int NCW, bool ZERO>
+__global__ __launch_bounds__((Both<T, KP, VEC, NCW, ZERO>::kThreads),
+                             (Back<T, KP, VEC, NCW>::kWaves)) void
+    delta_both_kernel(BackArgs g, WalkArgs f, uint32_t nback) {
+  typedef Both<T, KP, VEC, NCW, ZERO> W;
+  extern __shared__ __attribute__((aligned(16))) char raw[];
+  if (blockIdx.x < nback) {
+    if (threadIdx.x < W::B::kThreads) back_body<T, KP, VEC, NCW, ZERO>(g, raw, blockIdx.x);
+  } else {
+    if (threadIdx.x < W::F::kThreads)
+      walk_body<T, KP, VEC, 2, W::MODE>(f, raw, blockIdx.x - nback);
+  }
+}
+
+template <typename T, int KP, bool VEC, int NCW, bool ZERO>
+int both_launch(BackArgs& g, WalkArgs& f, hipStream_t s) {
+  typedef Both<T, KP, VEC, NCW, ZERO> W;
   g.nvb = (uint32_t)cdiv64(g.a.V, 16 * NCW);
-  const int64_t runs = g.a.B * g.a.Hv * (ZERO ? g.nseg - 1 : g.nseg);
-  const int64_t wgs = cdiv64(runs, 8) * 8 * g.nvb;
-  if (wgs > 0x7fffffff) return TSSM_ERR_UNSUPPORTED;
-  constexpr int bytes = (int)sizeof(typename W::Lds);
-  static_assert(bytes <= 160 * 1024, "LDS of a CU");
-  auto* f = delta_back_kernel<T, KP, VEC, NCW, ZERO>;
-  if (bytes > 64 * 1024) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(f),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  const int64_t nb = cdiv64(g.a.B * g.a.Hv * (ZERO ? g.nseg - 1 : g.nseg), 8) * 8 * g.nvb;
+  const int64_t nf = walk_wgs<KP, 2, W::MODE>(f);
+  if (nb > 0x3fffffff || nf < 0) return TSSM_ERR_UNSUPPORTED;
+  static_assert(W::kBytes <= 160 * 1024, "LDS of a CU");
+  auto* k = delta_both_kernel<T, KP, VEC, NCW, ZERO>;
+  if (W::kBytes > 64 * 1024) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, W::kBytes);
     if (e != hipSuccess) return (int)e;
   }
-  f<<<(unsigned)wgs, W::kThreads, bytes, s>>>(g);
+  k<<<(unsigned)(nb + nf), W::kThreads, W::kBytes, s>>>(g, f, (uint32_t)nb);
   return launch_status();
 }
 
 template <typename T, bool ZERO>
-int back_any(BackArgs& g, bool vec, hipStream_t s) {
+int both_any(BackArgs& g, WalkArgs& f, bool vec, hipStream_t s) {
   constexpr int NW = std::is_same<T, bf16_t>::value ? 2 : 1;
   if (g.a.K <= 32)
-    return vec ? back_launch<T, 32, true, 2, ZERO>(g, s) : back_launch<T, 32, false, 2, ZERO>(g, s);
+    return vec ? both_launch<T, 32, true, 2, ZERO>(g, f, s)
+               : both_launch<T, 32, false, 2, ZERO>(g, f, s);
   if (g.a.K <= 64)
-    return vec ? back_launch<T, 64, true, 2, ZERO>(g, s) : back_launch<T, 64, false, 2, ZERO>(g, s);
-  return vec ? back_launch<T, 128, true, NW, ZERO>(g, s)
-             : back_launch<T, 128, false, NW, ZERO>(g, s);
+    return vec ? both_launch<T, 64, true, 2, ZERO>(g, f, s)
+               : both_launch<T, 64, false, 2, ZERO>(g, f, s);
+  return vec ? both_launch<T, 128, true, NW, ZERO>(g, f, s)
+             : both_launch<T, 128, false, NW, ZERO>(g, f, s);
 }
 
 template <bool ZERO>
-int back(int dtype, BackArgs& g, bool vec, hipStream_t s) {
+int both(int dtype, BackArgs& g, WalkArgs& f, bool vec, hipStream_t s) {
   switch (dtype) {
-    case TSSM_F32: return back_any<float, ZERO>(g, vec, s);
-    case TSSM_BF16: return back_any<bf16_t, ZERO>(g, vec, s);
-    default: return back_any<f16_t, ZERO>(g, vec, s);
+    case TSSM_F32: return both_any<float, ZERO>(g, f, vec, s);
+    case TSSM_BF16: return both_any<bf16_t, ZERO>(g, f, vec, s);
+    default: return both_any<f16_t, ZERO>(g, f, vec, s);
   }
 }
 
 }  // namespace
 
-int delta_back_launch(int dtype, const DeltaArgs& a, bool vec, const DeltaPlan& p, hipStream_t s) {
+int delta_both_launch(int dtype, const DeltaArgs& a, const DeltaArgs& way, bool vec,
+                      const DeltaPlan& p, hipStream_t s) {
+  WalkArgs f = {};
+  f.a = a;
+  f.ws = reinterpret_cast<const ChunkWs*>(p.chunks);
+  f.nch = p.nch;
+  f.per = p.per;
+  f.nseg = f.walked = p.nseg;
   BackArgs g = {};
-  g.a = a;
-  g.ws = reinterpret_cast<const ChunkWs*>(p.chunks);
+  g.a = way;
+  g.ws = f.ws;
   g.nch = p.nch;
   g.per = p.per;
   g.nseg = p.nseg;
-  if (p.nseg > 1) {
+  if (p.nseg > 1) {  // all segments' transfer: the last one's is for the way back
+    f.states = p.transfer;
     g.grads = p.back;
-    int rc = back<true>(dtype, g, vec, s);
-    if (!rc) rc = delta_fold_back(a, p, s);
+    int rc = both<true>(dtype, g, f, vec, s);
+    if (!rc) rc = delta_fold(a, p, s);
+    if (!rc) rc = delta_fold_back(way, p, s);
     if (rc) return rc;
   }
+  f.entry = p.entry;
+  f.states = p.states;
   g.entry = p.gentry;
   g.grads = p.grads;
-  return back<false>(dtype, g, vec, s);
+  return both<false>(dtype, g, f, vec, s);
 }
 
 }  // namespace tssm

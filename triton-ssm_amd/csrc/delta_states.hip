@@ -1,5 +1,5 @@
-// Gated delta rule, chunked: the walks that form no outputs, and the joining
-// of a long sequence's segments.
+// Gated delta rule, chunked: the segments of a long sequence, walked from zero
+// and joined.
 #include "delta_walk.h"
 
 namespace tssm {
@@ -89,19 +89,7 @@ int fold(const FoldArgs& f, hipStream_t s) {
 
 }  // namespace
 
-int delta_transfer_launch(int dtype, const DeltaArgs& a, bool vec, const DeltaPlan& p,
-                          hipStream_t s) {
-  WalkArgs g = {};
-  g.a = a;
-  g.ws = reinterpret_cast<const ChunkWs*>(p.chunks);
-  g.nch = p.nch;
-  g.per = p.per;
-  g.nseg = p.nseg;
-  // the last one's is for the way back
-  g.walked = p.back ? p.nseg : p.nseg - 1;
-  g.states = p.transfer;
-  const int rc = walk_mode<kTransfer>(dtype, g, vec, s);
-  if (rc) return rc;
+int delta_fold(const DeltaArgs& a, const DeltaPlan& p, hipStream_t s) {
   const FoldArgs f = {a.h0, p.transfer, nullptr, p.entry, a.B * a.Hv, a.V, (int)a.K, p.nseg,
                       (int)cdiv64(a.V, 16)};
   return fold<false>(f, s);
@@ -113,17 +101,18 @@ int delta_fold_back(const DeltaArgs& a, const DeltaPlan& p, hipStream_t s) {
   return fold<true>(f, s);
 }
 
-int delta_states_launch(int dtype, const DeltaArgs& a, bool vec, const DeltaPlan& p,
-                        hipStream_t s) {
+int delta_transfer_launch(int dtype, const DeltaArgs& a, bool vec, const DeltaPlan& p,
+                          hipStream_t s) {
   WalkArgs g = {};
   g.a = a;
   g.ws = reinterpret_cast<const ChunkWs*>(p.chunks);
   g.nch = p.nch;
   g.per = p.per;
-  g.nseg = g.walked = p.nseg;
-  g.entry = p.entry;
-  g.states = p.states;
-  return walk_mode<kStates>(dtype, g, vec, s);
+  g.nseg = p.nseg;
+  g.walked = p.nseg - 1;
+  g.states = p.transfer;
+  const int rc = walk_mode<kTransfer>(dtype, g, vec, s);
+  return rc ? rc : delta_fold(a, p, s);
 }
 
 }  // namespace tssm

@@ -478,21 +478,18 @@ __device__ inline void outputs(const DeltaArgs& a, typename Walk<T, KP, VEC, NCW
 }
 
 template <typename T, int KP, bool VEC, int NCW, int MODE>
-__global__ __launch_bounds__((Walk<T, KP, VEC, NCW, MODE>::kThreads),
-                             (Walk<T, KP, VEC, NCW, MODE>::kWaves)) void
-    delta_walk_kernel(WalkArgs g) {
+__device__ inline void walk_body(const WalkArgs& g, char* raw, uint32_t block) {
   typedef Walk<T, KP, VEC, NCW, MODE> W;
-  extern __shared__ __attribute__((aligned(16))) char raw[];
   typename W::Lds& lds = *reinterpret_cast<typename W::Lds*>(raw);
   const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   // workgroups of one head and segment on one XCD: they share its keys and queries
   const int64_t runs = g.a.B * g.a.Hv * g.walked;
-  const int64_t run = (int64_t)(blockIdx.x / (8 * g.nvb)) * 8 + (blockIdx.x & 7);
+  const int64_t run = (int64_t)(block / (8 * g.nvb)) * 8 + (block & 7);
   if (run >= runs) return;
   const int64_t bh = run % (g.a.B * g.a.Hv);
   const int seg = (int)(run / (g.a.B * g.a.Hv));
   const int n0 = seg * g.per, n1 = n0 + g.per < g.nch ? n0 + g.per : g.nch;
-  const int64_t v0 = (int64_t)(blockIdx.x / 8 % g.nvb) * 16 * NCW;
+  const int64_t v0 = (int64_t)(block / 8 % g.nvb) * 16 * NCW;
   if (wv < NCW)
     chain<W, NCW, MODE>(g, lds, bh, seg, v0 + 16 * wv + (threadIdx.x & 15), wv, n0, n1);
   else if (MODE != kOutputs || wv >= NCW + 2)
@@ -502,13 +499,27 @@ __global__ __launch_bounds__((Walk<T, KP, VEC, NCW, MODE>::kThreads),
 }
 
 template <typename T, int KP, bool VEC, int NCW, int MODE>
-int walk_launch(WalkArgs& g, hipStream_t s) {
-  typedef Walk<T, KP, VEC, NCW, MODE> W;
+__global__ __launch_bounds__((Walk<T, KP, VEC, NCW, MODE>::kThreads),
+                             (Walk<T, KP, VEC, NCW, MODE>::kWaves)) void
+    delta_walk_kernel(WalkArgs g) {
+  extern __shared__ __attribute__((aligned(16))) char raw[];
+  walk_body<T, KP, VEC, NCW, MODE>(g, raw, blockIdx.x);
+}
+
+// Workgroups of a walk (nvb is set), or -1.
+template <int KP, int NCW, int MODE>
+int64_t walk_wgs(WalkArgs& g) {
   const int64_t cols = MODE == kTransfer ? (g.a.V + 15) / 16 * 16 + KP : g.a.V;
   g.nvb = (uint32_t)cdiv64(cols, 16 * NCW);
-  const int64_t runs = g.a.B * g.a.Hv * g.walked;
-  const int64_t wgs = cdiv64(runs, 8) * 8 * g.nvb;
-  if (wgs > 0x7fffffff) return TSSM_ERR_UNSUPPORTED;
+  const int64_t wgs = cdiv64(g.a.B * g.a.Hv * g.walked, 8) * 8 * g.nvb;
+  return wgs > 0x3fffffff ? -1 : wgs;
+}
+
+template <typename T, int KP, bool VEC, int NCW, int MODE>
+int walk_launch(WalkArgs& g, hipStream_t s) {
+  typedef Walk<T, KP, VEC, NCW, MODE> W;
+  const int64_t wgs = walk_wgs<KP, NCW, MODE>(g);
+  if (wgs < 0) return TSSM_ERR_UNSUPPORTED;
   constexpr int bytes = (int)sizeof(typename W::Lds);
   static_assert(bytes <= 160 * 1024, "LDS of a CU");
   auto* f = delta_walk_kernel<T, KP, VEC, NCW, MODE>;
