@@ -579,7 +579,8 @@ int tssm_masked_fill_zero(int dtype, int mask_code, const void* x, const void* m
  * h0/h_last f32 contiguous [B,Hv,K,V] or NULL (h0 NULL: zero; they may be the
  * same buffer).  K <= 128.  State, sums and products that reach the state are
  * fp32 whatever the dtype.  Workspace: tssm_gated_delta_workspace_bytes()
- * bytes, 256-byte aligned, raw fp32 (not look-back words), no clearing. */
+ * bytes (0: may be NULL), 256-byte aligned, raw fp32 (not look-back words), no
+ * clearing. */
 int64_t tssm_gated_delta_workspace_bytes(int64_t nbatch, int64_t L, int64_t Hk, int64_t Hv,
                                          int64_t K, int64_t V);
 int tssm_gated_delta_forward(int dtype, const void* q, const void* k, const void* v,

@@ -9,8 +9,12 @@ bool sizes_ok(int64_t B, int64_t L, int64_t Hk, int64_t Hv, int64_t K, int64_t V
   return B >= 0 && L >= 0 && Hk > 0 && Hv > 0 && Hv % Hk == 0 && K > 0 && V > 0;
 }
 
-// Shorter sequences go step by step.
-constexpr int64_t kSeqMost = 16;
+// Sequences up to here go step by step.  That takes 3 us and 0.6 us a step (B =
+// 1, 8 heads of 64 x 64: 5.3, 7.6 and 12.3 us at L = 4, 8 and 16); one chunk's
+// way through the chunked kernels takes 10.5 us at any L, and 23 us once the
+// chip has more than two heads on each CU (512 heads: 10.3, 16.4, 21.7 and 26.8
+// us step by step at L = 8, 16, 24 and 32).
+bool by_steps(int64_t heads, int64_t L) { return L <= (heads >= 512 ? 24 : 12); }
 
 // How many segments a sequence of nch chunks is walked in, by the times that the
 // walks take (in tenths of a chunk's time of one workgroup on each CU, a
@@ -106,7 +110,8 @@ extern "C" int tssm_gated_delta_forward(
   const DeltaArgs a = {q, k, v, g, beta, h0, o, h_last, nbatch, L, Hk, Hv, K, V,
                        sq_b, sq_l, sq_h, sk_b, sk_l, sk_h, sv_b, sv_l, sv_h,
                        sg_b, sg_l, sg_h, sbe_b, sbe_l, sbe_h, so_b, so_l, so_h, scale};
-  if (L <= kSeqMost || !chunk_rows(dtype, a)) return delta_seq_launch(dtype, a, as_stream(stream));
+  if (by_steps(nbatch * Hv, L) || !chunk_rows(dtype, a))
+    return delta_seq_launch(dtype, a, as_stream(stream));
   TSSM_CHECK(nbatch * Hv <= 0x7fffffff / cdiv64(L, 32), TSSM_ERR_UNSUPPORTED);
   const DeltaPlan p = delta_plan(reinterpret_cast<char*>(workspace), nbatch, L, Hv, K, V, false);
   TSSM_CHECK(workspace && workspace_bytes >= p.bytes && aligned(workspace, 256),
@@ -140,7 +145,7 @@ extern "C" int64_t tssm_gated_delta_workspace_bytes(int64_t nbatch, int64_t L, i
                                                     int64_t Hv, int64_t K, int64_t V) {
   if (!sizes_ok(nbatch, L, Hk, Hv, K, V)) return TSSM_ERR_SHAPE;
   if (K > 128) return TSSM_ERR_UNSUPPORTED;
-  if (L <= kSeqMost || nbatch == 0) return 256;
+  if (nbatch == 0 || by_steps(nbatch * Hv, L)) return 0;
   return delta_plan(nullptr, nbatch, L, Hv, K, V, false).bytes;
 }
 

@@ -1,23 +1,27 @@
 // Gated delta rule, step by step: decoding (one step, the state in place) and
 // short sequences.
 //
-// A wave owns 32 columns of one head's state for the whole call: lane
-// (kg, cq) = (lane / 8, lane % 8) holds rows kg KR .. kg KR + KR - 1 of columns
+// A wave owns 4 CQ columns of one head's state for the whole call: lane
+// (kg, cq) = (lane / CQ, lane % CQ) holds rows kg KR .. kg KR + KR - 1 of columns
 // 4 cq .. 4 cq + 3 in registers.  Columns never meet (S^T k, the update and
 // S^T q are all per column), so waves are independent; the sums over k run in
-// each lane, then over the eight row groups by lane exchanges.  The state is
-// read and written once whatever L is, 128 bytes of a row at a time.
+// each lane, then over the row groups by lane exchanges.  The state is read and
+// written once whatever L is, 16 CQ bytes of a row at a time.
 //
-// One step of many streams is bound by that traffic; a few steps of one stream
-// by the launch and a chain of two such sums a step.
+// One step of many streams is bound by that traffic (S=4096 H=32 K=128 V=64: 8.7
+// GB at 5.2 TB/s, the rate of a copy); a few steps of one stream by the launch
+// and a chain of two such sums a step, which CQ = 4 shortens where the waves of
+// CQ = 8 leave SIMDs idle.
 #include "delta.h"
 
 namespace tssm {
 namespace {
 
-// Sum over the lanes that share lane % 8.
+// Sum over the lanes that share lane % CQ.
+template <int CQ>
 __device__ inline float sum_kg(float v) {
-  v += dpp_mov<0x128>(v);  // row_ror:8
+  if constexpr (CQ == 4) v += dpp_mov<0x124>(v);  // row_ror:4
+  v += dpp_mov<0x128>(v);                         // row_ror:8
   const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false,
                                                   false);
   v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
@@ -51,14 +55,14 @@ struct Row {
   }
 };
 
-template <typename T, int KR, bool VEC>
+template <typename T, int CQ, int KR, bool VEC>
 __global__ __launch_bounds__(256) void delta_seq_kernel(DeltaArgs a, uint32_t ncb, int64_t units) {
-  const int lane = threadIdx.x & 63, kg = lane >> 3, cq = lane & 7;
+  const int lane = threadIdx.x & 63, kg = lane / CQ, cq = lane % CQ;
   const int64_t unit = (int64_t)blockIdx.x * 4 +
                        __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   if (unit >= units) return;
   const int64_t bh = unit / ncb, b = bh / a.Hv, h = bh - b * a.Hv, hk = h / (a.Hv / a.Hk);
-  const int K = (int)a.K, k0 = kg * KR, c0 = (int)(unit - bh * ncb) * 32 + 4 * cq;
+  const int K = (int)a.K, k0 = kg * KR, c0 = (int)(unit - bh * ncb) * 4 * CQ + 4 * cq;
   const int64_t V = a.V;
   const int klim = K - k0 < 0 ? 0 : K - k0, clim = V - c0 > 4 ? 4 : (V - c0 < 0 ? 0 : (int)(V - c0));
   // lanes past K or V read row 0 or column 0 of their head, store nothing
@@ -70,24 +74,31 @@ __global__ __launch_bounds__(256) void delta_seq_kernel(DeltaArgs a, uint32_t nc
   const float* ep = a.beta + b * a.be_b + h * a.be_h;
   const int64_t sbase = bh * K * V + c0;
 
+  // Loads from rows and columns that exist, zeroes by selection: a branch
+  // around each load would wait for it alone.
   float S[KR][4];
 #pragma unroll
-  for (int i = 0; i < KR; ++i) {
+  for (int i = 0; i < KR; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) S[i][j] = 0.0f;
-    if (a.h0 && i < klim) {
-      const float* p = a.h0 + sbase + (int64_t)(k0 + i) * V;
+  if (a.h0) {
+    const float* hp = a.h0 + bh * K * V + (clim ? c0 : 0);
+#pragma unroll
+    for (int i = 0; i < KR; ++i) {
+      const float* p = hp + (int64_t)(i < klim ? k0 + i : 0) * V;
       if constexpr (VEC) {
-        if (clim) {
-          const float4 x = *reinterpret_cast<const float4*>(p);
-          S[i][0] = x.x; S[i][1] = x.y; S[i][2] = x.z; S[i][3] = x.w;
-        }
+        const float4 x = *reinterpret_cast<const float4*>(p);
+        S[i][0] = x.x; S[i][1] = x.y; S[i][2] = x.z; S[i][3] = x.w;
       } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (j < clim) S[i][j] = p[j];
+        for (int j = 0; j < 4; ++j) S[i][j] = p[j < clim ? j : 0];
       }
     }
+#pragma unroll
+    for (int i = 0; i < KR; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (!(i < klim && j < clim)) S[i][j] = 0.0f;
   }
 
   Row<T, KR, VEC> nq, nk, q, k;
@@ -116,7 +127,7 @@ __global__ __launch_bounds__(256) void delta_seq_kernel(DeltaArgs a, uint32_t nc
       }
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) r[j] = be * (v.get(j, clim) - sum_kg(r[j]));
+    for (int j = 0; j < 4; ++j) r[j] = be * (v.get(j, clim) - sum_kg<CQ>(r[j]));
 #pragma unroll
     for (int i = 0; i < KR; ++i) {
       const float qf = q.get(i, klim);
@@ -127,7 +138,7 @@ __global__ __launch_bounds__(256) void delta_seq_kernel(DeltaArgs a, uint32_t nc
       }
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) y[j] = a.scale * sum_kg(y[j]);
+    for (int j = 0; j < 4; ++j) y[j] = a.scale * sum_kg<CQ>(y[j]);
     if (kg == 0) {
       T* p = op + t * a.o_l;
       if (VEC && clim) {
@@ -139,53 +150,61 @@ __global__ __launch_bounds__(256) void delta_seq_kernel(DeltaArgs a, uint32_t nc
       }
     }
   }
-  if (!a.h_last) return;
+  if (!a.h_last || !clim) return;
 #pragma unroll
   for (int i = 0; i < KR; ++i) {
-    if (i < klim) {
-      float* p = a.h_last + sbase + (int64_t)(k0 + i) * V;
-      if (VEC && clim) {
-        *reinterpret_cast<float4*>(p) = make_float4(S[i][0], S[i][1], S[i][2], S[i][3]);
-      } else {
+    float* p = a.h_last + sbase + (int64_t)(k0 + i) * V;
+    if constexpr (VEC) {
+      *reinterpret_cast<float4*>(p) = make_float4(S[i][0], S[i][1], S[i][2], S[i][3]);
+    } else if (i < klim) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (j < clim) p[j] = S[i][j];
-      }
+      for (int j = 0; j < 4; ++j)
+        if (j < clim) p[j] = S[i][j];
     }
   }
 }
 
-template <typename T>
+template <typename T, int CQ>
 int launch(const DeltaArgs& a, hipStream_t s) {
-  const int64_t ncb = cdiv64(a.V, 32), units = a.B * a.Hv * ncb, wgs = cdiv64(units, 4);
+  constexpr int kR = CQ / 4;  // rows of a lane for every 16 of K
+  const int64_t ncb = cdiv64(a.V, 4 * CQ), units = a.B * a.Hv * ncb, wgs = cdiv64(units, 4);
   if (wgs > 0x7fffffff) return TSSM_ERR_UNSUPPORTED;
   const int E = (int)sizeof(T);
-  const int kr = a.K <= 16 ? 2 : (a.K <= 32 ? 4 : (a.K <= 64 ? 8 : 16));
+  const int kr = (a.K <= 16 ? 1 : (a.K <= 32 ? 2 : (a.K <= 64 ? 4 : 8))) * kR;
   // every row of every operand starts on the widest access a lane makes
   const int64_t kb = kr * E < 16 ? kr * E : 16, vb = 4 * E;
   const bool vec =
-      a.K == 8 * kr && a.V % 4 == 0 && aligned(a.q, kb) && aligned(a.k, kb) && aligned(a.v, vb) &&
-      aligned(a.o, vb) && (!a.h0 || aligned(a.h0, 16)) && (!a.h_last || aligned(a.h_last, 16)) &&
+      a.K == 64 / CQ * kr && a.V % 4 == 0 && aligned(a.q, kb) && aligned(a.k, kb) &&
+      aligned(a.v, vb) && aligned(a.o, vb) && (!a.h0 || aligned(a.h0, 16)) &&
+      (!a.h_last || aligned(a.h_last, 16)) &&
       (a.q_b | a.q_l | a.q_h | a.k_b | a.k_l | a.k_h) * E % kb == 0 &&
       (a.v_b | a.v_l | a.v_h | a.o_b | a.o_l | a.o_h) * E % vb == 0;
-#define TSSM_SEQ(KR)                                                                          \
-  if (vec) delta_seq_kernel<T, KR, true><<<(unsigned)wgs, 256, 0, s>>>(a, (uint32_t)ncb, units); \
-  else delta_seq_kernel<T, KR, false><<<(unsigned)wgs, 256, 0, s>>>(a, (uint32_t)ncb, units)
-  if (kr == 2) { TSSM_SEQ(2); }
-  else if (kr == 4) { TSSM_SEQ(4); }
-  else if (kr == 8) { TSSM_SEQ(8); }
-  else { TSSM_SEQ(16); }
+#define TSSM_SEQ(KR)                                                                       \
+  if (vec)                                                                                 \
+    delta_seq_kernel<T, CQ, KR, true><<<(unsigned)wgs, 256, 0, s>>>(a, (uint32_t)ncb, units); \
+  else                                                                                     \
+    delta_seq_kernel<T, CQ, KR, false><<<(unsigned)wgs, 256, 0, s>>>(a, (uint32_t)ncb, units)
+  if (a.K <= 16) { TSSM_SEQ(kR); }
+  else if (a.K <= 32) { TSSM_SEQ(2 * kR); }
+  else if (a.K <= 64) { TSSM_SEQ(4 * kR); }
+  else { TSSM_SEQ(8 * kR); }
 #undef TSSM_SEQ
   return launch_status();
+}
+
+// 16 columns a wave while that gives at most one wave to each SIMD.
+template <typename T>
+int columns(const DeltaArgs& a, hipStream_t s) {
+  return a.B * a.Hv * cdiv64(a.V, 16) <= 1024 ? launch<T, 4>(a, s) : launch<T, 8>(a, s);
 }
 
 }  // namespace
 
 int delta_seq_launch(int dtype, const DeltaArgs& a, hipStream_t s) {
   switch (dtype) {
-    case TSSM_F32: return launch<float>(a, s);
-    case TSSM_BF16: return launch<bf16_t>(a, s);
-    default: return launch<f16_t>(a, s);
+    case TSSM_F32: return columns<float>(a, s);
+    case TSSM_BF16: return columns<bf16_t>(a, s);
+    default: return columns<f16_t>(a, s);
   }
 }
 

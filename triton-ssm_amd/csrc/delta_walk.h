@@ -19,7 +19,7 @@
 // state before every chunk in the workspace (for the gradients), one walks
 // the segments of a long sequence from zero, and V + K columns: the K more
 // start as unit vectors and take no input, which gives the segment's transfer
-// matrix (delta_fold.hip joins them).
+// matrix (delta_states.hip joins them).
 //
 // A chunk whose U is not finite is done again step by step from S: zero
 // weights would otherwise carry a later step's NaN to earlier outputs.

@@ -20,7 +20,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib, workspace
-from .launch import as_f32, dcode, need_gpu, ptr, stream_handle
+from .launch import DTYPES, as_f32, dcode, need_gpu, ptr, stream_handle
 
 
 def _check(t, what, shape, dtype, device):
@@ -41,27 +41,58 @@ def _rows(t, what):
     return s[:-1]
 
 
+_F32 = torch.float32
+
+
 def _operands(q, k, v, g, beta, lead):
     """Checks q, k, v, g, beta with ``lead`` leading dimensions; returns (sizes,
-    dtype code, g, beta, scale of None)."""
+    dtype code, g, beta).  Decoding calls pay for every check, so what is right
+    passes in one expression, and _explain() names what is not."""
+    try:
+        dev, dtype, rows, heads, shape = q.get_device(), q.dtype, q.shape, v.shape, g.shape
+        right = (dev >= 0 and len(rows) == lead + 2 and rows == k.shape and shape == beta.shape
+                 and heads[:-1] == shape and rows[:lead] == shape[:lead]
+                 and dtype == k.dtype == v.dtype and dtype in DTYPES
+                 and g.dtype == beta.dtype == _F32
+                 and dev == k.get_device() == v.get_device() == g.get_device()
+                 == beta.get_device())
+    except (AttributeError, TypeError, IndexError):
+        right = False
+    if not right:
+        g, beta = _explain(q, k, v, g, beta, lead)
+        dtype, rows, heads = q.dtype, q.shape, v.shape
+    Hk, K = rows[lead:]
+    Hv, V = heads[lead:]
+    if not (Hk and Hv and V and 0 < K <= 128) or Hv % Hk:
+        _sizes(Hk, Hv, K, V)
+    return (*rows[:lead], Hk, Hv, K, V), DTYPES[dtype], g, beta
+
+
+def _sizes(Hk, Hv, K, V):
+    if not (Hk and Hv and K and V) or Hv % Hk:
+        raise ValueError(f"v's heads must be a multiple of q's, all sizes positive: Hk = {Hk}, "
+                         f"Hv = {Hv}, K = {K}, V = {V}")
+    if K > 128:
+        raise ValueError(f"K = {K}: the key dimension may be at most 128")
+
+
+def _explain(q, k, v, g, beta, lead):
+    """Raises what is wrong with the operands; returns g and beta as float32 if
+    it was their dtype alone."""
     for t, w in ((q, "q"), (k, "k"), (v, "v"), (g, "g"), (beta, "beta")):
         need_gpu(t, w)
     if q.dim() != lead + 2 or v.dim() != lead + 2:
         names = "[B, L, Hk, K] and v [B, L, Hv, V]" if lead == 2 else "[S, Hk, K] and v [S, Hv, V]"
         raise ValueError(f"expected q, k {names}")
     rows, (Hk, K), (Hv, V), dev = q.shape[:lead], q.shape[lead:], v.shape[lead:], q.get_device()
-    if Hk == 0 or Hv == 0 or K == 0 or V == 0 or Hv % Hk:
-        raise ValueError(f"v's heads must be a multiple of q's, all sizes positive: Hk = {Hk}, "
-                         f"Hv = {Hv}, K = {K}, V = {V}")
-    if K > 128:
-        raise ValueError(f"K = {K}: the key dimension may be at most 128")
-    code = dcode(q, "q")
+    _sizes(Hk, Hv, K, V)
+    dcode(q, "q")
     _check(k, "k", q.shape, q.dtype, dev)
     _check(v, "v", rows + (Hv, V), q.dtype, dev)
     g, beta = as_f32(g, "g"), as_f32(beta, "beta")
-    _check(g, "g", rows + (Hv,), torch.float32, dev)
-    _check(beta, "beta", rows + (Hv,), torch.float32, dev)
-    return (*rows, Hk, Hv, K, V), code, g, beta
+    _check(g, "g", rows + (Hv,), _F32, dev)
+    _check(beta, "beta", rows + (Hv,), _F32, dev)
+    return g, beta
 
 
 def _steps(t):
@@ -74,9 +105,27 @@ def _state(t, what, shape, device):
     if t is None:
         return None
     need_gpu(t, what)
-    t = as_f32(t, what).contiguous()
-    _check(t, what, shape, torch.float32, device)
+    if t.dtype != _F32 or not t.is_contiguous():
+        t = as_f32(t, what).contiguous()
+    _check(t, what, shape, _F32, device)
     return t
+
+
+def _out(out, v):
+    """``out`` checked, or a new one like v."""
+    if out is None:
+        return torch.empty_like(v, memory_format=torch.contiguous_format)
+    _check(out, "out", v.shape, v.dtype, v.get_device())
+    return out
+
+
+def _workspace(q, nbytes):
+    """(address, size, stream handle); short sequences need none."""
+    stream = stream_handle(q)
+    if nbytes <= 0:
+        return None, 0, stream
+    ws = workspace.get(q.device, stream, nbytes, workspace.SSD)
+    return ws.data_ptr(), ws.numel(), stream
 
 
 def gated_delta_forward(q, k, v, g, beta, *, scale=None, h0=None, return_state=False, out=None):
@@ -98,19 +147,19 @@ def gated_delta_forward(q, k, v, g, beta, *, scale=None, h0=None, return_state=F
     (B, L, Hk, Hv, K, V), code, g, beta = _operands(q, k, v, g, beta, 2)
     q, k, v = _steps(q), _steps(k), _steps(v)
     h0 = _state(h0, "h0", (B, Hv, K, V), q.get_device())
-    o = torch.empty(v.shape, device=v.device, dtype=v.dtype) if out is None else out
-    _check(o, "out", v.shape, v.dtype, q.get_device())
-    h_last = torch.empty(B, Hv, K, V, device=v.device, dtype=torch.float32) \
-        if return_state else None
+    o = _out(out, v)
+    h_last = None
+    if return_state:
+        h_last = torch.empty(B, Hv, K, V, device=v.device, dtype=_F32) if h0 is None else \
+            torch.empty_like(h0)
     if B:
-        stream = stream_handle(q)
-        ws = workspace.get(q.device, stream, _lib.lib().tssm_gated_delta_workspace_bytes(
-            B, L, Hk, Hv, K, V), workspace.SSD)
+        ws, nbytes, stream = _workspace(q, _lib.lib().tssm_gated_delta_workspace_bytes(
+            B, L, Hk, Hv, K, V))
         _lib.call("tssm_gated_delta_forward", code, q.data_ptr(), k.data_ptr(), v.data_ptr(),
                   g.data_ptr(), beta.data_ptr(), ptr(h0), o.data_ptr(), ptr(h_last), B, L, Hk,
                   Hv, K, V, *_rows(q, "q"), *_rows(k, "k"), *_rows(v, "v"), *g.stride(),
                   *beta.stride(), *_rows(o, "out"), K ** -0.5 if scale is None else float(scale),
-                  ws.data_ptr(), ws.numel(), stream)
+                  ws, nbytes, stream)
     return (o, h_last) if return_state else o
 
 
@@ -137,15 +186,14 @@ def gated_delta_backward(q, k, v, g, beta, do, *, scale=None, h0=None, dh_last=N
     dg, dbeta = torch.empty(2, B, L, Hv, device=q.device, dtype=torch.float32)
     dh0 = None if h0 is None else torch.empty(B, Hv, K, V, device=q.device, dtype=torch.float32)
     if B and L:
-        stream = stream_handle(q)
-        ws = workspace.get(q.device, stream, _lib.lib().tssm_gated_delta_backward_workspace_bytes(
-            B, L, Hk, Hv, K, V), workspace.SSD)
+        ws, nbytes, stream = _workspace(q, _lib.lib().tssm_gated_delta_backward_workspace_bytes(
+            B, L, Hk, Hv, K, V))
         _lib.call("tssm_gated_delta_backward", code, q.data_ptr(), k.data_ptr(), v.data_ptr(),
                   g.data_ptr(), beta.data_ptr(), ptr(h0), do.data_ptr(), ptr(dh_last),
                   dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dg.data_ptr(), dbeta.data_ptr(),
                   ptr(dh0), B, L, Hk, Hv, K, V, *_rows(q, "q"), *_rows(k, "k"), *_rows(v, "v"),
                   *g.stride(), *beta.stride(), *_rows(do, "do"),
-                  K ** -0.5 if scale is None else float(scale), ws.data_ptr(), ws.numel(), stream)
+                  K ** -0.5 if scale is None else float(scale), ws, nbytes, stream)
     elif dh0 is not None:
         dh0.zero_() if dh_last is None else dh0.copy_(dh_last)
     return dq, dk, dv, dg, dbeta, dh0
@@ -163,8 +211,7 @@ def gated_delta_step(q, k, v, g, beta, state, *, scale=None, out=None):
     _check(state, "state", (S, Hv, K, V), torch.float32, q.get_device())
     if not state.is_contiguous():
         raise ValueError("state must be contiguous")
-    o = torch.empty(v.shape, device=v.device, dtype=v.dtype) if out is None else out
-    _check(o, "out", v.shape, v.dtype, q.get_device())
+    o = _out(out, v)
     if S:
         _lib.call("tssm_gated_delta_step", code, q.data_ptr(), k.data_ptr(), v.data_ptr(),
                   g.data_ptr(), beta.data_ptr(), state.data_ptr(), o.data_ptr(), S, Hk, Hv, K, V,

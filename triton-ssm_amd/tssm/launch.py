@@ -72,12 +72,12 @@ def normalize_grid(g) -> tuple[int, int, int]:
 
 
 # ------------------------------------------------------------------ tensors
-_DCODE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 
 
 def dcode(t: torch.Tensor, what: str = "tensor") -> int:
     try:
-        return _DCODE[t.dtype]
+        return DTYPES[t.dtype]
     except KeyError:
         raise TypeError(f"{what}: unsupported dtype {t.dtype} (float32/bfloat16/float16)") from None
 
