@@ -21,6 +21,16 @@ struct DeltaArgs {
   float scale;
 };
 
+// Batch, value head and key head of one of the B Hv heads, which are fewer than
+// 2^32 (a 64-bit division is some 150 instructions, and kernels begin with it).
+struct HeadOf {
+  int64_t b, h, hk;
+};
+__device__ inline HeadOf head_of(const DeltaArgs& a, uint32_t bh) {
+  const uint32_t Hv = (uint32_t)a.Hv, b = bh / Hv, h = bh - b * Hv;
+  return {b, h, h / (Hv / (uint32_t)a.Hk)};
+}
+
 // delta_seq.hip: one step after another, the state in registers.
 int delta_seq_launch(int dtype, const DeltaArgs& a, hipStream_t s);
 

@@ -35,7 +35,6 @@ struct Back {
   static constexpr int kThreads = 64 * (NCW + 4);
   static constexpr int kLd = KP + 8;
   static constexpr int kNk = kC * KP / 8 / NT;
-  static constexpr int kTp = 3 * kC * kC / 8;
   static constexpr int kVp = 2 * NCW;
   static constexpr int kVld = NP == 1 ? 16 * NCW + 8 : 16 * NCW + 4;
   static constexpr bool kEarly = NP * KP <= 128;
@@ -271,7 +270,7 @@ __device__ inline void back_bring(const BackArgs& g, typename Back<T, KP, VEC, N
   const DeltaArgs& a = g.a;
   const ChunkWs* ws = g.ws + bh * (int64_t)g.nch;
   const int id = threadIdx.x - (W::kThreads - NT);
-  const int64_t b = bh / a.Hv, h = bh - b * a.Hv, hk = h / (a.Hv / a.Hk);
+  const auto [b, h, hk] = head_of(a, (uint32_t)bh);
   const int nv = a.V - v0 < 16 * NCW ? (int)(a.V - v0) : 16 * NCW, K = (int)a.K;
   ChunkRows rk, rq, rv;
   rk.init(reinterpret_cast<const T*>(a.k) + b * a.k_b + hk * a.k_h, a.k_l, K, a.L);
@@ -302,8 +301,8 @@ __device__ inline void back_bring(const BackArgs& g, typename Back<T, KP, VEC, N
     r.v.load(dv, ov);
 #pragma unroll
     for (int i = 0; i < 3; ++i)
-      r.t[i] = __builtin_amdgcn_raw_buffer_load_b128(dw, 16 * (id + NT * i), 0, 0);
-    r.f = __builtin_amdgcn_raw_buffer_load_b64(dw, 16 * W::kTp + 8 * id, 0, 0);
+      r.t[i] = __builtin_amdgcn_raw_buffer_load_b128(dw, t_at(i, id), 0, 0);
+    r.f = __builtin_amdgcn_raw_buffer_load_b64(dw, 3 * kPlane + 8 * id, 0, 0);
   };
   auto store = [&](const Regs& r, int n) {
     typename W::Operands& B = lds.op[n & 1];
@@ -358,11 +357,11 @@ __device__ inline void back_body(const BackArgs& g, char* raw, uint32_t block) {
   typedef Back<T, KP, VEC, NCW> W;
   typename W::Lds& lds = *reinterpret_cast<typename W::Lds*>(raw);
   const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const int64_t heads = g.a.B * g.a.Hv, runs = heads * (ZERO ? g.nseg - 1 : g.nseg);
-  const int64_t run = (int64_t)(block / (8 * g.nvb)) * 8 + (block & 7);
-  if (run >= runs) return;
-  const int64_t bh = run % heads;
+  const uint32_t heads = (uint32_t)(g.a.B * g.a.Hv);
+  const uint32_t run = block / (8 * g.nvb) * 8 + (block & 7);
   const int seg = (int)(run / heads) + (ZERO ? 1 : 0);
+  if (seg >= g.nseg) return;
+  const int64_t bh = run % heads;
   const int n0 = seg * g.per, n1 = n0 + g.per < g.nch ? n0 + g.per : g.nch;
   const int64_t v0 = (int64_t)(block / 8 % g.nvb) * 16 * NCW;
   if (wv < NCW)

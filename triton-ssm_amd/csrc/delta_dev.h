@@ -204,10 +204,22 @@ __device__ inline u32x4 lds_col16(const uint16_t* m, int ld, int col, int lane) 
 // With G the sums of g within the chunk:
 //   fac: e^{G_t}, beta_t, e^{G_last - G_t}, g_t, and G_t log2(e) in two parts
 enum { kEg, kBeta, kEnd, kG, kGhi, kGlo, kFac = 8 };
+//   T: planes of (I + A)^-1, which is 0 above the diagonal: rows 16 to 31, then
+//   the left half of rows 0 to 15
 struct ChunkWs {
-  uint16_t T[3][kC][kC];    // planes of (I + A)^-1
+  struct {
+    uint16_t below[16][32], first[16][16];
+  } T[3];
   float fac[kFac][kC];
 };
+constexpr int kPlane = 16 * 48 * 2;  // bytes of a plane of T
+
+// The offset in ChunkWs of 8 elements of a plane from row id / 4, column
+// 8 (id % 4) on, or one past the end, where zeros are read.
+__device__ inline uint32_t t_at(int plane, int id) {
+  const int at = id >= 64 ? 16 * (id - 64) : 1024 + 16 * (id >> 2) * 2 + 16 * (id & 1);
+  return id < 64 && (id & 2) ? kPast : plane * kPlane + at;
+}
 
 __device__ inline const ChunkWs* chunk_at(const ChunkWs* ws, int n, int nch) {
   return ws + (n < 0 ? 0 : (n < nch ? n : nch - 1));

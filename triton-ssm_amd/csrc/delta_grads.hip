@@ -91,10 +91,12 @@ __global__ __launch_bounds__(256, (Grad<T, KP, VEC>::kWaves)) void delta_grads_k
   const DeltaArgs& a = g.a;
   const int tid = threadIdx.x, lane = tid & 63, j = lane >> 4, c = lane & 15;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6), tx = w >> 1, ty = w & 1;
-  const int K = (int)a.K, per = ONE ? 1 : (int)(a.Hv / a.Hk);
+  const uint32_t heads = (uint32_t)a.Hk;  // of the keys
+  const int K = (int)a.K, per = ONE ? 1 : (int)((uint32_t)a.Hv / heads);
   const int64_t Vp = (a.V + 15) / 16 * 16;
   // the chunks of one head follow each other
-  const int64_t n = blockIdx.x % g.nch, bk = blockIdx.x / g.nch, b = bk / a.Hk, hk = bk - b * a.Hk;
+  const uint32_t bk = blockIdx.x / (uint32_t)g.nch;
+  const int64_t n = blockIdx.x - bk * (uint32_t)g.nch, b = bk / heads, hk = bk % heads;
   const int64_t t0 = n * kC;
   const int rows = a.L - t0 < kC ? (int)(a.L - t0) : kC;
 
@@ -162,10 +164,11 @@ __global__ __launch_bounds__(256, (Grad<T, KP, VEC>::kWaves)) void delta_grads_k
         *reinterpret_cast<u32x4*>(&lds.D[m][sr * W::kVld + scol]) = p[m];
     };
     {
-      const u32x4* tp = reinterpret_cast<const u32x4*>(g.ws + unit);
+      const auto wp = rsrc_of(g.ws + unit, (int)sizeof(ChunkWs));
       u32x4 t[2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) t[i] = tp[tid + 256 * i < 384 ? tid + 256 * i : 0];
+      for (int i = 0; i < 2; ++i)
+        t[i] = __builtin_amdgcn_raw_buffer_load_b128(wp, t_at(2 * i + tid / 128, tid % 128), 0, 0);
       const float f = (&g.ws[unit].fac[0][0])[tid];
       slice(0);
       __syncthreads();

@@ -22,39 +22,39 @@ __device__ inline void wave_order() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// Row lane / 2, columns 16 (lane & 1) .. + 15 of an fp32 matrix into planes.
-template <int NP>
-__device__ inline void put_planes(const float* m, uint16_t (*out)[kC][kC], int lane) {
-  const int r = lane >> 1, c = 16 * (lane & 1);
-#pragma unroll
-  for (int x = 0; x < 2; ++x) {
+// T into planes, a KiB of one after the other at a time.
+__device__ inline void put_planes(const float* m, ChunkWs& out, int lane) {
+  auto put = [&](int row, int col, auto dst) {
     float v[8];
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-      const float4 f = *reinterpret_cast<const float4*>(m + r * kLd + c + 8 * x + 4 * q);
+      const float4 f = *reinterpret_cast<const float4*>(m + row * kLd + col + 4 * q);
       v[4 * q] = f.x; v[4 * q + 1] = f.y; v[4 * q + 2] = f.z; v[4 * q + 3] = f.w;
     }
-    u32x4 p[NP];
-    split8<NP>(v, p);
+    u32x4 p[3];
+    split8<3>(v, p);
 #pragma unroll
-    for (int n = 0; n < NP; ++n) *reinterpret_cast<u32x4*>(&out[n][r][c + 8 * x]) = p[n];
-  }
+    for (int n = 0; n < 3; ++n) *reinterpret_cast<u32x4*>(dst(n)) = p[n];
+  };
+  const int r4 = lane >> 2, c4 = 8 * (lane & 3), r2 = lane >> 1, c2 = 8 * (lane & 1);
+  put(16 + r4, c4, [&](int n) { return &out.T[n].below[r4][c4]; });
+  if (lane < 32) put(r2, c2, [&](int n) { return &out.T[n].first[r2][c2]; });
 }
 
 template <typename T, int KP, bool VEC>
-__global__ __launch_bounds__(256) void delta_prep_kernel(DeltaArgs a, ChunkWs* ws, int64_t nch,
-                                                         int64_t units) {
+__global__ __launch_bounds__(256) void delta_prep_kernel(DeltaArgs a, ChunkWs* ws, uint32_t nch,
+                                                         uint32_t units) {
   constexpr int NP = Piece<T, VEC>::NP;
   __shared__ __attribute__((aligned(16))) float mat[4][2][kC * kLd];
-  __shared__ double sums[4][kC];
-  __shared__ float bet[4][kC];
+  __shared__ __attribute__((aligned(16))) float sums[4][2][kC], bet[4][kC];  // G log2(e) in two parts, beta
   const int lane = threadIdx.x & 63, j = lane >> 4, c = lane & 15;
   const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const int64_t unit = (int64_t)blockIdx.x * 4 + wv;
+  const uint32_t unit = blockIdx.x * 4 + wv;
   if (unit >= units) return;
   // units run over the value heads of one chunk first: a group shares its keys
-  const int64_t bn = unit / a.Hv, h = unit - bn * a.Hv, b = bn / nch, n = bn - b * nch;
-  const int64_t hk = h / (a.Hv / a.Hk), t0 = n * kC;
+  const uint32_t Hv = (uint32_t)a.Hv, bn = unit / Hv, nth = bn / nch;
+  const int64_t n = bn - nth * nch, t0 = n * kC;
+  const auto [b, h, hk] = head_of(a, nth * Hv + (unit - bn * Hv));
   const int rows = a.L - t0 < kC ? (int)(a.L - t0) : kC;
   ChunkWs& out = ws[(b * a.Hv + h) * nch + n];
   float *mA = mat[wv][0], *mT = mat[wv][1];
@@ -74,15 +74,17 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(DeltaArgs a, ChunkWs* w
   }
   const double Gl = __shfl(G, 31, 32);
   if (lane < kC) {
-    sums[wv][t] = G;
+    const double log2e = 1.4426950408889634074, G2 = G * log2e;
+    const float hi = (float)G2, lo = (float)(G2 - (double)hi);
+    sums[wv][0][t] = hi;
+    sums[wv][1][t] = lo;
     bet[wv][t] = beta;
-    out.fac[kEg][t] = exp_acc((float)G);
+    out.fac[kEg][t] = exp2_fast(hi);
     out.fac[kBeta][t] = beta;
-    out.fac[kEnd][t] = exp_acc((float)(Gl - G));
+    out.fac[kEnd][t] = exp2_fast((float)((Gl - G) * log2e));
     out.fac[kG][t] = on ? g0 : 0.0f;
-    const double G2 = G * 1.4426950408889634074;
-    out.fac[kGhi][t] = (float)G2;
-    out.fac[kGlo][t] = (float)(G2 - (double)(float)G2);
+    out.fac[kGhi][t] = hi;
+    out.fac[kGlo][t] = lo;
   }
 
   // Gram product: tiles (0,0), (1,0), (1,1)
@@ -110,16 +112,17 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(DeltaArgs a, ChunkWs* w
 #pragma unroll
   for (int x = 0; x < 3; ++x) {
     const int i = 16 * (x > 1) + c;
-    const double Gi = sums[wv][i];
+    const float hi = sums[wv][0][i], lo = sums[wv][1][i];
+    const int at = 16 * (x > 0) + 4 * j;
+    const float4 h4 = *reinterpret_cast<const float4*>(&sums[wv][0][at]);
+    const float4 l4 = *reinterpret_cast<const float4*>(&sums[wv][1][at]);
+    const float4 b4 = *reinterpret_cast<const float4*>(&bet[wv][at]);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int row = 16 * (x > 0) + 4 * j + r;
-      const float d = exp_acc((float)(sums[wv][row] - Gi));
-      mA[row * kLd + i] = i < row ? bet[wv][row] * d * kk[x][r] : 0.0f;
+      const float d = exp2_fast(((&h4.x)[r] - hi) + ((&l4.x)[r] - lo));
+      mA[(at + r) * kLd + i] = i < at + r ? (&b4.x)[r] * d * kk[x][r] : 0.0f;
     }
   }
-#pragma unroll
-  for (int r = 0; r < 4; ++r) mT[(4 * j + r) * kLd + 16 + c] = 0.0f;  // above the diagonal
   wave_order();
   // diagonal blocks: lane (d, c) solves for column c of block d
   {
@@ -162,15 +165,15 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(DeltaArgs a, ChunkWs* w
     for (int r = 0; r < 4; ++r) mT[(16 + 4 * j + r) * kLd + c] = -y[r];
   }
   wave_order();
-  put_planes<3>(mT, out.T, lane);
+  put_planes(mT, out, lane);
 }
 
 template <typename T, int KP>
 void launch(const DeltaArgs& a, bool vec, ChunkWs* ws, hipStream_t s) {
   const int64_t nch = cdiv64(a.L, kC), units = a.B * a.Hv * nch;
   const unsigned wgs = (unsigned)cdiv64(units, 4);
-  if (vec) delta_prep_kernel<T, KP, true><<<wgs, 256, 0, s>>>(a, ws, nch, units);
-  else delta_prep_kernel<T, KP, false><<<wgs, 256, 0, s>>>(a, ws, nch, units);
+  if (vec) delta_prep_kernel<T, KP, true><<<wgs, 256, 0, s>>>(a, ws, (uint32_t)nch, (uint32_t)units);
+  else delta_prep_kernel<T, KP, false><<<wgs, 256, 0, s>>>(a, ws, (uint32_t)nch, (uint32_t)units);
 }
 
 template <typename T>

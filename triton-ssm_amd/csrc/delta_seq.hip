@@ -56,13 +56,15 @@ struct Row {
 };
 
 template <typename T, int CQ, int KR, bool VEC>
-__global__ __launch_bounds__(256) void delta_seq_kernel(DeltaArgs a, uint32_t ncb, int64_t units) {
+__global__ __launch_bounds__(256) void delta_seq_kernel(DeltaArgs a, uint32_t ncb, uint32_t units) {
   const int lane = threadIdx.x & 63, kg = lane / CQ, cq = lane % CQ;
-  const int64_t unit = (int64_t)blockIdx.x * 4 +
-                       __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const uint32_t unit = blockIdx.x * 4 +
+                        __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   if (unit >= units) return;
-  const int64_t bh = unit / ncb, b = bh / a.Hv, h = bh - b * a.Hv, hk = h / (a.Hv / a.Hk);
-  const int K = (int)a.K, k0 = kg * KR, c0 = (int)(unit - bh * ncb) * 4 * CQ + 4 * cq;
+  const uint32_t nth = unit / ncb;
+  const auto [b, h, hk] = head_of(a, nth);
+  const int64_t bh = nth;
+  const int K = (int)a.K, k0 = kg * KR, c0 = (int)(unit - nth * ncb) * 4 * CQ + 4 * cq;
   const int64_t V = a.V;
   const int klim = K - k0 < 0 ? 0 : K - k0, clim = V - c0 > 4 ? 4 : (V - c0 < 0 ? 0 : (int)(V - c0));
   // lanes past K or V read row 0 or column 0 of their head, store nothing
@@ -168,7 +170,7 @@ template <typename T, int CQ>
 int launch(const DeltaArgs& a, hipStream_t s) {
   constexpr int kR = CQ / 4;  // rows of a lane for every 16 of K
   const int64_t ncb = cdiv64(a.V, 4 * CQ), units = a.B * a.Hv * ncb, wgs = cdiv64(units, 4);
-  if (wgs > 0x7fffffff) return TSSM_ERR_UNSUPPORTED;
+  if (units > 0x7fffffff || a.B > 0x7fffffff / a.Hv) return TSSM_ERR_UNSUPPORTED;
   const int E = (int)sizeof(T);
   const int kr = (a.K <= 16 ? 1 : (a.K <= 32 ? 2 : (a.K <= 64 ? 4 : 8))) * kR;
   // every row of every operand starts on the widest access a lane makes
@@ -181,9 +183,9 @@ int launch(const DeltaArgs& a, hipStream_t s) {
       (a.v_b | a.v_l | a.v_h | a.o_b | a.o_l | a.o_h) * E % vb == 0;
 #define TSSM_SEQ(KR)                                                                       \
   if (vec)                                                                                 \
-    delta_seq_kernel<T, CQ, KR, true><<<(unsigned)wgs, 256, 0, s>>>(a, (uint32_t)ncb, units); \
+    delta_seq_kernel<T, CQ, KR, true><<<(unsigned)wgs, 256, 0, s>>>(a, (uint32_t)ncb, (uint32_t)units); \
   else                                                                                     \
-    delta_seq_kernel<T, CQ, KR, false><<<(unsigned)wgs, 256, 0, s>>>(a, (uint32_t)ncb, units)
+    delta_seq_kernel<T, CQ, KR, false><<<(unsigned)wgs, 256, 0, s>>>(a, (uint32_t)ncb, (uint32_t)units)
   if (a.K <= 16) { TSSM_SEQ(kR); }
   else if (a.K <= 32) { TSSM_SEQ(2 * kR); }
   else if (a.K <= 64) { TSSM_SEQ(4 * kR); }

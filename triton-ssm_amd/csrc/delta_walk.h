@@ -52,7 +52,6 @@ struct Walk {
   static constexpr int kThreads = 64 * (NCW + (MODE == kOutputs ? 4 : 2));
   static constexpr int kLd = KP + 8;            // bf16 elements of a row of K or Q in LDS
   static constexpr int kNk = kC * KP / 8 / NT;  // 8-element pieces of K a thread brings
-  static constexpr int kTp = 3 * kC * kC / 8;   // 16-byte pieces of T
   static constexpr int kVp = 2 * NCW;           // pieces of a row of V
   static constexpr int kVld = NP == 1 ? 16 * NCW + 8 : 16 * NCW + 4;  // elements of V's row
   // 256 registers where they suffice: with more to give out the compiler puts
@@ -281,7 +280,7 @@ __device__ inline void bring(const WalkArgs& wa, typename Walk<T, KP, VEC, NCW, 
   const ChunkWs* ws = wa.ws + bh * (int64_t)wa.nch;
   constexpr int NP = W::NP, NT = W::NT, kE = (int)sizeof(T);
   const int id = threadIdx.x - (W::kThreads - NT);
-  const int64_t b = bh / a.Hv, h = bh - b * a.Hv, hk = h / (a.Hv / a.Hk);
+  const auto [b, h, hk] = head_of(a, (uint32_t)bh);
   // columns past V (a transfer's unit vectors) have no input
   const int nv = a.V - v0 < 16 * NCW ? (a.V - v0 < 0 ? 0 : (int)(a.V - v0)) : 16 * NCW;
   const int K = (int)a.K;
@@ -317,8 +316,8 @@ __device__ inline void bring(const WalkArgs& wa, typename Walk<T, KP, VEC, NCW, 
     g.v.load(dv, ov);
 #pragma unroll
     for (int i = 0; i < 3; ++i)
-      g.t[i] = __builtin_amdgcn_raw_buffer_load_b128(dw, 16 * (id + NT * i), 0, 0);
-    g.f = __builtin_amdgcn_raw_buffer_load_b64(dw, 16 * W::kTp + 8 * id, 0, 0);
+      g.t[i] = __builtin_amdgcn_raw_buffer_load_b128(dw, t_at(i, id), 0, 0);
+    g.f = __builtin_amdgcn_raw_buffer_load_b64(dw, 3 * kPlane + 8 * id, 0, 0);
   };
   // Only whole pieces are read with VEC, and what lies past a row or the
   // sequence reads zero; without it a piece may run into what follows its row.
@@ -356,7 +355,7 @@ __device__ inline void bring(const WalkArgs& wa, typename Walk<T, KP, VEC, NCW, 
     }
     *reinterpret_cast<u32x2v*>(&B.fac[0][0] + 2 * id) = g.f;
   };
-  static_assert(W::kTp == 3 * NT && kFac * kC == 2 * NT, "pieces of a chunk");
+  static_assert(kC * kC == 8 * NT && kFac * kC == 2 * NT, "pieces of a chunk");
 
   Regs g0, g1;
   load(g0, n0);
@@ -383,7 +382,7 @@ __device__ inline void outputs(const DeltaArgs& a, typename Walk<T, KP, VEC, NCW
   constexpr int NP = W::NP, NO = W::NO, NS = W::NS, kE = (int)sizeof(T);
   const int lane = threadIdx.x & 63, j = lane >> 4, c = lane & 15;
   const int ar = 8 * (c >> 2) + (c & 3);
-  const int64_t b = bh / a.Hv, h = bh - b * a.Hv;
+  const auto [b, h, hk] = head_of(a, (uint32_t)bh);
   const int nv = a.V - v0 < 16 * NCW ? (int)(a.V - v0) : 16 * NCW;
   ChunkRows ro;
   ro.init(reinterpret_cast<T*>(a.o) + b * a.o_b + h * a.o_h + v0, a.o_l, nv, a.L);
@@ -483,11 +482,11 @@ __device__ inline void walk_body(const WalkArgs& g, char* raw, uint32_t block) {
   typename W::Lds& lds = *reinterpret_cast<typename W::Lds*>(raw);
   const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   // workgroups of one head and segment on one XCD: they share its keys and queries
-  const int64_t runs = g.a.B * g.a.Hv * g.walked;
-  const int64_t run = (int64_t)(block / (8 * g.nvb)) * 8 + (block & 7);
-  if (run >= runs) return;
-  const int64_t bh = run % (g.a.B * g.a.Hv);
-  const int seg = (int)(run / (g.a.B * g.a.Hv));
+  const uint32_t heads = (uint32_t)(g.a.B * g.a.Hv);
+  const uint32_t run = block / (8 * g.nvb) * 8 + (block & 7);
+  const int seg = (int)(run / heads);
+  if (seg >= g.walked) return;
+  const int64_t bh = run - seg * heads;
   const int n0 = seg * g.per, n1 = n0 + g.per < g.nch ? n0 + g.per : g.nch;
   const int64_t v0 = (int64_t)(block / 8 % g.nvb) * 16 * NCW;
   if (wv < NCW)
