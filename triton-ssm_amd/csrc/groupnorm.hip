@@ -298,7 +298,8 @@ __global__ __launch_bounds__(256) void gn_row_fwd(GnArgs a, int gw, uint32_t ngb
 // dw and db of the workgroup's rows go to ws[row block][2][C].
 template <typename T, int VW, int LG, int NV>
 __global__ __launch_bounds__(256) void gn_row_bwd(GnArgs a, int gw, uint32_t ngb, uint32_t nrb) {
-  __shared__ float red[256][VW + 1];
+  constexpr int kB = NV > 1 ? 4 : 2;  // sums of VW channels that meet at once
+  __shared__ float red[kB][256][VW + 1];
   const RowMap<LG> m(a, gw, blockIdx.x % ngb);
   const uint32_t rb = blockIdx.x / ngb;
   const int l = threadIdx.x % LG;
@@ -378,25 +379,37 @@ __global__ __launch_bounds__(256) void gn_row_bwd(GnArgs a, int gw, uint32_t ngb
     load(q0, base + 2 * hop + m.row);
     if (base + hop < a.N) row(q1, base + hop + m.row);
   }
-  float* part = a.ws + (int64_t)rb * 2 * a.G * a.Cg;
-  const int t = threadIdx.x, lanes = gw * LG;  // distinct (group, place) pairs
+  // sum i of w or b, 2 i or 2 i + 1, is one wave's of kB: a workgroup's lanes
+  // that hold the same (group, place) are `lanes` <= 64 apart
+  const int t = threadIdx.x, lanes = gw * LG, mine = t >> 6;
+  const int64_t C = a.G * a.Cg;
+  const bool head = mine < kB && (t & 63) < lanes;
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+  for (int q = 0; q < 2 * NV; q += kB) {
+    if (q) __syncthreads();
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      __syncthreads();
+    for (int k = 0; k < kB; ++k)
 #pragma unroll
-      for (int v = 0; v < VW; ++v) red[t][v] = k ? sb[i][v] : sw[i][v];
-      __syncthreads();
-      if (t < lanes && in[i]) {
+      for (int v = 0; v < VW; ++v)
+        red[k][t][v] = k & 1 ? sb[(q + k) / 2][v] : sw[(q + k) / 2][v];
+    __syncthreads();
+    const int64_t c = (int64_t)((q + mine) / 2 * LG + l) * VW;
+    if (head && on && c < a.Cg) {
+      float x[VW] = {};
+      for (int p = t & 63; p < 256; p += lanes)
 #pragma unroll
-        for (int v = 0; v < VW; ++v) {
-          float s = 0.0f;
-          for (int p = t; p < 256; p += lanes) s += red[p][v];
-          part[k * a.G * a.Cg + ch[i] + v] = s;
-        }
+        for (int v = 0; v < VW; ++v) x[v] += red[mine][p][v];
+      float* part = a.ws + (int64_t)rb * 2 * C + (mine & 1) * C + m.g * a.Cg + c;
+      if constexpr (VW % 4 == 0) {
+#pragma unroll
+        for (int v = 0; v < VW; v += 4)
+          *reinterpret_cast<float4*>(part + v) = make_float4(x[v], x[v + 1], x[v + 2], x[v + 3]);
+      } else {
+#pragma unroll
+        for (int v = 0; v < VW; ++v) part[v] = x[v];
       }
     }
+  }
 }
 
 // out0, out1 [C] = sums of ws [np][2][C] over np, in a fixed order; for every
@@ -407,23 +420,23 @@ __global__ __launch_bounds__(256) void gn_sum_kernel(const float* ws, float* out
   const int c = threadIdx.x & 15, p = threadIdx.x >> 4;
   const int64_t i = (int64_t)blockIdx.x * 16 + c;
   ws += (int64_t)blockIdx.y * np * 2 * C;
-  float s0 = 0.0f, s1 = 0.0f;
+  // eight loads in flight: np is in the hundreds and the workgroups few
+  float s[8] = {};
   if (i < 2 * C) {
     int64_t k = p;
-    for (; k + 16 < np; k += 32) {
-      s0 += ws[k * 2 * C + i];
-      s1 += ws[(k + 16) * 2 * C + i];
-    }
-    if (k < np) s0 += ws[k * 2 * C + i];
+    for (; k + 112 < np; k += 128)
+#pragma unroll
+      for (int q = 0; q < 8; ++q) s[q] += ws[(k + 16 * q) * 2 * C + i];
+    for (; k < np; k += 16) s[0] += ws[k * 2 * C + i];
   }
-  red[p][c] = s0 + s1;
+  red[p][c] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
   __syncthreads();
   if (p == 0 && i < 2 * C) {
-    float s = 0.0f;
+    float all = 0.0f;
 #pragma unroll
-    for (int k = 0; k < 16; ++k) s += red[k][c];
-    if (i < C) out0[blockIdx.y * out_step + i] = s;
-    else out1[blockIdx.y * out_step + i - C] = s;
+    for (int k = 0; k < 16; ++k) all += red[k][c];
+    if (i < C) out0[blockIdx.y * out_step + i] = all;
+    else out1[blockIdx.y * out_step + i - C] = all;
   }
 }
 
@@ -782,9 +795,11 @@ inline bool row_fits(int64_t S, int64_t Cg, int vw) {
 inline bool series_fits(int64_t C, int64_t G, int vw) {
   return cdiv64(C, vw) <= 1024 && G <= 2048;
 }
-// Row blocks of the rows' backward: about 1024 workgroups.
+// Row blocks of the rows' backward: two workgroups on each CU, with two rows of
+// every lane in flight (N = 8192 and 32768 of 16 x 64 channels, gated, bf16: 27
+// and 64 us; with four 32 and 74, with one 29 and 81).
 inline int64_t row_blocks(int64_t N, int64_t step, int64_t ngb) {
-  const int64_t all = cdiv64(N, step), want = cdiv64(1024, ngb);
+  const int64_t all = cdiv64(N, step), want = cdiv64(512, ngb);
   return all < want ? all : want;
 }
 struct RowPlan {
