@@ -15,6 +15,9 @@
 // Two barriers a chunk: before the first the loaders put the next chunk into
 // LDS while the chain waves multiply K G', after it the helpers work on that
 // chunk.
+// Bound like the walk by the chain waves' instructions.  B=4 L=4096 H=16 K=V=64
+// bf16, 256 workgroups of both kinds: 190 us in one launch, which also writes 268
+// MB of states and gradients; one after the other 124 and 185.
 #include "delta_walk.h"
 
 namespace tssm {
