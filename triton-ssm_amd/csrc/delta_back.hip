@@ -34,10 +34,10 @@ struct BackArgs {
 
 template <typename T, int KP, bool VEC, int NCW>
 struct Back {
-  static constexpr int NP = Piece<T, VEC>::NP, NS = KP / 32, NT = 128;
-  static constexpr int kThreads = 64 * (NCW + 4);
+  static constexpr int NP = Piece<T, VEC>::NP, NS = KP / 32, NT = NP == 1 ? 128 : 256;
+  static constexpr int kThreads = 64 * (NCW + 2) + NT;
   static constexpr int kLd = KP + 8;
-  static constexpr int kNk = kC * KP / 8 / NT;
+  static constexpr int kNk = (kC * KP / 8 + NT - 1) / NT;
   static constexpr int kVp = 2 * NCW;
   static constexpr int kVld = NP == 1 ? 16 * NCW + 8 : 16 * NCW + 4;
   static constexpr bool kEarly = NP * KP <= 128;
@@ -283,10 +283,11 @@ __device__ inline void back_bring(const BackArgs& g, typename Back<T, KP, VEC, N
 #pragma unroll
   for (int i = 0; i < W::kNk; ++i) {
     const int r = (id + NT * i) / (KP / 8), col = (id + NT * i) % (KP / 8) * 8;
-    ok[i] = col < K ? r * rk.row + col * kE : kPast;
-    oq[i] = col < K ? r * rq.row + col * kE : kPast;
+    ok[i] = r < kC && col < K ? r * rk.row + col * kE : kPast;
+    oq[i] = r < kC && col < K ? r * rq.row + col * kE : kPast;
   }
-  const int vr = id / W::kVp, vcol = id % W::kVp * 8;
+  const uint32_t vid = id - (NT - 128);
+  const int vr = (int)(vid / W::kVp), vcol = (int)(vid % W::kVp) * 8;
   const uint32_t ov = vr < kC && vcol < nv ? vr * rv.row + vcol * kE : kPast;
   struct Regs {
     Piece<T, VEC> k[W::kNk], q[W::kNk], v;
@@ -304,8 +305,8 @@ __device__ inline void back_bring(const BackArgs& g, typename Back<T, KP, VEC, N
     r.v.load(dv, ov);
 #pragma unroll
     for (int i = 0; i < 3; ++i)
-      r.t[i] = __builtin_amdgcn_raw_buffer_load_b128(dw, t_at(i, id), 0, 0);
-    r.f = __builtin_amdgcn_raw_buffer_load_b64(dw, 3 * kPlane + 8 * id, 0, 0);
+      r.t[i] = __builtin_amdgcn_raw_buffer_load_b128(dw, id < 128 ? t_at(i, id) : kPast, 0, 0);
+    r.f = __builtin_amdgcn_raw_buffer_load_b64(dw, 3 * kPlane + 8 * (id & 127), 0, 0);
   };
   auto store = [&](const Regs& r, int n) {
     typename W::Operands& B = lds.op[n & 1];
@@ -313,6 +314,7 @@ __device__ inline void back_bring(const BackArgs& g, typename Back<T, KP, VEC, N
 #pragma unroll
     for (int i = 0; i < W::kNk; ++i) {
       const int row = (id + NT * i) / (KP / 8), col = (id + NT * i) % (KP / 8) * 8;
+      if (kC * KP / 8 < NT && row >= kC) continue;
       const int lim = VEC ? 8 : K - col;
       r.k[i].planes(lim, p);
 #pragma unroll
@@ -332,10 +334,13 @@ __device__ inline void back_bring(const BackArgs& g, typename Back<T, KP, VEC, N
           B.D[vr * W::kVld + vcol + e] = e < lim ? ldf(&r.v.e[e]) : 0.0f;
       }
     }
+    if (NT == 128 || id < 128) {
 #pragma unroll
-    for (int i = 0; i < 3; ++i)
-      *reinterpret_cast<u32x4*>(&B.M[i][id / 4 * kTld + id % 4 * 8]) = r.t[i];
-    *reinterpret_cast<u32x2v*>(&B.fac[0][0] + 2 * id) = r.f;
+      for (int i = 0; i < 3; ++i)
+        *reinterpret_cast<u32x4*>(&B.M[i][id / 4 * kTld + id % 4 * 8]) = r.t[i];
+    }
+    if (NT == 128 || id >= 128)
+      *reinterpret_cast<u32x2v*>(&B.fac[0][0] + 2 * (id & 127)) = r.f;
   };
   Regs g0, g1;
   load(g0, n1 - 1);

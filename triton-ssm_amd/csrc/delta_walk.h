@@ -57,10 +57,13 @@ template <typename T, int KP, bool VEC, int NCW, int MODE>
 struct Walk {
   static constexpr int NP = Piece<T, VEC>::NP;  // planes of the inputs
   static constexpr int NO = NP == 1 ? 2 : 3;    // of S, P and U in the outputs' products
-  static constexpr int NS = KP / 32, NT = 128;  // threads of the loaders
-  static constexpr int kThreads = 64 * (NCW + (MODE == kOutputs ? 4 : 2));
+  static constexpr int NS = KP / 32;
+  // threads of the loaders: those of fp32 and fp16 split what they bring (B=3 L=1111
+  // 12 heads of 40 x 72: 57.4 us with 128, 55.7 with 256)
+  static constexpr int NT = NP == 1 ? 128 : 256;
+  static constexpr int kThreads = 64 * (NCW + (MODE == kOutputs ? 2 : 0)) + NT;
   static constexpr int kLd = KP + 8;            // bf16 elements of a row of K or Q in LDS
-  static constexpr int kNk = kC * KP / 8 / NT;  // 8-element pieces of K a thread brings
+  static constexpr int kNk = (kC * KP / 8 + NT - 1) / NT;  // 8-element pieces of K a thread brings
   static constexpr int kVp = 2 * NCW;           // pieces of a row of V
   static constexpr int kVld = NP == 1 ? 16 * NCW + 8 : 16 * NCW + 4;  // elements of V's row
   // 256 registers where they suffice: with more to give out the compiler puts
@@ -302,10 +305,12 @@ __device__ inline void bring(const WalkArgs& wa, typename Walk<T, KP, VEC, NCW, 
 #pragma unroll
   for (int i = 0; i < W::kNk; ++i) {
     const int r = (id + NT * i) / (KP / 8), col = (id + NT * i) % (KP / 8) * 8;
-    ok[i] = col < K ? r * rk.row + col * kE : kPast;
-    oq[i] = col < K ? r * rq.row + col * kE : kPast;
+    ok[i] = r < kC && col < K ? r * rk.row + col * kE : kPast;
+    oq[i] = r < kC && col < K ? r * rq.row + col * kE : kPast;
   }
-  const int vr = id / W::kVp, vcol = id % W::kVp * 8;   // this thread's piece of V
+  // this thread's piece of V: with 256 the first half brings T, the second V
+  const uint32_t vid = id - (NT - 128);
+  const int vr = (int)(vid / W::kVp), vcol = (int)(vid % W::kVp) * 8;
   const uint32_t ov = vr < kC && vcol < nv ? vr * rv.row + vcol * kE : kPast;
 
   // as they lie in memory: a conversion on the way would wait for the load
@@ -325,8 +330,8 @@ __device__ inline void bring(const WalkArgs& wa, typename Walk<T, KP, VEC, NCW, 
     g.v.load(dv, ov);
 #pragma unroll
     for (int i = 0; i < 3; ++i)
-      g.t[i] = __builtin_amdgcn_raw_buffer_load_b128(dw, t_at(i, id), 0, 0);
-    g.f = __builtin_amdgcn_raw_buffer_load_b64(dw, 3 * kPlane + 8 * id, 0, 0);
+      g.t[i] = __builtin_amdgcn_raw_buffer_load_b128(dw, id < 128 ? t_at(i, id) : kPast, 0, 0);
+    g.f = __builtin_amdgcn_raw_buffer_load_b64(dw, 3 * kPlane + 8 * (id & 127), 0, 0);
   };
   // Only whole pieces are read with VEC, and what lies past a row or the
   // sequence reads zero; without it a piece may run into what follows its row.
@@ -336,6 +341,7 @@ __device__ inline void bring(const WalkArgs& wa, typename Walk<T, KP, VEC, NCW, 
 #pragma unroll
     for (int i = 0; i < W::kNk; ++i) {
       const int r = (id + NT * i) / (KP / 8), col = (id + NT * i) % (KP / 8) * 8;
+      if (kC * KP / 8 < NT && r >= kC) continue;
       const int lim = VEC ? 8 : K - col;
       g.k[i].planes(lim, p);
 #pragma unroll
@@ -357,14 +363,15 @@ __device__ inline void bring(const WalkArgs& wa, typename Walk<T, KP, VEC, NCW, 
           B.V[vr * W::kVld + vcol + e] = e < lim ? ldf(&g.v.e[e]) : 0.0f;
       }
     }
+    if (NT == 128 || id < 128) {
 #pragma unroll
-    for (int i = 0; i < 3; ++i) {
-      const int r = id / 4, col = id % 4 * 8;  // NT pieces are one plane
-      *reinterpret_cast<u32x4*>(&B.M[i][r * kTld + col]) = g.t[i];
+      for (int i = 0; i < 3; ++i)  // 128 pieces are one plane
+        *reinterpret_cast<u32x4*>(&B.M[i][id / 4 * kTld + id % 4 * 8]) = g.t[i];
     }
-    *reinterpret_cast<u32x2v*>(&B.fac[0][0] + 2 * id) = g.f;
+    if (NT == 128 || id >= 128)
+      *reinterpret_cast<u32x2v*>(&B.fac[0][0] + 2 * (id & 127)) = g.f;
   };
-  static_assert(kC * kC == 8 * NT && kFac * kC == 2 * NT, "pieces of a chunk");
+  static_assert(kC * kC == 8 * 128 && kFac * kC == 2 * 128, "pieces of a chunk");
 
   Regs g0, g1;
   load(g0, n0);
