@@ -71,6 +71,19 @@ def test_forward(dev, dtype, B, L, Hk, Hv, K, V):
     assert_close(S, S_ref, TOL[F32], "state")
 
 
+@pytest.mark.parametrize("B,Hv,K,V", [(1, 4, 64, 40), (64, 8, 16, 16), (1, 2, 128, 8),
+                                      (300, 4, 16, 70)])
+@pytest.mark.parametrize("L", [2, 12, 13, 24, 25])
+def test_few_tokens(dev, B, Hv, K, V, L):
+    """Around the lengths where the forward turns from steps to chunks, with few
+    and with many heads, narrow and wide waves."""
+    d = inputs(dev, B, L, Hv // 2, Hv, K, V, BF16, seed=L + V, h0=True)
+    o, S = run(d)
+    o_ref, S_ref = oracle(d)
+    assert_close(o, o_ref, TOL[BF16], "o")
+    assert_close(S, S_ref, TOL[F32], "state")
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_forward_strides(dev, dtype):
     """q, k and v as slices of one projection, heads before steps, a shared g."""

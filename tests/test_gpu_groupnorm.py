@@ -197,3 +197,10 @@ def test_refusals(dev):
 ])
 def test_wide(dev, dtype, N, S, G, C):
     check(inputs(dev, N, S, C, dtype, True, seed=C), G, "silu", dtype)
+
+
+@pytest.mark.parametrize("N,G,C,dtype", [(140000, 1, 8, F32), (9000, 2, 64, BF16),
+                                         (5000, 1, 2048, F16)])
+def test_many_rows(dev, N, G, C, dtype):
+    """More rows than the gradients' workgroups take at once."""
+    check(inputs(dev, N, 1, C, dtype, True, seed=11), G, "silu", dtype)

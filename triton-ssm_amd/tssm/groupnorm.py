@@ -23,9 +23,11 @@ _ACT = {"none": 0, "silu": 1}
 def _view(t, what):
     """t [N, ..., C] as (N, S, C, stride of n, stride of s): the middle
     dimensions must be one run of positions."""
-    if t.dim() < 2:
-        raise ValueError(f"{what} must be [N, ..., C]")
     shape, stride = t.shape, t.stride()
+    if len(shape) == 2 and stride[1] == 1:
+        return shape[0], 1, shape[1], stride[0], shape[1]
+    if len(shape) < 2:
+        raise ValueError(f"{what} must be [N, ..., C]")
     if stride[-1] != 1 and shape[-1] != 1:
         raise ValueError(f"{what}: innermost dimension must be contiguous")
     S, step = 1, None
