@@ -123,6 +123,25 @@ def test_segments(dev, dtype, B, L, Hk, Hv, K, V, rate, h0):
     assert_close(S, S_ref, TOL[F32], "state")
 
 
+@pytest.mark.parametrize("B,L,H,K,V", [(1, 8200, 2, 64, 64), (2, 100, 2, 64, 48), (2, 9, 3, 32, 32)])
+def test_state_in_place(dev, B, L, H, K, V):
+    """The C entry point with one buffer for the state before and after, in
+    segments, in one walk and step by step: the bits of two buffers."""
+    from tssm import _lib
+    d = inputs(dev, B, L, H, H, K, V, BF16, seed=9, h0=True, rate=0.05)
+    o_ref, S_ref = run(d)
+    o, S = torch.empty_like(o_ref), d["h0"].clone()
+    n = _lib.lib().tssm_gated_delta_workspace_bytes(B, L, H, H, K, V)
+    ws = torch.empty(max(n, 1), dtype=torch.uint8, device=dev)
+    t = [d[x] for x in ("q", "k", "v")]
+    _lib.call("tssm_gated_delta_forward", 1, *(x.data_ptr() for x in t), d["g"].data_ptr(),
+              d["beta"].data_ptr(), S.data_ptr(), o.data_ptr(), S.data_ptr(), B, L, H, H, K, V,
+              *(s for x in t for s in x.stride()[:3]), *d["g"].stride(), *d["beta"].stride(),
+              *o.stride()[:3], K ** -0.5, ws.data_ptr() if n else None, n,
+              torch.cuda.current_stream().cuda_stream)
+    assert torch.equal(o, o_ref) and torch.equal(S, S_ref)
+
+
 @pytest.mark.parametrize("L", [0, 1])
 def test_empty(dev, L):
     d = inputs(dev, 2, L, 2, 2, 32, 32, F32, h0=True)

@@ -28,7 +28,7 @@ struct BackArgs {
   const ChunkWs* ws;
   int nch, per, nseg;
   uint32_t nvb;
-  const float* entry;  // [bh][nseg][Vp][KP], the gradient after the segment (its last one's: a.h0)
+  const float* entry;  // [bh][nseg][Vp][KP], the gradient after the segment (of one: a.h0)
   float* grads;        // [bh][nch][Vp][KP] after every chunk; from zero: [bh][nseg][Vp][KP] before it
 };
 
@@ -70,7 +70,7 @@ __device__ inline void back_chain(const BackArgs& g, typename W::Lds& lds, int64
   if (ZERO || vc >= Vp) {
 #pragma unroll
     for (int i = 0; i < 2 * NS; ++i) S[i] = zero4();
-  } else if (seg == g.nseg - 1) {
+  } else if (g.nseg == 1) {
     get_state<NS>(a.h0 ? a.h0 + bh * K * a.V : nullptr, S, vc, a.V, K, j);
   } else {
     get_cols<NS>(g.entry + (bh * g.nseg + seg) * Vp * KP, S, vc, j);

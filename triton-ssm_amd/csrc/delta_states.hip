@@ -67,6 +67,13 @@ __global__ __launch_bounds__(128 * NS) void delta_fold_kernel(FoldArgs f) {
 #pragma unroll
     for (int t = 0; t < 2 * NS; ++t) S[t] = tiles[i & 1][t][lane];
   };
+  // the first entry state too: the walks then read no buffer that they write
+  // (h0 may be h_last)
+#pragma unroll
+  for (int t = 0; t < 2 * NS; ++t)
+    if (t == x)
+      *reinterpret_cast<f32x4*>(f.entry + ((bh * f.nseg + (REV ? f.nseg - 1 : 0)) * Vp + col) * KP +
+                                row + 8 * j) = S[t];
   In g0, g1, g2;
   load(g0, 0);
   load(g1, 1);

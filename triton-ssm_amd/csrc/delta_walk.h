@@ -42,7 +42,7 @@ namespace {
 enum { kOutputs, kStates, kTransfer };
 
 // Sequences are walked in nseg segments of `per` chunks; a segment's entry
-// state is entry[bh][seg] (the first's: a.h0).
+// state is entry[bh][seg] (a.h0 where there is one).
 struct WalkArgs {
   DeltaArgs a;
   const ChunkWs* ws;
@@ -109,7 +109,7 @@ __device__ inline void chain(const WalkArgs& g, typename W::Lds& lds, int64_t bh
 #pragma unroll
       for (int r = 0; r < 4; ++r)
         S[i][r] = vc - Vp == 32 * (i >> 1) + 8 * j + 4 * (i & 1) + r ? 1.0f : 0.0f;
-  } else if (seg == 0) {
+  } else if (g.nseg == 1) {
     get_state<NS>(a.h0 ? a.h0 + bh * K * a.V : nullptr, S, vc, a.V, K, j);
   } else if (vc < Vp) {
     get_cols<NS>(g.entry + (bh * g.nseg + seg) * Vp * KP, S, vc, j);
