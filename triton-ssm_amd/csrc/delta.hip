@@ -175,7 +175,11 @@ extern "C" int tssm_gated_delta_backward(
                  sq_b, sq_l, sq_h, sk_b, sk_l, sk_h, sv_b, sv_l, sv_h,
                  sg_b, sg_l, sg_h, sbe_b, sbe_l, sbe_h, V, V, V, scale};
   TSSM_CHECK(V <= (INT64_C(1) << 21), TSSM_ERR_UNSUPPORTED);  // a state takes 31 bits
-  TSSM_CHECK((chunk_rows(dtype, a) && fits(dtype, sd_l, V)) || L == 1, TSSM_ERR_STRIDE);
+  if (L == 1) {  // the strides of one step say nothing: those that chunks are read by
+    a.q_l = a.k_l = K;
+    a.v_l = sd_l = V;
+  }
+  TSSM_CHECK(chunk_rows(dtype, a) && fits(dtype, sd_l, V), TSSM_ERR_STRIDE);
   const DeltaPlan p = delta_plan(reinterpret_cast<char*>(workspace), nbatch, L, Hv, K, V, true);
   TSSM_CHECK(workspace && workspace_bytes >= p.bytes && aligned(workspace, 256),
              TSSM_ERR_WORKSPACE);
