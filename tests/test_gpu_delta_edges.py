@@ -41,3 +41,26 @@ def test_backward_of_one_step(dev, dtype, layout, step):
         d[n] = one_step(d[n], layout)
         assert d[n].stride(1) == step
     compare_gradients(d, one_step(do, layout), dh, dtype)
+
+
+def test_many_streams(dev):
+    """More waves than one dimension of a grid holds work-items for: 7e7 streams
+    of a 1 x 1 state, whose step is a handful of products."""
+    from tssm import gated_delta_step
+    S = 70_000_000
+    r = torch.Generator(device=dev).manual_seed(26)
+    q, k, v, state = (torch.randn(S, generator=r, device=dev) for _ in range(4))
+    beta = torch.rand(S, generator=r, device=dev)
+    g = -torch.rand(S, generator=r, device=dev)
+    before = state.clone()
+    o = gated_delta_step(q.view(S, 1, 1), k.view(S, 1, 1), v.view(S, 1, 1), g.view(S, 1),
+                         beta.view(S, 1), state.view(S, 1, 1, 1)).view(S)
+    for lo in range(0, S, 10_000_000):
+        s = slice(lo, lo + 10_000_000)
+        x = torch.exp(g[s].double()) * before[s].double()
+        k64 = k[s].double()
+        x = x + k64 * beta[s].double() * (v[s].double() - k64 * x)
+        for got, want in ((state[s], x), (o[s], q[s].double() * x)):
+            # a step's few roundings of values that are all below `size`
+            size = want.abs().max()
+            assert (got.double() - want).abs().max() <= 1e-5 * size, lo

@@ -1,0 +1,32 @@
+"""GPU tests of the group norm at its edges."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def test_many_short_series(dev):
+    """20 million series of two positions: more workgroups than 2^32 work-items."""
+    from tssm import group_norm_act_backward, group_norm_act_forward
+    N, S, C = 20_000_000, 2, 4
+    r = torch.Generator(device=dev).manual_seed(33)
+    x = torch.randn(N, S, C, generator=r, device=dev)
+    dy = torch.randn(N, S, C, generator=r, device=dev)
+    y, mean, rstd = group_norm_act_forward(x, 1, act="none", return_stats=True)
+    w = torch.ones(C, device=dev)
+    dx, dw, _, _ = group_norm_act_backward(dy, x, mean, rstd, 1, w, act="none")
+    total = torch.zeros(C, dtype=torch.float64, device=dev)
+    for lo in range(0, N, 4_000_000):
+        s = slice(lo, lo + 4_000_000)
+        x64, d64 = x[s].double(), dy[s].double()
+        m = x64.mean((1, 2), keepdim=True)
+        rs = ((x64 - m).square().mean((1, 2), keepdim=True) + 1e-5).rsqrt()
+        xh = (x64 - m) * rs
+        want = rs * (d64 - d64.mean((1, 2), keepdim=True)
+                     - xh * (d64 * xh).mean((1, 2), keepdim=True))
+        assert (y[s].double() - xh).abs().max() <= 1e-5 * xh.abs().max(), lo
+        assert (dx[s].double() - want).abs().max() <= 1e-5 * want.abs().max(), lo
+        total += (d64 * xh).sum((0, 1))
+    # dw is some 6e3, joined from 128 fp32 sums of 1.6e5 terms of both signs that reach
+    # 6e2: roundings of at most 4e-5 each, 2e-2 a sum, 2e-1 in all
+    assert (dw.double() - total).abs().max() <= 1.0

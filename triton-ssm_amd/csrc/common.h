@@ -351,6 +351,16 @@ inline bool aligned(const void* p, uintptr_t a) {
 
 inline int64_t cdiv64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// Grids of any number of workgroups below 2^31.  A grid's dimension of 2^32
+// work-items or more is cut off modulo 2^32 without an error, so larger grids
+// go on in the second dimension, whose last row may hold workgroups past the
+// end: kernels return for those.
+constexpr uint32_t kGridX = 1u << 21;  // workgroups, of up to 1024 threads
+inline dim3 grid_of(int64_t wgs) {
+  return wgs <= kGridX ? dim3((unsigned)wgs) : dim3(kGridX, (unsigned)cdiv64(wgs, kGridX));
+}
+__device__ inline uint32_t block_of() { return blockIdx.y * kGridX + blockIdx.x; }
+
 inline hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }
 
 }  // namespace tssm

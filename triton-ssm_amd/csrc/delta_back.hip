@@ -397,11 +397,12 @@ __global__ __launch_bounds__((Both<T, KP, VEC, NCW, ZERO>::kThreads),
     delta_both_kernel(BackArgs g, WalkArgs f, uint32_t nback) {
   typedef Both<T, KP, VEC, NCW, ZERO> W;
   extern __shared__ __attribute__((aligned(16))) char raw[];
-  if (blockIdx.x < nback) {
-    if (threadIdx.x < W::B::kThreads) back_body<T, KP, VEC, NCW, ZERO>(g, raw, blockIdx.x);
+  const uint32_t block = block_of();
+  if (block < nback) {
+    if (threadIdx.x < W::B::kThreads) back_body<T, KP, VEC, NCW, ZERO>(g, raw, block);
   } else {
     if (threadIdx.x < W::F::kThreads)
-      walk_body<T, KP, VEC, 2, W::MODE>(f, raw, blockIdx.x - nback);
+      walk_body<T, KP, VEC, 2, W::MODE>(f, raw, block - nback);
   }
 }
 
@@ -419,7 +420,7 @@ int both_launch(BackArgs& g, WalkArgs& f, hipStream_t s) {
                                              hipFuncAttributeMaxDynamicSharedMemorySize, W::kBytes);
     if (e != hipSuccess) return (int)e;
   }
-  k<<<(unsigned)(nb + nf), W::kThreads, W::kBytes, s>>>(g, f, (uint32_t)nb);
+  k<<<grid_of(nb + nf), W::kThreads, W::kBytes, s>>>(g, f, (uint32_t)nb);
   return launch_status();
 }
 

@@ -100,8 +100,9 @@ __global__ __launch_bounds__(256, (Grad<T, KP, VEC>::kWaves)) void delta_grads_k
   const int K = (int)a.K, per = ONE ? 1 : (int)((uint32_t)a.Hv / heads);
   const int64_t Vp = (a.V + 15) / 16 * 16;
   // the chunks of one head follow each other
-  const uint32_t bk = blockIdx.x / (uint32_t)g.nch;
-  const int64_t n = blockIdx.x - bk * (uint32_t)g.nch, b = bk / heads, hk = bk % heads;
+  const uint32_t block = block_of(), bk = block / (uint32_t)g.nch;
+  const int64_t n = block - bk * (uint32_t)g.nch, b = bk / heads, hk = bk % heads;
+  if (b >= a.B) return;
   const int64_t t0 = n * kC;
   const int rows = a.L - t0 < kC ? (int)(a.L - t0) : kC;
 
@@ -605,7 +606,7 @@ int grads_launch(const GradArgs& g, bool vec, hipStream_t s) {
                                                hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
       if (e != hipSuccess) return (int)e;
     }
-    f<<<(unsigned)wgs, 256, bytes, s>>>(g);
+    f<<<grid_of(wgs), 256, bytes, s>>>(g);
     return launch_status();
   };
   static_assert(sizeof(typename Grad<T, KP, true>::Lds) <= 160 * 1024, "LDS of a CU");

@@ -55,7 +55,7 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(DeltaArgs a, ChunkWs* w
   __shared__ __attribute__((aligned(16))) float sums[4][2][kC], bet[4][kC];  // G log2(e) in two parts, beta
   const int lane = threadIdx.x & 63, j = lane >> 4, c = lane & 15;
   const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const uint32_t unit = blockIdx.x * 4 + wv;
+  const uint32_t unit = block_of() * 4 + wv;
   if (unit >= units) return;
   // units run over the value heads of one chunk first: a group shares its keys
   const uint32_t Hv = (uint32_t)a.Hv, bn = unit / Hv, nth = bn / nch;
@@ -177,7 +177,7 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(DeltaArgs a, ChunkWs* w
 template <typename T, int KP>
 void launch(const DeltaArgs& a, bool vec, ChunkWs* ws, hipStream_t s) {
   const int64_t nch = cdiv64(a.L, kC), units = a.B * a.Hv * nch;
-  const unsigned wgs = (unsigned)cdiv64(units, 4);
+  const dim3 wgs = grid_of(cdiv64(units, 4));
   if (vec) delta_prep_kernel<T, KP, true><<<wgs, 256, 0, s>>>(a, ws, (uint32_t)nch, (uint32_t)units);
   else delta_prep_kernel<T, KP, false><<<wgs, 256, 0, s>>>(a, ws, (uint32_t)nch, (uint32_t)units);
 }

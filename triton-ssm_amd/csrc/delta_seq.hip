@@ -58,7 +58,7 @@ struct Row {
 template <typename T, int CQ, int KR, bool VEC>
 __global__ __launch_bounds__(256) void delta_seq_kernel(DeltaArgs a, uint32_t ncb, uint32_t units) {
   const int lane = threadIdx.x & 63, kg = lane / CQ, cq = lane % CQ;
-  const uint32_t unit = blockIdx.x * 4 +
+  const uint32_t unit = block_of() * 4 +
                         __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   if (unit >= units) return;
   const uint32_t nth = unit / ncb;
@@ -169,8 +169,9 @@ __global__ __launch_bounds__(256) void delta_seq_kernel(DeltaArgs a, uint32_t nc
 template <typename T, int CQ>
 int launch(const DeltaArgs& a, hipStream_t s) {
   constexpr int kR = CQ / 4;  // rows of a lane for every 16 of K
-  const int64_t ncb = cdiv64(a.V, 4 * CQ), units = a.B * a.Hv * ncb, wgs = cdiv64(units, 4);
+  const int64_t ncb = cdiv64(a.V, 4 * CQ), units = a.B * a.Hv * ncb;
   if (units > 0x7fffffff || a.B > 0x7fffffff / a.Hv) return TSSM_ERR_UNSUPPORTED;
+  const dim3 wgs = grid_of(cdiv64(units, 4));
   const int E = (int)sizeof(T);
   const int kr = (a.K <= 16 ? 1 : (a.K <= 32 ? 2 : (a.K <= 64 ? 4 : 8))) * kR;
   // every row of every operand starts on the widest access a lane makes
@@ -183,9 +184,9 @@ int launch(const DeltaArgs& a, hipStream_t s) {
       (a.v_b | a.v_l | a.v_h | a.o_b | a.o_l | a.o_h) * E % vb == 0;
 #define TSSM_SEQ(KR)                                                                       \
   if (vec)                                                                                 \
-    delta_seq_kernel<T, CQ, KR, true><<<(unsigned)wgs, 256, 0, s>>>(a, (uint32_t)ncb, (uint32_t)units); \
+    delta_seq_kernel<T, CQ, KR, true><<<wgs, 256, 0, s>>>(a, (uint32_t)ncb, (uint32_t)units); \
   else                                                                                     \
-    delta_seq_kernel<T, CQ, KR, false><<<(unsigned)wgs, 256, 0, s>>>(a, (uint32_t)ncb, (uint32_t)units)
+    delta_seq_kernel<T, CQ, KR, false><<<wgs, 256, 0, s>>>(a, (uint32_t)ncb, (uint32_t)units)
   if (a.K <= 16) { TSSM_SEQ(kR); }
   else if (a.K <= 32) { TSSM_SEQ(2 * kR); }
   else if (a.K <= 64) { TSSM_SEQ(4 * kR); }

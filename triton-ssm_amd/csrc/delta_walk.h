@@ -518,7 +518,7 @@ __global__ __launch_bounds__((Walk<T, KP, VEC, NCW, MODE>::kThreads),
                              (Walk<T, KP, VEC, NCW, MODE>::kWaves)) void
     delta_walk_kernel(WalkArgs g) {
   extern __shared__ __attribute__((aligned(16))) char raw[];
-  walk_body<T, KP, VEC, NCW, MODE>(g, raw, blockIdx.x);
+  walk_body<T, KP, VEC, NCW, MODE>(g, raw, block_of());
 }
 
 // Workgroups of a walk (nvb is set), or -1.
@@ -543,7 +543,7 @@ int walk_launch(WalkArgs& g, hipStream_t s) {
                                              hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != hipSuccess) return (int)e;
   }
-  f<<<(unsigned)wgs, W::kThreads, bytes, s>>>(g);
+  f<<<grid_of(wgs), W::kThreads, bytes, s>>>(g);
   return launch_status();
 }
 

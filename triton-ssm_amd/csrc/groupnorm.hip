@@ -67,7 +67,8 @@ __device__ inline float block_sum(float v, float* red) {
 template <typename T>
 __global__ __launch_bounds__(256) void gn_fwd_kernel(GnArgs a) {
   __shared__ float red[4];
-  const int64_t n = blockIdx.x / a.G, g = blockIdx.x - n * a.G, E = a.S * a.Cg;
+  const int64_t ng = block_of(), n = ng / a.G, g = ng - n * a.G, E = a.S * a.Cg;
+  if (n >= a.N) return;
   const T* x = reinterpret_cast<const T*>(a.x) + n * a.x_n + g * a.Cg;
   const T* gt = reinterpret_cast<const T*>(a.gate) + n * a.gt_n + g * a.Cg;
   T* y = reinterpret_cast<T*>(a.y) + n * a.y_n + g * a.Cg;
@@ -85,8 +86,8 @@ __global__ __launch_bounds__(256) void gn_fwd_kernel(GnArgs a) {
   const float lo = block_sum(t, red) / (float)E;
   const float rstd = 1.0f / sqrtf(block_sum(s, red) / (float)E - lo * lo + a.eps);
   if (a.mean && threadIdx.x == 0) {
-    a.mean[blockIdx.x] = (double)mean + (double)lo;
-    a.rstd[blockIdx.x] = rstd;
+    a.mean[ng] = (double)mean + (double)lo;
+    a.rstd[ng] = rstd;
   }
   for (int64_t e = threadIdx.x; e < E; e += 256) {
     const int64_t r = e / a.Cg, c = e % a.Cg;
@@ -119,9 +120,10 @@ __device__ inline float gn_dz(const GnArgs& a, int64_t n, int64_t r, int64_t c, 
 template <typename T>
 __global__ __launch_bounds__(256) void gn_dx_kernel(GnArgs a) {
   __shared__ float red[4];
-  const int64_t n = blockIdx.x / a.G, g = blockIdx.x - n * a.G, E = a.S * a.Cg;
-  const float mean = (float)a.mean[blockIdx.x], rstd = a.rstd[blockIdx.x];
-  const float lo = (float)(a.mean[blockIdx.x] - (double)mean);
+  const int64_t ng = block_of(), n = ng / a.G, g = ng - n * a.G, E = a.S * a.Cg;
+  if (n >= a.N) return;
+  const float mean = (float)a.mean[ng], rstd = a.rstd[ng];
+  const float lo = (float)(a.mean[ng] - (double)mean);
   float s1 = 0.0f, s2 = 0.0f, xh;
   for (int64_t e = threadIdx.x; e < E; e += 256) {
     const int64_t r = e / a.Cg, c = g * a.Cg + e % a.Cg;
@@ -142,7 +144,7 @@ __global__ __launch_bounds__(256) void gn_dx_kernel(GnArgs a) {
 template <typename T>
 __global__ __launch_bounds__(256) void gn_dw_kernel(GnArgs a) {
   __shared__ float red[2][4][64];
-  const int64_t C = a.G * a.Cg, c = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
+  const int64_t C = a.G * a.Cg, c = (int64_t)block_of() * 64 + (threadIdx.x & 63);
   const int part = threadIdx.x >> 6;
   float sw = 0.0f, sb = 0.0f, xh;
   if (c < C) {
@@ -228,9 +230,10 @@ struct RowMap {
 
 template <typename T, int VW, int LG, int NV, int U>
 __global__ __launch_bounds__(256) void gn_row_fwd(GnArgs a, int gw, uint32_t ngb) {
-  const RowMap<LG> m(a, gw, blockIdx.x % ngb);
+  const uint32_t block = block_of(), rb = block / ngb;
+  const RowMap<LG> m(a, gw, block - rb * ngb);
   const int l = threadIdx.x % LG;
-  const int64_t step = 4 * m.rw, r0 = (int64_t)(blockIdx.x / ngb) * U * step + m.row;
+  const int64_t step = 4 * m.rw, r0 = (int64_t)rb * U * step + m.row;
   const bool on = m.g < a.G, gated = a.gate != nullptr;
   int64_t ch[NV];
   bool in[NV];
@@ -300,8 +303,9 @@ template <typename T, int VW, int LG, int NV>
 __global__ __launch_bounds__(256) void gn_row_bwd(GnArgs a, int gw, uint32_t ngb, uint32_t nrb) {
   constexpr int kB = NV > 1 ? 4 : 2;  // sums of VW channels that meet at once
   __shared__ float red[kB][256][VW + 1];
-  const RowMap<LG> m(a, gw, blockIdx.x % ngb);
-  const uint32_t rb = blockIdx.x / ngb;
+  const uint32_t block = block_of(), rb = block / ngb;
+  if (rb >= nrb) return;
+  const RowMap<LG> m(a, gw, block - rb * ngb);
   const int l = threadIdx.x % LG;
   const int64_t step = 4 * m.rw;
   const bool on = m.g < a.G, gated = a.gate != nullptr;
@@ -413,13 +417,13 @@ __global__ __launch_bounds__(256) void gn_row_bwd(GnArgs a, int gw, uint32_t ngb
 }
 
 // out0, out1 [C] = sums of ws [np][2][C] over np, in a fixed order; for every
-// blockIdx.y, np 2 C floats and out_step apart.
+// blockIdx.z, np 2 C floats and out_step apart.
 __global__ __launch_bounds__(256) void gn_sum_kernel(const float* ws, float* out0, float* out1,
                                                      int64_t C, int64_t np, int64_t out_step) {
   __shared__ float red[16][17];
   const int c = threadIdx.x & 15, p = threadIdx.x >> 4;
-  const int64_t i = (int64_t)blockIdx.x * 16 + c;
-  ws += (int64_t)blockIdx.y * np * 2 * C;
+  const int64_t i = (int64_t)block_of() * 16 + c;
+  ws += (int64_t)blockIdx.z * np * 2 * C;
   // eight loads in flight: np is in the hundreds and the workgroups few
   float s[8] = {};
   if (i < 2 * C) {
@@ -435,8 +439,8 @@ __global__ __launch_bounds__(256) void gn_sum_kernel(const float* ws, float* out
     float all = 0.0f;
 #pragma unroll
     for (int k = 0; k < 16; ++k) all += red[k][c];
-    if (i < C) out0[blockIdx.y * out_step + i] = all;
-    else out1[blockIdx.y * out_step + i - C] = all;
+    if (i < C) out0[blockIdx.z * out_step + i] = all;
+    else out1[blockIdx.z * out_step + i - C] = all;
   }
 }
 
@@ -507,7 +511,8 @@ __global__ __launch_bounds__(256) void gn_series_stats(GnArgs a, int tpr, int64_
   extern __shared__ double dyn[];
   double *mean = dyn, *sq = dyn + a.G;
   float *t0 = reinterpret_cast<float*>(dyn + 2 * a.G), *t1 = t0 + a.G, *t2 = t1 + a.G;
-  const int64_t n = blockIdx.x / nb, blk = blockIdx.x - n * nb;
+  const int64_t block = block_of(), n = block / nb, blk = block - n * nb;
+  if (n >= a.N) return;
   const Columns<VW, NC> m(a.G * a.Cg, tpr);
   const int rows = 256 / tpr;
   const int64_t s0 = blk * per, s1 = s0 + per < a.S ? s0 + per : a.S;
@@ -579,7 +584,8 @@ template <typename T, int VW, int NC>
 __global__ __launch_bounds__(256) void gn_series_fwd(GnArgs a, int tpr, int64_t nb, int64_t per) {
   extern __shared__ double dyn[];
   float *hi = reinterpret_cast<float*>(dyn), *lo = hi + a.G, *rs = lo + a.G;
-  const int64_t n = blockIdx.x / nb, blk = blockIdx.x - n * nb;
+  const int64_t block = block_of(), n = block / nb, blk = block - n * nb;
+  if (n >= a.N) return;
   {  // the blocks' statistics join, 16 threads a group
     const double* st = reinterpret_cast<const double*>(a.ws) + n * nb * 2 * a.G;
     const int part = threadIdx.x & 15;
@@ -647,7 +653,8 @@ template <typename T, int VW, int NC>
 __global__ __launch_bounds__(256) void gn_series_sums(GnArgs a, int tpr, int64_t nb, int64_t per,
                                                       float* part) {
   __shared__ float red[256][VW + 1];
-  const int64_t n = blockIdx.x / nb, blk = blockIdx.x - n * nb, C = a.G * a.Cg;
+  const int64_t block = block_of(), n = block / nb, blk = block - n * nb, C = a.G * a.Cg;
+  if (n >= a.N) return;
   const Columns<VW, NC> m(C, tpr);
   const bool gated = a.gate != nullptr;
   float w[NC][VW], b[NC][VW], h[NC], l[NC], r_[NC], sw[NC][VW], sb[NC][VW];
@@ -711,7 +718,8 @@ __global__ __launch_bounds__(256) void gn_series_dx(GnArgs a, int tpr, int64_t n
                                                     const float* chan) {
   extern __shared__ double dyn[];
   float *m1 = reinterpret_cast<float*>(dyn), *m2 = m1 + a.G;
-  const int64_t n = blockIdx.x / nb, blk = blockIdx.x - n * nb, C = a.G * a.Cg;
+  const int64_t block = block_of(), n = block / nb, blk = block - n * nb, C = a.G * a.Cg;
+  if (n >= a.N) return;
   {
     const float* cs = chan + n * 2 * C;
     const int part = threadIdx.x & 15;
@@ -875,18 +883,18 @@ int gn_fwd_vw(const GnArgs& a, hipStream_t s) {
       // rows in flight: where a row is one access of a lane, one is too few
       constexpr int U = NV == 1 ? 4 : (NV == 2 ? 2 : 1);
       gn_row_fwd<T, VW, LG, NV, U>
-          <<<(unsigned)(p.ngb * cdiv64(a.N, U * p.step)), 256, 0, s>>>(a, p.gw, (uint32_t)p.ngb);
+          <<<grid_of(p.ngb * cdiv64(a.N, U * p.step)), 256, 0, s>>>(a, p.gw, (uint32_t)p.ngb);
     });
   } else if (series_fits(C, a.G, VW)) {
     const SeriesPlan p = series_plan(a.N, a.S, C, VW);
     series_dispatch(p, [&](auto nc) {
       constexpr int NC = decltype(nc)::value, R = VW * NC >= 16 ? 2 : (VW * NC >= 8 ? 4 : 8);
-      const unsigned wgs = (unsigned)(a.N * p.nb);
+      const dim3 wgs = grid_of(a.N * p.nb);
       gn_series_stats<T, VW, NC, R><<<wgs, 256, (size_t)a.G * 28, s>>>(a, p.tpr, p.nb, p.per);
       gn_series_fwd<T, VW, NC><<<wgs, 256, (size_t)a.G * 12 + 8, s>>>(a, p.tpr, p.nb, p.per);
     });
   } else {
-    gn_fwd_kernel<T><<<(unsigned)(a.N * a.G), 256, 0, s>>>(a);
+    gn_fwd_kernel<T><<<grid_of(a.N * a.G), 256, 0, s>>>(a);
   }
   return launch_status();
 }
@@ -898,7 +906,7 @@ int gn_fwd(const GnArgs& a, hipStream_t s) {
 template <typename T, int VW>
 int gn_bwd_vw(const GnArgs& a, hipStream_t s) {
   const int64_t C = a.G * a.Cg;
-  const dim3 sums((unsigned)cdiv64(2 * C, 16));
+  const dim3 sums = grid_of(cdiv64(2 * C, 16));
   if (a.N * a.S == 0) {
     gn_sum_kernel<<<sums, 256, 0, s>>>(nullptr, a.dw, a.db, C, 0, 0);
   } else if (row_fits(a.S, a.Cg, VW)) {
@@ -906,7 +914,7 @@ int gn_bwd_vw(const GnArgs& a, hipStream_t s) {
     const int64_t nrb = row_blocks(a.N, p.step, p.ngb);
     row_dispatch<T, VW>(p, [&](auto lg, auto nv) {
       gn_row_bwd<T, VW, decltype(lg)::value, decltype(nv)::value>
-          <<<(unsigned)(p.ngb * nrb), 256, 0, s>>>(a, p.gw, (uint32_t)p.ngb, (uint32_t)nrb);
+          <<<grid_of(p.ngb * nrb), 256, 0, s>>>(a, p.gw, (uint32_t)p.ngb, (uint32_t)nrb);
     });
     gn_sum_kernel<<<sums, 256, 0, s>>>(a.ws, a.dw, a.db, C, nrb, 0);
   } else if (series_fits(C, a.G, VW)) {
@@ -914,19 +922,19 @@ int gn_bwd_vw(const GnArgs& a, hipStream_t s) {
     float* chan = a.ws + a.N * p.nb * 2 * C;
     series_dispatch(p, [&](auto nc) {
       constexpr int NC = decltype(nc)::value;
-      const unsigned wgs = (unsigned)(a.N * p.nb);
+      const dim3 wgs = grid_of(a.N * p.nb);
       gn_series_sums<T, VW, NC><<<wgs, 256, 0, s>>>(a, p.tpr, p.nb, p.per, a.ws);
       for (int64_t n = 0; n < a.N; n += 65535) {
         const unsigned ns = (unsigned)(a.N - n < 65535 ? a.N - n : 65535);
-        gn_sum_kernel<<<dim3(sums.x, ns), 256, 0, s>>>(a.ws + n * p.nb * 2 * C, chan + n * 2 * C,
+        gn_sum_kernel<<<dim3(sums.x, sums.y, ns), 256, 0, s>>>(a.ws + n * p.nb * 2 * C, chan + n * 2 * C,
                                                        chan + n * 2 * C + C, C, p.nb, 2 * C);
       }
       gn_series_dx<T, VW, NC><<<wgs, 256, (size_t)a.G * 8 + 8, s>>>(a, p.tpr, p.nb, p.per, chan);
     });
     gn_sum_kernel<<<sums, 256, 0, s>>>(chan, a.dw, a.db, C, a.N, 0);
   } else {
-    gn_dx_kernel<T><<<(unsigned)(a.N * a.G), 256, 0, s>>>(a);
-    gn_dw_kernel<T><<<(unsigned)cdiv64(C, 64), 256, 0, s>>>(a);
+    gn_dx_kernel<T><<<grid_of(a.N * a.G), 256, 0, s>>>(a);
+    gn_dw_kernel<T><<<grid_of(cdiv64(C, 64)), 256, 0, s>>>(a);
   }
   return launch_status();
 }
