@@ -119,15 +119,6 @@ def _out(out, v):
     return out
 
 
-def _workspace(q, nbytes):
-    """(address, size, stream handle); short sequences need none."""
-    stream = stream_handle(q)
-    if nbytes <= 0:
-        return None, 0, stream
-    ws = workspace.get(q.device, stream, nbytes, workspace.SSD)
-    return ws.data_ptr(), ws.numel(), stream
-
-
 def gated_delta_forward(q, k, v, g, beta, *, scale=None, h0=None, return_state=False, out=None):
     """Gated delta rule over whole sequences.
 
@@ -153,13 +144,12 @@ def gated_delta_forward(q, k, v, g, beta, *, scale=None, h0=None, return_state=F
         h_last = torch.empty(B, Hv, K, V, device=v.device, dtype=_F32) if h0 is None else \
             torch.empty_like(h0)
     if B:
-        ws, nbytes, stream = _workspace(q, _lib.lib().tssm_gated_delta_workspace_bytes(
-            B, L, Hk, Hv, K, V))
-        _lib.call("tssm_gated_delta_forward", code, q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                  g.data_ptr(), beta.data_ptr(), ptr(h0), o.data_ptr(), ptr(h_last), B, L, Hk,
-                  Hv, K, V, *_rows(q, "q"), *_rows(k, "k"), *_rows(v, "v"), *g.stride(),
-                  *beta.stride(), *_rows(o, "out"), K ** -0.5 if scale is None else float(scale),
-                  ws, nbytes, stream)
+        nbytes = _lib.lib().tssm_gated_delta_workspace_bytes(B, L, Hk, Hv, K, V)
+        workspace.call("tssm_gated_delta_forward", q, stream_handle(q), nbytes, code,
+                       q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(),
+                       ptr(h0), o.data_ptr(), ptr(h_last), B, L, Hk, Hv, K, V, *_rows(q, "q"),
+                       *_rows(k, "k"), *_rows(v, "v"), *g.stride(), *beta.stride(),
+                       *_rows(o, "out"), K ** -0.5 if scale is None else float(scale))
     return (o, h_last) if return_state else o
 
 
@@ -186,14 +176,14 @@ def gated_delta_backward(q, k, v, g, beta, do, *, scale=None, h0=None, dh_last=N
     dg, dbeta = torch.empty(2, B, L, Hv, device=q.device, dtype=torch.float32)
     dh0 = None if h0 is None else torch.empty(B, Hv, K, V, device=q.device, dtype=torch.float32)
     if B and L:
-        ws, nbytes, stream = _workspace(q, _lib.lib().tssm_gated_delta_backward_workspace_bytes(
-            B, L, Hk, Hv, K, V))
-        _lib.call("tssm_gated_delta_backward", code, q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                  g.data_ptr(), beta.data_ptr(), ptr(h0), do.data_ptr(), ptr(dh_last),
-                  dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dg.data_ptr(), dbeta.data_ptr(),
-                  ptr(dh0), B, L, Hk, Hv, K, V, *_rows(q, "q"), *_rows(k, "k"), *_rows(v, "v"),
-                  *g.stride(), *beta.stride(), *_rows(do, "do"),
-                  K ** -0.5 if scale is None else float(scale), ws, nbytes, stream)
+        nbytes = _lib.lib().tssm_gated_delta_backward_workspace_bytes(B, L, Hk, Hv, K, V)
+        workspace.call("tssm_gated_delta_backward", q, stream_handle(q), nbytes, code,
+                       q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(),
+                       ptr(h0), do.data_ptr(), ptr(dh_last), dq.data_ptr(), dk.data_ptr(),
+                       dv.data_ptr(), dg.data_ptr(), dbeta.data_ptr(), ptr(dh0), B, L, Hk, Hv, K,
+                       V, *_rows(q, "q"), *_rows(k, "k"), *_rows(v, "v"), *g.stride(),
+                       *beta.stride(), *_rows(do, "do"),
+                       K ** -0.5 if scale is None else float(scale))
     elif dh0 is not None:
         dh0.zero_() if dh_last is None else dh0.copy_(dh_last)
     return dq, dk, dv, dg, dbeta, dh0

@@ -101,11 +101,16 @@ def multihead_ssm_forward(u, A_log, B, C, dt, D=None, *, chunk=128, disc="euler"
     return (y, h_last) if return_state else y
 
 
-def _ws(nbytes, t, what, kind=workspace.LOOKBACK):
+def _call(nbytes, t, what, kind, name, *args):
+    """Entry point ``name`` with a workspace of ``kind``, for what is called ``what``."""
     if nbytes < 0:
         raise ValueError(f"{what}: unsupported shape for the fused kernel")
     stream = stream_handle(t)
-    return workspace.get(t.device, stream, nbytes, kind), stream
+    if kind == workspace.SSD:
+        workspace.call(name, t, stream, max(nbytes, 1), *args)
+    else:
+        ws = workspace.get(t.device, stream, nbytes, kind)
+        _lib.call(name, *args, ws.data_ptr(), ws.numel(), stream)
 
 
 def ssd_scan_forward(x, dt, A_log, B, C, D=None, *, chunk=256, disc="zoh", h0=None,
@@ -164,15 +169,11 @@ def ssd_scan_forward(x, dt, A_log, B, C, D=None, *, chunk=256, disc="zoh", h0=No
     # (the one-launch form exists for bf16 and N = 16 only: no need to ask for others)
     if fused and N == 16 and code == _lib.BF16 and L_.tssm_ssd_scan_fused_supported(code, *args):
         # one launch with a decoupled look-back: a look-back workspace
-        ws, stream = _ws(L_.tssm_ssd_scan_fused_workspace_bytes(Bsz, L, H, P, N, int(chunk)), x,
-                         "ssd_scan")
-        _lib.call("tssm_ssd_scan_fused", code, _disc_code(disc), *args, ws.data_ptr(),
-                  ws.numel(), stream)
+        _call(L_.tssm_ssd_scan_fused_workspace_bytes(Bsz, L, H, P, N, int(chunk)), x, "ssd_scan",
+              workspace.LOOKBACK, "tssm_ssd_scan_fused", code, _disc_code(disc), *args)
     else:
-        ws, stream = _ws(L_.tssm_ssd_scan_workspace_bytes(Bsz, L, H, P, N, int(chunk)), x,
-                         "ssd_scan", workspace.SSD)
-        _lib.call("tssm_ssd_scan", code, _disc_code(disc), *args, ws.data_ptr(), ws.numel(),
-                  stream)
+        _call(L_.tssm_ssd_scan_workspace_bytes(Bsz, L, H, P, N, int(chunk)), x, "ssd_scan",
+              workspace.SSD, "tssm_ssd_scan", code, _disc_code(disc), *args)
     return (y, h_last) if return_state else y
 
 
@@ -273,12 +274,11 @@ def _selective_scan_bcproj(x, dt, A_log, W_bc, D, disc, h0, return_state, dt_is_
         raise ValueError("out must match x in shape and dtype")
     _inner_unit(y, "out")
     h_last = torch.empty(Bsz, Dc, N, device=x.device, dtype=torch.float32) if return_state else None
-    ws, stream = _ws(_lib.lib().tssm_selective_scan_bcproj_workspace_bytes(Bsz, L, Dc, N), x,
-                     "selective_scan bc_proj", workspace.SSD)
-    _lib.call("tssm_selective_scan_bcproj", _disc_code(disc), x.data_ptr(), dt.data_ptr(),
-              int(bool(dt_is_tau)), A_log.data_ptr(), W_bc.data_ptr(), W_bc.stride(0), ptr(D),
-              ptr(h0), y.data_ptr(), ptr(h_last), Bsz, L, Dc, N, x.stride(0), x.stride(1),
-              *sdt, y.stride(0), y.stride(1), ws.data_ptr(), ws.numel(), stream)
+    _call(_lib.lib().tssm_selective_scan_bcproj_workspace_bytes(Bsz, L, Dc, N), x,
+          "selective_scan bc_proj", workspace.SSD, "tssm_selective_scan_bcproj",
+          _disc_code(disc), x.data_ptr(), dt.data_ptr(), int(bool(dt_is_tau)), A_log.data_ptr(),
+          W_bc.data_ptr(), W_bc.stride(0), ptr(D), ptr(h0), y.data_ptr(), ptr(h_last), Bsz, L,
+          Dc, N, x.stride(0), x.stride(1), *sdt, y.stride(0), y.stride(1))
     return (y, h_last) if return_state else y
 
 
@@ -332,13 +332,12 @@ def _selective_scan_xproj(x, A_log, xp, D, disc, h0, return_state, out):
         raise ValueError("out must match x in shape and dtype")
     _inner_unit(y, "out")
     h_last = torch.empty(Bsz, Dc, N, device=x.device, dtype=torch.float32) if return_state else None
-    ws, stream = _ws(_lib.lib().tssm_selective_scan_xproj_workspace_bytes(Bsz, L, Dc, N), x,
-                     "selective_scan x_proj", workspace.SSD)
-    _lib.call("tssm_selective_scan_xproj", _disc_code(disc), x.data_ptr(), A_log.data_ptr(),
-              W_x.data_ptr(), W_x.stride(0), R, W_dt.data_ptr(), W_dt.stride(0),
-              bias.data_ptr(), float(dt_min), float(dt_max), ptr(D), ptr(h0), y.data_ptr(),
-              ptr(h_last), Bsz, L, Dc, N, x.stride(0), x.stride(1), y.stride(0), y.stride(1),
-              ws.data_ptr(), ws.numel(), stream)
+    _call(_lib.lib().tssm_selective_scan_xproj_workspace_bytes(Bsz, L, Dc, N), x,
+          "selective_scan x_proj", workspace.SSD, "tssm_selective_scan_xproj", _disc_code(disc),
+          x.data_ptr(), A_log.data_ptr(), W_x.data_ptr(), W_x.stride(0), R, W_dt.data_ptr(),
+          W_dt.stride(0), bias.data_ptr(), float(dt_min), float(dt_max), ptr(D), ptr(h0),
+          y.data_ptr(), ptr(h_last), Bsz, L, Dc, N, x.stride(0), x.stride(1), y.stride(0),
+          y.stride(1))
     return (y, h_last) if return_state else y
 
 
@@ -453,19 +452,18 @@ def selective_scan_forward(x, dt, A_log, B=None, C=None, D=None, *, chunk=128, d
             code, Bsz, L, Dc, N, sdt[2], int(bool(dt_is_tau)), dt.data_ptr(), None, None, 0,
             0, 0, 0)
         nbytes = L_.tssm_selective_scan_workspace_bytes(Bsz, L, Dc, N, int(chunk))
-    ws, stream = _ws(nbytes, x, "selective_scan",
-                     workspace.SSD if passes else workspace.LOOKBACK)
+    kind = workspace.SSD if passes else workspace.LOOKBACK
     if proj is not None:
-        _lib.call("tssm_selective_scan_dtproj", code, _disc_code(disc), x.data_ptr(),
-                  dt.data_ptr(), W.data_ptr(), bias.data_ptr(), dt_min, dt_max,
-                  A_log.data_ptr(), B.data_ptr(), C.data_ptr(), ptr(D), ptr(h0), y.data_ptr(),
-                  ptr(h_last), Bsz, L, Dc, N, rank, *sx, dt.stride(0), dt.stride(1), W.stride(0),
-                  *sB, *sC, *sy, int(chunk), ws.data_ptr(), ws.numel(), stream)
+        _call(nbytes, x, "selective_scan", kind, "tssm_selective_scan_dtproj", code,
+              _disc_code(disc), x.data_ptr(), dt.data_ptr(), W.data_ptr(), bias.data_ptr(),
+              dt_min, dt_max, A_log.data_ptr(), B.data_ptr(), C.data_ptr(), ptr(D), ptr(h0),
+              y.data_ptr(), ptr(h_last), Bsz, L, Dc, N, rank, *sx, dt.stride(0), dt.stride(1),
+              W.stride(0), *sB, *sC, *sy, int(chunk))
     else:
-        _lib.call("tssm_selective_scan", code, _disc_code(disc), x.data_ptr(), dt.data_ptr(),
-                  int(bool(dt_is_tau)), A_log.data_ptr(), B.data_ptr(), C.data_ptr(), ptr(D),
-                  ptr(h0), y.data_ptr(), ptr(h_last), Bsz, L, Dc, N, *sx, *sdt, *sB, *sC, *sy,
-                  int(chunk), ws.data_ptr(), ws.numel(), stream)
+        _call(nbytes, x, "selective_scan", kind, "tssm_selective_scan", code, _disc_code(disc),
+              x.data_ptr(), dt.data_ptr(), int(bool(dt_is_tau)), A_log.data_ptr(), B.data_ptr(),
+              C.data_ptr(), ptr(D), ptr(h0), y.data_ptr(), ptr(h_last), Bsz, L, Dc, N, *sx, *sdt,
+              *sB, *sC, *sy, int(chunk))
     return (y, h_last) if return_state else y
 
 
@@ -502,15 +500,13 @@ def _interp_scan_fused(V, M, tau32, A_log, B, C, D, Vhat, K, FTILE, disc, h0, re
         h0 = as_f32(h0, "h0").contiguous()
     y = torch.empty(Bsz, T, F, device=V.device, dtype=V.dtype)
     h_last = torch.empty(Bsz, F, N, device=V.device, dtype=torch.float32) if return_state else None
-    ws, stream = _ws(L_.tssm_interp_selective_scan_workspace_bytes(Bsz, T, F, N), V,
-                     "interp_selective_scan", workspace.SSD)
-    _lib.call("tssm_interp_selective_scan", code, _disc_code(disc), V.data_ptr(), M.data_ptr(),
-              tau32.data_ptr(), A_log.data_ptr(), B.data_ptr(), C.data_ptr(), ptr(D), ptr(h0),
-              Vhat.data_ptr(), y.data_ptr(), ptr(h_last), Bsz, T, F, N, V.stride(0),
-              V.stride(1), M.stride(0), M.stride(1), tau32.stride(0), tau32.stride(1),
-              B.stride(0), B.stride(1), C.stride(0), C.stride(1), Vhat.stride(0),
-              Vhat.stride(1), y.stride(0), y.stride(1), int(K), int(FTILE), ws.data_ptr(),
-              ws.numel(), stream)
+    _call(L_.tssm_interp_selective_scan_workspace_bytes(Bsz, T, F, N), V, "interp_selective_scan",
+          workspace.SSD, "tssm_interp_selective_scan", code, _disc_code(disc), V.data_ptr(),
+          M.data_ptr(), tau32.data_ptr(), A_log.data_ptr(), B.data_ptr(), C.data_ptr(), ptr(D),
+          ptr(h0), Vhat.data_ptr(), y.data_ptr(), ptr(h_last), Bsz, T, F, N, V.stride(0),
+          V.stride(1), M.stride(0), M.stride(1), tau32.stride(0), tau32.stride(1), B.stride(0),
+          B.stride(1), C.stride(0), C.stride(1), Vhat.stride(0), Vhat.stride(1), y.stride(0),
+          y.stride(1), int(K), int(FTILE))
     return (Vhat, y, h_last) if return_state else (Vhat, y)
 
 

@@ -77,10 +77,9 @@ def _operands(x, groups, weight, bias, gate, act):
             _channels(weight, "weight", C), _channels(bias, "bias", C))
 
 
-def _ws(x, N, S, G, Cg):
-    stream = stream_handle(x)
-    nbytes = _lib.lib().tssm_group_norm_workspace_bytes(N, S, G, Cg)
-    return workspace.get(x.device, stream, nbytes, workspace.SSD), stream
+def _call(name, x, sizes, *args):
+    workspace.call(name, x, stream_handle(x),
+                   _lib.lib().tssm_group_norm_workspace_bytes(*sizes), *args)
 
 
 def group_norm_act_forward(x, groups, weight=None, bias=None, gate=None, *, act="silu",
@@ -102,10 +101,9 @@ def group_norm_act_forward(x, groups, weight=None, bias=None, gate=None, *, act=
         mean = torch.empty(N, G, device=x.device, dtype=torch.float64)
         rstd = torch.empty(N, G, device=x.device, dtype=torch.float32)
     if N * S:
-        ws, stream = _ws(x, N, S, G, Cg)
-        _lib.call("tssm_group_norm_act_fwd", code, act_, x.data_ptr(), ptr(w), ptr(b), ptr(gate),
-                  y.data_ptr(), ptr(mean), ptr(rstd), N, S, G, Cg, *sx, *sg, *sy, float(eps),
-                  ws.data_ptr(), ws.numel(), stream)
+        _call("tssm_group_norm_act_fwd", x, (N, S, G, Cg), code, act_, x.data_ptr(), ptr(w),
+              ptr(b), ptr(gate), y.data_ptr(), ptr(mean), ptr(rstd), N, S, G, Cg, *sx, *sg, *sy,
+              float(eps))
     return (y, mean, rstd) if return_stats else y
 
 
@@ -125,10 +123,8 @@ def group_norm_act_backward(dy, x, mean, rstd, groups, weight=None, bias=None, g
     dx = torch.empty(x.shape, device=x.device, dtype=x.dtype)
     dgate = torch.empty(x.shape, device=x.device, dtype=x.dtype) if gate is not None else None
     dw, db = torch.empty(2, G * Cg, device=x.device, dtype=torch.float32)
-    ws, stream = _ws(x, N, S, G, Cg)
     sdx = _view(dx, "dx")[3:]
-    _lib.call("tssm_group_norm_act_bwd", code, act_, dy.data_ptr(), x.data_ptr(),
-              mean.data_ptr(), rstd.data_ptr(), ptr(w), ptr(b), ptr(gate), dx.data_ptr(),
-              dw.data_ptr(), db.data_ptr(), ptr(dgate), N, S, G, Cg, *sdy, *sx, *sg, *sdx, *sdx,
-              ws.data_ptr(), ws.numel(), stream)
+    _call("tssm_group_norm_act_bwd", x, (N, S, G, Cg), code, act_, dy.data_ptr(), x.data_ptr(),
+          mean.data_ptr(), rstd.data_ptr(), ptr(w), ptr(b), ptr(gate), dx.data_ptr(),
+          dw.data_ptr(), db.data_ptr(), ptr(dgate), N, S, G, Cg, *sdy, *sx, *sg, *sdx, *sdx)
     return (dx, dw if weight is not None else None, db if bias is not None else None, dgate)

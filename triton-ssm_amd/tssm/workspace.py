@@ -15,7 +15,10 @@ launches.  Two kinds never share a buffer:
               word could carry a current epoch in its upper half.
 
 One buffer is kept per (device, stream, kind) and grown when a launch needs
-more; launches on different streams therefore never share one.
+more; launches on different streams therefore never share one.  An ``ssd`` call
+enqueues several launches that hand data on through the buffer, so it goes
+through ``call()``, which keeps other threads of that stream from getting
+between them and the buffer from being replaced meanwhile.
 
 A bounded look-back wait that expires (a predecessor tile that never
 published, ~1 s of polling) sets the sticky flag and the kernel finishes with
@@ -89,6 +92,25 @@ def get(device: torch.device, stream: int, nbytes: int, kind: str = LOOKBACK) ->
                 # after the zero fill above
                 _lib.call("tssm_workspace_attach_host_flag", buf.data_ptr(), flag.data_ptr())
         return buf
+
+
+_call_locks: dict[tuple[int, int], threading.Lock] = {}
+
+
+def call(name: str, t: torch.Tensor, stream: int, nbytes: int, *args) -> None:
+    """Entry point ``name`` with ``args``, then the address and size of the ssd
+    workspace of t's device and ``stream`` (none for nbytes <= 0), and the
+    stream; the workspace is this call's alone until its launches are enqueued."""
+    if nbytes <= 0:
+        _lib.call(name, *args, None, 0, stream)
+        return
+    key = (_dev_index(t.device), stream)
+    lock = _call_locks.get(key)
+    if lock is None:
+        lock = _call_locks.setdefault(key, threading.Lock())
+    with lock:
+        buf = get(t.device, stream, nbytes, SSD)
+        _lib.call(name, *args, buf.data_ptr(), buf.numel(), stream)
 
 
 def host_flag(device: torch.device, stream: int) -> torch.Tensor | None:
