@@ -32,6 +32,7 @@ def stub(monkeypatch):
         monkeypatch.setattr(module, "stream_handle", lambda t: 7)
     monkeypatch.setattr(workspace, "_dev_index", lambda device: 0)
     monkeypatch.setattr(workspace, "_cache", {})
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
     monkeypatch.setattr(_lib, "lib", lambda: library)
     get = workspace.get
 
@@ -112,3 +113,19 @@ def test_a_failing_call_lets_others_in(stub, monkeypatch):
     done.start()
     done.join(10)
     assert not done.is_alive() and stub[-1][0] == "end"
+
+
+@pytest.mark.parametrize("f", [delta_forward, delta_backward, norm_forward, norm_backward,
+                               ssd_forward])
+def test_captured_calls_have_memory_of_their_own(stub, monkeypatch, f):
+    """A graph may outlive the stream's buffer, which larger calls replace."""
+    seen = []
+    norm_forward()                                   # the stream has a buffer
+    before = dict(workspace._cache)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    monkeypatch.setattr(_lib, "call", lambda name, *args: seen.append(args[-3:-1]))
+    f()
+    (address, size), buf = seen[0], before[(0, 7, workspace.SSD)]
+    assert size > 0 and address % 64 == 0
+    assert not buf.data_ptr() <= address < buf.data_ptr() + buf.numel()
+    assert list(workspace._cache) == list(before) and workspace._cache[(0, 7, workspace.SSD)] is buf

@@ -18,7 +18,10 @@ One buffer is kept per (device, stream, kind) and grown when a launch needs
 more; launches on different streams therefore never share one.  An ``ssd`` call
 enqueues several launches that hand data on through the buffer, so it goes
 through ``call()``, which keeps other threads of that stream from getting
-between them and the buffer from being replaced meanwhile.
+between them and the buffer from being replaced meanwhile.  A replaced buffer
+goes back to the allocator, which a graph that was captured on it would not
+know: a captured ``ssd`` call therefore takes its workspace from the graph's own
+memory, which lives as long as the graph.
 
 A bounded look-back wait that expires (a predecessor tile that never
 published, ~1 s of polling) sets the sticky flag and the kernel finishes with
@@ -100,7 +103,8 @@ _call_locks: dict[tuple[int, int], threading.Lock] = {}
 def call(name: str, t: torch.Tensor, stream: int, nbytes: int, *args) -> None:
     """Entry point ``name`` with ``args``, then the address and size of the ssd
     workspace of t's device and ``stream`` (none for nbytes <= 0), and the
-    stream; the workspace is this call's alone until its launches are enqueued."""
+    stream; the workspace is this call's alone until its launches are enqueued.
+    A call that is captured in a graph gets memory of the graph's own."""
     if nbytes <= 0:
         _lib.call(name, *args, None, 0, stream)
         return
@@ -109,7 +113,10 @@ def call(name: str, t: torch.Tensor, stream: int, nbytes: int, *args) -> None:
     if lock is None:
         lock = _call_locks.setdefault(key, threading.Lock())
     with lock:
-        buf = get(t.device, stream, nbytes, SSD)
+        if torch.cuda.is_current_stream_capturing():
+            buf = torch.empty(nbytes, dtype=torch.uint8, device=t.device)
+        else:
+            buf = get(t.device, stream, nbytes, SSD)
         _lib.call(name, *args, buf.data_ptr(), buf.numel(), stream)
 
 
