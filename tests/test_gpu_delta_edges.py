@@ -64,3 +64,37 @@ def test_many_streams(dev):
             # a step's few roundings of values that are all below `size`
             size = want.abs().max()
             assert (got.double() - want).abs().max() <= 1e-5 * size, lo
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("odd", ["dq", "dk", "dv"])
+def test_packed_gradients(dev, dtype, odd):
+    """The C entry point with gradients in one allocation, one of which starts on
+    no 16-byte boundary."""
+    from tssm import _lib
+    B, L, H, K, V = 2, 70, 2, 64, 48
+    r = torch.Generator().manual_seed(29)
+    d = inputs(dev, B, L, H, H, K, V, dtype, seed=30, h0=True)
+    do = torch.randn(B, L, H, V, generator=r).to(dtype).to(dev)
+    want = gradients(d, do)
+    sizes = dict(dq=d["q"], dk=d["k"], dv=d["v"])
+    pack = torch.full((sum(t.numel() for t in sizes.values()) + 64,), 7.0, device=dev, dtype=dtype)
+    got, used, at = {}, torch.zeros_like(pack, dtype=torch.bool), 8
+    for name, t in sizes.items():
+        at += 1 if name == odd else 0
+        got[name] = pack[at:at + t.numel()].view(t.shape)
+        used[at:at + t.numel()] = True
+        at = (at + t.numel() + 7) // 8 * 8
+    dg, dbeta, dh0 = (torch.empty_like(d[n]) for n in ("g", "beta", "h0"))
+    n = _lib.lib().tssm_gated_delta_backward_workspace_bytes(B, L, H, H, K, V)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    t = [d[x] for x in ("q", "k", "v")]
+    _lib.call("tssm_gated_delta_backward", {F32: 0, BF16: 1}[dtype], *(x.data_ptr() for x in t),
+              d["g"].data_ptr(), d["beta"].data_ptr(), d["h0"].data_ptr(), do.data_ptr(), None,
+              *(g.data_ptr() for g in got.values()), dg.data_ptr(), dbeta.data_ptr(),
+              dh0.data_ptr(), B, L, H, H, K, V, *(s for x in t for s in x.stride()[:3]),
+              *d["g"].stride(), *d["beta"].stride(), *do.stride()[:3], K ** -0.5, ws.data_ptr(), n,
+              torch.cuda.current_stream().cuda_stream)
+    for name, x, y in zip(NAMES, (*got.values(), dg, dbeta, dh0), want):
+        assert_close(x, np64(y), 2.0 ** -8 if dtype == BF16 and name in got else 1e-6, name)
+    assert (pack[~used] == 7.0).all()

@@ -191,7 +191,9 @@ extern "C" int tssm_gated_delta_backward(
   way.h0 = dh_last;
   way.h_last = dh0;
   const DeltaGrads d = {dout, sd_b, sd_l, sd_h, dq, dk, dv, dg, dbeta};
-  const bool vec = vec_rows(dtype, a) && vec_rows(dtype, way);
+  // (the gradients of the inputs are written as the inputs are read)
+  const bool vec = vec_rows(dtype, a) && vec_rows(dtype, way) && aligned(dq, 16) &&
+                   aligned(dk, 16) && aligned(dv, 16);
   hipStream_t st = as_stream(stream);
   int rc = delta_prep_launch(dtype, a, vec, p.chunks, st);
   if (!rc) rc = delta_both_launch(dtype, a, way, vec, p, st);
