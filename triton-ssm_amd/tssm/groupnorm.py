@@ -54,12 +54,14 @@ def _same(t, what, x):
     return _view(t, what)[3:]
 
 
-def _channels(t, what, C):
+def _channels(t, what, C, x):
     if t is None:
         return None
     need_gpu(t, what)
     if t.shape != (C,):
         raise ValueError(f"{what} must be [{C}], got {list(t.shape)}")
+    if t.get_device() != x.get_device():
+        raise ValueError(f"{what} must be on x's device")
     return as_f32(t, what).contiguous()
 
 
@@ -74,7 +76,7 @@ def _operands(x, groups, weight, bias, gate, act):
         raise ValueError(f"act must be 'none' or 'silu', got {act!r}")
     sg = _same(gate, "gate", x) if gate is not None else (0, 0)
     return (code, _ACT[act], N, S, groups, C // groups, (sx_n, sx_s), sg,
-            _channels(weight, "weight", C), _channels(bias, "bias", C))
+            _channels(weight, "weight", C, x), _channels(bias, "bias", C, x))
 
 
 def _call(name, x, sizes, *args):
@@ -120,6 +122,8 @@ def group_norm_act_backward(dy, x, mean, rstd, groups, weight=None, bias=None, g
         need_gpu(t, what)
         if t.shape != (N, G) or t.dtype != dtype or not t.is_contiguous():
             raise ValueError(f"{what} must be contiguous {dtype} [{N}, {G}]")
+        if t.get_device() != x.get_device():
+            raise ValueError(f"{what} must be on x's device")
     dx = torch.empty(x.shape, device=x.device, dtype=x.dtype)
     dgate = torch.empty(x.shape, device=x.device, dtype=x.dtype) if gate is not None else None
     dw, db = torch.empty(2, G * Cg, device=x.device, dtype=torch.float32)
