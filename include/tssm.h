@@ -630,9 +630,9 @@ int tssm_gated_delta_step(int dtype, const void* q, const void* k, const void* v
  * over each group's S x Cg elements (S = 1: per row).  xhat = (x - mean) rstd,
  * z = xhat w + b (w, b f32 [C] or NULL), y = act(z), or z act(gate) where gate
  * [N,S,C] is given.  mean (64 bits: groups whose values almost agree need it)
- * and rstd f32 [N,G] are written where not NULL (both or neither) and read by
- * the backward, which writes dx, dgate (NULL without a
- * gate) of `dtype` and dw, db f32 [C], summed in a fixed order.  No reference
+ * and rstd f32 [N,G] are written where not NULL (both or neither; NaN with S =
+ * 0) and read by the backward, which writes dx, dgate (NULL without a gate) of
+ * `dtype` and dw, db f32 [C], summed in a fixed order.  No reference
  * counterpart.  Workspace: tssm_group_norm_workspace_bytes() bytes, 256-byte
  * aligned, no clearing. */
 int64_t tssm_group_norm_workspace_bytes(int64_t N, int64_t S, int64_t G, int64_t Cg);

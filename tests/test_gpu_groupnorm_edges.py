@@ -30,3 +30,13 @@ def test_many_short_series(dev):
     # dw is some 6e3, joined from 128 fp32 sums of 1.6e5 terms of both signs that reach
     # 6e2: roundings of at most 4e-5 each, 2e-2 a sum, 2e-1 in all
     assert (dw.double() - total).abs().max() <= 1.0
+
+
+@pytest.mark.parametrize("shape", [(4, 0, 32), (3, 2, 0, 5, 32)])
+def test_statistics_of_no_positions(dev, shape):
+    """A mean over nothing is 0 / 0."""
+    from tssm import group_norm_act_forward
+    torch.full((4, 2), 7.0, device=dev, dtype=torch.float64)      # what free memory may hold
+    y, mean, rstd = group_norm_act_forward(torch.empty(shape, device=dev), 2, return_stats=True)
+    assert y.shape == shape and mean.shape == rstd.shape == (shape[0], 2)
+    assert torch.isnan(mean).all() and torch.isnan(rstd).all()

@@ -19,7 +19,8 @@
 //   and dz xhat of every channel, from which the group's two means follow;
 // * groups wider than the registers of a wave (rows: 2048 channels, 512
 //   without vector access) or rows wider than a workgroup's (series: 1024
-//   accesses): one workgroup a group, element by element.
+//   accesses): one workgroup a group, element by element (with S = 0 the
+//   statistics of nothing, 0 / 0).
 #include <type_traits>
 
 #include "common.h"
@@ -885,7 +886,7 @@ int gn_fwd_vw(const GnArgs& a, hipStream_t s) {
       gn_row_fwd<T, VW, LG, NV, U>
           <<<grid_of(p.ngb * cdiv64(a.N, U * p.step)), 256, 0, s>>>(a, p.gw, (uint32_t)p.ngb);
     });
-  } else if (series_fits(C, a.G, VW)) {
+  } else if (a.S && series_fits(C, a.G, VW)) {
     const SeriesPlan p = series_plan(a.N, a.S, C, VW);
     series_dispatch(p, [&](auto nc) {
       constexpr int NC = decltype(nc)::value, R = VW * NC >= 16 ? 2 : (VW * NC >= 8 ? 4 : 8);
@@ -962,8 +963,9 @@ extern "C" int tssm_group_norm_act_fwd(int dtype, int act, const void* x, const 
   TSSM_CHECK(dtype >= TSSM_F32 && dtype <= TSSM_F16, TSSM_ERR_DTYPE);
   TSSM_CHECK(act == TSSM_ACT_NONE || act == TSSM_ACT_SILU, TSSM_ERR_UNSUPPORTED);
   TSSM_CHECK(N >= 0 && S >= 0 && G > 0 && Cg > 0, TSSM_ERR_SHAPE);
-  if (N == 0 || S == 0) return TSSM_OK;
-  TSSM_CHECK(x && y && !mean == !rstd, TSSM_ERR_NULL);
+  if (N == 0) return TSSM_OK;
+  TSSM_CHECK((S == 0 || (x && y)) && !mean == !rstd, TSSM_ERR_NULL);
+  if (S == 0 && !mean) return TSSM_OK;
   TSSM_CHECK(N <= 0x7fffffff / G && G * Cg <= 0x7fffffff, TSSM_ERR_UNSUPPORTED);
   GnArgs a = {};
   a.x = x; a.w = w; a.b = b; a.gate = gate; a.y = y; a.mean = mean; a.rstd = rstd;

@@ -31,6 +31,8 @@ def _view(t, what):
     if stride[-1] != 1 and shape[-1] != 1:
         raise ValueError(f"{what}: innermost dimension must be contiguous")
     S, step = 1, None
+    if 0 in shape[1:-1]:
+        return shape[0], 0, shape[-1], stride[0], shape[-1]
     for n, s in zip(reversed(shape[1:-1]), reversed(stride[1:-1])):
         if n == 1:
             continue
@@ -93,7 +95,7 @@ def group_norm_act_forward(x, groups, weight=None, bias=None, gate=None, *, act=
 
     Returns y (dtype of x; ``out`` if given) and, with ``return_stats``, mean
     (float64: groups whose values almost agree need it) and rstd (float32)
-    [N, groups], which the backward needs.
+    [N, groups], which the backward needs (NaN where there are no positions).
     """
     code, act_, N, S, G, Cg, sx, sg, w, b = _operands(x, groups, weight, bias, gate, act)
     y = torch.empty(x.shape, device=x.device, dtype=x.dtype) if out is None else out
@@ -102,7 +104,7 @@ def group_norm_act_forward(x, groups, weight=None, bias=None, gate=None, *, act=
     if return_stats:
         mean = torch.empty(N, G, device=x.device, dtype=torch.float64)
         rstd = torch.empty(N, G, device=x.device, dtype=torch.float32)
-    if N * S:
+    if N and (S or return_stats):
         _call("tssm_group_norm_act_fwd", x, (N, S, G, Cg), code, act_, x.data_ptr(), ptr(w),
               ptr(b), ptr(gate), y.data_ptr(), ptr(mean), ptr(rstd), N, S, G, Cg, *sx, *sg, *sy,
               float(eps))
