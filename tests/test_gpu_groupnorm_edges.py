@@ -40,3 +40,18 @@ def test_statistics_of_no_positions(dev, shape):
     y, mean, rstd = group_norm_act_forward(torch.empty(shape, device=dev), 2, return_stats=True)
     assert y.shape == shape and mean.shape == rstd.shape == (shape[0], 2)
     assert torch.isnan(mean).all() and torch.isnan(rstd).all()
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("N,S,C", [(6, 1, 64), (3, 70, 64), (2, 1, 4 * 4099)])
+def test_statistics_that_are_not_finite(dev, N, S, C, value):
+    """rstd tells of a group that is not finite, in every form of the kernels."""
+    from tssm import group_norm_act_forward
+    x = torch.randn(N, S, C, generator=torch.Generator().manual_seed(31)).to(dev)
+    x[1, 0, C // 4 + 4] = value
+    y, mean, rstd = group_norm_act_forward(x, 4, return_stats=True)
+    bad = torch.zeros(N, 4, dtype=torch.bool, device=dev)
+    bad[1, 1] = True
+    assert torch.equal(torch.isnan(rstd), bad)
+    assert torch.equal(~torch.isfinite(mean), bad)
+    assert torch.isnan(y[1, :, C // 4:C // 2]).all()

@@ -279,8 +279,8 @@ __global__ __launch_bounds__(256) void gn_row_fwd(GnArgs a, int gw, uint32_t ngb
         t = __builtin_fmaf(d[i][v], d[i][v], t);
       }
     const float lo = group_sum<LG>(s) * inv;
-    const float var = fmaxf(__builtin_fmaf(-lo, lo, group_sum<LG>(t) * inv), 0.0f);
-    const float rstd = __builtin_amdgcn_rsqf(var + a.eps);
+    const float var = __builtin_fmaf(-lo, lo, group_sum<LG>(t) * inv);
+    const float rstd = __builtin_amdgcn_rsqf((var < 0.0f ? 0.0f : var) + a.eps);  // (NaN stays)
     if (r >= a.N) continue;
     if (a.mean && l == 0 && on) {
       a.mean[r * a.G + m.g] = (double)mean + (double)lo;
