@@ -2,6 +2,8 @@
 import pytest
 import torch
 
+from test_gpu_groupnorm import F32
+
 pytestmark = pytest.mark.gpu
 
 
@@ -55,3 +57,16 @@ def test_statistics_that_are_not_finite(dev, N, S, C, value):
     assert torch.equal(torch.isnan(rstd), bad)
     assert torch.equal(~torch.isfinite(mean), bad)
     assert torch.isnan(y[1, :, C // 4:C // 2]).all()
+
+
+@pytest.mark.parametrize("N,S,G,C", [(64, 1, 4, 256), (64, 1, 4, 192), (5, 1, 2, 4099 * 2), (2, 500, 4, 256),
+                                     (3, 7, 2, 24), (2, 9, 513, 1026)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_offsets_of_many_deviations(dev, N, S, G, C, gated):
+    """Values of 1e5 with a deviation of 1, in every form of the kernels.  x - mean is
+    exact where the mean is what its two parts say (a 24-bit mean would be off by up
+    to 4e-3), so the tolerance is the usual one."""
+    from test_gpu_groupnorm import check, inputs
+    d = inputs(dev, N, S, C, F32, gated, seed=C + S)
+    d["x"] = d["x"] + 1e5
+    check(d, G, "silu", F32)

@@ -57,6 +57,13 @@ __device__ inline float act_df(float x, int act, float& d) {
   return x * s;
 }
 
+// sum / count as a 32-bit value of its own: fused into the differences from it,
+// the product would not be the mean that is kept (off by up to 2^-24 of it).
+__device__ inline float mean_of(float sum, float inv) {
+#pragma clang fp contract(off)
+  return sum * inv;
+}
+
 __device__ inline float block_sum(float v, float* red) {
   v = group_sum<64>(v);
   __syncthreads();
@@ -268,7 +275,7 @@ __global__ __launch_bounds__(256) void gn_row_fwd(GnArgs a, int gw, uint32_t ngb
         d[i][v] = x[u][i].get(v);
         s += in[i] ? d[i][v] : 0.0f;
       }
-    const float mean = group_sum<LG>(s) * inv;
+    const float mean = mean_of(group_sum<LG>(s), inv);
     s = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -541,7 +548,7 @@ __global__ __launch_bounds__(256) void gn_series_stats(GnArgs a, int tpr, int64_
     const float inv = 1.0f / (float)(cnt * a.Cg);
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      const float mu = t0[m.ch[i] / a.Cg] * inv;
+      const float mu = mean_of(t0[m.ch[i] / a.Cg], inv);
       d1[i] = d2[i] = 0.0f;
 #pragma unroll
       for (int u = 0; u < R; ++u)
@@ -556,7 +563,7 @@ __global__ __launch_bounds__(256) void gn_series_stats(GnArgs a, int tpr, int64_
     group_totals<VW, NC>(d2, red, t2, a, tpr);
     const double before = (double)((at - s0) * a.Cg), now = (double)(cnt * a.Cg);
     for (int g = threadIdx.x; g < a.G; g += 256) {
-      const double mu = (double)(t0[g] * inv), c = (double)t1[g] / now;
+      const double mu = (double)mean_of(t0[g], inv), c = (double)t1[g] / now;
       const double q = (double)t2[g] - c * c * now;  // about the mean mu + c
       if (at == s0) {
         mean[g] = mu + c;
