@@ -70,3 +70,19 @@ def test_offsets_of_many_deviations(dev, N, S, G, C, gated):
     d = inputs(dev, N, S, C, F32, gated, seed=C + S)
     d["x"] = d["x"] + 1e5
     check(d, G, "silu", F32)
+
+
+@pytest.mark.parametrize("N,S,C,size", [(64, 1, 24, 1e10), (64, 333, 24, 1e10), (64, 5, 16800, 1e10),
+                                        (64, 1, 16800, 1e15), (3, 400, 16800, 1e15)])
+def test_large_constant_groups(dev, N, S, C, size):
+    """Groups of one large value each: what rounding leaves of their variance may
+    be below 0, which is no reason for NaN.  x - mean stays within 2^-46 of x (the
+    mean's second part is good to 2^-24 of some 2^-24), rstd within eps^-1/2."""
+    from tssm import group_norm_act_forward
+    r = torch.Generator().manual_seed(32)
+    x = (size * (1.0 + torch.rand(N, 1, 8, 1, generator=r))).expand(N, S, 8, C // 8)
+    y, mean, rstd = group_norm_act_forward(x.reshape(N, S, C).to(dev), 8, act="none",
+                                           return_stats=True)
+    assert torch.isfinite(y).all()
+    assert (rstd > 0).all() and (rstd <= 316.3).all()
+    assert y.abs().max() <= 2.0 ** -45 * size * 316.3

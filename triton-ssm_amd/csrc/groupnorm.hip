@@ -64,6 +64,9 @@ __device__ inline float mean_of(float sum, float inv) {
   return sum * inv;
 }
 
+// A variance that rounding put below 0 is 0 (NaN stays).
+__device__ inline float not_below_0(float var) { return var < 0.0f ? 0.0f : var; }
+
 __device__ inline float block_sum(float v, float* red) {
   v = group_sum<64>(v);
   __syncthreads();
@@ -92,7 +95,7 @@ __global__ __launch_bounds__(256) void gn_fwd_kernel(GnArgs a) {
     s = __builtin_fmaf(d, d, s);
   }
   const float lo = block_sum(t, red) / (float)E;
-  const float rstd = 1.0f / sqrtf(block_sum(s, red) / (float)E - lo * lo + a.eps);
+  const float rstd = 1.0f / sqrtf(not_below_0(block_sum(s, red) / (float)E - lo * lo) + a.eps);
   if (a.mean && threadIdx.x == 0) {
     a.mean[ng] = (double)mean + (double)lo;
     a.rstd[ng] = rstd;
@@ -287,7 +290,7 @@ __global__ __launch_bounds__(256) void gn_row_fwd(GnArgs a, int gw, uint32_t ngb
       }
     const float lo = group_sum<LG>(s) * inv;
     const float var = __builtin_fmaf(-lo, lo, group_sum<LG>(t) * inv);
-    const float rstd = __builtin_amdgcn_rsqf((var < 0.0f ? 0.0f : var) + a.eps);  // (NaN stays)
+    const float rstd = __builtin_amdgcn_rsqf(not_below_0(var) + a.eps);
     if (r >= a.N) continue;
     if (a.mean && l == 0 && on) {
       a.mean[r * a.G + m.g] = (double)mean + (double)lo;
@@ -610,7 +613,7 @@ __global__ __launch_bounds__(256) void gn_series_fwd(GnArgs a, int tpr, int64_t 
         const double d = st[k * 2 * a.G + g] - mean;
         q += st[(k * 2 + 1) * a.G + g] + d * d * (double)(cnt * a.Cg);
       }
-      const float rstd = 1.0f / sqrtf((float)(sum16(q) / all) + a.eps);
+      const float rstd = 1.0f / sqrtf(not_below_0((float)(sum16(q) / all)) + a.eps);
       if (part == 0) {
         hi[g] = (float)mean;
         lo[g] = (float)(mean - (double)(float)mean);
