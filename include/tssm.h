@@ -596,8 +596,9 @@ int tssm_gated_delta_forward(int dtype, const void* q, const void* k, const void
 /* Gradients of the forward for dout [B,L,Hv,V] (strides sd) and dh_last f32
  * [B,Hv,K,V] or NULL (zero): dq, dk [B,L,Hk,K] (summed over the value heads
  * that share a key head, in order), dv [B,L,Hv,V] of `dtype`, dg, dbeta f32
- * [B,L,Hv], all contiguous, dh0 f32 [B,Hv,K,V] or NULL.  The rows of q, k, v
- * and dout must not overlap (L > 1).  The states are formed again from the
+ * [B,L,Hv], all contiguous, dh0 f32 [B,Hv,K,V] or NULL.  With L > 1 the rows of
+ * q, k, v and dout must not overlap, and 33 of their steps must lie within 2^31
+ * bytes (TSSM_ERR_STRIDE).  The states are formed again from the
  * inputs and kept in the workspace
  * (tssm_gated_delta_backward_workspace_bytes() bytes, else as the forward's):
  * 8 K V bytes for every 32 steps of a value head.  With L = 0 nothing is

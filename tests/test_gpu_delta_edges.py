@@ -98,3 +98,17 @@ def test_packed_gradients(dev, dtype, odd):
     for name, x, y in zip(NAMES, (*got.values(), dg, dbeta, dh0), want):
         assert_close(x, np64(y), 2.0 ** -8 if dtype == BF16 and name in got else 1e-6, name)
     assert (pack[~used] == 7.0).all()
+
+
+def test_backward_of_far_steps(dev):
+    """Steps that lie further apart than a chunk's 31 bits reach."""
+    L, H, N, far = 3, 2, 16, 17_000_000
+    r = torch.Generator().manual_seed(24)
+    d = inputs(dev, 1, L, H, H, N, N, F32, seed=25, h0=True)
+    do = torch.randn(1, L, H, N, generator=r).to(dev)
+    base = torch.empty(4 * H * N + (L - 1) * far, device=dev)
+    views = [base.as_strided((1, L, H, N), (1, far, N, 1), i * H * N) for i in range(4)]
+    for view, t in zip(views, (d["q"], d["k"], d["v"], do)):
+        view.copy_(t)
+    d["q"], d["k"], d["v"], do = views
+    compare_gradients(d, do, torch.randn(1, H, N, N, generator=r).to(dev), F32)

@@ -95,10 +95,15 @@ def _explain(q, k, v, g, beta, lead):
     return g, beta
 
 
-def _steps(t):
+def _steps(t, chunks=False):
     """t [B, L, H, N], copied where its steps overlap in memory (as expanded
-    ones do): the chunked kernels take steps that lie one after the other."""
-    return t.contiguous() if t.shape[1] > 1 and t.stride(1) < t.shape[3] else t
+    ones do): the chunked kernels take steps that lie one after the other.  With
+    ``chunks`` (nothing but chunked kernels) also where a chunk of 32 steps and
+    one more would pass 31 bits."""
+    if t.shape[1] > 1 and (t.stride(1) < t.shape[3] or chunks and
+                           t.stride(1) >= (1 << 31) // (33 * t.element_size())):
+        return t.contiguous()
+    return t
 
 
 def _state(t, what, shape, device):
@@ -168,7 +173,7 @@ def gated_delta_backward(q, k, v, g, beta, do, *, scale=None, h0=None, dh_last=N
     (B, L, Hk, Hv, K, V), code, g, beta = _operands(q, k, v, g, beta, 2)
     dev = q.get_device()
     _check(do, "do", v.shape, v.dtype, dev)
-    q, k, v, do = _steps(q), _steps(k), _steps(v), _steps(do)
+    q, k, v, do = (_steps(t, chunks=True) for t in (q, k, v, do))
     h0, dh_last = _state(h0, "h0", (B, Hv, K, V), dev), \
         _state(dh_last, "dh_last", (B, Hv, K, V), dev)
     dq = torch.empty(B, L, Hk, K, device=q.device, dtype=q.dtype)
