@@ -6,7 +6,7 @@ import torch
 
 from helpers import assert_close, np64
 from oracle import mixer_oracle as M
-from test_gpu_delta import BF16, F32, NAMES, TOL, gradients, inputs
+from test_gpu_delta import BF16, F16, F32, NAMES, TOL, gradients, inputs, oracle, run
 
 pytestmark = pytest.mark.gpu
 
@@ -112,3 +112,77 @@ def test_backward_of_far_steps(dev):
         view.copy_(t)
     d["q"], d["k"], d["v"], do = views
     compare_gradients(d, do, torch.randn(1, H, N, N, generator=r).to(dev), F32)
+
+
+@pytest.mark.parametrize("dtype,B,L,H,K,V,t0", [
+    (BF16, 1, 8200, 2, 64, 64, 4000),     # in segments, far from their ends
+    (F32, 1, 5001, 1, 40, 72, 3203),
+    (F16, 1, 150, 2, 64, 64, 75),
+    (F16, 2, 3000, 1, 128, 30, 31),       # in the first chunk of a segmented sequence
+    (BF16, 1, 150, 2, 128, 128, 149),     # the last step
+    (F32, 1, 150, 2, 128, 64, 64),        # the first step of a chunk
+    (BF16, 2, 70, 2, 24, 40, 40),         # K and V that fill no tile
+])
+@pytest.mark.parametrize("name", ["v", "k", "q", "beta", "g"])
+def test_not_finite_in_every_form(dev, dtype, B, L, H, K, V, t0, name):
+    """A NaN at one step of one head changes no earlier output and no other head;
+    in v no other column, in q no other step."""
+    d = inputs(dev, B, L, H, H, K, V, dtype, seed=L + K, h0=True, rate=0.05)
+    o_ref, S_ref = oracle(d)
+    if name in ("beta", "g"):
+        d[name][B - 1, t0, H - 1] = float("nan")
+    else:
+        d[name][B - 1, t0, H - 1, 5] = float("nan")
+    o, S = run(d)
+    assert_close(o[:, :t0], o_ref[:, :t0], TOL[dtype], "earlier steps")
+    rest = [i for i in range(B * H) if i != B * H - 1]
+    if rest:
+        heads = o.transpose(1, 2).reshape(B * H, L, V)[rest]
+        want = o_ref.swapaxes(1, 2).reshape(B * H, L, V)[rest]
+        assert_close(heads, want, TOL[dtype], "other heads")
+        assert_close(S.reshape(B * H, K, V)[rest], S_ref.reshape(B * H, K, V)[rest], TOL[F32],
+                     "other heads' states")
+    one, one_ref = o[B - 1, :, H - 1], o_ref[B - 1, :, H - 1]
+    last, last_ref = S[B - 1, H - 1], S_ref[B - 1, H - 1]
+    if name == "v":
+        keep = [c for c in range(V) if c != 5]
+        assert torch.isnan(one[t0, 5]) and torch.isnan(last[:, 5]).all()
+        assert_close(one[:, keep], one_ref[:, keep], TOL[dtype], "other columns")
+        assert_close(last[:, keep], last_ref[:, keep], TOL[F32], "their state")
+    elif name == "q":
+        assert torch.isnan(one[t0]).all()
+        if t0 + 1 < L:
+            assert_close(one[t0 + 1:], one_ref[t0 + 1:], TOL[dtype], "later steps")
+        assert_close(last, last_ref, TOL[F32], "state")
+    else:
+        assert torch.isnan(one[t0:]).all() and torch.isnan(last).all()
+
+
+@pytest.mark.parametrize("dtype,B,L,Hk,Hv,K,V", [
+    (BF16, 2, 70, 2, 4, 128, 128), (BF16, 1, 33, 1, 3, 128, 72), (BF16, 1, 3000, 1, 2, 128, 64),
+    (F16, 2, 100, 1, 2, 128, 128), (BF16, 1, 5000, 1, 1, 24, 20), (F32, 1, 70, 1, 2, 128, 200)])
+def test_backward_wide(dev, dtype, B, L, Hk, Hv, K, V):
+    """Keys of 128, shared key heads, V in several slices, segments."""
+    r = torch.Generator().manual_seed(27)
+    d = inputs(dev, B, L, Hk, Hv, K, V, dtype, seed=L + V, h0=True, rate=0.1)
+    do = torch.randn(B, L, Hv, V, generator=r).to(dtype).to(dev)
+    compare_gradients(d, do, torch.randn(B, Hv, K, V, generator=r).to(dev), dtype)
+
+
+def test_long_sequence_of_shared_rows(dev):
+    """The C entry point with one key and one query for all steps (stride 0): rows
+    that overlap go step by step at any length, without a workspace."""
+    from tssm import _lib
+    B, L, H, K, V = 2, 100, 2, 64, 48
+    d = inputs(dev, B, L, H, H, K, V, BF16, seed=28, h0=True)
+    d["q"], d["k"] = d["q"][:, :1].expand(B, L, H, K), d["k"][:, :1].expand(B, L, H, K)
+    o, S = torch.empty_like(d["v"]), torch.empty_like(d["h0"])
+    t = [d[x] for x in ("q", "k", "v")]
+    assert d["q"].stride(1) == 0
+    _lib.call("tssm_gated_delta_forward", 1, *(x.data_ptr() for x in t), d["g"].data_ptr(),
+              d["beta"].data_ptr(), d["h0"].data_ptr(), o.data_ptr(), S.data_ptr(), B, L, H, H, K,
+              V, *(s for x in t for s in x.stride()[:3]), *d["g"].stride(), *d["beta"].stride(),
+              *o.stride()[:3], K ** -0.5, None, 0, torch.cuda.current_stream().cuda_stream)
+    o_ref, S_ref = oracle(d)
+    assert_close(o, o_ref, TOL[BF16], "o")
+    assert_close(S, S_ref, TOL[F32], "state")
