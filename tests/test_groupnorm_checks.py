@@ -26,7 +26,7 @@ class OnOther(On):
 def no_library(monkeypatch):
     def called(*args):
         raise AssertionError("the library was called")
-    monkeypatch.setattr(groupnorm, "_call", called)
+    monkeypatch.setattr(groupnorm.workspace, "call", called)
 
 
 def on(t, other=False):

@@ -30,7 +30,7 @@ def stub(monkeypatch):
     for module in (delta, fused, groupnorm, launch):
         monkeypatch.setattr(module, "need_gpu", lambda t, what: t)
         monkeypatch.setattr(module, "stream_handle", lambda t: 7)
-    monkeypatch.setattr(workspace, "_dev_index", lambda device: 0)
+    monkeypatch.setattr(workspace, "_dev_index", lambda device: -1)
     monkeypatch.setattr(workspace, "_cache", {})
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
     monkeypatch.setattr(_lib, "lib", lambda: library)
@@ -44,7 +44,7 @@ def stub(monkeypatch):
     def call(name, *args):
         events.append(("begin", threading.get_ident()))
         time.sleep(0.005)          # the launches: other threads run meanwhile
-        held = workspace._cache[(0, 7, workspace.SSD)].data_ptr()
+        held = workspace._cache[(-1, 7, workspace.SSD)].data_ptr()
         events.append(("end" if held == args[-3] else "buffer replaced", threading.get_ident()))
 
     monkeypatch.setattr(workspace, "get", recorded)
@@ -125,7 +125,7 @@ def test_captured_calls_have_memory_of_their_own(stub, monkeypatch, f):
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
     monkeypatch.setattr(_lib, "call", lambda name, *args: seen.append(args[-3:-1]))
     f()
-    (address, size), buf = seen[0], before[(0, 7, workspace.SSD)]
+    (address, size), buf = seen[0], before[(-1, 7, workspace.SSD)]
     assert size > 0 and address % 64 == 0
     assert not buf.data_ptr() <= address < buf.data_ptr() + buf.numel()
-    assert list(workspace._cache) == list(before) and workspace._cache[(0, 7, workspace.SSD)] is buf
+    assert list(workspace._cache) == list(before) and workspace._cache[(-1, 7, workspace.SSD)] is buf

@@ -56,15 +56,15 @@ def _same(t, what, x):
     return _view(t, what)[3:]
 
 
-def _channels(t, what, C, x):
+def _channels(t, what, C, device):
     if t is None:
         return None
     need_gpu(t, what)
     if t.shape != (C,):
         raise ValueError(f"{what} must be [{C}], got {list(t.shape)}")
-    if t.get_device() != x.get_device():
+    if t.get_device() != device:
         raise ValueError(f"{what} must be on x's device")
-    return as_f32(t, what).contiguous()
+    return t if t.dtype == torch.float32 and t.is_contiguous() else as_f32(t, what).contiguous()
 
 
 def _operands(x, groups, weight, bias, gate, act):
@@ -77,13 +77,9 @@ def _operands(x, groups, weight, bias, gate, act):
     if act not in _ACT:
         raise ValueError(f"act must be 'none' or 'silu', got {act!r}")
     sg = _same(gate, "gate", x) if gate is not None else (0, 0)
+    device = x.get_device()
     return (code, _ACT[act], N, S, groups, C // groups, (sx_n, sx_s), sg,
-            _channels(weight, "weight", C, x), _channels(bias, "bias", C, x))
-
-
-def _call(name, x, sizes, *args):
-    workspace.call(name, x, stream_handle(x),
-                   _lib.lib().tssm_group_norm_workspace_bytes(*sizes), *args)
+            _channels(weight, "weight", C, device), _channels(bias, "bias", C, device))
 
 
 def group_norm_act_forward(x, groups, weight=None, bias=None, gate=None, *, act="silu",
@@ -105,9 +101,10 @@ def group_norm_act_forward(x, groups, weight=None, bias=None, gate=None, *, act=
         mean = torch.empty(N, G, device=x.device, dtype=torch.float64)
         rstd = torch.empty(N, G, device=x.device, dtype=torch.float32)
     if N and (S or return_stats):
-        _call("tssm_group_norm_act_fwd", x, (N, S, G, Cg), code, act_, x.data_ptr(), ptr(w),
-              ptr(b), ptr(gate), y.data_ptr(), ptr(mean), ptr(rstd), N, S, G, Cg, *sx, *sg, *sy,
-              float(eps))
+        workspace.call("tssm_group_norm_act_fwd", x, stream_handle(x),
+                       _lib.lib().tssm_group_norm_workspace_bytes(N, S, G, Cg), code, act_,
+                       x.data_ptr(), ptr(w), ptr(b), ptr(gate), y.data_ptr(), ptr(mean),
+                       ptr(rstd), N, S, G, Cg, *sx, *sg, *sy, float(eps))
     return (y, mean, rstd) if return_stats else y
 
 
@@ -130,7 +127,9 @@ def group_norm_act_backward(dy, x, mean, rstd, groups, weight=None, bias=None, g
     dgate = torch.empty(x.shape, device=x.device, dtype=x.dtype) if gate is not None else None
     dw, db = torch.empty(2, G * Cg, device=x.device, dtype=torch.float32)
     sdx = _view(dx, "dx")[3:]
-    _call("tssm_group_norm_act_bwd", x, (N, S, G, Cg), code, act_, dy.data_ptr(), x.data_ptr(),
-          mean.data_ptr(), rstd.data_ptr(), ptr(w), ptr(b), ptr(gate), dx.data_ptr(),
-          dw.data_ptr(), db.data_ptr(), ptr(dgate), N, S, G, Cg, *sdy, *sx, *sg, *sdx, *sdx)
+    workspace.call("tssm_group_norm_act_bwd", x, stream_handle(x),
+                   _lib.lib().tssm_group_norm_workspace_bytes(N, S, G, Cg), code, act_,
+                   dy.data_ptr(), x.data_ptr(), mean.data_ptr(), rstd.data_ptr(), ptr(w), ptr(b),
+                   ptr(gate), dx.data_ptr(), dw.data_ptr(), db.data_ptr(), ptr(dgate), N, S, G,
+                   Cg, *sdy, *sx, *sg, *sdx, *sdx)
     return (dx, dw if weight is not None else None, db if bias is not None else None, dgate)

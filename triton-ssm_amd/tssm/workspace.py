@@ -97,7 +97,7 @@ def get(device: torch.device, stream: int, nbytes: int, kind: str = LOOKBACK) ->
         return buf
 
 
-_call_locks: dict[tuple[int, int], threading.Lock] = {}
+_call_locks: dict[tuple[int, int, str], threading.Lock] = {}
 
 
 def call(name: str, t: torch.Tensor, stream: int, nbytes: int, *args) -> None:
@@ -108,14 +108,17 @@ def call(name: str, t: torch.Tensor, stream: int, nbytes: int, *args) -> None:
     if nbytes <= 0:
         _lib.call(name, *args, None, 0, stream)
         return
-    key = (_dev_index(t.device), stream)
+    if stream and torch.cuda.is_current_stream_capturing():   # (stream 0 takes no captures)
+        buf = torch.empty(nbytes, dtype=torch.uint8, device=t.device)
+        _lib.call(name, *args, buf.data_ptr(), nbytes, stream)
+        return
+    key = (t.get_device(), stream, SSD)
     lock = _call_locks.get(key)
     if lock is None:
         lock = _call_locks.setdefault(key, threading.Lock())
     with lock:
-        if torch.cuda.is_current_stream_capturing():
-            buf = torch.empty(nbytes, dtype=torch.uint8, device=t.device)
-        else:
+        buf = _cache.get(key)
+        if buf is None or buf.numel() < nbytes:
             buf = get(t.device, stream, nbytes, SSD)
         _lib.call(name, *args, buf.data_ptr(), buf.numel(), stream)
 
