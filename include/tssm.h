@@ -579,7 +579,8 @@ int tssm_masked_fill_zero(int dtype, int mask_code, const void* x, const void* m
  * h0/h_last f32 contiguous [B,Hv,K,V] or NULL (h0 NULL: zero; they may be the
  * same buffer).  K <= 128.  State, sums and products that reach the state are
  * fp32 whatever the dtype.  Workspace: tssm_gated_delta_workspace_bytes()
- * bytes (0: may be NULL), 256-byte aligned, raw fp32 (not look-back words), no
+ * bytes (0: may be NULL; else 5632 for every 32 steps of a value head, and the
+ * segments' matrices), 256-byte aligned, raw fp32 (not look-back words), no
  * clearing. */
 int64_t tssm_gated_delta_workspace_bytes(int64_t nbatch, int64_t L, int64_t Hk, int64_t Hv,
                                          int64_t K, int64_t V);
@@ -600,9 +601,11 @@ int tssm_gated_delta_forward(int dtype, const void* q, const void* k, const void
  * q, k, v and dout must not overlap, and 33 of their steps must lie within 2^31
  * bytes (TSSM_ERR_STRIDE).  The states are formed again from the
  * inputs and kept in the workspace
- * (tssm_gated_delta_backward_workspace_bytes() bytes, else as the forward's):
- * 8 K V bytes for every 32 steps of a value head.  With L = 0 nothing is
- * written (dh0 would be dh_last). */
+ * (tssm_gated_delta_backward_workspace_bytes() bytes, else as the forward's): 8
+ * K' V' + 5632 bytes for every 32 steps of a value head, K' being K rounded up
+ * to 32, 64 or 128 and V' V to a multiple of 16, and for few heads and long
+ * sequences 4 K' (4 V' + K') for each of at most 512 segments of a head.  With L
+ * = 0 nothing is written (dh0 would be dh_last). */
 int64_t tssm_gated_delta_backward_workspace_bytes(int64_t nbatch, int64_t L, int64_t Hk,
                                                   int64_t Hv, int64_t K, int64_t V);
 int tssm_gated_delta_backward(int dtype, const void* q, const void* k, const void* v,

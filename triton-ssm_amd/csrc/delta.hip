@@ -13,7 +13,10 @@ bool sizes_ok(int64_t B, int64_t L, int64_t Hk, int64_t Hv, int64_t K, int64_t V
 // 1, 8 heads of 64 x 64: 5.3, 7.6 and 12.3 us at L = 4, 8 and 16); one chunk's
 // way through the chunked kernels takes 10.5 us at any L, and 23 us once the
 // chip has more than two heads on each CU (512 heads: 10.3, 16.4, 21.7 and 26.8
-// us step by step at L = 8, 16, 24 and 32).
+// us step by step at L = 8, 16, 24 and 32).  That is 64 x 64 in bf16; the two
+// ways meet at 10 tokens for 12 heads of 40 x 72 in fp32, at 16 to 19 for 16 and 32
+// of 128 x 128, and beyond 32 for 512 of 128 x 128 (25 tokens: 47 us step by step,
+// 100 in chunks) and 1024 of 40 x 72.
 bool by_steps(int64_t heads, int64_t L) { return L <= (heads >= 512 ? 24 : 12); }
 
 // How many segments a sequence of nch chunks is walked in, by the times that the
@@ -21,8 +24,12 @@ bool by_steps(int64_t heads, int64_t L) { return L <= (heads >= 512 ? 24 : 12); 
 // microsecond): the outputs' walk fills a CU with one workgroup of 32 columns;
 // the walk from zero over V + KP columns, which s > 1 segments add, takes 1.5
 // and 2 times as long a chunk with two and four workgroups on a CU; joining
-// takes a chunk's time a segment, the two launches more twelve.  B = 1, L = 65536, H = 8, K = V = 64,
-// bf16: 1780 us in one segment; with 8, 16, 32 and 64: 513, 375, 332 and 406.
+// takes a chunk's time a segment, the two launches more twelve.  B = 1, L = 65536,
+// H = 8, K = V = 64, bf16: 1780 us in one segment; with 8, 16, 32 and 64: 513, 375,
+// 332 and 406.  The rule compares times only, and other sizes keep about these
+// proportions: with 128 x 128 and 40 x 72, in fp32 and fp16, and in the gradients,
+// whose two walks go side by side, seven more calls took at most 7% more than
+// with the best of ten counts.
 int64_t segments(int64_t heads, int64_t nch, int64_t KP, int64_t V) {
   const int64_t out = heads * cdiv64(V, 32), all = heads * (cdiv64(V, 32) + KP / 32);
   int64_t best = 1, least = nch * 10 * cdiv64(out, 256);

@@ -16,8 +16,9 @@
 // LDS while the chain waves multiply K G', after it the helpers work on that
 // chunk.
 // Bound like the walk by the chain waves' instructions.  B=4 L=4096 H=16 K=V=64
-// bf16, 256 workgroups of both kinds: 190 us in one launch, which also writes 268
-// MB of states and gradients; one after the other 124 and 185.
+// bf16, 256 workgroups of both kinds: 178 us in one launch, which also writes 268
+// MB of states and gradients (190 in a first call, where one after the other took
+// 124 and 185).
 #include "delta_walk.h"
 
 namespace tssm {

@@ -11,7 +11,7 @@
 // slow step; a decay below e^-200 is 0 in fp32 either way.
 //
 // Bound by memory: 4 KiB of keys and 0.25 of g and beta in, 5.25 out a chunk (B=8
-// L=4096 H=16 K=64 bf16: 172 MB in 36 us, 4.8 TB/s; 43 us with T's zeros stored
+// L=4096 H=16 K=64 bf16: 172 MB in 34 to 36 us, 5 TB/s; 43 us with T's zeros stored
 // and 16 bytes of every 32 written at a time).  T in fp32 would be less to write
 // (36 us with its zeros), but the walks' loaders then split it into planes, and
 // the chain waves on their SIMDs lose more to that than is gained here.

@@ -25,13 +25,14 @@
 // weights would otherwise carry a later step's NaN to earlier outputs.
 //
 // What bounds it is the chain waves' own instructions, one after the other from one
-// wave: about 300 a chunk of K = 64 bf16, 2061 cycles with the rest of the
-// workgroup idle and 2077 with it at work (an 8-byte instruction leaves a wave
-// every 6.5 cycles).  112 of them split S, R and U into planes, 36 are matrix
-// instructions.  B=8 L=4096 H=16 K=V=64 bf16: 121 to 148 us by the card's clock,
-// 128 chunks in a row; B=2 L=2000 Hv=16 K=V=128: 100 us.  With its operands
-// straight from memory, two chunks ahead, it took 145 against 128 us, with three
-// chunks in LDS and reads a chunk ahead 127 against 122.
+// wave: about 300 a chunk of K = 64 bf16, 2100 cycles with the rest of the
+// workgroup idle and 2170 with it at work (an 8-byte instruction leaves a wave
+// every 6.5 cycles); 2980 of 3180 at K = 128, 2710 of 3150 in fp32 at K = 40.  112
+// of the 300 split S, R and U into planes, 36 are matrix instructions.  B=8 L=4096
+// H=16 K=V=64 bf16: 122 us once the clock has settled (148 in a first call), 128
+// chunks in a row; B=2 L=2000 Hv=16 K=V=128: 96 us.  With its operands straight
+// from memory, two chunks ahead, it took 145 against 128 us, with three chunks in
+// LDS and reads a chunk ahead 127 against 122.
 #pragma once
 
 #include "delta_dev.h"
@@ -56,7 +57,11 @@ struct WalkArgs {
 template <typename T, int KP, bool VEC, int NCW, int MODE>
 struct Walk {
   static constexpr int NP = Piece<T, VEC>::NP;  // planes of the inputs
-  static constexpr int NO = NP == 1 ? 2 : 3;    // of S, P and U in the outputs' products
+  // of S, P and U in the products that reach the outputs alone: with bf16's two
+  // (2^-17 of a value that is rounded to 2^-9) 0.34% of the outputs are the bf16
+  // next to the nearest, with three 0.016%, at the same error against 64 bits
+  // (1.7e-3, normwise) and 155 against 165 us for B=8 L=4096 H=16 K=V=64
+  static constexpr int NO = NP == 1 ? 2 : 3;
   static constexpr int NS = KP / 32;
   // threads of the loaders: those of fp32 and fp16 split what they bring (B=3 L=1111
   // 12 heads of 40 x 72: 57.4 us with 128, 55.7 with 256)

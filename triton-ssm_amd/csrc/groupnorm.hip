@@ -12,15 +12,19 @@
 // need x - mean exactly, and the variance is formed about it.
 //
 // Three forms, all bound by memory where the problem is large:
-// * rows (S = 1): a group in LG lanes' registers, one pass over the data;
+// * rows (S = 1): a group in LG lanes' registers, one pass over the data (32768
+//   rows of 16 x 64, gated, bf16: 43 us, 4.7 TB/s);
 // * series (S > 1): blocks of positions in registers, their means and squared
 //   deviations joined by Chan's formula, then a second pass over x (which the
 //   last-level cache mostly serves); the backward needs only the sums of dz
 //   and dz xhat of every channel, from which the group's two means follow;
 // * groups wider than the registers of a wave (rows: 2048 channels, 512
 //   without vector access) or rows wider than a workgroup's (series: 1024
-//   accesses): one workgroup a group, element by element (with S = 0 the
-//   statistics of nothing, 0 / 0).
+//   accesses, 1024 channels without vector access): one workgroup a group,
+//   element by element (with S = 0 the statistics of nothing, 0 / 0).  This form
+//   is bound by its index arithmetic and by few workgroups: one series of 4096
+//   positions of 30 groups of 50 channels, bf16, 990 us, with gradients 3550
+//   (floors 5 and 10; in torch's elementary operations 220 and 680).
 #include <type_traits>
 
 #include "common.h"
