@@ -10,6 +10,7 @@ callable taking the dict of bound arguments (Triton's ``grid(meta)`` form).
 from __future__ import annotations
 
 import torch
+import torch._prims_common
 
 from . import _lib
 
@@ -102,7 +103,7 @@ def as_f32(t: torch.Tensor, what: str) -> torch.Tensor:
         return t
     if not t.is_floating_point():
         raise TypeError(f"{what}: expected a float tensor, got {t.dtype}")
-    if not t.is_non_overlapping_and_dense():
+    if not torch._prims_common.is_non_overlapping_and_dense(t):
         raise TypeError(f"{what}: a non-fp32 tensor must be dense to be read as fp32")
     return t.to(torch.float32)  # preserve_format keeps strides of dense tensors
 
@@ -136,6 +137,15 @@ def stream_handle(t: torch.Tensor) -> int:
     ``torch.cuda.current_stream(t.device).cuda_stream`` holds, read without
     building the stream object (0.2 against 2.0 us)."""
     return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
+def on_device(device: int, f, *args):
+    """f(*args) with ``device`` as the current one: a launch on a default stream
+    goes to the current device, whatever device the tensors are on."""
+    if torch._C._cuda_getDevice() == device:
+        return f(*args)
+    with torch.cuda.device(device):
+        return f(*args)
 
 
 def ival(x, what: str) -> int:
