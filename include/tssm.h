@@ -629,6 +629,37 @@ int tssm_gated_delta_step(int dtype, const void* q, const void* k, const void* v
                           int64_t sg_h, int64_t sbe_s, int64_t sbe_h, int64_t so_s, int64_t so_h,
                           float scale, void* stream);
 
+/* ------------------------------------------------------------------ linear attention
+ * Per batch and value head h, key head h / (Hv / Hk), state S [K][V] f32:
+ *   S = exp(g) S + k v^T,  o = scale S^T q
+ * q, k [B,L,Hk,K], v, o [B,L,Hv,V] of one dtype, innermost stride 1, the other
+ * strides (b, l, h) free; g f32 [B,L,Hv], three strides.  h0, h_last f32
+ * contiguous [B,Hv,K,V] or NULL (zero, not returned); they may be one buffer.
+ * K <= 128, V <= 2^21.  No reference counterpart.  The state and the sums that
+ * reach it are fp32 whatever the dtype.  Workspace:
+ * tssm_linear_attention_workspace_bytes() bytes (0: may be NULL), 256-byte
+ * aligned, raw fp32 (not look-back words), no clearing. */
+int64_t tssm_linear_attention_workspace_bytes(int64_t nbatch, int64_t L, int64_t Hk, int64_t Hv,
+                                              int64_t K, int64_t V);
+int tssm_linear_attention_forward(int dtype, const void* q, const void* k, const void* v,
+                                  const float* g, const float* h0, void* o, float* h_last,
+                                  int64_t nbatch, int64_t L, int64_t Hk, int64_t Hv, int64_t K,
+                                  int64_t V, int64_t sq_b, int64_t sq_l, int64_t sq_h,
+                                  int64_t sk_b, int64_t sk_l, int64_t sk_h, int64_t sv_b,
+                                  int64_t sv_l, int64_t sv_h, int64_t sg_b, int64_t sg_l,
+                                  int64_t sg_h, int64_t so_b, int64_t so_l, int64_t so_h,
+                                  float scale, void* workspace, int64_t workspace_bytes,
+                                  void* stream);
+
+/* One step of S streams, state f32 contiguous [S,Hv,K,V] updated in place:
+ * q, k [S,Hk,K], v, o [S,Hv,V], g [S,Hv], strides (s, h). */
+int tssm_linear_attention_step(int dtype, const void* q, const void* k, const void* v,
+                               const float* g, float* state, void* o, int64_t S, int64_t Hk,
+                               int64_t Hv, int64_t K, int64_t V, int64_t sq_s, int64_t sq_h,
+                               int64_t sk_s, int64_t sk_h, int64_t sv_s, int64_t sv_h,
+                               int64_t sg_s, int64_t sg_h, int64_t so_s, int64_t so_h,
+                               float scale, void* stream);
+
 /* ------------------------------------------------------------------ group norm, activation
  * x [N,S,C], C = G Cg, unit channel stride, strides (n, s); mean and variance
  * over each group's S x Cg elements (S = 1: per row).  xhat = (x - mean) rstd,

@@ -1,0 +1,34 @@
+// Shared argument block of linear attention's kernels (linattn.hip and its
+// translation units).  Per batch b, value head h (key head h / per):
+//   S_t = e^{g_t} S_{t-1} + k_t v_t^T,  o_t = scale S_t^T q_t,   S [K, V] fp32.
+#pragma once
+
+#include "common.h"
+
+namespace tssm {
+
+struct LinArgs {
+  const void *q, *k, *v;
+  const float *g, *h0;
+  void* o;
+  float* h_last;
+  int64_t B, L, Hk, Hv, K, V;
+  int64_t q_b, q_l, q_h, k_b, k_l, k_h, v_b, v_l, v_h;
+  int64_t g_b, g_l, g_h, o_b, o_l, o_h;
+  float scale;
+};
+
+// Batch, value head and key head of one of the B Hv heads, which are fewer than
+// 2^32 (a 64-bit division is some 150 instructions, and kernels begin with it).
+struct LinHead {
+  int64_t b, h, hk;
+};
+__device__ inline LinHead lin_head(const LinArgs& a, uint32_t bh) {
+  const uint32_t Hv = (uint32_t)a.Hv, b = bh / Hv, h = bh - b * Hv;
+  return {b, h, h / (Hv / (uint32_t)a.Hk)};
+}
+
+// linattn_seq.hip: one step after another, the state in registers.
+int lin_seq_launch(int dtype, const LinArgs& a, hipStream_t s);
+
+}  // namespace tssm
