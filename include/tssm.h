@@ -660,6 +660,49 @@ int tssm_linear_attention_step(int dtype, const void* q, const void* k, const vo
                                int64_t sg_s, int64_t sg_h, int64_t so_s, int64_t so_h,
                                float scale, void* stream);
 
+/* ------------------------------------------------------------------ norm and rotation of queries and keys
+ * For each row x [K] of q [B,L,Hq,K] and k [B,L,Hk,K] (unit innermost stride,
+ * strides (b, l, h)): n = r x w with r = (mean x^2 + eps)^-1/2 (TSSM_NORM_RMS),
+ * (sum x^2 + eps)^-1/2 (TSSM_NORM_L2) or 1 (TSSM_NORM_NONE), w f32 [K] or NULL
+ * (1); then the R/2 pairs of the first R channels, (j, j + R/2) or with
+ * `interleaved` (2j, 2j + 1), turned by the angle pos freq[j] and scaled by
+ * `amplitude`; the other channels stay n.  pos [B,L], strides (b, l), of a
+ * TSSM_POS_* type, freq f64 [R/2]; the angle is formed in 64 bits.  R = 0: no
+ * rotation, pos and freq may be NULL.  K <= 256 (and
+ * K > 1 with a norm: one channel's norm is its sign), B L < 2^31.  The outputs (of
+ * `dtype`, strides like the inputs') may be the inputs.  The backward takes the
+ * outputs' gradients and writes dq, dk of `dtype` and dwq, dwk f32 [K] (NULL
+ * where not wanted), summed in a fixed order through a workspace of
+ * tssm_qk_norm_rotary_workspace_bytes() bytes (16-byte aligned, no clearing;
+ * NULL with neither).  No reference counterpart. */
+#define TSSM_NORM_NONE 0
+#define TSSM_NORM_RMS 1
+#define TSSM_NORM_L2 2
+#define TSSM_POS_F32 0
+#define TSSM_POS_F64 1
+#define TSSM_POS_I32 2
+#define TSSM_POS_I64 3
+int tssm_qk_norm_rotary_fwd(int dtype, int norm, int interleaved, const void* q, const void* k,
+                            const void* pos, int pos_type, const double* freq, const float* wq,
+                            const float* wk, void* yq, void* yk, int64_t nbatch, int64_t L,
+                            int64_t Hq, int64_t Hk, int64_t K, int64_t R, int64_t sq_b,
+                            int64_t sq_l, int64_t sq_h, int64_t sk_b, int64_t sk_l, int64_t sk_h,
+                            int64_t sp_b, int64_t sp_l, int64_t syq_b, int64_t syq_l,
+                            int64_t syq_h, int64_t syk_b, int64_t syk_l, int64_t syk_h, float eps,
+                            float amplitude, void* stream);
+int64_t tssm_qk_norm_rotary_workspace_bytes(int64_t K);
+int tssm_qk_norm_rotary_bwd(int dtype, int norm, int interleaved, const void* dyq,
+                            const void* dyk, const void* q, const void* k, const void* pos,
+                            int pos_type, const double* freq, const float* wq, const float* wk,
+                            void* dq, void* dk, float* dwq, float* dwk, int64_t nbatch, int64_t L,
+                            int64_t Hq, int64_t Hk, int64_t K, int64_t R, int64_t sdyq_b,
+                            int64_t sdyq_l, int64_t sdyq_h, int64_t sdyk_b, int64_t sdyk_l,
+                            int64_t sdyk_h, int64_t sq_b, int64_t sq_l, int64_t sq_h,
+                            int64_t sk_b, int64_t sk_l, int64_t sk_h, int64_t sp_b, int64_t sp_l,
+                            int64_t sdq_b, int64_t sdq_l, int64_t sdq_h, int64_t sdk_b,
+                            int64_t sdk_l, int64_t sdk_h, float eps, float amplitude,
+                            void* workspace, int64_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------------ group norm, activation
  * x [N,S,C], C = G Cg, unit channel stride, strides (n, s); mean and variance
  * over each group's S x Cg elements (S = 1: per row).  xhat = (x - mean) rstd,

@@ -4,8 +4,9 @@ Tolerances, normwise (largest difference over largest value).  fp32 outputs
 (states, and everything with fp32 inputs): 1e-5 -- a sum of n products in a fixed
 order carries about sqrt(n) 2^-24; here n is K (at most 128), the steps that a
 decay leaves (at most some thousands) and the chunks' states, so 100 x 6e-8 = 6e-6.
-16-bit outputs: twice the rounding of the largest value, 2^-8 for bfloat16 and
-2^-11 for float16.
+16-bit outputs: one rounding, 2^-8 (bfloat16) or 2^-11 (float16) of the largest
+value, and a fiftieth of it for what precedes it (weights of two planes, 2^-16,
+with up to 100 terms that count).
 """
 import numpy as np
 import pytest
@@ -17,7 +18,7 @@ from oracle import mixer_oracle as M
 pytestmark = pytest.mark.gpu
 
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
-TOL = {F32: 1e-5, BF16: 2.0 ** -8, F16: 2.0 ** -11}
+TOL = {F32: 1e-5, BF16: 1.02 * 2.0 ** -8, F16: 1.02 * 2.0 ** -11}
 
 
 def inputs(dev, B, L, Hk, Hv, K, V, dtype, seed=0, h0=False, rate=1.0):
