@@ -31,4 +31,20 @@ __device__ inline LinHead lin_head(const LinArgs& a, uint32_t bh) {
 // linattn_seq.hip: one step after another, the state in registers.
 int lin_seq_launch(int dtype, const LinArgs& a, hipStream_t s);
 
+// Chunked form.  Sequences of few heads are walked in segments: each one's end
+// state from zero, joined to its entry state (ends, in place) by the sums of g.  For
+// the gradients also the states before the chunks, and the gradients of those after
+// them (`back`: the same of the way back).
+struct LinPlan {
+  int64_t steps, nseg;       // steps of a segment, segments
+  float *ends, *back;        // nseg > 1
+  double *sums, *back_sums;
+  float *states, *grads;     // gradients only
+  int64_t bytes;
+};
+// vec: the rows of q, k, v and o are whole 16-byte accesses.
+int lin_walk_launch(int dtype, const LinArgs& a, bool vec, const LinPlan& p, hipStream_t s);
+// The segments' entry states, forward.
+int lin_entry_launch(int dtype, const LinArgs& a, bool vec, const LinPlan& p, hipStream_t s);
+
 }  // namespace tssm

@@ -10,6 +10,59 @@ bool sizes_ok(int64_t B, int64_t L, int64_t Hk, int64_t Hv, int64_t K, int64_t V
 // A head's state takes 31 bits.
 bool takes(int64_t K, int64_t V) { return K <= 128 && V <= (INT64_C(1) << 21); }
 
+// Sequences up to here go step by step.
+bool by_steps(int64_t heads, int64_t L) { return L <= 16; }
+
+// Segments of a sequence: as many as fill the chip with two workgroups for each CU.
+int64_t segments(int64_t heads, int64_t L, int64_t V) {
+  const int64_t wgs = heads * cdiv64(V, 32);
+  if (wgs >= 256) return 1;
+  const int64_t most = cdiv64(L, 512);
+  const int64_t want = cdiv64(512, wgs);
+  return want < most ? want : most;
+}
+
+LinPlan lin_plan(char* base, int64_t B, int64_t L, int64_t Hv, int64_t K, int64_t V) {
+  LinPlan p = {};
+  const int64_t heads = B * Hv, elems = (K <= 32 ? 32 : (K <= 64 ? 64 : 128)) * cdiv64(V, 32) * 32;
+  int64_t at = 0;
+  const auto take = [&](int64_t bytes) {
+    char* q = base + at;
+    at += cdiv64(bytes, 256) * 256;
+    return q;
+  };
+  const int64_t nseg = segments(heads, L, V);
+  p.steps = cdiv64(cdiv64(L, nseg), 128) * 128;
+  p.nseg = cdiv64(L, p.steps);
+  if (p.nseg > 1) {
+    p.ends = reinterpret_cast<float*>(take(heads * p.nseg * elems * 4));
+    p.sums = reinterpret_cast<double*>(take(heads * p.nseg * 8));
+  }
+  p.bytes = at;
+  return p;
+}
+
+// The rows of q, k, v and o are whole 16-byte accesses.
+bool vec_rows(int dtype, const LinArgs& a) {
+  const int64_t E = dtype == TSSM_F32 ? 4 : 2;
+  return a.K % 8 == 0 && a.V % 8 == 0 && aligned(a.q, 16) && aligned(a.k, 16) &&
+         aligned(a.v, 16) && aligned(a.o, 16) &&
+         (a.q_b | a.q_l | a.q_h | a.k_b | a.k_l | a.k_h | a.v_b | a.v_l | a.v_h | a.o_b | a.o_l |
+          a.o_h) * E % 16 == 0;
+}
+
+bool fits(int dtype, int64_t stride, int64_t cols) {
+  const int64_t most = (INT64_C(1) << 31) / (129 * (dtype == TSSM_F32 ? 4 : 2));
+  return stride >= cols && stride < most;
+}
+
+// What the chunked kernels' buffer accesses ask for: the rows of q, k, v and o
+// do not overlap, and a chunk's lie within 31 bits of its first.
+bool chunk_rows(int dtype, const LinArgs& a) {
+  return fits(dtype, a.q_l, a.K) && fits(dtype, a.k_l, a.K) && fits(dtype, a.v_l, a.V) &&
+         fits(dtype, a.o_l, a.V);
+}
+
 }  // namespace
 }  // namespace tssm
 
@@ -19,7 +72,8 @@ extern "C" int64_t tssm_linear_attention_workspace_bytes(int64_t nbatch, int64_t
                                                          int64_t Hv, int64_t K, int64_t V) {
   if (!sizes_ok(nbatch, L, Hk, Hv, K, V)) return TSSM_ERR_SHAPE;
   if (!takes(K, V)) return TSSM_ERR_UNSUPPORTED;
-  return 0;
+  if (nbatch == 0 || by_steps(nbatch * Hv, L)) return 0;
+  return lin_plan(nullptr, nbatch, L, Hv, K, V).bytes;
 }
 
 extern "C" int tssm_linear_attention_forward(
@@ -37,9 +91,15 @@ extern "C" int tssm_linear_attention_forward(
   const LinArgs a = {q, k, v, g, h0, o, h_last, nbatch, L, Hk, Hv, K, V,
                      sq_b, sq_l, sq_h, sk_b, sk_l, sk_h, sv_b, sv_l, sv_h,
                      sg_b, sg_l, sg_h, so_b, so_l, so_h, scale};
-  (void)workspace;
-  (void)workspace_bytes;
-  return lin_seq_launch(dtype, a, as_stream(stream));
+  hipStream_t st = as_stream(stream);
+  if (by_steps(nbatch * Hv, L) || !chunk_rows(dtype, a)) return lin_seq_launch(dtype, a, st);
+  TSSM_CHECK(L < (INT64_C(1) << 31) && nbatch <= 0x7fffffff / Hv, TSSM_ERR_UNSUPPORTED);
+  const LinPlan p = lin_plan(reinterpret_cast<char*>(workspace), nbatch, L, Hv, K, V);
+  TSSM_CHECK(p.bytes == 0 || (workspace && workspace_bytes >= p.bytes && aligned(workspace, 256)),
+             TSSM_ERR_WORKSPACE);
+  const bool vec = vec_rows(dtype, a);
+  const int rc = p.nseg > 1 ? lin_entry_launch(dtype, a, vec, p, st) : TSSM_OK;
+  return rc ? rc : lin_walk_launch(dtype, a, vec, p, st);
 }
 
 extern "C" int tssm_linear_attention_step(int dtype, const void* q, const void* k, const void* v,

@@ -1,0 +1,161 @@
+// Device pieces of linear attention's chunked kernels (planes.h: the products).
+#pragma once
+
+#include "linattn.h"
+#include "planes.h"
+
+namespace tssm {
+namespace {
+
+// Planes of an input (fp32 three, fp16 two, bf16 one: exactly), and of what is
+// formed on the way to the outputs alone (two, 2^-17 of a value that is rounded to
+// 2^-9 or 2^-12; three where nothing is rounded).  What reaches the state always
+// has three.
+template <typename T>
+constexpr int kPlanes = sizeof(T) == 4 ? 3 : (std::is_same<T, bf16_t>::value ? 1 : 2);
+template <typename T>
+constexpr int kOutPlanes = sizeof(T) == 4 ? 3 : 2;
+
+// A state in the workspace lies as the waves hold it: tiles [Vp / 16][KP / 16] of
+// 64 lanes x 4, tile (vt, 2 s + x) lane (j, c) register r holding S[32 s + 8 j + 4 x
+// + r][16 vt + c]; Vp is V rounded up to 32, zero past K and V.
+__host__ __device__ inline int64_t lin_state_elems(int64_t KP, int64_t V) {
+  return KP * ((V + 31) / 32 * 32);
+}
+
+// A tile's lane of a caller's [K][V] state, zero past K and V or without one.
+__device__ inline f32x4 get_tile(const float* m, int kt, int64_t col, int64_t V, int K, int j) {
+  const bool on = m && col < V;
+  f32x4 S;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int k = 32 * (kt >> 1) + 8 * j + 4 * (kt & 1) + r;
+    const float x = m ? m[(int64_t)(k < K ? k : 0) * V + (on ? col : 0)] : 0.0f;
+    S[r] = on && k < K ? x : 0.0f;
+  }
+  return S;
+}
+__device__ inline void put_tile(float* m, const f32x4& S, int kt, int64_t col, int64_t V, int K,
+                                int j) {
+  if (!m || col >= V) return;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int k = 32 * (kt >> 1) + 8 * j + 4 * (kt & 1) + r;
+    if (k < K) m[(int64_t)k * V + col] = S[r];
+  }
+}
+
+// Decays of a chunk of C steps.  With G the sums of g from the chunk's start in
+// units of log 2, formed in 64 bits: hi + lo = G_t in two parts, whose differences
+// keep 24 bits where the decay between two steps counts, and u = e^(G_end - G_t),
+// end being the last of the step's 32.  g below -200 counts as -200 (e^-200 is 0 in
+// fp32, and sums stay finite).
+template <int C>
+struct Decays {
+  float hi[C], lo[C], u[C];
+};
+
+__device__ inline float diff2(float hi, float lo, float hi0, float lo0) {
+  return exp2_fast((hi - hi0) + (lo - lo0));
+}
+
+// g of a lane's steps: steps lane E .. lane E + E - 1, E = max(C / 64, 1).
+template <int C>
+struct Gaps {
+  static constexpr int E = C > 64 ? C / 64 : 1;
+  float g[E];
+  // steps past `rows` count as 0
+  __device__ inline void load(const float* p, int64_t stride, int lane, int rows) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int t = lane * E + e;
+      const float x = p[t < rows ? t * stride : 0];
+      g[e] = t < rows ? x : 0.0f;
+    }
+  }
+  // One wave forms a chunk's decays.
+  __device__ inline void decays(Decays<C>& d, int lane) const {
+    double s[E], sum = 0.0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float x = g[e] < -200.0f ? -200.0f : g[e];
+      sum += (double)x;
+      s[e] = sum;
+    }
+    double run = sum;
+#pragma unroll
+    for (int n = 1; n < 64; n *= 2) {
+      const double y = __shfl_up(run, n);
+      if (lane >= n) run += y;
+    }
+    const double before = __shfl_up(run, 1);
+    float hi[E], lo[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const double G = ((lane ? before : 0.0) + s[e]) * 1.4426950408889634;
+      hi[e] = (float)G;
+      lo[e] = (float)(G - (double)hi[e]);
+    }
+    constexpr int kBlock = 32 / E;  // lanes of 32 steps
+    const int end = lane | (kBlock - 1);
+    const float hE = __shfl(hi[E - 1], end), lE = __shfl(lo[E - 1], end);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int t = lane * E + e;
+      if (t < C) {
+        d.hi[t] = hi[e];
+        d.lo[t] = lo[e];
+        d.u[t] = diff2(hE, lE, hi[e], lo[e]);
+      }
+    }
+  }
+};
+
+// The planes of a piece of K or V, whose channels must not meet: take_plane() takes
+// the planes of a pair together, where a value that is not finite would reach its
+// neighbour.
+template <typename T, bool VEC, int NP>
+__device__ inline void planes_apart(const Piece<T, VEC, NP>& x, int lim, u32x4* out) {
+  if constexpr (NP == 1) {
+    x.planes(lim, out);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float a = 2 * i < lim ? ldf(&x.e[2 * i]) : 0.0f;
+      float b = 2 * i + 1 < lim ? ldf(&x.e[2 * i + 1]) : 0.0f;
+#pragma unroll
+      for (int n = 0; n < NP; ++n) {
+        const uint32_t w = pk_bf16(a, b);
+        out[n][i] = w;
+        a -= __uint_as_float(w << 16);
+        b -= __uint_as_float(w & 0xffff0000u);
+      }
+    }
+  }
+}
+
+// Eight consecutive floats of LDS.
+__device__ inline void lds8(const float* p, float* x) {
+  *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(p);
+  *reinterpret_cast<float4*>(x + 4) = *reinterpret_cast<const float4*>(p + 4);
+}
+
+// The B operand X[8 j + e][c] of 32 rows from `row` on and 16 columns from `col`
+// on of planes [NP][rows][ld] in LDS, as floats.
+template <int NP>
+__device__ inline void lds_values(const uint16_t* m, int plane, int ld, int row, int col, int lane,
+                                  float* x) {
+#pragma unroll
+  for (int p = NP - 1; p >= 0; --p) {
+    const u32x4 w = lds_col16(m + p * plane + row * ld, ld, col, lane);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float a = __uint_as_float(w[e] << 16), b = __uint_as_float(w[e] & 0xffff0000u);
+      x[2 * e] = p == NP - 1 ? a : x[2 * e] + a;
+      x[2 * e + 1] = p == NP - 1 ? b : x[2 * e + 1] + b;
+    }
+  }
+}
+
+}  // namespace
+}  // namespace tssm

@@ -92,6 +92,12 @@ def _explain(q, k, v, g, lead):
     return g.to(_F32)
 
 
+def _steps(t):
+    """t [B, L, H, N], copied where its steps overlap in memory (as expanded ones
+    do): the chunked kernels take steps that lie one after the other."""
+    return t.contiguous() if t.shape[1] > 1 and t.stride(1) < t.shape[3] else t
+
+
 def _state(t, what, shape, device):
     if t is None:
         return None
@@ -129,6 +135,7 @@ def linear_attention_forward(q, k, v, g, *, scale=None, h0=None, return_state=Fa
     """
     (B, L, Hk, Hv, K, V), code, g = _operands(q, k, v, g, 2)
     dev = q.get_device()
+    q, k, v = _steps(q), _steps(k), _steps(v)
     h0 = _state(h0, "h0", (B, Hv, K, V), dev)
     o = _out(out, v)
     h_last = None
