@@ -651,6 +651,31 @@ int tssm_linear_attention_forward(int dtype, const void* q, const void* k, const
                                   float scale, void* workspace, int64_t workspace_bytes,
                                   void* stream);
 
+/* Gradients of the forward for dout [B,L,Hv,V] (strides sd) and dh_last f32
+ * [B,Hv,K,V] or NULL (zero): dq, dk [B,L,Hk,K] (summed over the value heads
+ * that share a key head, in order), dv [B,L,Hv,V] of `dtype`, dg f32 [B,L,Hv],
+ * all contiguous, dh0 f32 [B,Hv,K,V] or NULL.  With L > 1 the rows of q, k, v
+ * and dout must not overlap, and 129 of their steps must lie within 2^31 bytes
+ * (TSSM_ERR_STRIDE).  The states are formed again from the inputs and kept in the
+ * workspace (tssm_linear_attention_backward_workspace_bytes() bytes, else as
+ * the forward's): 8 K' V' bytes for every 64 steps of a value head (32 in fp32
+ * with K > 64), K' being K rounded up to 32, 64 or 128 and V' V to a multiple of
+ * 32, and for few heads and long sequences as much for each segment of a head.
+ * With L = 0 nothing is written (dh0 would be dh_last). */
+int64_t tssm_linear_attention_backward_workspace_bytes(int dtype, int64_t nbatch, int64_t L,
+                                                       int64_t Hk, int64_t Hv, int64_t K,
+                                                       int64_t V);
+int tssm_linear_attention_backward(int dtype, const void* q, const void* k, const void* v,
+                                   const float* g, const float* h0, const void* dout,
+                                   const float* dh_last, void* dq, void* dk, void* dv, float* dg,
+                                   float* dh0, int64_t nbatch, int64_t L, int64_t Hk, int64_t Hv,
+                                   int64_t K, int64_t V, int64_t sq_b, int64_t sq_l,
+                                   int64_t sq_h, int64_t sk_b, int64_t sk_l, int64_t sk_h,
+                                   int64_t sv_b, int64_t sv_l, int64_t sv_h, int64_t sg_b,
+                                   int64_t sg_l, int64_t sg_h, int64_t sd_b, int64_t sd_l,
+                                   int64_t sd_h, float scale, void* workspace,
+                                   int64_t workspace_bytes, void* stream);
+
 /* One step of S streams, state f32 contiguous [S,Hv,K,V] updated in place:
  * q, k [S,Hk,K], v, o [S,Hv,V], g [S,Hv], strides (s, h). */
 int tssm_linear_attention_step(int dtype, const void* q, const void* k, const void* v,

@@ -320,3 +320,170 @@ def test_many_streams(dev):
             # a step's few roundings of values that are all below `size`
             size = want.abs().max()
             assert (got.double() - want).abs().max() <= 1e-6 * size, lo
+
+
+# ------------------------------------------------------------------ gradients
+NAMES = ("dq", "dk", "dv", "dg", "dh0")
+
+
+def gradients(d, do, dh=None, **kw):
+    from tssm import linear_attention_backward
+    return linear_attention_backward(d["q"], d["k"], d["v"], d["g"], do, h0=d["h0"], dh_last=dh,
+                                     **kw)
+
+
+def compare_gradients(d, do, dh, dtype, **kw):
+    got = gradients(d, do, dh, **kw)
+    ref = M.linear_backward(**{n: None if t is None else np64(t) for n, t in d.items()},
+                            do=np64(do), dh_last=None if dh is None else np64(dh), **kw)
+    for name, x, y in zip(NAMES, got, ref):
+        if name == "dh0" and d["h0"] is None:
+            assert x is None
+        else:
+            assert_close(x, y, TOL[dtype] if name in ("dq", "dk", "dv") else TOL[F32], name)
+    return got
+
+
+def check_gradients(dev, d, dtype, seed, dh=True, **kw):
+    r = torch.Generator().manual_seed(seed)
+    B, L, Hv, V = d["v"].shape
+    K = d["q"].shape[-1]
+    do = torch.randn(B, L, Hv, V, generator=r).to(dtype).to(dev)
+    dh = torch.randn(B, Hv, K, V, generator=r).to(dev) if dh else None
+    return do, dh, compare_gradients(d, do, dh, dtype, **kw)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("B,L,Hk,Hv,K,V", SIZES)
+def test_backward(dev, dtype, B, L, Hk, Hv, K, V):
+    d = inputs(dev, B, L, Hk, Hv, K, V, dtype, seed=L + K, h0=L % 2 == 1)
+    check_gradients(dev, d, dtype, seed=V, dh=L % 2 == 1)
+
+
+@pytest.mark.parametrize("dtype,B,L,Hk,Hv,K,V,rate", [
+    (BF16, 1, 6000, 1, 2, 64, 64, 0.05), (F32, 1, 3001, 1, 1, 40, 72, 0.05),
+    (F16, 1, 2500, 1, 1, 128, 30, 0.02)])
+def test_backward_segments(dev, dtype, B, L, Hk, Hv, K, V, rate):
+    d = inputs(dev, B, L, Hk, Hv, K, V, dtype, seed=L, h0=True, rate=rate)
+    check_gradients(dev, d, dtype, seed=1)
+
+
+@pytest.mark.parametrize("dtype,B,L,Hk,Hv,K,V", [
+    (BF16, 2, 70, 2, 4, 128, 128), (BF16, 1, 33, 1, 3, 128, 72), (BF16, 1, 3000, 1, 2, 128, 64),
+    (F16, 2, 100, 1, 2, 128, 128), (BF16, 1, 5000, 1, 1, 24, 20), (F32, 1, 70, 1, 2, 128, 200),
+    (F32, 1, 100, 1, 3, 64, 130)])
+def test_backward_wide(dev, dtype, B, L, Hk, Hv, K, V):
+    """Keys of 128, shared key heads, V in several slices, segments."""
+    d = inputs(dev, B, L, Hk, Hv, K, V, dtype, seed=L + V, h0=True, rate=0.1)
+    check_gradients(dev, d, dtype, seed=27)
+
+
+@pytest.mark.parametrize("rate", [30.0, 1.0, 0.01])
+def test_gradient_of_the_decays(dev, rate):
+    """dg alone at strong and slow decays: each chunk sums its own terms, so that what
+    strong decays leave is not the difference of large sums."""
+    d = inputs(dev, 1, 700, 1, 2, 32, 32, F32, seed=31, h0=True, rate=rate)
+    check_gradients(dev, d, F32, seed=32)
+
+
+def test_backward_resets(dev):
+    """g = -inf and the lowest value: nothing flows past, and dg is 0 there."""
+    d = inputs(dev, 2, 150, 1, 2, 64, 48, F32, seed=33, h0=True, rate=0.1)
+    d["g"][0, 40], d["g"][0, 64] = -float("inf"), -float("inf")
+    d["g"][1, 41] = torch.finfo(F32).min
+    dg = check_gradients(dev, d, F32, seed=34)[2][3]
+    assert not dg[0, 40].any() and not dg[0, 64].any() and not dg[1, 41].any()
+
+
+def test_backward_against_differences(dev):
+    """Central differences of the forward itself, in fp32: a step of 2^-6 of inputs of
+    size 1 leaves a truncation of 2^-12 / 6 of third derivatives (none in q, k, v and
+    h0, of which the loss is linear one at a time) and a rounding of 64 x 2^-24 of the
+    loss over the step: 1e-3 of the largest gradient holds both."""
+    B, L, H, K, V = 1, 9, 1, 5, 4
+    d = inputs(dev, B, L, H, H, K, V, F32, seed=35, h0=True)
+    r = torch.Generator().manual_seed(36)
+    do = torch.randn(B, L, H, V, generator=r).to(dev)
+    dh = torch.randn(B, H, K, V, generator=r).to(dev)
+
+    def loss():
+        o, S = run(d)
+        return float((o.double() * do.double()).sum() + (S.double() * dh.double()).sum())
+
+    for name, got in zip(("q", "k", "v", "g", "h0"), gradients(d, do, dh)):
+        flat, want, eps = d[name].view(-1), [], 2.0 ** -6
+        for i in range(flat.numel()):
+            old = flat[i].item()
+            flat[i] = old + eps
+            hi = loss()
+            flat[i] = old - eps
+            lo = loss()
+            flat[i] = old
+            want.append((hi - lo) / (2 * eps))
+        assert_close(got.reshape(-1), np.array(want), 1e-3, name)
+
+
+def one_step(t, layout):
+    """t [B, 1, H, N] as a view whose step stride is no row's length."""
+    B, _, H, N = t.shape
+    if layout == "innermost":       # [B, H, N, L] with L = 1
+        return t.new_empty(B, H, N, 1).permute(0, 3, 1, 2).copy_(t)
+    if layout == "shared":          # one head for all
+        return t[:, 0, 0][:, None].expand(B, H, N).unsqueeze(1)
+    # 31 rows of this stride pass 32 bits
+    return t.contiguous().as_strided(t.shape, (H * N, 1 << 30, N, 1))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("layout", ["innermost", "shared", "far"])
+def test_backward_of_one_step(dev, dtype, layout):
+    """The stride of a dimension of one element says nothing."""
+    r = torch.Generator().manual_seed(22)
+    d = inputs(dev, 2, 1, 3, 3, 32, 32, dtype, seed=21, h0=True)
+    do = torch.randn(2, 1, 3, 32, generator=r).to(dtype).to(dev)
+    dh = torch.randn(2, 3, 32, 32, generator=r).to(dev)
+    for n in ("q", "k", "v"):
+        d[n] = one_step(d[n], layout)
+    compare_gradients(d, one_step(do, layout), dh, dtype)
+
+
+def test_backward_strides(dev):
+    """Slices of one projection, rows that overlap, steps further apart than a chunk's
+    31 bits reach, shared rates, an expanded gradient."""
+    B, L, H, K, V = 2, 77, 2, 32, 32
+    d = inputs(dev, B, L, H, H, K, V, F32, seed=5, h0=True)
+    packed = torch.zeros(B, L, H * (2 * K + V) + 3, device=dev)
+    for name, at in (("q", 0), ("k", H * K), ("v", 2 * H * K)):
+        view = packed[..., at + 1:at + 1 + H * K].view(B, L, H, K)
+        view.copy_(d[name])
+        d[name] = view
+    d["g"] = d["g"][:1, :1].expand(B, L, H)
+    check_gradients(dev, d, F32, seed=6)
+    d["k"] = d["k"][:, :1].expand(B, L, H, K)
+    compare_gradients(d, torch.ones(B, 1, H, V, device=dev).expand(B, L, H, V), None, F32)
+    far = 17_000_000
+    base = torch.empty(3 * H * K + 2 * far, device=dev)
+    e = {n: t if t is None or n == "h0" else t[:1, :3] for n, t in d.items()}
+    e["h0"] = d["h0"][:1]
+    for i, n in enumerate(("q", "k", "v")):
+        view = base.as_strided((1, 3, H, K), (1, far, K, 1), i * H * K)
+        view.copy_(e[n])
+        e[n] = view
+    check_gradients(dev, e, F32, seed=7)
+
+
+def test_backward_empty_and_repeat(dev):
+    d = inputs(dev, 2, 0, 2, 2, 32, 32, F32, h0=True)
+    dh = torch.ones_like(d["h0"])
+    assert torch.equal(gradients(d, d["v"], dh)[4], dh)
+    assert not gradients(d, d["v"])[4].any()
+    for L in (300, 9000):
+        d = inputs(dev, 1, L, 1, 2, 64, 64, BF16, seed=41)
+        do = d["v"].flip(1).contiguous()
+        want = gradients(d, do)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            got = gradients(d, do)
+        torch.cuda.current_stream().wait_stream(side)
+        assert all(x is y is None or torch.equal(x, y) for x, y in zip(got, want))

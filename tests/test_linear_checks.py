@@ -38,6 +38,30 @@ def test_workspace():
     assert f(1, 4, 2, 3, 8, 8) == -2 and f(1, 4, 1, 1, 129, 8) == -6
 
 
+def test_backward_status():
+    L = _lib.lib()
+
+    def back(dtype=1, q=P, dg=P, B=2, n=400, Hk=2, Hv=4, K=64, V=64, sq=512, sv=256, ws=P,
+             nbytes=1 << 40):
+        s = [0, sq, 64, 0, sq, 64, 0, sv, 64, 0, 4, 1, 0, sv, 64]
+        return L.tssm_linear_attention_backward(dtype, q, P, P, P, None, P, None, P, P, P, dg,
+                                                None, B, n, Hk, Hv, K, V, *s, 0.125, ws, nbytes,
+                                                None)
+
+    assert back(dtype=5) == -4 and back(q=None) == -1 and back(dg=None) == -1
+    assert back(Hv=3) == -2 and back(K=129) == -6 and back(V=1 << 22) == -6
+    assert back(sq=8) == -3 and back(sv=0) == -3        # rows that overlap
+    assert back(sq=1 << 24) == -3                       # too far apart
+    assert back(ws=None) == -5 and back(nbytes=1 << 10) == -5 and back(ws=P + 8) == -5
+    assert back(B=0) == 0 and back(n=0) == 0
+    f = L.tssm_linear_attention_backward_workspace_bytes
+    assert f(1, 2, 400, 2, 4, 64, 64) > L.tssm_linear_attention_workspace_bytes(2, 400, 2, 4, 64,
+                                                                               64)
+    assert f(0, 2, 384, 2, 4, 128, 64) == 2 * f(1, 2, 384, 2, 4, 128, 64)   # chunks of 32
+    assert f(3, 1, 4, 1, 1, 8, 8) == -4 and f(1, 1, 4, 2, 3, 8, 8) == -2
+    assert f(1, 1, 4, 1, 1, 129, 8) == -6
+
+
 class On(torch.Tensor):
     """A CPU tensor that is on device ``dev`` by its own account."""
     dev = 0
@@ -111,6 +135,24 @@ def test_shapes_and_types():
         forward(dict(operands(), q=None))
     with pytest.raises(ValueError, match="HIP device"):
         forward(dict(operands(), q=torch.zeros(2, 5, 2, 8)))
+
+
+def test_backward_refusals():
+    d, do = operands(), on(torch.zeros(2, 5, 4, 6))
+
+    def back(do, **kw):
+        return linear.linear_attention_backward(d["q"], d["k"], d["v"], d["g"], do, **kw)
+
+    with pytest.raises(ValueError, match="do must be"):
+        back(on(torch.zeros(2, 5, 4, 7)))
+    with pytest.raises(TypeError, match="do must be"):
+        back(do.half())
+    with pytest.raises(ValueError, match="do must be on device 0"):
+        back(on(torch.zeros(2, 5, 4, 6), True))
+    with pytest.raises(ValueError, match="dh_last must be"):
+        back(do, dh_last=on(torch.zeros(2, 4, 6, 8)))
+    with pytest.raises(ValueError, match="dh_last must be on device 0"):
+        back(do, dh_last=on(torch.zeros(2, 4, 8, 6), True))
 
 
 def test_states_and_outputs():

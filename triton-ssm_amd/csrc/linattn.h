@@ -46,5 +46,19 @@ struct LinPlan {
 int lin_walk_launch(int dtype, const LinArgs& a, bool vec, const LinPlan& p, hipStream_t s);
 // The segments' entry states, forward.
 int lin_entry_launch(int dtype, const LinArgs& a, bool vec, const LinPlan& p, hipStream_t s);
+// The states before the chunks and the gradients of those after them (way: q for k, dO
+// for v, dh_last for h0, dh0 for h_last), segments included.
+int lin_states_launch(int dtype, const LinArgs& a, const LinArgs& way, bool vec, const LinPlan& p,
+                      hipStream_t s);
+int64_t lin_state_steps(int dtype, int64_t K);  // steps of such a chunk
+// Gradients of the inputs; outputs contiguous, dO with strides.
+struct LinGrads {
+  const void* dout;
+  int64_t d_b, d_l, d_h;
+  void *dq, *dk, *dv;
+  float* dg;
+};
+int lin_grads_launch(int dtype, const LinArgs& a, const LinGrads& d, bool vec, const LinPlan& p,
+                     hipStream_t s);
 
 }  // namespace tssm

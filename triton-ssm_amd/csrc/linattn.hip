@@ -22,7 +22,10 @@ int64_t segments(int64_t heads, int64_t L, int64_t V) {
   return want < most ? want : most;
 }
 
-LinPlan lin_plan(char* base, int64_t B, int64_t L, int64_t Hv, int64_t K, int64_t V) {
+// The chunked form's plan over a workspace at base (which may be null: sizes).  chunk:
+// steps between the states that the gradients keep, 0 for the forward.
+LinPlan lin_plan(char* base, int64_t B, int64_t L, int64_t Hv, int64_t K, int64_t V,
+                 int64_t chunk) {
   LinPlan p = {};
   const int64_t heads = B * Hv, elems = (K <= 32 ? 32 : (K <= 64 ? 64 : 128)) * cdiv64(V, 32) * 32;
   int64_t at = 0;
@@ -37,6 +40,14 @@ LinPlan lin_plan(char* base, int64_t B, int64_t L, int64_t Hv, int64_t K, int64_
   if (p.nseg > 1) {
     p.ends = reinterpret_cast<float*>(take(heads * p.nseg * elems * 4));
     p.sums = reinterpret_cast<double*>(take(heads * p.nseg * 8));
+    if (chunk) {
+      p.back = reinterpret_cast<float*>(take(heads * p.nseg * elems * 4));
+      p.back_sums = reinterpret_cast<double*>(take(heads * p.nseg * 8));
+    }
+  }
+  if (chunk) {
+    p.states = reinterpret_cast<float*>(take(heads * cdiv64(L, chunk) * elems * 4));
+    p.grads = reinterpret_cast<float*>(take(heads * cdiv64(L, chunk) * elems * 4));
   }
   p.bytes = at;
   return p;
@@ -73,7 +84,7 @@ extern "C" int64_t tssm_linear_attention_workspace_bytes(int64_t nbatch, int64_t
   if (!sizes_ok(nbatch, L, Hk, Hv, K, V)) return TSSM_ERR_SHAPE;
   if (!takes(K, V)) return TSSM_ERR_UNSUPPORTED;
   if (nbatch == 0 || by_steps(nbatch * Hv, L)) return 0;
-  return lin_plan(nullptr, nbatch, L, Hv, K, V).bytes;
+  return lin_plan(nullptr, nbatch, L, Hv, K, V, 0).bytes;
 }
 
 extern "C" int tssm_linear_attention_forward(
@@ -94,7 +105,7 @@ extern "C" int tssm_linear_attention_forward(
   hipStream_t st = as_stream(stream);
   if (by_steps(nbatch * Hv, L) || !chunk_rows(dtype, a)) return lin_seq_launch(dtype, a, st);
   TSSM_CHECK(L < (INT64_C(1) << 31) && nbatch <= 0x7fffffff / Hv, TSSM_ERR_UNSUPPORTED);
-  const LinPlan p = lin_plan(reinterpret_cast<char*>(workspace), nbatch, L, Hv, K, V);
+  const LinPlan p = lin_plan(reinterpret_cast<char*>(workspace), nbatch, L, Hv, K, V, 0);
   TSSM_CHECK(p.bytes == 0 || (workspace && workspace_bytes >= p.bytes && aligned(workspace, 256)),
              TSSM_ERR_WORKSPACE);
   const bool vec = vec_rows(dtype, a);
@@ -117,4 +128,61 @@ extern "C" int tssm_linear_attention_step(int dtype, const void* q, const void* 
                      sq_s, 0, sq_h, sk_s, 0, sk_h, sv_s, 0, sv_h,
                      sg_s, 0, sg_h, so_s, 0, so_h, scale};
   return lin_seq_launch(dtype, a, as_stream(stream));
+}
+
+extern "C" int64_t tssm_linear_attention_backward_workspace_bytes(int dtype, int64_t nbatch,
+                                                                  int64_t L, int64_t Hk,
+                                                                  int64_t Hv, int64_t K,
+                                                                  int64_t V) {
+  if (dtype < TSSM_F32 || dtype > TSSM_F16) return TSSM_ERR_DTYPE;
+  if (!sizes_ok(nbatch, L, Hk, Hv, K, V)) return TSSM_ERR_SHAPE;
+  if (!takes(K, V)) return TSSM_ERR_UNSUPPORTED;
+  if (L == 0 || nbatch == 0) return 256;
+  return lin_plan(nullptr, nbatch, L, Hv, K, V, lin_state_steps(dtype, K)).bytes;
+}
+
+extern "C" int tssm_linear_attention_backward(
+    int dtype, const void* q, const void* k, const void* v, const float* g, const float* h0,
+    const void* dout, const float* dh_last, void* dq, void* dk, void* dv, float* dg, float* dh0,
+    int64_t nbatch, int64_t L, int64_t Hk, int64_t Hv, int64_t K, int64_t V, int64_t sq_b,
+    int64_t sq_l, int64_t sq_h, int64_t sk_b, int64_t sk_l, int64_t sk_h, int64_t sv_b,
+    int64_t sv_l, int64_t sv_h, int64_t sg_b, int64_t sg_l, int64_t sg_h, int64_t sd_b,
+    int64_t sd_l, int64_t sd_h, float scale, void* workspace, int64_t workspace_bytes,
+    void* stream) {
+  TSSM_CHECK(dtype >= TSSM_F32 && dtype <= TSSM_F16, TSSM_ERR_DTYPE);
+  TSSM_CHECK(sizes_ok(nbatch, L, Hk, Hv, K, V), TSSM_ERR_SHAPE);
+  TSSM_CHECK(takes(K, V), TSSM_ERR_UNSUPPORTED);
+  if (nbatch == 0 || L == 0) return TSSM_OK;
+  TSSM_CHECK(q && k && v && g && dout && dq && dk && dv && dg, TSSM_ERR_NULL);
+  TSSM_CHECK(L < (INT64_C(1) << 31) && nbatch <= 0x7fffffff / Hv, TSSM_ERR_UNSUPPORTED);
+  // (no outputs: o stands for dV in the checks of rows, as they are read)
+  LinArgs a = {q, k, v, g, h0, dv, nullptr, nbatch, L, Hk, Hv, K, V,
+               sq_b, sq_l, sq_h, sk_b, sk_l, sk_h, sv_b, sv_l, sv_h,
+               sg_b, sg_l, sg_h, V, V, V, scale};
+  if (L == 1) {  // the strides of one step say nothing: those that chunks are read by
+    a.q_l = a.k_l = K;
+    a.v_l = sd_l = V;
+  }
+  TSSM_CHECK(chunk_rows(dtype, a) && fits(dtype, sd_l, V), TSSM_ERR_STRIDE);
+  const LinPlan p = lin_plan(reinterpret_cast<char*>(workspace), nbatch, L, Hv, K, V,
+                             lin_state_steps(dtype, K));
+  TSSM_CHECK(workspace && workspace_bytes >= p.bytes && aligned(workspace, 256),
+             TSSM_ERR_WORKSPACE);
+  LinArgs way = a;  // the way back reads queries for keys and dO for v
+  way.k = q;
+  way.k_b = sq_b;
+  way.k_l = a.q_l;
+  way.k_h = sq_h;
+  way.v = dout;
+  way.v_b = sd_b;
+  way.v_l = sd_l;
+  way.v_h = sd_h;
+  way.h0 = dh_last;
+  way.h_last = dh0;
+  const LinGrads d = {dout, sd_b, sd_l, sd_h, dq, dk, dv, dg};
+  // (the gradients of the inputs are written as the inputs are read)
+  const bool vec = vec_rows(dtype, a) && vec_rows(dtype, way) && aligned(dq, 16) && aligned(dk, 16);
+  hipStream_t st = as_stream(stream);
+  const int rc = lin_states_launch(dtype, a, way, vec, p, st);
+  return rc ? rc : lin_grads_launch(dtype, a, d, vec, p, st);
 }

@@ -1,4 +1,5 @@
-// Linear attention, chunked: the segments of a long sequence and how they are joined.
+// Linear attention, chunked: the segments of a long sequence and how they are joined,
+// and for the gradients the states before the chunks and the gradients after them.
 #include "linattn_walk.h"
 
 namespace tssm {
@@ -54,18 +55,65 @@ int fold(const LinArgs& a, float* ends, const double* sums, int nseg, int rev, h
   return launch_status();
 }
 
-}  // namespace
+template <typename T, int MODE>
+int by_keys(const LinWalkArgs& f, const LinWalkArgs& b, bool vec, hipStream_t s) {
+#define TSSM_WALK(KP) \
+  (vec ? lin_states<T, KP, true, MODE>(f, b, s) : lin_states<T, KP, false, MODE>(f, b, s))
+  if (f.a.K <= 32) return TSSM_WALK(32);
+  if (f.a.K <= 64) return TSSM_WALK(64);
+  return TSSM_WALK(128);
+#undef TSSM_WALK
+}
 
-int lin_entry_launch(int dtype, const LinArgs& a, bool vec, const LinPlan& p, hipStream_t s) {
+template <int MODE>
+int walk(int dtype, const LinWalkArgs& f, const LinWalkArgs& b, bool vec, hipStream_t s) {
+  switch (dtype) {
+    case TSSM_F32: return by_keys<float, MODE>(f, b, vec, s);
+    case TSSM_BF16: return by_keys<bf16_t, MODE>(f, b, vec, s);
+    default: return by_keys<f16_t, MODE>(f, b, vec, s);
+  }
+}
+
+// The walk of all segments but the last one (forward) or the first (back).
+LinWalkArgs ends_of(const LinArgs& a, const LinPlan& p, bool rev) {
   LinWalkArgs g = {};
   g.a = a;
   g.steps = p.steps;
   g.nseg = (int)p.nseg;
   g.walked = g.nseg - 1;
-  g.states = p.ends;
-  g.sums = p.sums;
-  const int rc = lin_walk_mode<kEnds>(dtype, g, vec, s);
-  return rc ? rc : fold(a, p.ends, p.sums, g.nseg, 0, s);
+  g.first = rev ? 1 : 0;
+  g.states = rev ? p.back : p.ends;
+  g.sums = rev ? p.back_sums : p.sums;
+  return g;
 }
+
+}  // namespace
+
+int lin_entry_launch(int dtype, const LinArgs& a, bool vec, const LinPlan& p, hipStream_t s) {
+  LinWalkArgs none = ends_of(a, p, false);
+  none.walked = 0;
+  const int rc = walk<kEnds>(dtype, ends_of(a, p, false), none, vec, s);
+  return rc ? rc : fold(a, p.ends, p.sums, (int)p.nseg, 0, s);
+}
+
+int lin_states_launch(int dtype, const LinArgs& a, const LinArgs& way, bool vec, const LinPlan& p,
+                      hipStream_t s) {
+  LinWalkArgs f = ends_of(a, p, false), b = ends_of(way, p, true);
+  if (p.nseg > 1) {
+    int rc = walk<kEnds>(dtype, f, b, vec, s);
+    if (!rc) rc = fold(a, p.ends, p.sums, (int)p.nseg, 0, s);
+    if (!rc) rc = fold(way, p.back, p.back_sums, (int)p.nseg, 1, s);
+    if (rc) return rc;
+  }
+  f.walked = b.walked = (int)p.nseg;
+  b.first = 0;
+  f.entry = p.ends;
+  b.entry = p.back;
+  f.states = p.states;
+  b.states = p.grads;
+  return walk<kStates>(dtype, f, b, vec, s);
+}
+
+int64_t lin_state_steps(int dtype, int64_t K) { return dtype == TSSM_F32 && K > 64 ? 32 : 64; }
 
 }  // namespace tssm

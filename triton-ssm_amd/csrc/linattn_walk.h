@@ -43,7 +43,6 @@ struct LinWalkArgs {
   int64_t steps;
   int nseg;
   int first, walked;   // the segments that are walked
-  int rev;
   int nch, per;        // chunks, chunks of a segment        (the launch sets these)
   uint32_t nvb, units; // blocks of 32 columns; heads times segments walked
   const float* entry;  // [bh][nseg][state]
@@ -71,16 +70,15 @@ struct LinWalk {
   };
 };
 
-template <typename T, int KP, bool VEC, int C, int MODE>
-__global__ __launch_bounds__(4 * C) void lin_walk_kernel(LinWalkArgs g) {
+template <typename T, int KP, bool VEC, int C, int MODE, bool REV>
+__device__ inline void lin_walk_body(const LinWalkArgs& g, char* smem, uint32_t id) {
   typedef LinWalk<T, KP, C, MODE> W;
   constexpr int NP = W::NP, NO = W::NO, NS = W::NS, KT = W::KT, NT = W::NT, NIQ = W::NIQ,
                 OWN = W::OWN, kE = (int)sizeof(T);
-  extern __shared__ char smem[];
   typename W::Lds& lds = *reinterpret_cast<typename W::Lds*>(smem);
   const LinArgs& a = g.a;
   // workgroups of one head's segment, which share Q and K, on one XCD
-  const uint32_t id = block_of(), vb = (id >> 3) % g.nvb, u = (id >> 3) / g.nvb * 8 + (id & 7);
+  const uint32_t vb = (id >> 3) % g.nvb, u = (id >> 3) / g.nvb * 8 + (id & 7);
   if (u >= g.units) return;
   const int64_t bh = u / (uint32_t)g.walked;
   const int seg = g.first + (int)(u - (uint32_t)bh * (uint32_t)g.walked);
@@ -112,7 +110,7 @@ __global__ __launch_bounds__(4 * C) void lin_walk_kernel(LinWalkArgs g) {
   } in;
   const auto chunk = [&](int m) {   // the chunk of step m of the walk
     const int x = m < cnt ? m : cnt - 1;
-    return g.rev ? n1 - 1 - x : n0 + x;
+    return REV ? n1 - 1 - x : n0 + x;
   };
   const auto fetch = [&](int m) {
     const int n = chunk(m);
@@ -278,7 +276,7 @@ __global__ __launch_bounds__(4 * C) void lin_walk_kernel(LinWalkArgs g) {
     // this wave's 32 steps of K^T V
     float v8[8], e8[8];
     lds_values<NP>(&B.V[0][0], C * W::kVld, W::kVld, 32 * iq, 16 * vt, lane, v8);
-    if (g.rev) {
+    if constexpr (REV) {
       float h8[8], l8[8];
       lds8(&B.d.hi[32 * iq + 8 * j], h8);
       lds8(&B.d.lo[32 * iq + 8 * j], l8);
@@ -385,7 +383,7 @@ __global__ __launch_bounds__(4 * C) void lin_walk_kernel(LinWalkArgs g) {
 #pragma unroll
     for (int i = 0; i < OWN; ++i) *reinterpret_cast<f32x4*>(p + 256 * i) = S[i];
     if (vb == 0 && threadIdx.x == 0) g.sums[bh * g.nseg + seg] = total;
-  } else if (g.rev ? n0 == 0 : n1 == g.nch) {
+  } else if (REV ? n0 == 0 : n1 == g.nch) {
     float* p = a.h_last ? a.h_last + bh * K * a.V : nullptr;
 #pragma unroll
     for (int i = 0; i < OWN; ++i) put_tile(p, S[i], iq * OWN + i, col, a.V, K, j);
@@ -400,43 +398,70 @@ constexpr int kWalkSteps = kPlanes<T> == 1 && KP == 64 ? 128
 template <typename T, int KP>
 constexpr int kStateSteps = kPlanes<T> == 3 && KP == 128 ? 32 : 64;
 
+template <typename T, int KP, bool VEC>
+__global__ __launch_bounds__((4 * kWalkSteps<T, KP>)) void lin_walk_kernel(LinWalkArgs g) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  lin_walk_body<T, KP, VEC, kWalkSteps<T, KP>, kOutputs, false>(g, smem, block_of());
+}
+
+// The states' walk and its way back, side by side: the first nf workgroups go forward.
 template <typename T, int KP, bool VEC, int MODE>
-int lin_walk(LinWalkArgs g, hipStream_t s) {
-  constexpr int C = MODE == kOutputs ? kWalkSteps<T, KP> : kStateSteps<T, KP>;
-  typedef LinWalk<T, KP, C, MODE> W;
+__global__ __launch_bounds__((4 * kStateSteps<T, KP>)) void lin_states_kernel(LinWalkArgs f,
+                                                                              LinWalkArgs back,
+                                                                              uint32_t nf) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const uint32_t id = block_of();
+  if (id < nf)
+    lin_walk_body<T, KP, VEC, kStateSteps<T, KP>, MODE, false>(f, smem, id);
+  else
+    lin_walk_body<T, KP, VEC, kStateSteps<T, KP>, MODE, true>(back, smem, id - nf);
+}
+
+// Sizes that a launch sets; returns its workgroups, or -1.
+inline int64_t lin_walk_sizes(LinWalkArgs& g, int C) {
   g.nvb = (uint32_t)cdiv64(g.a.V, 32);
   g.nch = (int)cdiv64(g.a.L, C);
   g.per = (int)cdiv64(g.steps, C);
   const int64_t units = g.a.B * g.a.Hv * g.walked, wgs = cdiv64(units, 8) * 8 * g.nvb;
-  if (wgs > 0x7fffffff) return TSSM_ERR_UNSUPPORTED;
+  if (wgs > 0x3fffffff) return -1;
   g.units = (uint32_t)units;
-  if (g.walked == 0) return TSSM_OK;
-  static_assert(sizeof(typename W::Lds) <= 163840, "LDS of one workgroup");
-  const auto kernel = lin_walk_kernel<T, KP, VEC, C, MODE>;
-  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                           hipFuncAttributeMaxDynamicSharedMemorySize,
-                                           (int)sizeof(typename W::Lds));
-  if (e != hipSuccess) return (int)e;
+  return wgs;
+}
+
+template <typename K>
+int lin_lds(K kernel, int bytes) {
+  return bytes <= 65536 ? TSSM_OK
+                        : (int)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                                   hipFuncAttributeMaxDynamicSharedMemorySize,
+                                                   bytes);
+}
+
+template <typename T, int KP, bool VEC>
+int lin_walk(LinWalkArgs g, hipStream_t s) {
+  typedef LinWalk<T, KP, kWalkSteps<T, KP>, kOutputs> W;
+  static_assert(sizeof(typename W::Lds) <= 160 * 1024, "LDS of a CU");
+  const int64_t wgs = lin_walk_sizes(g, kWalkSteps<T, KP>);
+  if (wgs < 0) return TSSM_ERR_UNSUPPORTED;
+  const auto kernel = lin_walk_kernel<T, KP, VEC>;
+  const int rc = lin_lds(kernel, (int)sizeof(typename W::Lds));
+  if (rc) return rc;
   kernel<<<grid_of(wgs), W::NT, sizeof(typename W::Lds), s>>>(g);
   return launch_status();
 }
 
-template <typename T, int MODE>
-int lin_walk_keys(const LinWalkArgs& g, bool vec, hipStream_t s) {
-#define TSSM_WALK(KP) (vec ? lin_walk<T, KP, true, MODE>(g, s) : lin_walk<T, KP, false, MODE>(g, s))
-  if (g.a.K <= 32) return TSSM_WALK(32);
-  if (g.a.K <= 64) return TSSM_WALK(64);
-  return TSSM_WALK(128);
-#undef TSSM_WALK
-}
-
-template <int MODE>
-int lin_walk_mode(int dtype, const LinWalkArgs& g, bool vec, hipStream_t s) {
-  switch (dtype) {
-    case TSSM_F32: return lin_walk_keys<float, MODE>(g, vec, s);
-    case TSSM_BF16: return lin_walk_keys<bf16_t, MODE>(g, vec, s);
-    default: return lin_walk_keys<f16_t, MODE>(g, vec, s);
-  }
+// back.walked = 0: forward alone.
+template <typename T, int KP, bool VEC, int MODE>
+int lin_states(LinWalkArgs f, LinWalkArgs back, hipStream_t s) {
+  typedef LinWalk<T, KP, kStateSteps<T, KP>, MODE> W;
+  static_assert(sizeof(typename W::Lds) <= 160 * 1024, "LDS of a CU");
+  const int64_t nf = lin_walk_sizes(f, kStateSteps<T, KP>);
+  const int64_t nb = lin_walk_sizes(back, kStateSteps<T, KP>);
+  if (nf < 0 || nb < 0) return TSSM_ERR_UNSUPPORTED;
+  const auto kernel = lin_states_kernel<T, KP, VEC, MODE>;
+  const int rc = lin_lds(kernel, (int)sizeof(typename W::Lds));
+  if (rc) return rc;
+  kernel<<<grid_of(nf + nb), W::NT, sizeof(typename W::Lds), s>>>(f, back, (uint32_t)nf);
+  return launch_status();
 }
 
 }  // namespace

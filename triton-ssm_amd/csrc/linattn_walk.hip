@@ -2,6 +2,18 @@
 #include "linattn_walk.h"
 
 namespace tssm {
+namespace {
+
+template <typename T>
+int by_keys(const LinWalkArgs& g, bool vec, hipStream_t s) {
+#define TSSM_WALK(KP) (vec ? lin_walk<T, KP, true>(g, s) : lin_walk<T, KP, false>(g, s))
+  if (g.a.K <= 32) return TSSM_WALK(32);
+  if (g.a.K <= 64) return TSSM_WALK(64);
+  return TSSM_WALK(128);
+#undef TSSM_WALK
+}
+
+}  // namespace
 
 int lin_walk_launch(int dtype, const LinArgs& a, bool vec, const LinPlan& p, hipStream_t s) {
   LinWalkArgs g = {};
@@ -9,7 +21,11 @@ int lin_walk_launch(int dtype, const LinArgs& a, bool vec, const LinPlan& p, hip
   g.steps = p.steps;
   g.nseg = g.walked = (int)p.nseg;
   g.entry = p.ends;
-  return lin_walk_mode<kOutputs>(dtype, g, vec, s);
+  switch (dtype) {
+    case TSSM_F32: return by_keys<float>(g, vec, s);
+    case TSSM_BF16: return by_keys<bf16_t>(g, vec, s);
+    default: return by_keys<f16_t>(g, vec, s);
+  }
 }
 
 }  // namespace tssm

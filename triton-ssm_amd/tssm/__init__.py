@@ -18,7 +18,8 @@ from .delta import gated_delta_backward, gated_delta_forward, gated_delta_step  
 from .fused import (fused_interp_ssm_forward, multihead_ssm_forward,  # noqa: F401
                     selective_scan_forward, ssd_scan_forward, ssd_stream_step)
 from .groupnorm import group_norm_act_backward, group_norm_act_forward  # noqa: F401
-from .linear import linear_attention_forward, linear_attention_step  # noqa: F401
+from .linear import (linear_attention_backward, linear_attention_forward,  # noqa: F401
+                     linear_attention_step)
 from .qknorm import (qk_norm_rotary_backward, qk_norm_rotary_forward,  # noqa: F401
                      rotary_amplitude, rotary_frequencies)
 from .workspace import check  # noqa: F401
@@ -26,7 +27,7 @@ from .workspace import check  # noqa: F401
 __all__ = ["multihead_ssm_forward", "selective_scan_forward", "ssd_scan_forward",
            "ssd_stream_step", "fused_interp_ssm_forward", "time_aware_interp_corrected",
            "streaming_interp_step_corrected", "gated_delta_forward", "gated_delta_backward",
-           "gated_delta_step", "linear_attention_forward", "linear_attention_step",
-           "qk_norm_rotary_forward", "qk_norm_rotary_backward", "rotary_frequencies",
+           "gated_delta_step", "linear_attention_forward",
+           "linear_attention_backward", "linear_attention_step", "qk_norm_rotary_forward", "qk_norm_rotary_backward", "rotary_frequencies",
            "rotary_amplitude", "group_norm_act_forward", "group_norm_act_backward", "check",
            "TssmError"]

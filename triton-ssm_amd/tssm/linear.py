@@ -92,10 +92,15 @@ def _explain(q, k, v, g, lead):
     return g.to(_F32)
 
 
-def _steps(t):
+def _steps(t, chunks=False):
     """t [B, L, H, N], copied where its steps overlap in memory (as expanded ones
-    do): the chunked kernels take steps that lie one after the other."""
-    return t.contiguous() if t.shape[1] > 1 and t.stride(1) < t.shape[3] else t
+    do): the chunked kernels take steps that lie one after the other.  With
+    ``chunks`` (nothing but chunked kernels) also where a chunk of 128 steps and one
+    more would pass 31 bits."""
+    if t.shape[1] > 1 and (t.stride(1) < t.shape[3] or chunks and
+                           t.stride(1) >= (1 << 31) // (129 * t.element_size())):
+        return t.contiguous()
+    return t
 
 
 def _state(t, what, shape, device):
@@ -150,6 +155,42 @@ def linear_attention_forward(q, k, v, g, *, scale=None, h0=None, return_state=Fa
                   *_rows(v, "v"), *g.stride(), *_rows(o, "out"),
                   K ** -0.5 if scale is None else float(scale))
     return (o, h_last) if return_state else o
+
+
+def linear_attention_backward(q, k, v, g, do, *, scale=None, h0=None, dh_last=None):
+    """Gradients of ``linear_attention_forward`` for its inputs and do [B, L, Hv, V]
+    (dtype of v), the gradient of o, and dh_last [B, Hv, K, V] float32 or None,
+    that of the final state.
+
+    Returns (dq, dk, dv, dg, dh0): dq, dk and dv of q's dtype, dg [B, L, Hv] and dh0
+    float32 (dh0 is None without h0).  dq and dk are summed over the value heads
+    that share a key head; repeated calls give identical bits.  The states are
+    formed again from the inputs: nothing but the inputs needs to be kept between
+    the passes.  An input or gradient that is not finite makes its chunk of 64 steps,
+    and what depends on it, not finite.
+    """
+    (B, L, Hk, Hv, K, V), code, g = _operands(q, k, v, g, 2)
+    dev = q.get_device()
+    _check(do, "do", v.shape, v.dtype, dev)
+    q, k, v, do = (_steps(t, chunks=True) for t in (q, k, v, do))
+    h0, dh_last = _state(h0, "h0", (B, Hv, K, V), dev), \
+        _state(dh_last, "dh_last", (B, Hv, K, V), dev)
+    dq = torch.empty(B, L, Hk, K, device=q.device, dtype=q.dtype)
+    dk, dv = torch.empty_like(dq), torch.empty(B, L, Hv, V, device=q.device, dtype=q.dtype)
+    dg = torch.empty(B, L, Hv, device=q.device, dtype=_F32)
+    dh0 = None if h0 is None else torch.empty(B, Hv, K, V, device=q.device, dtype=_F32)
+    if B and L:
+        nbytes = _lib.lib().tssm_linear_attention_backward_workspace_bytes(code, B, L, Hk, Hv, K,
+                                                                          V)
+        on_device(dev, workspace.call, "tssm_linear_attention_backward", q, stream_handle(q),
+                  nbytes, code, q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), ptr(h0),
+                  do.data_ptr(), ptr(dh_last), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                  dg.data_ptr(), ptr(dh0), B, L, Hk, Hv, K, V, *_rows(q, "q"), *_rows(k, "k"),
+                  *_rows(v, "v"), *g.stride(), *_rows(do, "do"),
+                  K ** -0.5 if scale is None else float(scale))
+    elif dh0 is not None:
+        dh0.zero_() if dh_last is None else dh0.copy_(dh_last)
+    return dq, dk, dv, dg, dh0
 
 
 def linear_attention_step(q, k, v, g, state, *, scale=None, out=None):
