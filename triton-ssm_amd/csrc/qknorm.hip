@@ -13,12 +13,18 @@
 // rate of 1 leaves 20 bits of an fp32 angle before the point), are formed once
 // for a token by the workgroup and shared by its heads through LDS.
 //
+// The forward reaches 4.4 to 5.0 TB/s (B=8 L=4096, 16 + 16 heads of 64, bf16: 54 us;
+// B=4 L=4096, 16 + 8 of 128: 45), a copy 5.15.  It is waves in flight that decide: rows
+// are asked for before the angles are formed, and the weights, which both would hold 32
+// registers, are in LDS (with them in registers and the next rows ahead, 200 registers
+// and two waves a SIMD, 65 us each).
+//
 // A workgroup has TB tokens; a group of LG lanes holds one row, TB groups beside
 // each other take tokens, the others heads, so a lane keeps its token's cosines in
 // registers over the heads it goes through.  A lane holds both members of its
 // pairs: two 16-byte vectors R/2 apart (or next to each other), or, where sizes or
 // alignment do not fit those, single elements.
-#include "common.h"
+#include "planes.h"
 
 namespace tssm {
 namespace {
@@ -147,30 +153,29 @@ struct Part {
 template <int LG>
 __device__ inline float row_sum(float v) { return group_sum<LG>(v); }
 
-constexpr int kThreads = 256, kTable = 4096;  // entries of the table of angles
+constexpr int kThreads = 256, kTable = 1024;  // entries of the table of angles
 
 template <typename T, int FORM, int LG, int NS, bool BACK>
-__global__ __launch_bounds__(kThreads) void qk_kernel(QkArgs a) {
+__global__ __launch_bounds__(kThreads, BACK ? 3 : 1) void qk_kernel(QkArgs a) {
   typedef Part<T, FORM, LG, NS> P;
   typedef Form<T, FORM, LG, NS> F;
-  constexpr int NP = F::NP, NI = BACK ? 2 : 4;  // rows that a lane has in flight
+  constexpr int NP = F::NP, NI = BACK ? 1 : 4;  // rows that a lane has in flight
   constexpr int kGroups = kThreads / LG;
   __shared__ float2 table[kTable];
+  __shared__ __attribute__((aligned(16))) float weights[2 * LG * 2 * NP];
   __shared__ float sums[BACK ? 2 * LG * 2 * NP * 4 : 1];
   const int g = threadIdx.x / LG, l = threadIdx.x % LG, half = a.R / 2;
   const int t = g / a.HS, h0 = g % a.HS;
   const bool on = FORM == kSingle || l * 2 * F::VE < a.K;   // this lane has elements
-  float wq[2 * NP], wk[2 * NP], sq[BACK ? 2 * NP : 1], sk[BACK ? 2 * NP : 1];
-#pragma unroll
-  for (int i = 0; i < NP; ++i) {
+  float sq[BACK ? 2 * NP : 1], sk[BACK ? 2 * NP : 1];
+  // both weights, as a lane reads them: [q, k][lane][2 NP]
+  for (int i = threadIdx.x; i < 2 * LG * 2 * NP; i += kThreads) {
+    const int e = i % (2 * NP), ll = i / (2 * NP) % LG, isk = i / (2 * NP * LG);
     int ea, eb;
-    F::places(a, l, i, ea, eb);
-    if (!on || ea >= a.K) ea = 0;
-    if (!on || eb >= a.K) eb = 0;
-    wq[2 * i] = a.wq ? a.wq[ea] : 1.0f;
-    wq[2 * i + 1] = a.wq ? a.wq[eb] : 1.0f;
-    wk[2 * i] = a.wk ? a.wk[ea] : 1.0f;
-    wk[2 * i + 1] = a.wk ? a.wk[eb] : 1.0f;
+    F::places(a, ll, e / 2, ea, eb);
+    const int at = e & 1 ? eb : ea;
+    const float* w = isk ? a.wk : a.wq;
+    weights[i] = w && at < a.K ? w[at] : 1.0f;
   }
   if constexpr (BACK) {
 #pragma unroll
@@ -179,48 +184,56 @@ __global__ __launch_bounds__(kThreads) void qk_kernel(QkArgs a) {
   const float m = a.norm == TSSM_NORM_RMS ? 1.0f / (float)a.K : (a.norm == TSSM_NORM_L2 ? 1.0f : 0.0f);
   for (uint32_t block = block_of(); block < a.blocks; block += gridDim.x * gridDim.y) {
     const uint32_t first = block * (uint32_t)a.TB;
-    // the table of this block's angles
-    for (int i = threadIdx.x; i < a.TB * half; i += kThreads) {
-      const int tt = i / half, j = i - tt * half;
-      const uint32_t tok = first + (uint32_t)tt < a.tokens ? first + (uint32_t)tt : a.tokens - 1;
-      const uint32_t b = tok / a.L, at = tok - b * a.L;
-      const double turns = position(a, b * a.p_b + at * a.p_l) * a.freq[j] * 0.15915494309189535;
-      float s, c;
-      sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
-      table[i] = make_float2(a.amplitude * c, a.amplitude * s);
-    }
-    __syncthreads();
     const uint32_t tok = first + (uint32_t)t;
     const bool live = tok < a.tokens;
     const uint32_t tk = live ? tok : a.tokens - 1, b = tk / a.L, at = tk - b * a.L;
-    float c[NP], s[NP];
-    bool rot[NP];
-#pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const int j = FORM == kSingle ? l + LG * i : l * F::VE + i;
-      rot[i] = j < half;
-      const float2 x = table[t * half + (rot[i] ? j : 0)];
-      c[i] = rot[i] ? x.x : 1.0f;
-      s[i] = rot[i] ? x.y : 0.0f;
-    }
     const T* q = reinterpret_cast<const T*>(a.q) + b * a.q_b + at * a.q_l;
     const T* k = reinterpret_cast<const T*>(a.k) + b * a.k_b + at * a.k_l;
     T* yq = reinterpret_cast<T*>(a.yq) + b * a.yq_b + at * a.yq_l;
     T* yk = reinterpret_cast<T*>(a.yk) + b * a.yk_b + at * a.yk_l;
     const T* dq = reinterpret_cast<const T*>(a.dq) + (BACK ? b * a.dq_b + at * a.dq_l : 0);
     const T* dk = reinterpret_cast<const T*>(a.dk) + (BACK ? b * a.dk_b + at * a.dk_l : 0);
-    for (int hb = h0; hb < a.H; hb += NI * a.HS) {
-      P x[NI], d[BACK ? NI : 1];
+    P x[NI], d[BACK ? NI : 1];
+    // rows past the last head are this lane's first ones again (no branch: it would
+    // make every load wait)
+    const auto fetch = [&](int hb) {
 #pragma unroll
       for (int n = 0; n < NI; ++n) {
-        const int h = hb + n * a.HS < a.H ? hb + n * a.HS : hb;
+        int h = hb + n * a.HS + h0;
+        h = h < a.H ? h : (h0 < a.H ? h0 : 0);
         x[n].load(a, h < a.Hq ? q + h * a.q_h : k + (h - a.Hq) * a.k_h, l, on);
         if constexpr (BACK)
           d[n].load(a, h < a.Hq ? dq + h * a.dq_h : dk + (h - a.Hq) * a.dk_h, l, on);
       }
+    };
+    fetch(0);  // in flight while the angles are formed
+    // the table of this block's angles
+    for (int i = threadIdx.x; i < a.TB * half; i += kThreads) {
+      const int tt = i / half, j = i - tt * half;
+      const uint32_t tok2 = first + (uint32_t)tt < a.tokens ? first + (uint32_t)tt : a.tokens - 1;
+      const uint32_t b2 = tok2 / a.L, at2 = tok2 - b2 * a.L;
+      const double turns =
+          position(a, b2 * a.p_b + at2 * a.p_l) * a.freq[j] * 0.15915494309189535;
+      float s, c;
+      sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
+      table[i] = make_float2(a.amplitude * c, a.amplitude * s);
+    }
+    lds_barrier();
+    float c[NP], s[NP];
+    bool rot[NP];
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int j = FORM == kSingle ? l + LG * i : l * F::VE + i;
+      rot[i] = j < half;
+      const float2 y = table[t * half + (rot[i] ? j : 0)];
+      c[i] = rot[i] ? y.x : 1.0f;
+      s[i] = rot[i] ? y.y : 0.0f;
+    }
+    for (int hb = 0; hb < a.H; hb += NI * a.HS) {
+      if (hb) fetch(hb);
 #pragma unroll
       for (int n = 0; n < NI; ++n) {
-        const int h = hb + n * a.HS;
+        const int h = hb + n * a.HS + h0;
         if (h >= a.H || !live) continue;   // (whole groups)
         const bool isq = h < a.Hq;
         float u[NP], v[NP], sum = 0.0f, r = 1.0f;
@@ -230,12 +243,16 @@ __global__ __launch_bounds__(kThreads) void qk_kernel(QkArgs a) {
           for (int i = 0; i < NP; ++i) sum = __builtin_fmaf(u[i], u[i], __builtin_fmaf(v[i], v[i], sum));
           r = 1.0f / sqrtf(__builtin_fmaf(row_sum<LG>(sum), m, a.eps));
         }
+        float w[2 * NP];
+        const float* wp = &weights[((isq ? 0 : LG) + l) * 2 * NP];
+#pragma unroll
+        for (int i = 0; i < 2 * NP; ++i) w[i] = wp[i];
         T* out = isq ? yq + h * a.yq_h : yk + (h - a.Hq) * a.yk_h;
         if constexpr (!BACK) {
 #pragma unroll
           for (int i = 0; i < NP; ++i) {
-            const float f = u[i] * r * (isq ? wq[2 * i] : wk[2 * i]);
-            const float e = v[i] * r * (isq ? wq[2 * i + 1] : wk[2 * i + 1]);
+            const float f = u[i] * r * w[2 * i];
+            const float e = v[i] * r * w[2 * i + 1];
             u[i] = rot[i] ? f * c[i] - e * s[i] : f;
             v[i] = rot[i] ? f * s[i] + e * c[i] : e;
           }
@@ -254,8 +271,8 @@ __global__ __launch_bounds__(kThreads) void qk_kernel(QkArgs a) {
               sk[2 * i] += g0;
               sk[2 * i + 1] += g1;
             }
-            f[i] = x0 * (isq ? wq[2 * i] : wk[2 * i]);
-            e[i] = x1 * (isq ? wq[2 * i + 1] : wk[2 * i + 1]);
+            f[i] = x0 * w[2 * i];
+            e[i] = x1 * w[2 * i + 1];
             dot = __builtin_fmaf(f[i], u[i], __builtin_fmaf(e[i], v[i], dot));
           }
           if (a.norm != TSSM_NORM_NONE) dot = row_sum<LG>(dot) * (m * r * r);
@@ -268,7 +285,7 @@ __global__ __launch_bounds__(kThreads) void qk_kernel(QkArgs a) {
         x[n].put(a, out, l, on, u, v);
       }
     }
-    __syncthreads();  // the table is read
+    lds_barrier();  // the table is read
   }
   if constexpr (BACK) {
     if (!a.part) return;
@@ -303,27 +320,38 @@ __global__ __launch_bounds__(kThreads) void qk_kernel(QkArgs a) {
   }
 }
 
-// dw = sum of the workgroups' parts, in order: 16 columns of [rows][n] a workgroup.
-__global__ __launch_bounds__(256) void qk_sum_kernel(const float* part, int rows, int n, int K,
-                                                     float* dwq, float* dwk) {
-  __shared__ float sums[16][16];
+// dw = sum of the workgroups' parts, in order: 16 columns of [rows][n] a workgroup, 64
+// rows at a time, eight loads in flight (768 rows of 2 x 128: 4.5 us).
+__global__ __launch_bounds__(1024) void qk_sum_kernel(const float* part, int rows, int n, int K,
+                                                      float* dwq, float* dwk) {
+  __shared__ float sums[64][17];
   const int c = threadIdx.x & 15, r = threadIdx.x >> 4, col = blockIdx.x * 16 + c;
+  const float* p = part + (col < n ? col : 0);
   float s = 0.0f;
-  if (col < n)
-    for (int i = r; i < rows; i += 16) s += part[(int64_t)i * n + col];
+  for (int i = r; i < rows; i += 8 * 64) {
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = p[(int64_t)(i + 64 * e < rows ? i + 64 * e : i) * n];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s += i + 64 * e < rows ? x[e] : 0.0f;
+  }
   sums[r][c] = s;
   __syncthreads();
   if (r == 0 && col < n) {
-    for (int i = 1; i < 16; ++i) s += sums[i][c];
+    for (int i = 1; i < 64; ++i) s += sums[i][c];
     if (col < K && dwq) dwq[col] = s;
     if (col >= K && dwk) dwk[col - K] = s;
   }
 }
 
-constexpr int64_t kBackGroups = 1024;  // workgroups of the gradients
+// Workgroups of the gradients: the three that a CU holds, each with blocks of its own
+// to go through, so that few sums of the weights' gradients are left to join (16384
+// tokens of 16 + 8 heads of 128, bf16: 68 us; 82 with 1024, which leaves a third of the
+// CUs a workgroup more than the others, 100 with one for each of 4096 blocks).
+constexpr int64_t kBackGroups = 768;
 
 int sum_parts(const QkArgs& a, int rows, hipStream_t st) {
-  qk_sum_kernel<<<(unsigned)cdiv64(2 * a.K, 16), 256, 0, st>>>(a.part, rows, 2 * a.K, a.K, a.dwq,
+  qk_sum_kernel<<<(unsigned)cdiv64(2 * a.K, 16), 1024, 0, st>>>(a.part, rows, 2 * a.K, a.K, a.dwq,
                                                              a.dwk);
   return launch_status();
 }

@@ -89,7 +89,7 @@ def _like(t, what, x):
 
 def _out(t, what, x):
     if t is None:
-        return torch.empty(x.shape, device=x.device, dtype=x.dtype)
+        return torch.empty_like(x, memory_format=torch.contiguous_format)
     _like(t, what, x)
     if any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
         raise ValueError(f"{what}: elements must not share memory")
@@ -109,7 +109,45 @@ def _weight(t, what, K, device):
 
 def _operands(q, k, positions, freqs, weight_q, weight_k, norm):
     """Checks; returns (dtype code, norm code, sizes, positions' pointer, type and
-    strides, freqs, weights)."""
+    strides, freqs, weights).  Decoding calls pay for every check, so what is right
+    passes in one expression, and _explain() names what is not."""
+    R, pos = 0, (None, 0, 0, 0)
+    try:
+        dev, dtype, sq, sk = q.get_device(), q.dtype, q.shape, k.shape
+        lead, K = sq[:-2], sq[-1]
+        right = (dev >= 0 and 3 <= len(sq) <= 4 and sk[:-2] == lead and sk[-1] == K
+                 and dtype == k.dtype and dtype in DTYPES and k.get_device() == dev
+                 and sq[-2] and sk[-2] and (1 < K <= 256 or K == 1 and norm == "none")
+                 and norm in _NORM)
+        if right and freqs is not None:
+            R = 2 * freqs.shape[0]
+            right = (freqs.dim() == 1 and freqs.dtype == torch.float64 and R <= K
+                     and freqs.is_contiguous() and positions.shape == lead
+                     and positions.dtype in _POS and freqs.get_device() == dev
+                     and positions.get_device() == dev)
+        elif positions is not None:
+            right = False
+        for w in (weight_q, weight_k):
+            if w is not None and not (w.shape == (K,) and w.dtype == torch.float32
+                                      and w.get_device() == dev and w.is_contiguous()):
+                right = False
+    except (AttributeError, TypeError, IndexError):
+        right = False
+    if not right:
+        R, positions, freqs, weight_q, weight_k = _explain(q, k, positions, freqs, weight_q,
+                                                           weight_k, norm)
+        dtype, sq, sk, lead, K = q.dtype, q.shape, k.shape, q.shape[:-2], q.shape[-1]
+    if R:
+        st = positions.stride()
+        st = st if len(st) == 2 else ((0, st[0]) if len(lead) == 2 else (st[0], 0))
+        pos = (positions.data_ptr(), _POS[positions.dtype], *st)
+    return (DTYPES[dtype], _NORM[norm], (lead[0], lead[1] if len(lead) == 2 else 1, sq[-2],
+                                         sk[-2], K, R), pos, freqs, weight_q, weight_k)
+
+
+def _explain(q, k, positions, freqs, weight_q, weight_k, norm):
+    """Raises what is wrong with the operands; returns R and the operands that
+    kernels read, converted where that is all."""
     need_gpu(q, "q")
     need_gpu(k, "k")
     if q.dim() not in (3, 4) or k.dim() != q.dim():
@@ -119,9 +157,7 @@ def _operands(q, k, positions, freqs, weight_q, weight_k, norm):
         raise ValueError(f"k must be [{', '.join(map(str, lead))}, Hk, {K}], got {list(k.shape)}")
     if k.get_device() != dev:
         raise ValueError(f"k must be on device {dev}")
-    code = DTYPES.get(q.dtype)
-    if code is None:
-        dcode(q, "q")
+    dcode(q, "q")
     if k.dtype != q.dtype:
         raise TypeError(f"k must be {q.dtype}, got {k.dtype}")
     if norm not in _NORM:
@@ -135,7 +171,7 @@ def _operands(q, k, positions, freqs, weight_q, weight_k, norm):
         raise ValueError("K = 1: the norm of one channel is its sign")
     if (positions is None) != (freqs is None):
         raise ValueError("positions and freqs go together")
-    R, pos = 0, (None, 0, 0, 0)
+    R = 0
     if freqs is not None:
         need_gpu(freqs, "freqs")
         need_gpu(positions, "positions")
@@ -153,14 +189,9 @@ def _operands(q, k, positions, freqs, weight_q, weight_k, norm):
         for t, what in ((freqs, "freqs"), (positions, "positions")):
             if t.get_device() != dev:
                 raise ValueError(f"{what} must be on device {dev}")
-        if freqs.dtype != torch.float64 or not freqs.is_contiguous():
-            freqs = freqs.to(torch.float64).contiguous()
-        st = positions.stride()
-        st = st if len(st) == 2 else ((0, st[0]) if len(lead) == 2 else (st[0], 0))
-        pos = (positions.data_ptr(), _POS[positions.dtype], *st)
-    B, L = lead if len(lead) == 2 else (lead[0], 1)
-    return (code, _NORM[norm], (B, L, Hq, Hk, K, R), pos, freqs,
-            _weight(weight_q, "weight_q", K, dev), _weight(weight_k, "weight_k", K, dev))
+        freqs = freqs.to(torch.float64).contiguous()
+    return (R, positions, freqs, _weight(weight_q, "weight_q", K, dev),
+            _weight(weight_k, "weight_k", K, dev))
 
 
 def qk_norm_rotary_forward(q, k, positions=None, freqs=None, weight_q=None, weight_k=None, *,
@@ -202,7 +233,7 @@ def qk_norm_rotary_backward(dq_out, dk_out, q, k, positions=None, freqs=None, we
     code, norm_, sizes, pos, freqs, wq, wk = _operands(q, k, positions, freqs, weight_q,
                                                        weight_k, norm)
     sdq, sdk = _like(dq_out, "dq_out", q), _like(dk_out, "dk_out", k)
-    dq, dk = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k))
+    dq, dk = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k))
     dwq, dwk = (None if w is None else torch.empty(sizes[4], device=q.device, dtype=torch.float32)
                 for w in (wq, wk))
     weights = dwq is not None or dwk is not None
