@@ -59,6 +59,25 @@ __device__ inline float diff2(float hi, float lo, float hi0, float lo0) {
   return exp2_fast((hi - hi0) + (lo - lo0));
 }
 
+// Inclusive sums over the wave's lanes: row shifts within 16 lanes, then the rows'
+// last lanes (scan_incl() of common.h, in 64 bits).
+template <int CTRL, int ROWS>
+__device__ inline double dpp_in64(double v) {
+  const uint64_t x = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, CTRL, ROWS, 0xf, true);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(x >> 32), CTRL, ROWS, 0xf, true);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ inline double wave_scan(double v) {
+  v += dpp_in64<0x111, 0xf>(v);
+  v += dpp_in64<0x112, 0xf>(v);
+  v += dpp_in64<0x114, 0xf>(v);
+  v += dpp_in64<0x118, 0xf>(v);
+  v += dpp_in64<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
+  v += dpp_in64<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
+  return v;
+}
+
 // g of a lane's steps: steps lane E .. lane E + E - 1, E = max(C / 64, 1).
 template <int C>
 struct Gaps {
@@ -82,17 +101,13 @@ struct Gaps {
       sum += (double)x;
       s[e] = sum;
     }
-    double run = sum;
-#pragma unroll
-    for (int n = 1; n < 64; n *= 2) {
-      const double y = __shfl_up(run, n);
-      if (lane >= n) run += y;
-    }
-    const double before = __shfl_up(run, 1);
+    // of the lanes before (wave_shr:1): subtracting the lane's own would carry a later
+    // step's NaN to an earlier one
+    const double before = dpp_in64<0x138, 0xf>(wave_scan(sum));
     float hi[E], lo[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const double G = ((lane ? before : 0.0) + s[e]) * 1.4426950408889634;
+      const double G = (before + s[e]) * 1.4426950408889634;
       hi[e] = (float)G;
       lo[e] = (float)(G - (double)hi[e]);
     }

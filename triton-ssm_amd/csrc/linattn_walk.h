@@ -206,51 +206,61 @@ __device__ inline void lin_walk_body(const LinWalkArgs& g, char* smem, uint32_t 
       const int db = tw >> 1, t = 16 * tw + c;
       const float ht = B.d.hi[t], lt = B.d.lo[t];
       eg = exp2_fast(ht + lt);
-      float p8[8];
-      u32x4 pb[NO];
-      const auto weights = [&](int ib) {  // rows i = 32 ib + 8 j + e of K Q^T
-        f32x4 p[2] = {zero4(), zero4()};
+      float p8[8];  // of the last block, the wave's own
+      // NB blocks of 32 steps, in one piece so that they overlap; the last is masked
+      const auto blocks = [&](auto count) {
+        constexpr int NB = decltype(count)::value;
+        f32x4 p[NB][2];
+        float from[NB];
 #pragma unroll
-        for (int s = 0; s < NS; ++s)
+        for (int ib = 0; ib < NB; ++ib) {
+          from[ib] = diff2(ht, lt, B.d.hi[32 * ib + 31], B.d.lo[32 * ib + 31]);
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            u32x4 fk[NP];
+            p[ib][x] = zero4();
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {  // rows i = 32 ib + 8 j + 4 x + r of K Q^T
+              u32x4 fk[NP];
+#pragma unroll
+              for (int y = 0; y < NP; ++y)
+                fk[y] = lds16(&B.K[y][(32 * ib + ar + 4 * x) * W::kLd + 32 * s + 8 * j]);
+              p[ib][x] = mfma_planes<NP, NP, NO>(fk, qb[s], p[ib][x]);
+            }
+          }
+        }
+#pragma unroll
+        for (int ib = 0; ib < NB; ++ib) {
+          if (ib + 1 < NB) {
+            float u8[8];
+            lds8(&B.d.u[32 * ib + 8 * j], u8);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) p8[e] = p[ib][e >> 2][e & 3] * (u8[e] * from[ib]);
+          } else {
+            float h8[8], l8[8];
+            lds8(&B.d.hi[32 * ib + 8 * j], h8);
+            lds8(&B.d.lo[32 * ib + 8 * j], l8);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              p8[e] = 32 * ib + 8 * j + e <= t
+                          ? p[ib][e >> 2][e & 3] * diff2(ht, lt, h8[e], l8[e]) : 0.0f;
+          }
+          u32x4 pb[NO];
+          split8<NO>(p8, pb);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {  // V^T P^T
+            u32x4 fv[NP];
 #pragma unroll
             for (int y = 0; y < NP; ++y)
-              fk[y] = lds16(&B.K[y][(32 * ib + ar + 4 * x) * W::kLd + 32 * s + 8 * j]);
-            p[x] = mfma_planes<NP, NP, NO>(fk, qb[s], p[x]);
+              fv[y] = lds_col(&B.V[y][32 * ib * W::kVld], W::kVld, 4 * x, lane);
+            f32x4& o = ib + 1 < NB ? acc[x] : own[x];
+            o = mfma_planes<NP, NO, NO>(fv, pb, o);
           }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) p8[e] = p[e >> 2][e & 3];
-      };
-      const auto add = [&](int ib, f32x4 (&o)[2]) {  // V^T P^T
-        split8<NO>(p8, pb);
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          u32x4 fv[NP];
-#pragma unroll
-          for (int y = 0; y < NP; ++y)
-            fv[y] = lds_col(&B.V[y][32 * ib * W::kVld], W::kVld, 4 * x, lane);
-          o[x] = mfma_planes<NP, NO, NO>(fv, pb, o[x]);
         }
       };
-      for (int ib = 0; ib < db; ++ib) {
-        weights(ib);
-        float u8[8];
-        lds8(&B.d.u[32 * ib + 8 * j], u8);
-        const float from = diff2(ht, lt, B.d.hi[32 * ib + 31], B.d.lo[32 * ib + 31]);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) p8[e] *= u8[e] * from;
-        add(ib, acc);
-      }
-      weights(db);
-      float h8[8], l8[8];
-      lds8(&B.d.hi[32 * db + 8 * j], h8);
-      lds8(&B.d.lo[32 * db + 8 * j], l8);
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        p8[e] = 32 * db + 8 * j + e <= t ? p8[e] * diff2(ht, lt, h8[e], l8[e]) : 0.0f;
-      add(db, own);
+      if (C == 32 || db == 0) blocks(std::integral_constant<int, 1>());
+      else if (C == 64 || db == 1) blocks(std::integral_constant<int, 2>());
+      else if (db == 2) blocks(std::integral_constant<int, 3>());
+      else blocks(std::integral_constant<int, 4>());
       float big = 0.0f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) big += __builtin_fabsf(own[e >> 2][e & 3]);
