@@ -155,14 +155,14 @@ __device__ inline void lds8(const float* p, float* x) {
   *reinterpret_cast<float4*>(x + 4) = *reinterpret_cast<const float4*>(p + 4);
 }
 
-// The B operand X[8 j + e][c] of 32 rows from `row` on and 16 columns from `col`
-// on of planes [NP][rows][ld] in LDS, as floats.
-template <int NP>
-__device__ inline void lds_values(const uint16_t* m, int plane, int ld, int row, int col, int lane,
+// The B operand X[8 j + e][c] of 32 rows from `row` on and 16 columns from `col` on of
+// planes [NP][rows][N] in LDS, as floats.
+template <int NP, int N>
+__device__ inline void lds_values(const uint16_t* m, int plane, int row, int col, int lane,
                                   float* x) {
 #pragma unroll
   for (int p = NP - 1; p >= 0; --p) {
-    const u32x4 w = lds_col16(m + p * plane + row * ld, ld, col, lane);
+    const u32x4 w = Swizzled<N>::col16(m + p * plane, row, col, lane);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float a = __uint_as_float(w[e] << 16), b = __uint_as_float(w[e] & 0xffff0000u);

@@ -58,7 +58,7 @@ int fold(const LinArgs& a, float* ends, const double* sums, int nseg, int rev, h
 template <typename T, int MODE>
 int by_keys(const LinWalkArgs& f, const LinWalkArgs& b, bool vec, hipStream_t s) {
 #define TSSM_WALK(KP) \
-  (vec ? lin_states<T, KP, true, MODE>(f, b, s) : lin_states<T, KP, false, MODE>(f, b, s))
+  (vec ? lin_states_run<T, KP, true, MODE>(f, b, s) : lin_states_run<T, KP, false, MODE>(f, b, s))
   if (f.a.K <= 32) return TSSM_WALK(32);
   if (f.a.K <= 64) return TSSM_WALK(64);
   return TSSM_WALK(128);

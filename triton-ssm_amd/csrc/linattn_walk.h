@@ -5,16 +5,17 @@
 //   O = scale (e^G Q S + (Q K^T D) V),   S' = e^(G_end) S + K^T (e^(G_end - G) V).
 // Only S' waits for S, by one product and a sum; all the rest of a chunk is its own.
 //
-// A workgroup of C / 16 waves walks 32 columns of V of one head's segment.  A wave
-// has 16 steps of the chunk for the outputs and a share of K^T V: 32 steps for 16
+// A workgroup walks 32 columns of V of one head's segment, with C / 16 waves for the
+// outputs and as many for the states.  An output wave has 16 steps of the chunk.  A
+// state wave brings its share of K and V to LDS and forms K^T V of 32 steps and 16
 // columns, all of K, of which it keeps the tiles of the state that are its own and
 // hands the others to their owners through LDS.  Everything is formed transposed
-// (planes.h): a wave's P^T = K Q^T is the next product's operand in place, queries
-// come to it straight from memory, and a lane ends up with 8 neighbouring columns of
-// one step's output.  Per chunk
-//   before the barrier: P and its part of the output, K^T V, the next chunk to LDS,
+// (planes.h): P^T = K Q^T is the next product's operand in place, queries come to
+// their wave straight from memory, and a lane ends up with 8 neighbouring columns of
+// one step's output.  One barrier a chunk:
+//   before it: P and its part of the output | K^T V, the next chunk to LDS,
 //   after it: the state's part of the output from planes that the owners left in
-//     LDS a chunk ago, and the next state.
+//     LDS a chunk ago | the next state and its planes.
 // K and V are in LDS twice, a third chunk's loads are in flight.
 //
 // D of the 32 steps before the wave's own is a product of two factors with the decay
@@ -55,118 +56,113 @@ struct LinWalk {
   static constexpr int NP = kPlanes<T>, NO = kOutPlanes<T>;
   static constexpr int NS = KP / 32, KT = KP / 16, NW = C / 16, NT = 64 * NW, NIQ = C / 32;
   static constexpr int OWN = KT / NIQ;       // tiles of the state that a wave keeps
-  static constexpr int kLd = KP + 8, kVld = 40;  // bf16 elements of a row in LDS
+  typedef Swizzled<KP> KR;                   // rows of K and of the state's planes
+  typedef Swizzled<32> VR;                   // of V
+  // outputs and states have waves of their own
+  static constexpr int kThreads = MODE == kOutputs ? 2 * NT : NT;
   static constexpr int kNk = C * KP / 8 / NT;    // 8-element pieces of K a thread brings
   static_assert(KT % NIQ == 0, "every wave owns tiles");
   struct Operands {  // of one chunk
-    uint16_t K[NP][C * kLd], V[NP][C * kVld];
+    uint16_t K[NP][C * KP], V[NP][C * 32];
     Decays<C> d;
   };
   struct Lds {
     Operands op[2];
     f32x4 part[2][NW][KT - OWN ? KT - OWN : 1][64];
     // planes of S^T, a row for each column of V
-    uint16_t S[MODE == kOutputs ? 2 : 1][NO][MODE == kOutputs ? 32 * kLd : 8];
+    uint16_t S[MODE == kOutputs ? 2 : 1][NO][MODE == kOutputs ? 32 * KP : 8];
   };
 };
 
-template <typename T, int KP, bool VEC, int C, int MODE, bool REV>
-__device__ inline void lin_walk_body(const LinWalkArgs& g, char* smem, uint32_t id) {
-  typedef LinWalk<T, KP, C, MODE> W;
-  constexpr int NP = W::NP, NO = W::NO, NS = W::NS, KT = W::KT, NT = W::NT, NIQ = W::NIQ,
-                OWN = W::OWN, kE = (int)sizeof(T);
-  typename W::Lds& lds = *reinterpret_cast<typename W::Lds*>(smem);
-  const LinArgs& a = g.a;
-  // workgroups of one head's segment, which share Q and K, on one XCD
-  const uint32_t vb = (id >> 3) % g.nvb, u = (id >> 3) / g.nvb * 8 + (id & 7);
-  if (u >= g.units) return;
-  const int64_t bh = u / (uint32_t)g.walked;
-  const int seg = g.first + (int)(u - (uint32_t)bh * (uint32_t)g.walked);
-  const int n0 = seg * g.per, n1 = n0 + g.per < g.nch ? n0 + g.per : g.nch, cnt = n1 - n0;
-  const int lane = threadIdx.x & 63, j = lane >> 4, c = lane & 15;
-  const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  // 16 steps for the outputs: waves w and w + 4, on one SIMD, have equal work together
-  const int tw = C == 128 && w >= 4 ? 11 - w : w;
-  const int iq = w >> 1, vt = w & 1;         // 32 steps, 16 columns for K^T V
-  const int ar = 8 * (c >> 2) + (c & 3);     // row of tile x of an A operand, less 4 x
-  const auto [b, h, hk] = lin_head(a, (uint32_t)bh);
-  const int64_t v0 = (int64_t)vb * 32;
-  const int nv = a.V - v0 < 32 ? (int)(a.V - v0) : 32, K = (int)a.K;
-  const int64_t elems = lin_state_elems(KP, a.V), col = v0 + 16 * vt + c;
-  const int64_t tile0 = ((int64_t)(2 * vb + vt) * KT + iq * OWN) * 256 + lane * 4;
-
-  RowsOf<C> rk, rq, rv, ro;
-  rk.init(reinterpret_cast<const T*>(a.k) + b * a.k_b + hk * a.k_h, a.k_l, K, a.L);
-  rv.init(reinterpret_cast<const T*>(a.v) + b * a.v_b + h * a.v_h + v0, a.v_l, nv, a.L);
-  if constexpr (MODE == kOutputs) {
-    rq.init(reinterpret_cast<const T*>(a.q) + b * a.q_b + hk * a.q_h, a.q_l, K, a.L);
-    ro.init(reinterpret_cast<const T*>(a.o) + b * a.o_b + h * a.o_h + v0, a.o_l, nv, a.L);
+// What a workgroup walks.
+template <int C>
+struct LinUnit {
+  int64_t bh, b, h, hk, v0;
+  int seg, n0, n1, nv;
+  // workgroups of one head's segment, which share Q and K, are on one XCD
+  __device__ inline bool init(const LinWalkArgs& g, uint32_t id) {
+    const uint32_t vb = (id >> 3) % g.nvb, u = (id >> 3) / g.nvb * 8 + (id & 7);
+    if (u >= g.units) return false;
+    bh = u / (uint32_t)g.walked;
+    seg = g.first + (int)(u - (uint32_t)bh * (uint32_t)g.walked);
+    n0 = seg * g.per;
+    n1 = n0 + g.per < g.nch ? n0 + g.per : g.nch;
+    const LinHead x = lin_head(g.a, (uint32_t)bh);
+    b = x.b;
+    h = x.h;
+    hk = x.hk;
+    v0 = (int64_t)vb * 32;
+    nv = g.a.V - v0 < 32 ? (int)(g.a.V - v0) : 32;
+    return true;
   }
-  const float* gp = a.g + b * a.g_b + h * a.g_h;
+};
 
-  struct Regs {
-    Piece<T, VEC, NP> k[W::kNk], v, q[MODE == kOutputs ? NS : 1];
-    Gaps<C> g;
-  } in;
+// The waves of the states, and of K and V's way to LDS.
+template <typename T, int KP, bool VEC, int C, int MODE, bool REV>
+__device__ inline void lin_states(const LinWalkArgs& g, const LinUnit<C>& u,
+                                  typename LinWalk<T, KP, C, MODE>::Lds& lds, int id) {
+  typedef LinWalk<T, KP, C, MODE> W;
+  typedef typename W::KR KR;
+  typedef typename W::VR VR;
+  constexpr int NP = W::NP, NO = W::NO, KT = W::KT, NT = W::NT, NIQ = W::NIQ, OWN = W::OWN,
+                kE = (int)sizeof(T);
+  const LinArgs& a = g.a;
+  const int lane = id & 63, j = lane >> 4, c = lane & 15, cnt = u.n1 - u.n0, K = (int)a.K;
+  const int w = __builtin_amdgcn_readfirstlane(id >> 6);
+  const int iq = w >> 1, vt = w & 1;         // 32 steps, 16 columns for K^T V
+  const int64_t elems = lin_state_elems(KP, a.V), col = u.v0 + 16 * vt + c;
+  const int64_t tile0 = ((u.v0 / 16 + vt) * KT + iq * OWN) * 256 + lane * 4;
+
+  RowsOf<C> rk, rv;
+  rk.init(reinterpret_cast<const T*>(a.k) + u.b * a.k_b + u.hk * a.k_h, a.k_l, K, a.L);
+  rv.init(reinterpret_cast<const T*>(a.v) + u.b * a.v_b + u.h * a.v_h + u.v0, a.v_l, u.nv, a.L);
+  const float* gp = a.g + u.b * a.g_b + u.h * a.g_h;
   const auto chunk = [&](int m) {   // the chunk of step m of the walk
     const int x = m < cnt ? m : cnt - 1;
-    return REV ? n1 - 1 - x : n0 + x;
+    return REV ? u.n1 - 1 - x : u.n0 + x;
   };
+  Piece<T, VEC, NP> ink[W::kNk], inv;
+  Gaps<C> gaps;
   const auto fetch = [&](int m) {
     const int n = chunk(m);
     const auto dk = rk.at(n), dv = rv.at(n);
 #pragma unroll
     for (int i = 0; i < W::kNk; ++i) {
-      const int at = (int)threadIdx.x + NT * i, r = at / (KP / 8), x = at % (KP / 8) * 8;
-      in.k[i].load(dk, x < K ? r * rk.row + x * kE : kPast);
+      const int at = id + NT * i, r = at / (KP / 8), x = at % (KP / 8) * 8;
+      ink[i].load(dk, x < K ? r * rk.row + x * kE : kPast);
     }
-    const int r = (int)threadIdx.x >> 2, x = ((int)threadIdx.x & 3) * 8;
-    in.v.load(dv, x < nv ? r * rv.row + x * kE : kPast);
-    if constexpr (MODE == kOutputs) {
-      const auto dq = rq.at(n);
-#pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        const int y = 32 * s + 8 * j;
-        in.q[s].load(dq, y < K ? (16 * tw + c) * rq.row + y * kE : kPast);
-      }
-    }
+    const int r = id >> 2, x = (id & 3) * 8;
+    inv.load(dv, x < u.nv ? r * rv.row + x * kE : kPast);
     if (w == 0) {
       const int64_t t0 = (int64_t)n * C, rest = a.L - t0;
-      in.g.load(gp + t0 * a.g_l, a.g_l, lane, rest < C ? (int)rest : C);
+      gaps.load(gp + t0 * a.g_l, a.g_l, lane, rest < C ? (int)rest : C);
     }
   };
   const auto leave = [&](typename W::Operands& o) {  // what fetch() brought, to LDS
 #pragma unroll
     for (int i = 0; i < W::kNk; ++i) {
-      const int at = (int)threadIdx.x + NT * i, r = at / (KP / 8), x = at % (KP / 8) * 8;
+      const int at = id + NT * i, r = at / (KP / 8), x = at % (KP / 8);
       u32x4 p[NP];
-      planes_apart(in.k[i], K - x, p);
+      planes_apart(ink[i], K - 8 * x, p);
 #pragma unroll
-      for (int y = 0; y < NP; ++y) *reinterpret_cast<u32x4*>(&o.K[y][r * W::kLd + x]) = p[y];
+      for (int y = 0; y < NP; ++y) *reinterpret_cast<u32x4*>(&o.K[y][KR::at(r, x)]) = p[y];
     }
-    const int r = (int)threadIdx.x >> 2, x = ((int)threadIdx.x & 3) * 8;
+    const int r = id >> 2, x = id & 3;
     u32x4 p[NP];
-    planes_apart(in.v, nv - x, p);
+    planes_apart(inv, u.nv - 8 * x, p);
 #pragma unroll
-    for (int y = 0; y < NP; ++y) *reinterpret_cast<u32x4*>(&o.V[y][r * W::kVld + x]) = p[y];
-    if (w == 0) in.g.decays(o.d, lane);
+    for (int y = 0; y < NP; ++y) *reinterpret_cast<u32x4*>(&o.V[y][VR::at(r, x)]) = p[y];
+    if (w == 0) gaps.decays(o.d, lane);
   };
-  u32x4 qb[NS][NP], qn[NS][NP];
-  const auto queries = [&](u32x4 (&q)[NS][NP]) {
-    if constexpr (MODE == kOutputs) {
-#pragma unroll
-      for (int s = 0; s < NS; ++s) in.q[s].planes(K - 32 * s - 8 * j, q[s]);
-    }
-  };
-
   f32x4 S[OWN];
 #pragma unroll
   for (int i = 0; i < OWN; ++i) {
     if constexpr (MODE == kEnds) S[i] = zero4();
     else if (g.nseg == 1)
-      S[i] = get_tile(a.h0 ? a.h0 + bh * K * a.V : nullptr, iq * OWN + i, col, a.V, K, j);
+      S[i] = get_tile(a.h0 ? a.h0 + u.bh * K * a.V : nullptr, iq * OWN + i, col, a.V, K, j);
     else
-      S[i] = *reinterpret_cast<const f32x4*>(g.entry + (bh * g.nseg + seg) * elems + tile0 + 256 * i);
+      S[i] = *reinterpret_cast<const f32x4*>(g.entry + (u.bh * g.nseg + u.seg) * elems + tile0 +
+                                             256 * i);
   }
   const auto show = [&](int par) {  // the state's planes, for the outputs
     if constexpr (MODE == kOutputs) {
@@ -177,8 +173,8 @@ __device__ inline void lin_walk_body(const LinWalkArgs& g, char* smem, uint32_t 
 #pragma unroll
         for (int p = 0; p < NO; ++p) {
           const uint32_t lo = pk_bf16(x0, x1), hi = pk_bf16(x2, x3);
-          *reinterpret_cast<uint2*>(&lds.S[par][p][(16 * vt + c) * W::kLd + 32 * (kt >> 1) +
-                                                   8 * j + 4 * (kt & 1)]) = make_uint2(lo, hi);
+          *reinterpret_cast<uint2*>(&lds.S[par][p][KR::at(16 * vt + c, 4 * (kt >> 1) + j) +
+                                                   4 * (kt & 1)]) = make_uint2(lo, hi);
           if (p + 1 < NO) {
             take_plane(lo, x0, x1);
             take_plane(hi, x2, x3);
@@ -190,102 +186,18 @@ __device__ inline void lin_walk_body(const LinWalkArgs& g, char* smem, uint32_t 
   double total = 0.0;
   fetch(0);
   leave(lds.op[0]);
-  queries(qb);
   show(0);
   fetch(1);
   lds_barrier();
   for (int m = 0; m < cnt; ++m) {
-    const int n = chunk(m), par = m & 1;
+    const int par = m & 1;
     const typename W::Operands& B = lds.op[par];
     const float hend = B.d.hi[C - 1], lend = B.d.lo[C - 1];
     const float last = exp2_fast(hend + lend);
-    float eg = 0.0f;
-    f32x4 acc[2] = {zero4(), zero4()}, own[2] = {zero4(), zero4()};
     if constexpr (MODE == kEnds) total += (double)hend + (double)lend;
-    if constexpr (MODE == kOutputs) {
-      const int db = tw >> 1, t = 16 * tw + c;
-      const float ht = B.d.hi[t], lt = B.d.lo[t];
-      eg = exp2_fast(ht + lt);
-      float p8[8];  // of the last block, the wave's own
-      // NB blocks of 32 steps, in one piece so that they overlap; the last is masked
-      const auto blocks = [&](auto count) {
-        constexpr int NB = decltype(count)::value;
-        f32x4 p[NB][2];
-        float from[NB];
-#pragma unroll
-        for (int ib = 0; ib < NB; ++ib) {
-          from[ib] = diff2(ht, lt, B.d.hi[32 * ib + 31], B.d.lo[32 * ib + 31]);
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            p[ib][x] = zero4();
-#pragma unroll
-            for (int s = 0; s < NS; ++s) {  // rows i = 32 ib + 8 j + 4 x + r of K Q^T
-              u32x4 fk[NP];
-#pragma unroll
-              for (int y = 0; y < NP; ++y)
-                fk[y] = lds16(&B.K[y][(32 * ib + ar + 4 * x) * W::kLd + 32 * s + 8 * j]);
-              p[ib][x] = mfma_planes<NP, NP, NO>(fk, qb[s], p[ib][x]);
-            }
-          }
-        }
-#pragma unroll
-        for (int ib = 0; ib < NB; ++ib) {
-          if (ib + 1 < NB) {
-            float u8[8];
-            lds8(&B.d.u[32 * ib + 8 * j], u8);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) p8[e] = p[ib][e >> 2][e & 3] * (u8[e] * from[ib]);
-          } else {
-            float h8[8], l8[8];
-            lds8(&B.d.hi[32 * ib + 8 * j], h8);
-            lds8(&B.d.lo[32 * ib + 8 * j], l8);
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              p8[e] = 32 * ib + 8 * j + e <= t
-                          ? p[ib][e >> 2][e & 3] * diff2(ht, lt, h8[e], l8[e]) : 0.0f;
-          }
-          u32x4 pb[NO];
-          split8<NO>(p8, pb);
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {  // V^T P^T
-            u32x4 fv[NP];
-#pragma unroll
-            for (int y = 0; y < NP; ++y)
-              fv[y] = lds_col(&B.V[y][32 * ib * W::kVld], W::kVld, 4 * x, lane);
-            f32x4& o = ib + 1 < NB ? acc[x] : own[x];
-            o = mfma_planes<NP, NO, NO>(fv, pb, o);
-          }
-        }
-      };
-      if (C == 32 || db == 0) blocks(std::integral_constant<int, 1>());
-      else if (C == 64 || db == 1) blocks(std::integral_constant<int, 2>());
-      else if (db == 2) blocks(std::integral_constant<int, 3>());
-      else blocks(std::integral_constant<int, 4>());
-      float big = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) big += __builtin_fabsf(own[e >> 2][e & 3]);
-      if (__builtin_expect(__ballot(!(big < __builtin_inff())) != 0, 0)) {
-        own[0] = own[1] = zero4();
-#pragma unroll 1
-        for (int i = 0; i < 32; ++i) {
-          float p = 0.0f;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) p = (i & 7) == e ? p8[e] : p;
-          p = __shfl(p, (i >> 3) * 16 + c);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            float v = 0.0f;
-#pragma unroll
-            for (int y = NP - 1; y >= 0; --y)
-              v += bf16_bits_to_f32(B.V[y][(32 * db + i) * W::kVld + 8 * j + e]);
-            if (32 * db + i <= t) own[e >> 2][e & 3] += p * v;
-          }
-        }
-      }
-    }
     // this wave's 32 steps of K^T V
     float v8[8], e8[8];
-    lds_values<NP>(&B.V[0][0], C * W::kVld, W::kVld, 32 * iq, 16 * vt, lane, v8);
+    lds_values<NP, 32>(&B.V[0][0], C * 32, 32 * iq, 16 * vt, lane, v8);
     if constexpr (REV) {
       float h8[8], l8[8];
       lds8(&B.d.hi[32 * iq + 8 * j], h8);
@@ -308,7 +220,7 @@ __device__ inline void lin_walk_body(const LinWalkArgs& g, char* smem, uint32_t 
       u32x4 fk[NP];
 #pragma unroll
       for (int y = 0; y < NP; ++y)
-        fk[y] = lds_col(&B.K[y][32 * iq * W::kLd], W::kLd, 32 * (kt >> 1) + 4 * (kt & 1), lane);
+        fk[y] = KR::col(B.K[y], 32 * iq, 32 * (kt >> 1) + 4 * (kt & 1), lane);
       const f32x4 x = mfma_planes<NP, 3, 3>(fk, vp, zero4());
       if (kt / OWN == iq) {
 #pragma unroll
@@ -319,11 +231,10 @@ __device__ inline void lin_walk_body(const LinWalkArgs& g, char* smem, uint32_t 
       }
     }
     leave(lds.op[par ^ 1]);
-    queries(qn);
     fetch(m + 2);
     lds_barrier();
     if constexpr (MODE == kStates) {
-      float* p = g.states + (bh * g.nch + n) * elems + tile0;
+      float* p = g.states + (u.bh * g.nch + chunk(m)) * elems + tile0;
 #pragma unroll
       for (int i = 0; i < OWN; ++i) *reinterpret_cast<f32x4*>(p + 256 * i) = S[i];
     }
@@ -338,65 +249,167 @@ __device__ inline void lin_walk_body(const LinWalkArgs& g, char* smem, uint32_t 
 #pragma unroll
       for (int r = 0; r < 4; ++r) S[i][r] = __builtin_fmaf(S[i][r], last, x[r]);
     }
-    if constexpr (MODE == kOutputs) {
-      show(par ^ 1);
-      f32x4 y[2] = {zero4(), zero4()};
-#pragma unroll
-      for (int s = 0; s < NS; ++s)
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          u32x4 fs[NO];
-#pragma unroll
-          for (int p = 0; p < NO; ++p)
-            fs[p] = lds16(&lds.S[par][p][(ar + 4 * x) * W::kLd + 32 * s + 8 * j]);
-          y[x] = mfma_planes<NO, NP, NO>(fs, qb[s], y[x]);
-        }
-      const auto dst = ro.at(n);
-      const uint32_t off = (uint32_t)((16 * tw + c) * ro.row + 8 * j * kE);
-      float o8[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        o8[e] = a.scale * __builtin_fmaf(y[e >> 2][e & 3], eg,
-                                         acc[e >> 2][e & 3] + own[e >> 2][e & 3]);
-      if constexpr (VEC) {
-        const uint32_t to = 8 * j < nv ? off : kPast;
-        if constexpr (kE == 4) {
-          typedef uint32_t vec4 __attribute__((ext_vector_type(4)));
-          __builtin_amdgcn_raw_buffer_store_b128(
-              vec4{__float_as_uint(o8[0]), __float_as_uint(o8[1]), __float_as_uint(o8[2]),
-                   __float_as_uint(o8[3])}, dst, to, 0, 0);
-          __builtin_amdgcn_raw_buffer_store_b128(
-              vec4{__float_as_uint(o8[4]), __float_as_uint(o8[5]), __float_as_uint(o8[6]),
-                   __float_as_uint(o8[7])}, dst, to + 16, 0, 0);
-        } else {
-          union {
-            T e[8];
-            u32x4 v;
-          } x;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) stf(&x.e[e], o8[e]);
-          __builtin_amdgcn_raw_buffer_store_b128(x.v, dst, to, 0, 0);
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          buf_put<T>(dst, 8 * j + e < nv ? off + e * kE : kPast, o8[e]);
-      }
-#pragma unroll
-      for (int s = 0; s < NS; ++s)
-#pragma unroll
-        for (int p = 0; p < NP; ++p) qb[s][p] = qn[s][p];
-    }
+    show(par ^ 1);
   }
   if constexpr (MODE == kEnds) {
-    float* p = g.states + (bh * g.nseg + seg) * elems + tile0;
+    float* p = g.states + (u.bh * g.nseg + u.seg) * elems + tile0;
 #pragma unroll
     for (int i = 0; i < OWN; ++i) *reinterpret_cast<f32x4*>(p + 256 * i) = S[i];
-    if (vb == 0 && threadIdx.x == 0) g.sums[bh * g.nseg + seg] = total;
-  } else if (REV ? n0 == 0 : n1 == g.nch) {
-    float* p = a.h_last ? a.h_last + bh * K * a.V : nullptr;
+    if (u.v0 == 0 && id == 0) g.sums[u.bh * g.nseg + u.seg] = total;
+  } else if (REV ? u.n0 == 0 : u.n1 == g.nch) {
+    float* p = a.h_last ? a.h_last + u.bh * K * a.V : nullptr;
 #pragma unroll
     for (int i = 0; i < OWN; ++i) put_tile(p, S[i], iq * OWN + i, col, a.V, K, j);
+  }
+}
+
+// The waves of the outputs.
+template <typename T, int KP, bool VEC, int C>
+__device__ inline void lin_outputs(const LinWalkArgs& g, const LinUnit<C>& u,
+                                   typename LinWalk<T, KP, C, kOutputs>::Lds& lds, int id) {
+  typedef LinWalk<T, KP, C, kOutputs> W;
+  typedef typename W::KR KR;
+  typedef typename W::VR VR;
+  constexpr int NP = W::NP, NO = W::NO, NS = W::NS, kE = (int)sizeof(T);
+  const LinArgs& a = g.a;
+  const int lane = id & 63, j = lane >> 4, c = lane & 15, cnt = u.n1 - u.n0, K = (int)a.K;
+  const int w = __builtin_amdgcn_readfirstlane(id >> 6);
+  // 16 steps: waves w and w + 4, on one SIMD, have equal work together
+  const int tw = C == 128 && w >= 4 ? 11 - w : w, db = tw >> 1, t = 16 * tw + c;
+  const int ar = 8 * (c >> 2) + (c & 3);     // row of tile x of an A operand, less 4 x
+  RowsOf<C> rq, ro;
+  rq.init(reinterpret_cast<const T*>(a.q) + u.b * a.q_b + u.hk * a.q_h, a.q_l, K, a.L);
+  ro.init(reinterpret_cast<const T*>(a.o) + u.b * a.o_b + u.h * a.o_h + u.v0, a.o_l, u.nv, a.L);
+  Piece<T, VEC, NP> in[NS];
+  const auto fetch = [&](int m) {
+    const auto d = rq.at(u.n0 + (m < cnt ? m : cnt - 1));
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      const int y = 32 * s + 8 * j;
+      in[s].load(d, y < K ? t * rq.row + y * kE : kPast);
+    }
+  };
+  fetch(0);
+  lds_barrier();
+  for (int m = 0; m < cnt; ++m) {
+    const int par = m & 1;
+    const typename W::Operands& B = lds.op[par];
+    u32x4 qb[NS][NP];
+#pragma unroll
+    for (int s = 0; s < NS; ++s) in[s].planes(K - 32 * s - 8 * j, qb[s]);
+    fetch(m + 1);
+    f32x4 acc[2] = {zero4(), zero4()}, own[2] = {zero4(), zero4()};
+    const float ht = B.d.hi[t], lt = B.d.lo[t], eg = exp2_fast(ht + lt);
+    float p8[8];  // of the last block, the wave's own
+    // NB blocks of 32 steps, in one piece so that they overlap; the last is masked
+    const auto blocks = [&](auto count) {
+      constexpr int NB = decltype(count)::value;
+      f32x4 p[NB][2];
+      float from[NB];
+#pragma unroll
+      for (int ib = 0; ib < NB; ++ib) {
+        from[ib] = diff2(ht, lt, B.d.hi[32 * ib + 31], B.d.lo[32 * ib + 31]);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          p[ib][x] = zero4();
+#pragma unroll
+          for (int s = 0; s < NS; ++s) {  // rows i = 32 ib + 8 j + 4 x + r of K Q^T
+            u32x4 fk[NP];
+#pragma unroll
+            for (int y = 0; y < NP; ++y)
+              fk[y] = lds16(&B.K[y][KR::at(ar, 4 * s + j) + (32 * ib + 4 * x) * KP]);
+            p[ib][x] = mfma_planes<NP, NP, NO>(fk, qb[s], p[ib][x]);
+          }
+        }
+      }
+#pragma unroll
+      for (int ib = 0; ib < NB; ++ib) {
+        if (ib + 1 < NB) {
+          float u8[8];
+          lds8(&B.d.u[32 * ib + 8 * j], u8);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) p8[e] = p[ib][e >> 2][e & 3] * (u8[e] * from[ib]);
+        } else {
+          float h8[8], l8[8];
+          lds8(&B.d.hi[32 * ib + 8 * j], h8);
+          lds8(&B.d.lo[32 * ib + 8 * j], l8);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            p8[e] = 32 * ib + 8 * j + e <= t
+                        ? p[ib][e >> 2][e & 3] * diff2(ht, lt, h8[e], l8[e]) : 0.0f;
+        }
+        u32x4 pb[NO];
+        split8<NO>(p8, pb);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {  // V^T P^T
+          u32x4 fv[NP];
+#pragma unroll
+          for (int y = 0; y < NP; ++y) fv[y] = VR::col(B.V[y], 32 * ib, 4 * x, lane);
+          f32x4& o = ib + 1 < NB ? acc[x] : own[x];
+          o = mfma_planes<NP, NO, NO>(fv, pb, o);
+        }
+      }
+    };
+    if (C == 32 || db == 0) blocks(std::integral_constant<int, 1>());
+    else if (C == 64 || db == 1) blocks(std::integral_constant<int, 2>());
+    else if (db == 2) blocks(std::integral_constant<int, 3>());
+    else blocks(std::integral_constant<int, 4>());
+    float big = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) big += __builtin_fabsf(own[e >> 2][e & 3]);
+    if (__builtin_expect(__ballot(!(big < __builtin_inff())) != 0, 0)) {
+      own[0] = own[1] = zero4();
+#pragma unroll 1
+      for (int i = 0; i < 32; ++i) {
+        float p = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) p = (i & 7) == e ? p8[e] : p;
+        p = __shfl(p, (i >> 3) * 16 + c);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float v = 0.0f;
+#pragma unroll
+          for (int y = NP - 1; y >= 0; --y)
+            v += bf16_bits_to_f32(B.V[y][VR::at(32 * db + i, j) + e]);
+          if (32 * db + i <= t) own[e >> 2][e & 3] += p * v;
+        }
+      }
+    }
+    lds_barrier();
+    f32x4 y[2] = {zero4(), zero4()};
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        u32x4 fs[NO];
+#pragma unroll
+        for (int p = 0; p < NO; ++p)
+          fs[p] = lds16(&lds.S[par][p][KR::at(ar, 4 * s + j) + 4 * x * KP]);
+        y[x] = mfma_planes<NO, NP, NO>(fs, qb[s], y[x]);
+      }
+    const auto dst = ro.at(u.n0 + m);
+    const uint32_t off = (uint32_t)(t * ro.row + 8 * j * kE);
+    float o8[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      o8[e] = a.scale * __builtin_fmaf(y[e >> 2][e & 3], eg,
+                                       acc[e >> 2][e & 3] + own[e >> 2][e & 3]);
+    if constexpr (VEC) {
+      const uint32_t to = 8 * j < u.nv ? off : kPast;
+      union {
+        T e[8];
+        u32x4 v[kE / 2];
+      } x;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) stf(&x.e[e], o8[e]);
+#pragma unroll
+      for (int i = 0; i < kE / 2; ++i)
+        __builtin_amdgcn_raw_buffer_store_b128(x.v[i], dst, to + 16 * i, 0, 0);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        buf_put<T>(dst, 8 * j + e < u.nv ? off + e * kE : kPast, o8[e]);
+    }
   }
 }
 
@@ -409,9 +422,16 @@ template <typename T, int KP>
 constexpr int kStateSteps = kPlanes<T> == 3 && KP == 128 ? 32 : 64;
 
 template <typename T, int KP, bool VEC>
-__global__ __launch_bounds__((4 * kWalkSteps<T, KP>)) void lin_walk_kernel(LinWalkArgs g) {
+__global__ __launch_bounds__((8 * kWalkSteps<T, KP>)) void lin_walk_kernel(LinWalkArgs g) {
+  constexpr int C = kWalkSteps<T, KP>;
+  typedef LinWalk<T, KP, C, kOutputs> W;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  lin_walk_body<T, KP, VEC, kWalkSteps<T, KP>, kOutputs, false>(g, smem, block_of());
+  typename W::Lds& lds = *reinterpret_cast<typename W::Lds*>(smem);
+  LinUnit<C> u;
+  if (!u.init(g, block_of())) return;
+  const int id = (int)threadIdx.x;
+  if (id < W::NT) lin_outputs<T, KP, VEC, C>(g, u, lds, id);
+  else lin_states<T, KP, VEC, C, kOutputs, false>(g, u, lds, id - W::NT);
 }
 
 // The states' walk and its way back, side by side: the first nf workgroups go forward.
@@ -419,12 +439,17 @@ template <typename T, int KP, bool VEC, int MODE>
 __global__ __launch_bounds__((4 * kStateSteps<T, KP>)) void lin_states_kernel(LinWalkArgs f,
                                                                               LinWalkArgs back,
                                                                               uint32_t nf) {
+  constexpr int C = kStateSteps<T, KP>;
+  typedef LinWalk<T, KP, C, MODE> W;
   extern __shared__ __attribute__((aligned(16))) char smem[];
+  typename W::Lds& lds = *reinterpret_cast<typename W::Lds*>(smem);
   const uint32_t id = block_of();
-  if (id < nf)
-    lin_walk_body<T, KP, VEC, kStateSteps<T, KP>, MODE, false>(f, smem, id);
-  else
-    lin_walk_body<T, KP, VEC, kStateSteps<T, KP>, MODE, true>(back, smem, id - nf);
+  LinUnit<C> u;
+  if (id < nf) {
+    if (u.init(f, id)) lin_states<T, KP, VEC, C, MODE, false>(f, u, lds, (int)threadIdx.x);
+  } else {
+    if (u.init(back, id - nf)) lin_states<T, KP, VEC, C, MODE, true>(back, u, lds, (int)threadIdx.x);
+  }
 }
 
 // Sizes that a launch sets; returns its workgroups, or -1.
@@ -447,7 +472,7 @@ int lin_lds(K kernel, int bytes) {
 }
 
 template <typename T, int KP, bool VEC>
-int lin_walk(LinWalkArgs g, hipStream_t s) {
+int lin_walk_run(LinWalkArgs g, hipStream_t s) {
   typedef LinWalk<T, KP, kWalkSteps<T, KP>, kOutputs> W;
   static_assert(sizeof(typename W::Lds) <= 160 * 1024, "LDS of a CU");
   const int64_t wgs = lin_walk_sizes(g, kWalkSteps<T, KP>);
@@ -455,13 +480,13 @@ int lin_walk(LinWalkArgs g, hipStream_t s) {
   const auto kernel = lin_walk_kernel<T, KP, VEC>;
   const int rc = lin_lds(kernel, (int)sizeof(typename W::Lds));
   if (rc) return rc;
-  kernel<<<grid_of(wgs), W::NT, sizeof(typename W::Lds), s>>>(g);
+  kernel<<<grid_of(wgs), W::kThreads, sizeof(typename W::Lds), s>>>(g);
   return launch_status();
 }
 
 // back.walked = 0: forward alone.
 template <typename T, int KP, bool VEC, int MODE>
-int lin_states(LinWalkArgs f, LinWalkArgs back, hipStream_t s) {
+int lin_states_run(LinWalkArgs f, LinWalkArgs back, hipStream_t s) {
   typedef LinWalk<T, KP, kStateSteps<T, KP>, MODE> W;
   static_assert(sizeof(typename W::Lds) <= 160 * 1024, "LDS of a CU");
   const int64_t nf = lin_walk_sizes(f, kStateSteps<T, KP>);
@@ -470,7 +495,7 @@ int lin_states(LinWalkArgs f, LinWalkArgs back, hipStream_t s) {
   const auto kernel = lin_states_kernel<T, KP, VEC, MODE>;
   const int rc = lin_lds(kernel, (int)sizeof(typename W::Lds));
   if (rc) return rc;
-  kernel<<<grid_of(nf + nb), W::NT, sizeof(typename W::Lds), s>>>(f, back, (uint32_t)nf);
+  kernel<<<grid_of(nf + nb), W::kThreads, sizeof(typename W::Lds), s>>>(f, back, (uint32_t)nf);
   return launch_status();
 }
 

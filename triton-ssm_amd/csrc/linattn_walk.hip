@@ -6,7 +6,7 @@ namespace {
 
 template <typename T>
 int by_keys(const LinWalkArgs& g, bool vec, hipStream_t s) {
-#define TSSM_WALK(KP) (vec ? lin_walk<T, KP, true>(g, s) : lin_walk<T, KP, false>(g, s))
+#define TSSM_WALK(KP) (vec ? lin_walk_run<T, KP, true>(g, s) : lin_walk_run<T, KP, false>(g, s))
   if (g.a.K <= 32) return TSSM_WALK(32);
   if (g.a.K <= 64) return TSSM_WALK(64);
   return TSSM_WALK(128);

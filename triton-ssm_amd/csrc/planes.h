@@ -202,5 +202,33 @@ __device__ inline u32x4 lds_col16(const uint16_t* m, int ld, int col, int lane) 
   return u32x4{a[0], a[1], b[0], b[1]};
 }
 
+// Rows of N (32, 64 or 128) bf16 elements in LDS without padding: the 16-byte units of
+// a row are permuted, so that neither the 16 rows that an A operand's lanes read (lds16
+// at 8 (c / 4) + c % 4) nor the four that a transposed read takes share banks.
+template <int N>
+struct Swizzled {
+  static constexpr int kHigh = N == 128 ? 0 : (N == 64 ? 1 : 2);
+  static __device__ inline int at(int row, int unit) {
+    return row * N + ((unit ^ ((((row & 3) >> kHigh) << 2) | (row >> 3 & 3))) << 3);
+  }
+  // lds16 of row `row`, elements 8 unit and up
+  static __device__ inline u32x4 get(const uint16_t* m, int row, int unit) {
+    return lds16(m + at(row, unit));
+  }
+  // lds_col and lds_col16 of the 32 rows from `row` (a multiple of 32) on
+  static __device__ inline u32x4 col(const uint16_t* m, int row, int col, int lane) {
+    const int j = lane >> 4, i = lane & 15, r = 8 * j + (i >> 2);
+    const uint16_t* p = m + row * N + at(r, (col >> 3) + (i & 3)) + (col & 7);
+    const u32x2v a = lds_tr(p), b = lds_tr(p + 4 * N);
+    return u32x4{a[0], a[1], b[0], b[1]};
+  }
+  static __device__ inline u32x4 col16(const uint16_t* m, int row, int col, int lane) {
+    const int j = lane >> 4, i = lane & 15, r = 8 * j + (i >> 2);
+    const uint16_t* p = m + row * N + at(r, (col >> 3) + ((i & 3) >> 1)) + 4 * (i & 1);
+    const u32x2v a = lds_tr(p), b = lds_tr(p + 4 * N);
+    return u32x4{a[0], a[1], b[0], b[1]};
+  }
+};
+
 }  // namespace
 }  // namespace tssm
