@@ -83,21 +83,19 @@ template <int C>
 struct Gaps {
   static constexpr int E = C > 64 ? C / 64 : 1;
   float g[E];
-  // steps past `rows` count as 0
-  __device__ inline void load(const float* p, int64_t stride, int lane, int rows) {
+  int rows;  // steps past these count as 0: when they are used, not here (a load whose
+             // value is looked at in a branch is waited for in it)
+  __device__ inline void load(const float* p, int64_t stride, int lane, int n) {
+    rows = n;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int t = lane * E + e;
-      const float x = p[t < rows ? t * stride : 0];
-      g[e] = t < rows ? x : 0.0f;
-    }
+    for (int e = 0; e < E; ++e) g[e] = p[lane * E + e < n ? (lane * E + e) * stride : 0];
   }
   // One wave forms a chunk's decays.
   __device__ inline void decays(Decays<C>& d, int lane) const {
     double s[E], sum = 0.0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const float x = g[e] < -200.0f ? -200.0f : g[e];
+      const float x = lane * E + e < rows ? (g[e] < -200.0f ? -200.0f : g[e]) : 0.0f;
       sum += (double)x;
       s[e] = sum;
     }

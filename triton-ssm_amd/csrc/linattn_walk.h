@@ -216,18 +216,18 @@ __device__ inline void lin_states(const LinWalkArgs& g, const LinUnit<C>& u,
     split8<3>(v8, vp);
     f32x4 mine[OWN];
 #pragma unroll
-    for (int kt = 0; kt < KT; ++kt) {
-      u32x4 fk[NP];
+    for (int o = 0; o < NIQ; ++o) {  // the tiles of this wave, then of the others
+      const int other = (iq + o) % NIQ;
 #pragma unroll
-      for (int y = 0; y < NP; ++y)
-        fk[y] = KR::col(B.K[y], 32 * iq, 32 * (kt >> 1) + 4 * (kt & 1), lane);
-      const f32x4 x = mfma_planes<NP, 3, 3>(fk, vp, zero4());
-      if (kt / OWN == iq) {
+      for (int i = 0; i < OWN; ++i) {
+        const int kt = other * OWN + i;
+        u32x4 fk[NP];
 #pragma unroll
-        for (int i = 0; i < OWN; ++i)
-          if (kt % OWN == i) mine[i] = x;
-      } else {
-        lds.part[par][w][kt / OWN < iq ? kt : kt - OWN][lane] = x;
+        for (int y = 0; y < NP; ++y)
+          fk[y] = KR::col(B.K[y], 32 * iq, 32 * (kt >> 1) + 4 * (kt & 1), lane);
+        const f32x4 x = mfma_planes<NP, 3, 3>(fk, vp, zero4());
+        if (o == 0) mine[i] = x;
+        else lds.part[par][w][other < iq ? kt : kt - OWN][lane] = x;
       }
     }
     leave(lds.op[par ^ 1]);
