@@ -124,18 +124,18 @@ struct Gaps {
   }
 };
 
-// The planes of a piece of K or V, whose channels must not meet: take_plane() takes
-// the planes of a pair together, where a value that is not finite would reach its
-// neighbour.
+// The planes of a piece of q, k or v.  (Pieces of whole vectors are zero past the row's
+// end as they were read.)  Channels must not meet: take_plane() takes the planes of a
+// pair together, where a value that is not finite would reach its neighbour.
 template <typename T, bool VEC, int NP>
 __device__ inline void planes_apart(const Piece<T, VEC, NP>& x, int lim, u32x4* out) {
-  if constexpr (NP == 1) {
-    x.planes(lim, out);
+  if constexpr (NP == 1 && VEC) {
+    out[0] = x.w[0];
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      float a = 2 * i < lim ? ldf(&x.e[2 * i]) : 0.0f;
-      float b = 2 * i + 1 < lim ? ldf(&x.e[2 * i + 1]) : 0.0f;
+      float a = VEC || 2 * i < lim ? ldf(&x.e[2 * i]) : 0.0f;
+      float b = VEC || 2 * i + 1 < lim ? ldf(&x.e[2 * i + 1]) : 0.0f;
 #pragma unroll
       for (int n = 0; n < NP; ++n) {
         const uint32_t w = pk_bf16(a, b);

@@ -5,29 +5,34 @@
 //   O = scale (e^G Q S + (Q K^T D) V),   S' = e^(G_end) S + K^T (e^(G_end - G) V).
 // Only S' waits for S, by one product and a sum; all the rest of a chunk is its own.
 //
-// A workgroup walks 32 columns of V of one head's segment, with C / 16 waves for the
-// outputs and as many for the states.  An output wave has 16 steps of the chunk.  A
-// state wave brings its share of K and V to LDS and forms K^T V of 32 steps and 16
-// columns, all of K, of which it keeps the tiles of the state that are its own and
-// hands the others to their owners through LDS.  Everything is formed transposed
-// (planes.h): P^T = K Q^T is the next product's operand in place, queries come to
-// their wave straight from memory, and a lane ends up with 8 neighbouring columns of
-// one step's output.  One barrier a chunk:
-//   before it: P and its part of the output | K^T V, the next chunk to LDS,
-//   after it: the state's part of the output from planes that the owners left in
-//     LDS a chunk ago | the next state and its planes.
-// K and V are in LDS twice, a third chunk's loads are in flight.
+// A workgroup walks 32 columns of V of one head's segment.  Its waves have roles, one
+// barrier a chunk:
+//   two teams of C / 32 output waves (one where LDS does not hold three chunks): 32
+//     steps of a chunk each, as two tiles of 16.  A team has every other chunk, and
+//     two chunks' time for it,
+//   2 state waves: 16 columns each.  K^T V of the whole chunk on top of the decayed
+//     state, whose planes go to LDS for the next chunk's outputs,
+//   loaders: the chunk after this one to LDS, from loads that are two chunks ahead.
+// Everything is formed transposed (planes.h): P^T = K Q^T is the next product's operand
+// in place, queries come to their wave straight from memory, and a lane ends up with 8
+// neighbouring columns of one step's output.
 //
-// D of the 32 steps before the wave's own is a product of two factors with the decay
-// from that block's end between them: one exponential for a lane and block and a
-// table of the chunk's, instead of one for every weight.
+// LDS sets the time: a 16-byte read takes it 16 cycles, so an operand that is read
+// should serve as many products as it can.  The two tiles of an output wave share K, V
+// and the state's planes (B=8 L=4096 H=16 64 x 64 bf16: WALKTIME us; 84 with a wave for
+// each tile), and a state wave that has all steps of its columns needs no exchange.
+// Tiles a and C / 16 - 1 - a are together, five blocks of K in all whatever a is.
+//
+// D of the 32 steps before a tile's own is a product of two factors with the decay from
+// that block's end between them: one exponential for a lane and block and a table of
+// the chunk's, instead of one for every weight.
 //
 // Two more forms leave out the outputs: the state at the end of a segment that starts
 // from zero, and the states before all chunks (for the gradients).  Walked backwards,
 // with queries for keys and dO for V, they give the gradients of the states.
 //
-// A wave whose own block's output is not finite forms it again without the steps
-// after each row: weights of zero would carry a later step's NaN to earlier outputs.
+// A tile whose own block's output is not finite forms it again without the steps after
+// each row: weights of zero would carry a later step's NaN to earlier outputs.
 #pragma once
 
 #include "linattn_dev.h"
@@ -51,26 +56,34 @@ struct LinWalkArgs {
   double* sums;        // kEnds: [bh][nseg], of g / log 2
 };
 
+// Teams of output waves, and steps of a chunk: as many as LDS holds (a chunk more of K's
+// and the state's planes than there are teams).
+constexpr int lin_teams(int NP, int KP) { return NP * KP <= 256 ? 2 : 1; }
+template <typename T, int KP>
+constexpr int kWalkSteps = kPlanes<T> * KP <= 64 ? 128 : (kPlanes<T> * KP <= 192 ? 64 : 32);
+// The gradients' kernel asks for chunks of its own.
+template <typename T, int KP>
+constexpr int kStateSteps = kPlanes<T> == 3 && KP == 128 ? 32 : 64;
+
 template <typename T, int KP, int C, int MODE>
 struct LinWalk {
   static constexpr int NP = kPlanes<T>, NO = kOutPlanes<T>;
-  static constexpr int NS = KP / 32, KT = KP / 16, NW = C / 16, NT = 64 * NW, NIQ = C / 32;
-  static constexpr int OWN = KT / NIQ;       // tiles of the state that a wave keeps
+  static constexpr int NS = KP / 32, KT = KP / 16, NB = C / 32;
+  static constexpr int TEAMS = MODE == kOutputs ? lin_teams(NP, KP) : 1, RING = TEAMS + 1;
+  static constexpr int NW = MODE == kOutputs ? TEAMS * C / 32 : 0;  // output waves
+  static constexpr int NT = 128;                            // threads of the loaders
+  static constexpr int kThreads = 64 * (NW + 2) + NT;
+  static constexpr int kNk = (C * KP / 8 + NT - 1) / NT, kNv = (C * 4 + NT - 1) / NT;
   typedef Swizzled<KP> KR;                   // rows of K and of the state's planes
   typedef Swizzled<32> VR;                   // of V
-  // outputs and states have waves of their own
-  static constexpr int kThreads = MODE == kOutputs ? 2 * NT : NT;
-  static constexpr int kNk = C * KP / 8 / NT;    // 8-element pieces of K a thread brings
-  static_assert(KT % NIQ == 0, "every wave owns tiles");
   struct Operands {  // of one chunk
     uint16_t K[NP][C * KP], V[NP][C * 32];
     Decays<C> d;
   };
   struct Lds {
-    Operands op[2];
-    f32x4 part[2][NW][KT - OWN ? KT - OWN : 1][64];
+    Operands op[RING];
     // planes of S^T, a row for each column of V
-    uint16_t S[MODE == kOutputs ? 2 : 1][NO][MODE == kOutputs ? 32 * KP : 8];
+    uint16_t S[MODE == kOutputs ? RING : 1][NO][MODE == kOutputs ? 32 * KP : 8];
   };
 };
 
@@ -97,358 +110,431 @@ struct LinUnit {
   }
 };
 
-// The waves of the states, and of K and V's way to LDS.
-template <typename T, int KP, bool VEC, int C, int MODE, bool REV>
-__device__ inline void lin_states(const LinWalkArgs& g, const LinUnit<C>& u,
-                                  typename LinWalk<T, KP, C, MODE>::Lds& lds, int id) {
-  typedef LinWalk<T, KP, C, MODE> W;
-  typedef typename W::KR KR;
-  typedef typename W::VR VR;
-  constexpr int NP = W::NP, NO = W::NO, KT = W::KT, NT = W::NT, NIQ = W::NIQ, OWN = W::OWN,
-                kE = (int)sizeof(T);
-  const LinArgs& a = g.a;
-  const int lane = id & 63, j = lane >> 4, c = lane & 15, cnt = u.n1 - u.n0, K = (int)a.K;
-  const int w = __builtin_amdgcn_readfirstlane(id >> 6);
-  const int iq = w >> 1, vt = w & 1;         // 32 steps, 16 columns for K^T V
-  const int64_t elems = lin_state_elems(KP, a.V), col = u.v0 + 16 * vt + c;
-  const int64_t tile0 = ((u.v0 / 16 + vt) * KT + iq * OWN) * 256 + lane * 4;
+// The chunk of step m of a walk.
+template <int C, bool REV>
+__device__ inline int lin_chunk(const LinUnit<C>& u, int m) {
+  const int cnt = u.n1 - u.n0, x = m < cnt ? m : cnt - 1;
+  return REV ? u.n1 - 1 - x : u.n0 + x;
+}
 
+// K's, V's and the decays' way to LDS.
+template <typename T, int KP, bool VEC, int C, int MODE, bool REV>
+__device__ inline void lin_bring(const LinWalkArgs& g, const LinUnit<C>& u,
+                                 typename LinWalk<T, KP, C, MODE>::Lds& lds, int id) {
+  typedef LinWalk<T, KP, C, MODE> W;
+  constexpr int NP = W::NP, NT = W::NT, kE = (int)sizeof(T), U = KP / 8;
+  const LinArgs& a = g.a;
+  const int lane = id & 63, cnt = u.n1 - u.n0, K = (int)a.K;
+  const bool first = __builtin_amdgcn_readfirstlane(id >> 6) == 0;
   RowsOf<C> rk, rv;
   rk.init(reinterpret_cast<const T*>(a.k) + u.b * a.k_b + u.hk * a.k_h, a.k_l, K, a.L);
   rv.init(reinterpret_cast<const T*>(a.v) + u.b * a.v_b + u.h * a.v_h + u.v0, a.v_l, u.nv, a.L);
   const float* gp = a.g + u.b * a.g_b + u.h * a.g_h;
-  const auto chunk = [&](int m) {   // the chunk of step m of the walk
-    const int x = m < cnt ? m : cnt - 1;
-    return REV ? u.n1 - 1 - x : u.n0 + x;
-  };
-  Piece<T, VEC, NP> ink[W::kNk], inv;
-  Gaps<C> gaps;
-  const auto fetch = [&](int m) {
-    const int n = chunk(m);
+  struct Regs {
+    Piece<T, VEC, NP> k[W::kNk], v[W::kNv];
+    Gaps<C> g;
+  } in0, in1;
+  const auto fetch = [&](Regs& in, int m) {
+    const int n = lin_chunk<C, REV>(u, m);
     const auto dk = rk.at(n), dv = rv.at(n);
 #pragma unroll
     for (int i = 0; i < W::kNk; ++i) {
-      const int at = id + NT * i, r = at / (KP / 8), x = at % (KP / 8) * 8;
-      ink[i].load(dk, x < K ? r * rk.row + x * kE : kPast);
+      const int at = id + NT * i, r = at / U, x = at % U * 8;
+      in.k[i].load(dk, r < C && x < K ? r * rk.row + x * kE : kPast);
     }
-    const int r = id >> 2, x = (id & 3) * 8;
-    inv.load(dv, x < u.nv ? r * rv.row + x * kE : kPast);
-    if (w == 0) {
+#pragma unroll
+    for (int i = 0; i < W::kNv; ++i) {
+      const int at = id + NT * i, r = at >> 2, x = (at & 3) * 8;
+      in.v[i].load(dv, r < C && x < u.nv ? r * rv.row + x * kE : kPast);
+    }
+    if (first) {
       const int64_t t0 = (int64_t)n * C, rest = a.L - t0;
-      gaps.load(gp + t0 * a.g_l, a.g_l, lane, rest < C ? (int)rest : C);
+      in.g.load(gp + t0 * a.g_l, a.g_l, lane, rest < C ? (int)rest : C);
     }
   };
-  const auto leave = [&](typename W::Operands& o) {  // what fetch() brought, to LDS
+  const auto leave = [&](const Regs& in, typename W::Operands& o) {
 #pragma unroll
     for (int i = 0; i < W::kNk; ++i) {
-      const int at = id + NT * i, r = at / (KP / 8), x = at % (KP / 8);
+      const int at = id + NT * i, r = at / U, x = at % U;
       u32x4 p[NP];
-      planes_apart(ink[i], K - 8 * x, p);
+      planes_apart(in.k[i], K - 8 * x, p);
+      if (C * U % NT == 0 || r < C) {
 #pragma unroll
-      for (int y = 0; y < NP; ++y) *reinterpret_cast<u32x4*>(&o.K[y][KR::at(r, x)]) = p[y];
+        for (int y = 0; y < NP; ++y)
+          *reinterpret_cast<u32x4*>(&o.K[y][W::KR::at(r, x)]) = p[y];
+      }
     }
-    const int r = id >> 2, x = id & 3;
-    u32x4 p[NP];
-    planes_apart(inv, u.nv - 8 * x, p);
 #pragma unroll
-    for (int y = 0; y < NP; ++y) *reinterpret_cast<u32x4*>(&o.V[y][VR::at(r, x)]) = p[y];
-    if (w == 0) gaps.decays(o.d, lane);
+    for (int i = 0; i < W::kNv; ++i) {
+      const int at = id + NT * i, r = at >> 2, x = at & 3;
+      u32x4 p[NP];
+      planes_apart(in.v[i], u.nv - 8 * x, p);
+      if (C * 4 % NT == 0 || r < C) {
+#pragma unroll
+        for (int y = 0; y < NP; ++y)
+          *reinterpret_cast<u32x4*>(&o.V[y][W::VR::at(r, x)]) = p[y];
+      }
+    }
+    if (first) in.g.decays(o.d, lane);
   };
-  f32x4 S[OWN];
+  fetch(in0, 0);
+  fetch(in1, 1);
+  leave(in0, lds.op[0]);
+  fetch(in0, 2);
+  lds_barrier();
+  int slot = 1;
+  const auto turn = [&](int m, Regs& in) {  // in holds chunk m + 1
+    leave(in, lds.op[slot]);
+    slot = slot + 1 < W::RING ? slot + 1 : 0;
+    fetch(in, m + 3);
+    lds_barrier();
+  };
+  for (int m = 0; m < cnt; m += 2) {
+    turn(m, in1);
+    if (m + 1 < cnt) turn(m + 1, in0);
+  }
+  if constexpr (W::TEAMS == 2) lds_barrier();
+}
+
+// The states' waves: vt, 16 columns.
+template <typename T, int KP, int C, int MODE, bool REV>
+__device__ inline void lin_states(const LinWalkArgs& g, const LinUnit<C>& u,
+                                  typename LinWalk<T, KP, C, MODE>::Lds& lds, int lane, int vt) {
+  typedef LinWalk<T, KP, C, MODE> W;
+  typedef typename W::KR KR;
+  constexpr int NP = W::NP, NO = W::NO, KT = W::KT, NB = W::NB;
+  const LinArgs& a = g.a;
+  const int j = lane >> 4, c = lane & 15, cnt = u.n1 - u.n0, K = (int)a.K;
+  const int64_t elems = lin_state_elems(KP, a.V), col = u.v0 + 16 * vt + c;
+  const int64_t tile0 = (u.v0 / 16 + vt) * KT * 256 + lane * 4;
+  f32x4 S[KT];
 #pragma unroll
-  for (int i = 0; i < OWN; ++i) {
+  for (int i = 0; i < KT; ++i) {
     if constexpr (MODE == kEnds) S[i] = zero4();
     else if (g.nseg == 1)
-      S[i] = get_tile(a.h0 ? a.h0 + u.bh * K * a.V : nullptr, iq * OWN + i, col, a.V, K, j);
+      S[i] = get_tile(a.h0 ? a.h0 + u.bh * K * a.V : nullptr, i, col, a.V, K, j);
     else
       S[i] = *reinterpret_cast<const f32x4*>(g.entry + (u.bh * g.nseg + u.seg) * elems + tile0 +
                                              256 * i);
   }
-  const auto show = [&](int par) {  // the state's planes, for the outputs
+  const auto show = [&](int slot) {  // the state's planes, for the outputs
     if constexpr (MODE == kOutputs) {
 #pragma unroll
-      for (int i = 0; i < OWN; ++i) {
-        const int kt = iq * OWN + i;
-        float x0 = S[i][0], x1 = S[i][1], x2 = S[i][2], x3 = S[i][3];
+      for (int s = 0; s < KT / 2; ++s) {
+        u32x4 p[NO];
+        split_tiles<NO>(S[2 * s], S[2 * s + 1], p);
 #pragma unroll
-        for (int p = 0; p < NO; ++p) {
-          const uint32_t lo = pk_bf16(x0, x1), hi = pk_bf16(x2, x3);
-          *reinterpret_cast<uint2*>(&lds.S[par][p][KR::at(16 * vt + c, 4 * (kt >> 1) + j) +
-                                                   4 * (kt & 1)]) = make_uint2(lo, hi);
-          if (p + 1 < NO) {
-            take_plane(lo, x0, x1);
-            take_plane(hi, x2, x3);
-          }
-        }
+        for (int y = 0; y < NO; ++y)
+          *reinterpret_cast<u32x4*>(&lds.S[slot][y][KR::at(16 * vt + c, 4 * s + j)]) = p[y];
       }
     }
   };
   double total = 0.0;
-  fetch(0);
-  leave(lds.op[0]);
+  int slot = 0;
   show(0);
-  fetch(1);
   lds_barrier();
   for (int m = 0; m < cnt; ++m) {
-    const int par = m & 1;
-    const typename W::Operands& B = lds.op[par];
+    const typename W::Operands& B = lds.op[slot];
     const float hend = B.d.hi[C - 1], lend = B.d.lo[C - 1];
     const float last = exp2_fast(hend + lend);
     if constexpr (MODE == kEnds) total += (double)hend + (double)lend;
-    // this wave's 32 steps of K^T V
-    float v8[8], e8[8];
-    lds_values<NP, 32>(&B.V[0][0], C * 32, 32 * iq, 16 * vt, lane, v8);
-    if constexpr (REV) {
-      float h8[8], l8[8];
-      lds8(&B.d.hi[32 * iq + 8 * j], h8);
-      lds8(&B.d.lo[32 * iq + 8 * j], l8);
+    if constexpr (MODE == kStates) {
+      float* p = g.states + (u.bh * g.nch + lin_chunk<C, REV>(u, m)) * elems + tile0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) e8[e] = a.scale * exp2_fast(h8[e] + l8[e]);
-    } else {
-      lds8(&B.d.u[32 * iq + 8 * j], e8);
-      const float from = diff2(hend, lend, B.d.hi[32 * iq + 31], B.d.lo[32 * iq + 31]);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) e8[e] *= from;
+      for (int i = 0; i < KT; ++i) *reinterpret_cast<f32x4*>(p + 256 * i) = S[i];
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v8[e] *= e8[e];
-    u32x4 vp[3];
-    split8<3>(v8, vp);
-    f32x4 mine[OWN];
+    for (int i = 0; i < KT; ++i)
 #pragma unroll
-    for (int o = 0; o < NIQ; ++o) {  // the tiles of this wave, then of the others
-      const int other = (iq + o) % NIQ;
+      for (int r = 0; r < 4; ++r) S[i][r] *= last;
 #pragma unroll
-      for (int i = 0; i < OWN; ++i) {
-        const int kt = other * OWN + i;
-        u32x4 fk[NP];
+    for (int ib = 0; ib < NB; ++ib) {  // operands asked for at once
+      float v8[8], e8[8], l8[8], from = 0.0f;
+      u32x4 fk[KT][NP];
+      lds_values<NP, 32>(&B.V[0][0], C * 32, 32 * ib, 16 * vt, lane, v8);
+      if constexpr (REV) {
+        lds8(&B.d.hi[32 * ib + 8 * j], e8);
+        lds8(&B.d.lo[32 * ib + 8 * j], l8);
+      } else {
+        lds8(&B.d.u[32 * ib + 8 * j], e8);
+        from = diff2(hend, lend, B.d.hi[32 * ib + 31], B.d.lo[32 * ib + 31]);
+      }
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
         for (int y = 0; y < NP; ++y)
-          fk[y] = KR::col(B.K[y], 32 * iq, 32 * (kt >> 1) + 4 * (kt & 1), lane);
-        const f32x4 x = mfma_planes<NP, 3, 3>(fk, vp, zero4());
-        if (o == 0) mine[i] = x;
-        else lds.part[par][w][other < iq ? kt : kt - OWN][lane] = x;
-      }
+          fk[kt][y] = KR::col(B.K[y], 32 * ib, 32 * (kt >> 1) + 4 * (kt & 1), lane);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        v8[e] *= REV ? a.scale * exp2_fast(e8[e] + l8[e]) : e8[e] * from;
+      u32x4 vp[3];
+      split8<3>(v8, vp);
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) S[kt] = mfma_planes<NP, 3, 3>(fk[kt], vp, S[kt]);
     }
-    leave(lds.op[par ^ 1]);
-    fetch(m + 2);
+    slot = slot + 1 < W::RING ? slot + 1 : 0;
+    show(slot);
     lds_barrier();
-    if constexpr (MODE == kStates) {
-      float* p = g.states + (u.bh * g.nch + chunk(m)) * elems + tile0;
-#pragma unroll
-      for (int i = 0; i < OWN; ++i) *reinterpret_cast<f32x4*>(p + 256 * i) = S[i];
-    }
-#pragma unroll
-    for (int i = 0; i < OWN; ++i) {
-      f32x4 x = mine[i];
-#pragma unroll
-      for (int o = 1; o < NIQ; ++o) {
-        const int other = (iq + o) % NIQ, kt = iq * OWN + i;
-        x += lds.part[par][2 * other + vt][iq < other ? kt : kt - OWN][lane];
-      }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) S[i][r] = __builtin_fmaf(S[i][r], last, x[r]);
-    }
-    show(par ^ 1);
   }
+  if constexpr (W::TEAMS == 2) lds_barrier();
   if constexpr (MODE == kEnds) {
     float* p = g.states + (u.bh * g.nseg + u.seg) * elems + tile0;
 #pragma unroll
-    for (int i = 0; i < OWN; ++i) *reinterpret_cast<f32x4*>(p + 256 * i) = S[i];
-    if (u.v0 == 0 && id == 0) g.sums[u.bh * g.nseg + u.seg] = total;
+    for (int i = 0; i < KT; ++i) *reinterpret_cast<f32x4*>(p + 256 * i) = S[i];
+    if (u.v0 == 0 && vt == 0 && lane == 0) g.sums[u.bh * g.nseg + u.seg] = total;
   } else if (REV ? u.n0 == 0 : u.n1 == g.nch) {
     float* p = a.h_last ? a.h_last + u.bh * K * a.V : nullptr;
 #pragma unroll
-    for (int i = 0; i < OWN; ++i) put_tile(p, S[i], iq * OWN + i, col, a.V, K, j);
+    for (int i = 0; i < KT; ++i) put_tile(p, S[i], i, col, a.V, K, j);
   }
 }
 
-// The waves of the outputs.
-template <typename T, int KP, bool VEC, int C>
+// The outputs' waves: tiles a0 and C / 16 - 1 - a0, whose own blocks of 32 steps are EB
+// and LB.
+template <typename T, int KP, bool VEC, int C, int EB, int LB>
 __device__ inline void lin_outputs(const LinWalkArgs& g, const LinUnit<C>& u,
-                                   typename LinWalk<T, KP, C, kOutputs>::Lds& lds, int id) {
+                                   typename LinWalk<T, KP, C, kOutputs>::Lds& lds, int lane,
+                                   int a0, int team) {
   typedef LinWalk<T, KP, C, kOutputs> W;
   typedef typename W::KR KR;
   typedef typename W::VR VR;
-  constexpr int NP = W::NP, NO = W::NO, NS = W::NS, kE = (int)sizeof(T);
+  constexpr int NP = W::NP, NO = W::NO, NS = W::NS, TEAMS = W::TEAMS, kE = (int)sizeof(T);
+  constexpr int kOwn[2] = {EB, LB};
   const LinArgs& a = g.a;
-  const int lane = id & 63, j = lane >> 4, c = lane & 15, cnt = u.n1 - u.n0, K = (int)a.K;
-  const int w = __builtin_amdgcn_readfirstlane(id >> 6);
-  // 16 steps: waves w and w + 4, on one SIMD, have equal work together
-  const int tw = C == 128 && w >= 4 ? 11 - w : w, db = tw >> 1, t = 16 * tw + c;
+  const int j = lane >> 4, c = lane & 15, cnt = u.n1 - u.n0, K = (int)a.K;
+  const int t[2] = {16 * a0 + c, 16 * (C / 16 - 1 - a0) + c};
   const int ar = 8 * (c >> 2) + (c & 3);     // row of tile x of an A operand, less 4 x
   RowsOf<C> rq, ro;
   rq.init(reinterpret_cast<const T*>(a.q) + u.b * a.q_b + u.hk * a.q_h, a.q_l, K, a.L);
   ro.init(reinterpret_cast<const T*>(a.o) + u.b * a.o_b + u.h * a.o_h + u.v0, a.o_l, u.nv, a.L);
-  Piece<T, VEC, NP> in[NS];
+  Piece<T, VEC, NP> in[2][NS];
   const auto fetch = [&](int m) {
-    const auto d = rq.at(u.n0 + (m < cnt ? m : cnt - 1));
+    const auto d = rq.at(lin_chunk<C, false>(u, m));
 #pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      const int y = 32 * s + 8 * j;
-      in[s].load(d, y < K ? t * rq.row + y * kE : kPast);
-    }
-  };
-  fetch(0);
-  lds_barrier();
-  for (int m = 0; m < cnt; ++m) {
-    const int par = m & 1;
-    const typename W::Operands& B = lds.op[par];
-    u32x4 qb[NS][NP];
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int s = 0; s < NS; ++s) in[s].planes(K - 32 * s - 8 * j, qb[s]);
-    fetch(m + 1);
-    f32x4 acc[2] = {zero4(), zero4()}, own[2] = {zero4(), zero4()};
-    const float ht = B.d.hi[t], lt = B.d.lo[t], eg = exp2_fast(ht + lt);
-    float p8[8];  // of the last block, the wave's own
-    // NB blocks of 32 steps, in one piece so that they overlap; the last is masked
-    const auto blocks = [&](auto count) {
-      constexpr int NB = decltype(count)::value;
-      f32x4 p[NB][2];
-      float from[NB];
-#pragma unroll
-      for (int ib = 0; ib < NB; ++ib) {
-        from[ib] = diff2(ht, lt, B.d.hi[32 * ib + 31], B.d.lo[32 * ib + 31]);
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          p[ib][x] = zero4();
-#pragma unroll
-          for (int s = 0; s < NS; ++s) {  // rows i = 32 ib + 8 j + 4 x + r of K Q^T
-            u32x4 fk[NP];
-#pragma unroll
-            for (int y = 0; y < NP; ++y)
-              fk[y] = lds16(&B.K[y][KR::at(ar, 4 * s + j) + (32 * ib + 4 * x) * KP]);
-            p[ib][x] = mfma_planes<NP, NP, NO>(fk, qb[s], p[ib][x]);
-          }
-        }
+      for (int s = 0; s < NS; ++s) {
+        const int y = 32 * s + 8 * j;
+        in[i][s].load(d, y < K ? t[i] * rq.row + y * kE : kPast);
       }
+  };
+  fetch(team);
+  lds_barrier();
+  if (team) lds_barrier();
+  int slot = team;
+  for (int m = team; m < cnt; m += TEAMS) {
+    const typename W::Operands& B = lds.op[slot];
+    const auto& Sp = lds.S[slot];
+    slot = slot + TEAMS < W::RING ? slot + TEAMS : slot + TEAMS - W::RING;
+    u32x4 qb[2][NS][NP], fk[2][NS][NP], fv[2][NP];
+    float u8[8], h8[8], l8[8], ht[2], lt[2];
+    const auto keys = [&](int ib) {
 #pragma unroll
-      for (int ib = 0; ib < NB; ++ib) {
-        if (ib + 1 < NB) {
-          float u8[8];
-          lds8(&B.d.u[32 * ib + 8 * j], u8);
+      for (int s = 0; s < NS; ++s)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) p8[e] = p[ib][e >> 2][e & 3] * (u8[e] * from[ib]);
-        } else {
-          float h8[8], l8[8];
-          lds8(&B.d.hi[32 * ib + 8 * j], h8);
-          lds8(&B.d.lo[32 * ib + 8 * j], l8);
+        for (int x = 0; x < 2; ++x)
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            p8[e] = 32 * ib + 8 * j + e <= t
-                        ? p[ib][e >> 2][e & 3] * diff2(ht, lt, h8[e], l8[e]) : 0.0f;
-        }
-        u32x4 pb[NO];
-        split8<NO>(p8, pb);
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {  // V^T P^T
-          u32x4 fv[NP];
-#pragma unroll
-          for (int y = 0; y < NP; ++y) fv[y] = VR::col(B.V[y], 32 * ib, 4 * x, lane);
-          f32x4& o = ib + 1 < NB ? acc[x] : own[x];
-          o = mfma_planes<NP, NO, NO>(fv, pb, o);
-        }
+          for (int y = 0; y < NP; ++y)
+            fk[x][s][y] = lds16(&B.K[y][KR::at(ar, 4 * s + j) + (32 * ib + 4 * x) * KP]);
+    };
+    const auto decays = [&](int ib) {
+      if (ib < LB) lds8(&B.d.u[32 * ib + 8 * j], u8);
+      if (ib == EB || ib == LB) {
+        lds8(&B.d.hi[32 * ib + 8 * j], h8);
+        lds8(&B.d.lo[32 * ib + 8 * j], l8);
       }
     };
-    if (C == 32 || db == 0) blocks(std::integral_constant<int, 1>());
-    else if (C == 64 || db == 1) blocks(std::integral_constant<int, 2>());
-    else if (db == 2) blocks(std::integral_constant<int, 3>());
-    else blocks(std::integral_constant<int, 4>());
-    float big = 0.0f;
+    const auto values = [&](int ib) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) big += __builtin_fabsf(own[e >> 2][e & 3]);
-    if (__builtin_expect(__ballot(!(big < __builtin_inff())) != 0, 0)) {
-      own[0] = own[1] = zero4();
-#pragma unroll 1
-      for (int i = 0; i < 32; ++i) {
-        float p = 0.0f;
+      for (int x = 0; x < 2; ++x)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) p = (i & 7) == e ? p8[e] : p;
-        p = __shfl(p, (i >> 3) * 16 + c);
+        for (int y = 0; y < NP; ++y) fv[x][y] = VR::col(B.V[y], 32 * ib, 4 * x, lane);
+    };
+    // Operands are asked for a product ahead: read where they are used, each would
+    // wait for LDS.
+    keys(0);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float v = 0.0f;
-#pragma unroll
-          for (int y = NP - 1; y >= 0; --y)
-            v += bf16_bits_to_f32(B.V[y][VR::at(32 * db + i, j) + e]);
-          if (32 * db + i <= t) own[e >> 2][e & 3] += p * v;
-        }
-      }
+    for (int i = 0; i < 2; ++i) {
+      ht[i] = B.d.hi[t[i]];
+      lt[i] = B.d.lo[t[i]];
     }
-    lds_barrier();
-    f32x4 y[2] = {zero4(), zero4()};
+    decays(0);
+    values(0);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int s = 0; s < NS; ++s) planes_apart(in[i][s], K - 32 * s - 8 * j, qb[i][s]);
+    fetch(m + TEAMS);
+    __builtin_amdgcn_sched_barrier(0);
+    f32x4 acc[2][2], own[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) acc[i][0] = acc[i][1] = zero4();
+#pragma unroll
+    for (int ib = 0; ib <= LB; ++ib) {
+      f32x4 p[2][2];  // rows i = 32 ib + 8 j + 4 x + r of K Q^T
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (ib > kOwn[i]) continue;
+        p[i][0] = p[i][1] = zero4();
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            p[i][x] = mfma_planes<NP, NP, NO>(fk[x][s], qb[i][s], p[i][x]);
+      }
+      if (ib < LB) keys(ib + 1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (ib > kOwn[i]) continue;
+        float w8[8];
+        if (ib < kOwn[i]) {
+          const float from = diff2(ht[i], lt[i], B.d.hi[32 * ib + 31], B.d.lo[32 * ib + 31]);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) w8[e] = p[i][e >> 2][e & 3] * (u8[e] * from);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            float y = p[i][e >> 2][e & 3] * diff2(ht[i], lt[i], h8[e], l8[e]);
+            asm("" : "+v"(y));  // formed for all, then chosen: no branch
+            w8[e] = 32 * ib + 8 * j + e <= t[i] ? y : 0.0f;
+          }
+        }
+        u32x4 pb[NO];
+        split8<NO>(w8, pb);
+        if (ib < kOwn[i]) {
+#pragma unroll
+          for (int x = 0; x < 2; ++x)  // V^T P^T
+            acc[i][x] = mfma_planes<NP, NO, NO>(fv[x], pb, acc[i][x]);
+          continue;
+        }
+        float big = 0.0f;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) own[x] = mfma_planes<NP, NO, NO>(fv[x], pb, zero4());
+#pragma unroll
+        for (int e = 0; e < 8; ++e) big += __builtin_fabsf(own[e >> 2][e & 3]);
+        if (__builtin_expect(__ballot(!(big < __builtin_inff())) != 0, 0)) {
+          own[0] = own[1] = zero4();
+#pragma unroll 1
+          for (int n = 0; n < 32; ++n) {
+            float w = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w = (n & 7) == e ? w8[e] : w;
+            w = __shfl(w, (n >> 3) * 16 + c);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              float v = 0.0f;
+#pragma unroll
+              for (int y = NP - 1; y >= 0; --y)
+                v += bf16_bits_to_f32(B.V[y][VR::at(32 * ib + n, j) + e]);
+              if (32 * ib + n <= t[i]) own[e >> 2][e & 3] += w * v;
+            }
+          }
+        }
+        acc[i][0] += own[0];
+        acc[i][1] += own[1];
+      }
+      if (ib < LB) {
+        decays(ib + 1);
+        values(ib + 1);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      // half of the work: the rest while the other team has its first half
+      if (TEAMS == 2 && ib == LB / 2) lds_barrier();
+    }
+    // the state's part
+    u32x4 fs[NS][2][NO];
 #pragma unroll
     for (int s = 0; s < NS; ++s)
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        u32x4 fs[NO];
+      for (int x = 0; x < 2; ++x)
 #pragma unroll
         for (int p = 0; p < NO; ++p)
-          fs[p] = lds16(&lds.S[par][p][KR::at(ar, 4 * s + j) + 4 * x * KP]);
-        y[x] = mfma_planes<NO, NP, NO>(fs, qb[s], y[x]);
-      }
+          fs[s][x][p] = lds16(&Sp[p][KR::at(ar, 4 * s + j) + 4 * x * KP]);
     const auto dst = ro.at(u.n0 + m);
-    const uint32_t off = (uint32_t)(t * ro.row + 8 * j * kE);
-    float o8[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      o8[e] = a.scale * __builtin_fmaf(y[e >> 2][e & 3], eg,
-                                       acc[e >> 2][e & 3] + own[e >> 2][e & 3]);
-    if constexpr (VEC) {
-      const uint32_t to = 8 * j < u.nv ? off : kPast;
-      union {
-        T e[8];
-        u32x4 v[kE / 2];
-      } x;
+    for (int i = 0; i < 2; ++i) {
+      f32x4 y[2] = {zero4(), zero4()};
 #pragma unroll
-      for (int e = 0; e < 8; ++e) stf(&x.e[e], o8[e]);
+      for (int s = 0; s < NS; ++s)
 #pragma unroll
-      for (int i = 0; i < kE / 2; ++i)
-        __builtin_amdgcn_raw_buffer_store_b128(x.v[i], dst, to + 16 * i, 0, 0);
-    } else {
+        for (int x = 0; x < 2; ++x) y[x] = mfma_planes<NO, NP, NO>(fs[s][x], qb[i][s], y[x]);
+      const float eg = exp2_fast(ht[i] + lt[i]);
+      const uint32_t off = (uint32_t)(t[i] * ro.row + 8 * j * kE);
+      float o8[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        buf_put<T>(dst, 8 * j + e < u.nv ? off + e * kE : kPast, o8[e]);
+        o8[e] = a.scale * __builtin_fmaf(y[e >> 2][e & 3], eg, acc[i][e >> 2][e & 3]);
+      if constexpr (VEC) {
+        const uint32_t to = 8 * j < u.nv ? off : kPast;
+        union {
+          T e[8];
+          u32x4 v[kE / 2];
+        } x;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) stf(&x.e[e], o8[e]);
+#pragma unroll
+        for (int n = 0; n < kE / 2; ++n)
+          __builtin_amdgcn_raw_buffer_store_b128(x.v[n], dst, to + 16 * n, 0, 0);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          buf_put<T>(dst, 8 * j + e < u.nv ? off + e * kE : kPast, o8[e]);
+      }
     }
+    lds_barrier();
   }
+  // the barriers that are left of cnt + 1: this team's chunks have had two each
+  if (TEAMS == 2 && ((cnt - team) & 1) == 0) lds_barrier();
 }
 
-// Steps of a chunk: as many as LDS holds (two chunks of K's planes).  The gradients'
-// kernel asks for chunks of its own.
-template <typename T, int KP>
-constexpr int kWalkSteps = kPlanes<T> == 1 && KP == 64 ? 128
-                           : (kPlanes<T> == 3 && KP == 128 ? 32 : 64);
-template <typename T, int KP>
-constexpr int kStateSteps = kPlanes<T> == 3 && KP == 128 ? 32 : 64;
-
 template <typename T, int KP, bool VEC>
-__global__ __launch_bounds__((8 * kWalkSteps<T, KP>)) void lin_walk_kernel(LinWalkArgs g) {
+__global__ __launch_bounds__((LinWalk<T, KP, kWalkSteps<T, KP>, kOutputs>::kThreads)) void
+    lin_walk_kernel(LinWalkArgs g) {
   constexpr int C = kWalkSteps<T, KP>;
   typedef LinWalk<T, KP, C, kOutputs> W;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   typename W::Lds& lds = *reinterpret_cast<typename W::Lds*>(smem);
   LinUnit<C> u;
   if (!u.init(g, block_of())) return;
-  const int id = (int)threadIdx.x;
-  if (id < W::NT) lin_outputs<T, KP, VEC, C>(g, u, lds, id);
-  else lin_states<T, KP, VEC, C, kOutputs, false>(g, u, lds, id - W::NT);
+  const int id = (int)threadIdx.x, lane = id & 63;
+  const int w = __builtin_amdgcn_readfirstlane(id >> 6);
+  if (w >= W::NW + 2) {
+    lin_bring<T, KP, VEC, C, kOutputs, false>(g, u, lds, id - 64 * (W::NW + 2));
+  } else if (w >= W::NW) {
+    lin_states<T, KP, C, kOutputs, false>(g, u, lds, lane, w - W::NW);
+  } else {
+    constexpr int kTeam = C / 32;  // waves of a team
+    const int team = w / kTeam, a0 = w % kTeam;
+    if constexpr (C == 128) {
+      if (a0 < 2) lin_outputs<T, KP, VEC, C, 0, 3>(g, u, lds, lane, a0, team);
+      else lin_outputs<T, KP, VEC, C, 1, 2>(g, u, lds, lane, a0, team);
+    } else {
+      lin_outputs<T, KP, VEC, C, 0, C / 32 - 1>(g, u, lds, lane, a0, team);
+    }
+  }
 }
 
 // The states' walk and its way back, side by side: the first nf workgroups go forward.
 template <typename T, int KP, bool VEC, int MODE>
-__global__ __launch_bounds__((4 * kStateSteps<T, KP>)) void lin_states_kernel(LinWalkArgs f,
-                                                                              LinWalkArgs back,
-                                                                              uint32_t nf) {
+__global__ __launch_bounds__((LinWalk<T, KP, kStateSteps<T, KP>, MODE>::kThreads)) void
+    lin_states_kernel(LinWalkArgs f, LinWalkArgs back, uint32_t nf) {
   constexpr int C = kStateSteps<T, KP>;
   typedef LinWalk<T, KP, C, MODE> W;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   typename W::Lds& lds = *reinterpret_cast<typename W::Lds*>(smem);
-  const uint32_t id = block_of();
+  const uint32_t block = block_of();
+  const int id = (int)threadIdx.x, lane = id & 63;
+  const int w = __builtin_amdgcn_readfirstlane(id >> 6);
   LinUnit<C> u;
-  if (id < nf) {
-    if (u.init(f, id)) lin_states<T, KP, VEC, C, MODE, false>(f, u, lds, (int)threadIdx.x);
+  if (block < nf) {
+    if (!u.init(f, block)) return;
+    if (w < 2) lin_states<T, KP, C, MODE, false>(f, u, lds, lane, w);
+    else lin_bring<T, KP, VEC, C, MODE, false>(f, u, lds, id - 128);
   } else {
-    if (u.init(back, id - nf)) lin_states<T, KP, VEC, C, MODE, true>(back, u, lds, (int)threadIdx.x);
+    if (!u.init(back, block - nf)) return;
+    if (w < 2) lin_states<T, KP, C, MODE, true>(back, u, lds, lane, w);
+    else lin_bring<T, KP, VEC, C, MODE, true>(back, u, lds, id - 128);
   }
 }
 
