@@ -48,11 +48,12 @@ __device__ inline void put_tile(float* m, const f32x4& S, int kt, int64_t col, i
 // Decays of a chunk of C steps.  With G the sums of g from the chunk's start in
 // units of log 2, formed in 64 bits: hi + lo = G_t in two parts, whose differences
 // keep 24 bits where the decay between two steps counts, and u = e^(G_end - G_t),
-// end being the last of the step's 32.  g below -200 counts as -200 (e^-200 is 0 in
+// end being the last of the step's 32; w is the step's weight in the state, e^(G_last -
+// G_t), or on the way back scale e^(G_t).  g below -200 counts as -200 (e^-200 is 0 in
 // fp32, and sums stay finite).
 template <int C>
 struct Decays {
-  float hi[C], lo[C], u[C];
+  float hi[C], lo[C], u[C], w[C];
 };
 
 __device__ inline float diff2(float hi, float lo, float hi0, float lo0) {
@@ -91,7 +92,8 @@ struct Gaps {
     for (int e = 0; e < E; ++e) g[e] = p[lane * E + e < n ? (lane * E + e) * stride : 0];
   }
   // One wave forms a chunk's decays.
-  __device__ inline void decays(Decays<C>& d, int lane) const {
+  template <bool REV = false>
+  __device__ inline void decays(Decays<C>& d, int lane, float scale = 1.0f) const {
     double s[E], sum = 0.0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -112,6 +114,9 @@ struct Gaps {
     constexpr int kBlock = 32 / E;  // lanes of 32 steps
     const int end = lane | (kBlock - 1);
     const float hE = __shfl(hi[E - 1], end), lE = __shfl(lo[E - 1], end);
+    constexpr int kLast = C / E - 1;  // lane of the last step
+    const float hL = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(hi[E - 1]), kLast));
+    const float lL = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(lo[E - 1]), kLast));
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const int t = lane * E + e;
@@ -119,6 +124,7 @@ struct Gaps {
         d.hi[t] = hi[e];
         d.lo[t] = lo[e];
         d.u[t] = diff2(hE, lE, hi[e], lo[e]);
+        d.w[t] = REV ? scale * exp2_fast(hi[e] + lo[e]) : diff2(hL, lL, hi[e], lo[e]);
       }
     }
   }
@@ -153,21 +159,17 @@ __device__ inline void lds8(const float* p, float* x) {
   *reinterpret_cast<float4*>(x + 4) = *reinterpret_cast<const float4*>(p + 4);
 }
 
-// The B operand X[8 j + e][c] of 32 rows from `row` on and 16 columns from `col` on of
-// planes [NP][rows][N] in LDS, as floats.
-template <int NP, int N>
-__device__ inline void lds_values(const uint16_t* m, int plane, int row, int col, int lane,
-                                  float* x) {
+// The values of an operand's planes.
+template <int NP>
+__device__ inline void operand_values(const u32x4 (&f)[NP], float* x) {
 #pragma unroll
-  for (int p = NP - 1; p >= 0; --p) {
-    const u32x4 w = Swizzled<N>::col16(m + p * plane, row, col, lane);
+  for (int p = NP - 1; p >= 0; --p)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float a = __uint_as_float(w[e] << 16), b = __uint_as_float(w[e] & 0xffff0000u);
+      const float a = __uint_as_float(f[p][e] << 16), b = __uint_as_float(f[p][e] & 0xffff0000u);
       x[2 * e] = p == NP - 1 ? a : x[2 * e] + a;
       x[2 * e + 1] = p == NP - 1 ? b : x[2 * e + 1] + b;
     }
-  }
 }
 
 }  // namespace

@@ -92,12 +92,16 @@ template <int C>
 struct LinUnit {
   int64_t bh, b, h, hk, v0;
   int seg, n0, n1, nv;
-  // workgroups of one head's segment, which share Q and K, are on one XCD
+  // Workgroups of one head's segment, which share Q and K, are on one XCD, and so are
+  // neighbouring heads: together they read whole rows (with every eighth head on an XCD
+  // one of them took 80 us where the others took 67).
   __device__ inline bool init(const LinWalkArgs& g, uint32_t id) {
-    const uint32_t vb = (id >> 3) % g.nvb, u = (id >> 3) / g.nvb * 8 + (id & 7);
-    if (u >= g.units) return false;
-    bh = u / (uint32_t)g.walked;
-    seg = g.first + (int)(u - (uint32_t)bh * (uint32_t)g.walked);
+    const uint32_t vb = (id >> 3) % g.nvb, each = (g.units + 7) / 8;
+    const uint32_t u = (id & 7) * each + (id >> 3) / g.nvb, heads = g.units / (uint32_t)g.walked;
+    if (u >= g.units || (id >> 3) / g.nvb >= each) return false;
+    const uint32_t s = u / heads;
+    bh = u - s * heads;
+    seg = g.first + (int)s;
     n0 = seg * g.per;
     n1 = n0 + g.per < g.nch ? n0 + g.per : g.nch;
     const LinHead x = lin_head(g.a, (uint32_t)bh);
@@ -175,7 +179,7 @@ __device__ inline void lin_bring(const LinWalkArgs& g, const LinUnit<C>& u,
           *reinterpret_cast<u32x4*>(&o.V[y][W::VR::at(r, x)]) = p[y];
       }
     }
-    if (first) in.g.decays(o.d, lane);
+    if (first) in.g.template decays<REV>(o.d, lane, a.scale);
   };
   fetch(in0, 0);
   fetch(in1, 1);
@@ -232,6 +236,7 @@ __device__ inline void lin_states(const LinWalkArgs& g, const LinUnit<C>& u,
   double total = 0.0;
   int slot = 0;
   show(0);
+  __builtin_amdgcn_s_setprio(3);  // the outputs have two chunks' time, this chain one
   lds_barrier();
   for (int m = 0; m < cnt; ++m) {
     const typename W::Operands& B = lds.op[slot];
@@ -247,30 +252,38 @@ __device__ inline void lin_states(const LinWalkArgs& g, const LinUnit<C>& u,
     for (int i = 0; i < KT; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) S[i][r] *= last;
+    // operands asked for a block ahead: waited for, they would be a third of the time
+    float w8[2][8];
+    u32x4 fk[2][KT][NP], fv[2][NP];
+    const auto ask = [&](int ib) {
 #pragma unroll
-    for (int ib = 0; ib < NB; ++ib) {  // operands asked for at once
-      float v8[8], e8[8], l8[8], from = 0.0f;
-      u32x4 fk[KT][NP];
-      lds_values<NP, 32>(&B.V[0][0], C * 32, 32 * ib, 16 * vt, lane, v8);
-      if constexpr (REV) {
-        lds8(&B.d.hi[32 * ib + 8 * j], e8);
-        lds8(&B.d.lo[32 * ib + 8 * j], l8);
-      } else {
-        lds8(&B.d.u[32 * ib + 8 * j], e8);
-        from = diff2(hend, lend, B.d.hi[32 * ib + 31], B.d.lo[32 * ib + 31]);
-      }
+      for (int y = 0; y < NP; ++y)
+        fv[ib & 1][y] = Swizzled<32>::col16(B.V[y], 32 * ib, 16 * vt, lane);
+      lds8(&B.d.w[32 * ib + 8 * j], w8[ib & 1]);
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
         for (int y = 0; y < NP; ++y)
-          fk[kt][y] = KR::col(B.K[y], 32 * ib, 32 * (kt >> 1) + 4 * (kt & 1), lane);
+          fk[ib & 1][kt][y] = KR::col(B.K[y], 32 * ib, 32 * (kt >> 1) + 4 * (kt & 1), lane);
+    };
+    ask(0);
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        v8[e] *= REV ? a.scale * exp2_fast(e8[e] + l8[e]) : e8[e] * from;
+    for (int ib = 0; ib < NB; ++ib) {
+      if (ib + 1 < NB) ask(ib + 1);
+      __builtin_amdgcn_sched_barrier(0);
+      float v8[8];
+      operand_values<NP>(fv[ib & 1], v8);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v8[e] *= w8[ib & 1][e];
       u32x4 vp[3];
       split8<3>(v8, vp);
+      // (tiles within planes: a tile's products wait for each other)
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt) S[kt] = mfma_planes<NP, 3, 3>(fk[kt], vp, S[kt]);
+      for (int x = 0; x < NP; ++x)
+#pragma unroll
+        for (int y = 0; y + x < 3; ++y)
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt) S[kt] = mfma32(fk[ib & 1][kt][x], vp[y], S[kt]);
     }
     slot = slot + 1 < W::RING ? slot + 1 : 0;
     show(slot);
@@ -289,29 +302,30 @@ __device__ inline void lin_states(const LinWalkArgs& g, const LinUnit<C>& u,
   }
 }
 
-// The outputs' waves: tiles a0 and C / 16 - 1 - a0, whose own blocks of 32 steps are EB
-// and LB.
-template <typename T, int KP, bool VEC, int C, int EB, int LB>
+// The outputs' waves: tiles of 16 steps, at 16 tile[i], whose own blocks of 32 steps are OWN.
+template <typename T, int KP, bool VEC, int C, int... OWN>
 __device__ inline void lin_outputs(const LinWalkArgs& g, const LinUnit<C>& u,
                                    typename LinWalk<T, KP, C, kOutputs>::Lds& lds, int lane,
-                                   int a0, int team) {
+                                   const int (&tile)[sizeof...(OWN)], int team) {
   typedef LinWalk<T, KP, C, kOutputs> W;
   typedef typename W::KR KR;
   typedef typename W::VR VR;
   constexpr int NP = W::NP, NO = W::NO, NS = W::NS, TEAMS = W::TEAMS, kE = (int)sizeof(T);
-  constexpr int kOwn[2] = {EB, LB};
+  constexpr int NI = sizeof...(OWN), kOwn[NI] = {OWN...}, LB = kOwn[NI - 1];  // the last is latest
   const LinArgs& a = g.a;
   const int j = lane >> 4, c = lane & 15, cnt = u.n1 - u.n0, K = (int)a.K;
-  const int t[2] = {16 * a0 + c, 16 * (C / 16 - 1 - a0) + c};
+  int t[NI];
+#pragma unroll
+  for (int i = 0; i < NI; ++i) t[i] = 16 * tile[i] + c;
   const int ar = 8 * (c >> 2) + (c & 3);     // row of tile x of an A operand, less 4 x
   RowsOf<C> rq, ro;
   rq.init(reinterpret_cast<const T*>(a.q) + u.b * a.q_b + u.hk * a.q_h, a.q_l, K, a.L);
   ro.init(reinterpret_cast<const T*>(a.o) + u.b * a.o_b + u.h * a.o_h + u.v0, a.o_l, u.nv, a.L);
-  Piece<T, VEC, NP> in[2][NS];
+  Piece<T, VEC, NP> in[NI][NS];
   const auto fetch = [&](int m) {
     const auto d = rq.at(lin_chunk<C, false>(u, m));
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < NI; ++i)
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
         const int y = 32 * s + 8 * j;
@@ -326,8 +340,8 @@ __device__ inline void lin_outputs(const LinWalkArgs& g, const LinUnit<C>& u,
     const typename W::Operands& B = lds.op[slot];
     const auto& Sp = lds.S[slot];
     slot = slot + TEAMS < W::RING ? slot + TEAMS : slot + TEAMS - W::RING;
-    u32x4 qb[2][NS][NP], fk[2][NS][NP], fv[2][NP];
-    float u8[8], h8[8], l8[8], ht[2], lt[2];
+    u32x4 qb[NI][NS][NP], fk[2][NS][NP], fv[2][NP];
+    float u8[8], h8[8], l8[8], ht[NI], lt[NI];
     const auto keys = [&](int ib) {
 #pragma unroll
       for (int s = 0; s < NS; ++s)
@@ -339,7 +353,7 @@ __device__ inline void lin_outputs(const LinWalkArgs& g, const LinUnit<C>& u,
     };
     const auto decays = [&](int ib) {
       if (ib < LB) lds8(&B.d.u[32 * ib + 8 * j], u8);
-      if (ib == EB || ib == LB) {
+      if (((ib == OWN) || ...)) {
         lds8(&B.d.hi[32 * ib + 8 * j], h8);
         lds8(&B.d.lo[32 * ib + 8 * j], l8);
       }
@@ -354,26 +368,26 @@ __device__ inline void lin_outputs(const LinWalkArgs& g, const LinUnit<C>& u,
     // wait for LDS.
     keys(0);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < NI; ++i) {
       ht[i] = B.d.hi[t[i]];
       lt[i] = B.d.lo[t[i]];
     }
     decays(0);
     values(0);
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < NI; ++i)
 #pragma unroll
       for (int s = 0; s < NS; ++s) planes_apart(in[i][s], K - 32 * s - 8 * j, qb[i][s]);
     fetch(m + TEAMS);
     __builtin_amdgcn_sched_barrier(0);
-    f32x4 acc[2][2], own[2];
+    f32x4 acc[NI][2], own[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) acc[i][0] = acc[i][1] = zero4();
+    for (int i = 0; i < NI; ++i) acc[i][0] = acc[i][1] = zero4();
 #pragma unroll
     for (int ib = 0; ib <= LB; ++ib) {
-      f32x4 p[2][2];  // rows i = 32 ib + 8 j + 4 x + r of K Q^T
+      f32x4 p[NI][2];  // rows i = 32 ib + 8 j + 4 x + r of K Q^T
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < NI; ++i) {
         if (ib > kOwn[i]) continue;
         p[i][0] = p[i][1] = zero4();
 #pragma unroll
@@ -385,7 +399,7 @@ __device__ inline void lin_outputs(const LinWalkArgs& g, const LinUnit<C>& u,
       if (ib < LB) keys(ib + 1);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < NI; ++i) {
         if (ib > kOwn[i]) continue;
         float w8[8];
         if (ib < kOwn[i]) {
@@ -453,7 +467,7 @@ __device__ inline void lin_outputs(const LinWalkArgs& g, const LinUnit<C>& u,
           fs[s][x][p] = lds16(&Sp[p][KR::at(ar, 4 * s + j) + 4 * x * KP]);
     const auto dst = ro.at(u.n0 + m);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < NI; ++i) {
       f32x4 y[2] = {zero4(), zero4()};
 #pragma unroll
       for (int s = 0; s < NS; ++s)
@@ -505,12 +519,12 @@ __global__ __launch_bounds__((LinWalk<T, KP, kWalkSteps<T, KP>, kOutputs>::kThre
     lin_states<T, KP, C, kOutputs, false>(g, u, lds, lane, w - W::NW);
   } else {
     constexpr int kTeam = C / 32;  // waves of a team
-    const int team = w / kTeam, a0 = w % kTeam;
+    const int team = w / kTeam, n = w % kTeam;
     if constexpr (C == 128) {
-      if (a0 < 2) lin_outputs<T, KP, VEC, C, 0, 3>(g, u, lds, lane, a0, team);
-      else lin_outputs<T, KP, VEC, C, 1, 2>(g, u, lds, lane, a0, team);
+      if (n < 2) lin_outputs<T, KP, VEC, C, 0, 1>(g, u, lds, lane, {n, 3 - n}, team);
+      else lin_outputs<T, KP, VEC, C, 2, 3>(g, u, lds, lane, {n + 2, 9 - n}, team);
     } else {
-      lin_outputs<T, KP, VEC, C, 0, C / 32 - 1>(g, u, lds, lane, a0, team);
+      lin_outputs<T, KP, VEC, C, 0, C / 32 - 1>(g, u, lds, lane, {n, C / 16 - 1 - n}, team);
     }
   }
 }
