@@ -35,19 +35,22 @@ struct Grad {
   static constexpr int NP = kPlanes<T>, NO = kOutPlanes<T>;
   static constexpr int VB = KP == 128 ? 32 : 64, NS = KP / 32, KT = KP / 16, VS = VB / 32,
                        VT = VB / 16, NW = C / 16, NT = 64 * NW;
-  static constexpr int kLd = KP + 8, kVld = VB + 8;
+  typedef Swizzled<KP> KR;  // rows of Q, K and the states' planes
+  typedef Swizzled<VB> VR;  // of V and dO
   static constexpr int kNk = C * KP / 8 / NT, kNv = C * VB / 8 / NT, kNs = VT * KT * 64 / NT;
   struct Lds {
-    uint16_t Q[NP][C * kLd], K[NP][C * kLd], V[NP][C * kVld], O[NP][C * kVld];
-    uint16_t S[3][VB * kLd];  // planes of S^T, then of dS^T
+    uint16_t Q[NP][C * KP], K[NP][C * KP], V[NP][C * VB], O[NP][C * VB];
+    uint16_t S[3][VB * KP];  // planes of S^T, then of dS^T
     Decays<C> d;
     float r[NW][C], c[C], x[C], y[C], z[NW];
   };
 };
 
 template <typename T, int KP, bool VEC, int C>
-__global__ __launch_bounds__(4 * C) void lin_grads_kernel(LinGradArgs g) {
+__global__ __launch_bounds__(4 * C, kPlanes<T> * KP <= 64 ? 2 : 1) void lin_grads_kernel(LinGradArgs g) {
   typedef Grad<T, KP, C> W;
+  typedef typename W::KR KR;
+  typedef typename W::VR VR;
   constexpr int NP = W::NP, NO = W::NO, NS = W::NS, KT = W::KT, VS = W::VS, VT = W::VT,
                 NT = W::NT, NW = W::NW, VB = W::VB, kE = (int)sizeof(T), NB = C / 32;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -55,9 +58,9 @@ __global__ __launch_bounds__(4 * C) void lin_grads_kernel(LinGradArgs g) {
   const LinArgs& a = g.a;
   const uint32_t id = block_of();
   if (id >= g.units) return;
-  const int n = (int)(id % (uint32_t)g.nch);
-  const uint32_t bk = id / (uint32_t)g.nch;
-  const int64_t b = bk / (uint32_t)a.Hk, hk = bk - (uint32_t)b * (uint32_t)a.Hk;
+  const uint32_t bn = id / (uint32_t)a.Hk;
+  const int64_t hk = id - bn * (uint32_t)a.Hk, b = bn / (uint32_t)g.nch;
+  const int n = (int)(bn - (uint32_t)b * (uint32_t)g.nch);
   const int per = (int)(a.Hv / a.Hk), K = (int)a.K;
   const int lane = threadIdx.x & 63, j = lane >> 4, c = lane & 15;
   const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -69,6 +72,35 @@ __global__ __launch_bounds__(4 * C) void lin_grads_kernel(LinGradArgs g) {
   RowsOf<C> rq, rk;
   rq.init(reinterpret_cast<const T*>(a.q) + b * a.q_b + hk * a.q_h, a.q_l, K, a.L);
   rk.init(reinterpret_cast<const T*>(a.k) + b * a.k_b + hk * a.k_h, a.k_l, K, a.L);
+  // A value head's block of V, dO and the states, on their way from memory: the first
+  // with Q and K, the next ones behind the last use of the registers before them.
+  Piece<T, VEC, NP> pv[W::kNv], po[W::kNv];
+  f32x4 st[W::kNs], gr[W::kNs];
+  Gaps<C> gaps;
+  const auto fetch = [&](int hi, int vb) {
+    const int64_t h = hk * per + hi, bh = b * a.Hv + h, v0 = (int64_t)vb * VB;
+    const int nv = a.V - v0 < VB ? (int)(a.V - v0) : VB;
+    RowsOf<C> rv, ro;
+    rv.init(reinterpret_cast<const T*>(a.v) + b * a.v_b + h * a.v_h + v0, a.v_l, nv, a.L);
+    ro.init(reinterpret_cast<const T*>(g.d.dout) + b * g.d.d_b + h * g.d.d_h + v0, g.d.d_l, nv,
+            a.L);
+    const auto dv = rv.at(n), dd = ro.at(n);
+#pragma unroll
+    for (int i = 0; i < W::kNv; ++i) {
+      const int at = (int)threadIdx.x + NT * i, r = at / (VB / 8), x = at % (VB / 8) * 8;
+      pv[i].load(dv, x < nv ? r * rv.row + x * kE : kPast);
+      po[i].load(dd, x < nv ? r * ro.row + x * kE : kPast);
+    }
+#pragma unroll
+    for (int i = 0; i < W::kNs; ++i) {
+      const int tile = w + NW * i, vt = vb * VT + tile / KT;
+      const int64_t at = (bh * g.nch + n) * elems +
+                         ((int64_t)(vt < tiles ? vt : 0) * KT + tile % KT) * 256 + lane * 4;
+      st[i] = *reinterpret_cast<const f32x4*>(g.states + at);
+      gr[i] = *reinterpret_cast<const f32x4*>(g.grads + at);
+    }
+    gaps.load(a.g + b * a.g_b + h * a.g_h + t0 * a.g_l, a.g_l, lane, rows);
+  };
   {
     const auto dq = rq.at(n), dk = rk.at(n);
     Piece<T, VEC, NP> pq[W::kNk], pk[W::kNk];
@@ -78,16 +110,17 @@ __global__ __launch_bounds__(4 * C) void lin_grads_kernel(LinGradArgs g) {
       pq[i].load(dq, x < K ? r * rq.row + x * kE : kPast);
       pk[i].load(dk, x < K ? r * rk.row + x * kE : kPast);
     }
+    fetch(0, 0);
 #pragma unroll
     for (int i = 0; i < W::kNk; ++i) {
-      const int at = (int)threadIdx.x + NT * i, r = at / (KP / 8), x = at % (KP / 8) * 8;
+      const int at = (int)threadIdx.x + NT * i, r = at / (KP / 8), x = at % (KP / 8);
       u32x4 p[NP];
-      pq[i].planes(K - x, p);
+      planes_apart(pq[i], K - 8 * x, p);
 #pragma unroll
-      for (int y = 0; y < NP; ++y) *reinterpret_cast<u32x4*>(&lds.Q[y][r * W::kLd + x]) = p[y];
-      pk[i].planes(K - x, p);
+      for (int y = 0; y < NP; ++y) *reinterpret_cast<u32x4*>(&lds.Q[y][KR::at(r, x)]) = p[y];
+      planes_apart(pk[i], K - 8 * x, p);
 #pragma unroll
-      for (int y = 0; y < NP; ++y) *reinterpret_cast<u32x4*>(&lds.K[y][r * W::kLd + x]) = p[y];
+      for (int y = 0; y < NP; ++y) *reinterpret_cast<u32x4*>(&lds.K[y][KR::at(r, x)]) = p[y];
     }
   }
   f32x4 dq[KT], dk[KT];
@@ -95,49 +128,27 @@ __global__ __launch_bounds__(4 * C) void lin_grads_kernel(LinGradArgs g) {
   for (int i = 0; i < KT; ++i) dq[i] = dk[i] = zero4();
 
   for (int hi = 0; hi < per; ++hi) {
-    const int64_t h = hk * per + hi, bh = b * a.Hv + h;
+    const int64_t h = hk * per + hi;
     float sumx = 0.0f, sumy = 0.0f, sumc = 0.0f, sumz = 0.0f;
-    Gaps<C> gaps;
     for (int vb = 0; vb < g.nvb; ++vb) {
       const int64_t v0 = (int64_t)vb * VB;
       const int nv = a.V - v0 < VB ? (int)(a.V - v0) : VB;
-      // this head's block of V, dO and the states
-      RowsOf<C> rv, ro;
-      rv.init(reinterpret_cast<const T*>(a.v) + b * a.v_b + h * a.v_h + v0, a.v_l, nv, a.L);
-      ro.init(reinterpret_cast<const T*>(g.d.dout) + b * g.d.d_b + h * g.d.d_h + v0, g.d.d_l, nv,
-              a.L);
-      Piece<T, VEC, NP> pv[W::kNv], po[W::kNv];
-      const auto dv = rv.at(n), dd = ro.at(n);
-#pragma unroll
-      for (int i = 0; i < W::kNv; ++i) {
-        const int at = (int)threadIdx.x + NT * i, r = at / (VB / 8), x = at % (VB / 8) * 8;
-        pv[i].load(dv, x < nv ? r * rv.row + x * kE : kPast);
-        po[i].load(dd, x < nv ? r * ro.row + x * kE : kPast);
-      }
-      f32x4 st[W::kNs], gr[W::kNs];
-#pragma unroll
-      for (int i = 0; i < W::kNs; ++i) {
-        const int tile = w + NW * i, vt = vb * VT + tile / KT;
-        const int64_t at = (bh * g.nch + n) * elems +
-                           ((int64_t)(vt < tiles ? vt : 0) * KT + tile % KT) * 256 + lane * 4;
-        st[i] = *reinterpret_cast<const f32x4*>(g.states + at);
-        gr[i] = *reinterpret_cast<const f32x4*>(g.grads + at);
-        if (vt >= tiles) st[i] = gr[i] = zero4();
-      }
-      if (vb == 0 && w == 0)
-        gaps.load(a.g + b * a.g_b + h * a.g_h + t0 * a.g_l, a.g_l, lane, rows);
+      if (vb > 0 || hi > 0) fetch(hi, vb);
       lds_barrier();  // the one before is done with LDS
 #pragma unroll
       for (int i = 0; i < W::kNv; ++i) {
-        const int at = (int)threadIdx.x + NT * i, r = at / (VB / 8), x = at % (VB / 8) * 8;
+        const int at = (int)threadIdx.x + NT * i, r = at / (VB / 8), x = at % (VB / 8);
         u32x4 p[NP];
-        pv[i].planes(nv - x, p);
+        planes_apart(pv[i], nv - 8 * x, p);
 #pragma unroll
-        for (int y = 0; y < NP; ++y) *reinterpret_cast<u32x4*>(&lds.V[y][r * W::kVld + x]) = p[y];
-        po[i].planes(nv - x, p);
+        for (int y = 0; y < NP; ++y) *reinterpret_cast<u32x4*>(&lds.V[y][VR::at(r, x)]) = p[y];
+        planes_apart(po[i], nv - 8 * x, p);
 #pragma unroll
-        for (int y = 0; y < NP; ++y) *reinterpret_cast<u32x4*>(&lds.O[y][r * W::kVld + x]) = p[y];
+        for (int y = 0; y < NP; ++y) *reinterpret_cast<u32x4*>(&lds.O[y][VR::at(r, x)]) = p[y];
       }
+#pragma unroll
+      for (int i = 0; i < W::kNs; ++i)  // (tiles past the state's read its first)
+        if (vb * VT + (w + NW * i) / KT >= tiles) st[i] = gr[i] = zero4();
       const auto show = [&](const f32x4 (&m)[W::kNs]) {
 #pragma unroll
         for (int i = 0; i < W::kNs; ++i) {
@@ -147,7 +158,7 @@ __global__ __launch_bounds__(4 * C) void lin_grads_kernel(LinGradArgs g) {
           for (int p = 0; p < 3; ++p) {
             const uint32_t lo = pk_bf16(x0, x1), hi2 = pk_bf16(x2, x3);
             *reinterpret_cast<uint2*>(
-                &lds.S[p][(16 * vt + c) * W::kLd + 32 * (kt >> 1) + 8 * j + 4 * (kt & 1)]) =
+                &lds.S[p][KR::at(16 * vt + c, 4 * (kt >> 1) + j) + 4 * (kt & 1)]) =
                 make_uint2(lo, hi2);
             if (p < 2) {
               take_plane(lo, x0, x1);
@@ -175,39 +186,43 @@ __global__ __launch_bounds__(4 * C) void lin_grads_kernel(LinGradArgs g) {
 #pragma unroll
       for (int s = 0; s < VS; ++s)
 #pragma unroll
-        for (int y = 0; y < NP; ++y) ob[s][y] = lds16(&lds.O[y][own * W::kVld + 32 * s + 8 * j]);
+        for (int y = 0; y < NP; ++y) ob[s][y] = VR::get(lds.O[y], own, 4 * s + j);
       // ---- 16 queries: dQ
       {
         for (int ib = 0; ib <= db; ++ib) {
+          u32x4 fv[VS][2][NP], fk[KT][NP];
+          float h8[8], l8[8], p8[8];
+#pragma unroll
+          for (int s = 0; s < VS; ++s)
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+              for (int y = 0; y < NP; ++y)
+                fv[s][x][y] = VR::get(lds.V[y], 32 * ib + ar + 4 * x, 4 * s + j);
+          lds8(&lds.d.hi[32 * ib + 8 * j], h8);
+          lds8(&lds.d.lo[32 * ib + 8 * j], l8);
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int y = 0; y < NP; ++y)
+              fk[kt][y] = KR::col(lds.K[y], 32 * ib, 32 * (kt >> 1) + 4 * (kt & 1), lane);
+          if constexpr (NP == 1) __builtin_amdgcn_sched_barrier(0);
           f32x4 q[2] = {zero4(), zero4()};  // V dO^T, rows i
 #pragma unroll
           for (int s = 0; s < VS; ++s)
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              u32x4 f[NP];
+            for (int x = 0; x < 2; ++x) q[x] = mfma_planes<NP, NP, NO>(fv[s][x], ob[s], q[x]);
 #pragma unroll
-              for (int y = 0; y < NP; ++y)
-                f[y] = lds16(&lds.V[y][(32 * ib + ar + 4 * x) * W::kVld + 32 * s + 8 * j]);
-              q[x] = mfma_planes<NP, NP, NO>(f, ob[s], q[x]);
-            }
-          float h8[8], l8[8], p8[8];
-          lds8(&lds.d.hi[32 * ib + 8 * j], h8);
-          lds8(&lds.d.lo[32 * ib + 8 * j], l8);
+          for (int e = 0; e < 8; ++e) p8[e] = a.scale * diff2(ht, lt, h8[e], l8[e]);
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            p8[e] = 32 * ib + 8 * j + e <= own
-                        ? q[e >> 2][e & 3] * (a.scale * diff2(ht, lt, h8[e], l8[e])) : 0.0f;
+          for (int e = 0; e < 8; ++e) {
+            asm("" : "+v"(p8[e]));  // no branch around the exponential
+            p8[e] = 32 * ib + 8 * j + e <= own ? q[e >> 2][e & 3] * p8[e] : 0.0f;
+          }
           u32x4 pb[NO];
           split8<NO>(p8, pb);
 #pragma unroll
-          for (int kt = 0; kt < KT; ++kt) {
-            u32x4 f[NP];
-#pragma unroll
-            for (int y = 0; y < NP; ++y)
-              f[y] = lds_col(&lds.K[y][32 * ib * W::kLd], W::kLd, 32 * (kt >> 1) + 4 * (kt & 1),
-                             lane);
-            dq[kt] = mfma_planes<NP, NO, NO>(f, pb, dq[kt]);
-          }
+          for (int kt = 0; kt < KT; ++kt) dq[kt] = mfma_planes<NP, NO, NO>(fk[kt], pb, dq[kt]);
         }
         const float from = a.scale * exp2_fast(ht + lt);
         float dot = 0.0f;
@@ -216,31 +231,35 @@ __global__ __launch_bounds__(4 * C) void lin_grads_kernel(LinGradArgs g) {
           float q8[8];
 #pragma unroll
           for (int y = NP - 1; y >= 0; --y) {
-            const u32x4 v = lds16(&lds.Q[y][own * W::kLd + 32 * s + 8 * j]);
+            const u32x4 v = KR::get(lds.Q[y], own, 4 * s + j);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
               const float x = __uint_as_float(e & 1 ? v[e >> 1] & 0xffff0000u : v[e >> 1] << 16);
               q8[e] = y == NP - 1 ? x : q8[e] + x;
             }
           }
+          u32x4 f[VS][2][3];
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            f32x4 q = zero4();
+          for (int vs = 0; vs < VS; ++vs)
 #pragma unroll
-            for (int vs = 0; vs < VS; ++vs) {
-              u32x4 f[3];
+            for (int x = 0; x < 2; ++x)
 #pragma unroll
               for (int p = 0; p < 3; ++p)
-                f[p] = lds_col(&lds.S[p][32 * vs * W::kLd], W::kLd, 32 * s + 4 * x, lane);
-              q = mfma_planes<3, NP, 3>(f, ob[vs], q);
-            }
+                f[vs][x][p] = KR::col(lds.S[p], 32 * vs, 32 * s + 4 * x, lane);
+          if constexpr (NP == 1) __builtin_amdgcn_sched_barrier(0);
+          f32x4 q[2] = {zero4(), zero4()};
+#pragma unroll
+          for (int vs = 0; vs < VS; ++vs)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) q[x] = mfma_planes<3, NP, 3>(f[vs][x], ob[vs], q[x]);
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              const float y = q[r] * from;
+              const float y = q[x][r] * from;
               dq[2 * s + x][r] += y;
               dot = __builtin_fmaf(q8[4 * x + r], y, dot);
             }
-          }
         }
         dot += __shfl_xor(dot, 16);
         dot += __shfl_xor(dot, 32);
@@ -251,44 +270,59 @@ __global__ __launch_bounds__(4 * C) void lin_grads_kernel(LinGradArgs g) {
 #pragma unroll
       for (int s = 0; s < NS; ++s)
 #pragma unroll
-        for (int y = 0; y < NP; ++y) kb[s][y] = lds16(&lds.K[y][own * W::kLd + 32 * s + 8 * j]);
+        for (int y = 0; y < NP; ++y) kb[s][y] = KR::get(lds.K[y], own, 4 * s + j);
 #pragma unroll
       for (int s = 0; s < VS; ++s)
 #pragma unroll
-        for (int y = 0; y < NP; ++y) vbf[s][y] = lds16(&lds.V[y][own * W::kVld + 32 * s + 8 * j]);
+        for (int y = 0; y < NP; ++y) vbf[s][y] = VR::get(lds.V[y], own, 4 * s + j);
       f32x4 dvt[VT];
 #pragma unroll
       for (int i = 0; i < VT; ++i) dvt[i] = zero4();
       for (int tb = db; tb < NB; ++tb) {
-        f32x4 qk[2] = {zero4(), zero4()}, ov[2] = {zero4(), zero4()};  // rows t
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-#pragma unroll
-          for (int s = 0; s < NS; ++s) {
-            u32x4 f[NP];
-#pragma unroll
-            for (int y = 0; y < NP; ++y)
-              f[y] = lds16(&lds.Q[y][(32 * tb + ar + 4 * x) * W::kLd + 32 * s + 8 * j]);
-            qk[x] = mfma_planes<NP, NP, 3>(f, kb[s], qk[x]);
-          }
-#pragma unroll
-          for (int s = 0; s < VS; ++s) {
-            u32x4 f[NP];
-#pragma unroll
-            for (int y = 0; y < NP; ++y)
-              f[y] = lds16(&lds.O[y][(32 * tb + ar + 4 * x) * W::kVld + 32 * s + 8 * j]);
-            ov[x] = mfma_planes<NP, NP, 3>(f, vbf[s], ov[x]);
-          }
-        }
+        u32x4 fq[NS][2][NP], fo[VS][2][NP];
         float h8[8], l8[8], p8[8], r8[8], w8[8];
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int y = 0; y < NP; ++y) {
+#pragma unroll
+            for (int s = 0; s < NS; ++s)
+              fq[s][x][y] = KR::get(lds.Q[y], 32 * tb + ar + 4 * x, 4 * s + j);
+#pragma unroll
+            for (int s = 0; s < VS; ++s)
+              fo[s][x][y] = VR::get(lds.O[y], 32 * tb + ar + 4 * x, 4 * s + j);
+          }
         lds8(&lds.d.hi[32 * tb + 8 * j], h8);
         lds8(&lds.d.lo[32 * tb + 8 * j], l8);
+        if constexpr (NP == 1) __builtin_amdgcn_sched_barrier(0);
+        f32x4 qk[2] = {zero4(), zero4()}, ov[2] = {zero4(), zero4()};  // rows t
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) qk[x] = mfma_planes<NP, NP, 3>(fq[s][x], kb[s], qk[x]);
+#pragma unroll
+        for (int s = 0; s < VS; ++s)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) ov[x] = mfma_planes<NP, NP, 3>(fo[s][x], vbf[s], ov[x]);
+        u32x4 co[VT][NP], cq[KT][NP];
+#pragma unroll
+        for (int y = 0; y < NP; ++y) {
+#pragma unroll
+          for (int i = 0; i < VT; ++i)
+            co[i][y] = VR::col(lds.O[y], 32 * tb, 32 * (i >> 1) + 4 * (i & 1), lane);
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt)
+            cq[kt][y] = KR::col(lds.Q[y], 32 * tb, 32 * (kt >> 1) + 4 * (kt & 1), lane);
+        }
+        float d8[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) d8[e] = a.scale * diff2(h8[e], l8[e], ht, lt);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
+          asm("" : "+v"(d8[e]));  // no branch around the exponential
           const int t = 32 * tb + 8 * j + e;
-          const float d = a.scale * diff2(h8[e], l8[e], ht, lt);
-          p8[e] = t >= own ? qk[e >> 2][e & 3] * d : 0.0f;
-          r8[e] = t >= own ? ov[e >> 2][e & 3] * d : 0.0f;
+          p8[e] = t >= own ? qk[e >> 2][e & 3] * d8[e] : 0.0f;
+          r8[e] = t >= own ? ov[e >> 2][e & 3] * d8[e] : 0.0f;
           w8[e] = t > own ? p8[e] * ov[e >> 2][e & 3] : 0.0f;
           sumc += w8[e];
           w8[e] = group_sum<16>(w8[e]);
@@ -302,21 +336,9 @@ __global__ __launch_bounds__(4 * C) void lin_grads_kernel(LinGradArgs g) {
         split8<NO>(p8, pb);
         split8<NO>(r8, rb);
 #pragma unroll
-        for (int i = 0; i < VT; ++i) {
-          u32x4 f[NP];
+        for (int i = 0; i < VT; ++i) dvt[i] = mfma_planes<NP, NO, NO>(co[i], pb, dvt[i]);
 #pragma unroll
-          for (int y = 0; y < NP; ++y)
-            f[y] = lds_col(&lds.O[y][32 * tb * W::kVld], W::kVld, 32 * (i >> 1) + 4 * (i & 1), lane);
-          dvt[i] = mfma_planes<NP, NO, NO>(f, pb, dvt[i]);
-        }
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt) {
-          u32x4 f[NP];
-#pragma unroll
-          for (int y = 0; y < NP; ++y)
-            f[y] = lds_col(&lds.Q[y][32 * tb * W::kLd], W::kLd, 32 * (kt >> 1) + 4 * (kt & 1), lane);
-          dk[kt] = mfma_planes<NP, NO, NO>(f, rb, dk[kt]);
-        }
+        for (int kt = 0; kt < KT; ++kt) dk[kt] = mfma_planes<NP, NO, NO>(cq[kt], rb, dk[kt]);
       }
       lds_barrier();  // S is read
       show(gr);
@@ -334,24 +356,28 @@ __global__ __launch_bounds__(4 * C) void lin_grads_kernel(LinGradArgs g) {
                 __uint_as_float(e & 1 ? kb[s][y][e >> 1] & 0xffff0000u : kb[s][y][e >> 1] << 16);
             k8[e] = y == NP - 1 ? x : k8[e] + x;
           }
+        u32x4 f[VS][2][3];
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          f32x4 q = zero4();
+        for (int vs = 0; vs < VS; ++vs)
 #pragma unroll
-          for (int vs = 0; vs < VS; ++vs) {
-            u32x4 f[3];
+          for (int x = 0; x < 2; ++x)
 #pragma unroll
             for (int p = 0; p < 3; ++p)
-              f[p] = lds_col(&lds.S[p][32 * vs * W::kLd], W::kLd, 32 * s + 4 * x, lane);
-            q = mfma_planes<3, NP, 3>(f, vbf[vs], q);
-          }
+              f[vs][x][p] = KR::col(lds.S[p], 32 * vs, 32 * s + 4 * x, lane);
+        if constexpr (NP == 1) __builtin_amdgcn_sched_barrier(0);
+        f32x4 q[2] = {zero4(), zero4()};
+#pragma unroll
+        for (int vs = 0; vs < VS; ++vs)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) q[x] = mfma_planes<3, NP, 3>(f[vs][x], vbf[vs], q[x]);
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float y = q[r] * to;
+            const float y = q[x][r] * to;
             dk[2 * s + x][r] += y;
             dot = __builtin_fmaf(k8[4 * x + r], y, dot);
           }
-        }
       }
       dot += __shfl_xor(dot, 16);
       dot += __shfl_xor(dot, 32);
@@ -364,7 +390,7 @@ __global__ __launch_bounds__(4 * C) void lin_grads_kernel(LinGradArgs g) {
           u32x4 f[NO];
 #pragma unroll
           for (int p = 0; p < NO; ++p)
-            f[p] = lds16(&lds.S[p][(32 * (i >> 1) + ar + 4 * (i & 1)) * W::kLd + 32 * s + 8 * j]);
+            f[p] = KR::get(lds.S[p], 32 * (i >> 1) + ar + 4 * (i & 1), 4 * s + j);
           q = mfma_planes<NO, NP, NO>(f, kb[s], q);
         }
 #pragma unroll
@@ -391,6 +417,11 @@ __global__ __launch_bounds__(4 * C) void lin_grads_kernel(LinGradArgs g) {
           }
         }
       }
+      // (that these are loaded again is more than the compiler sees)
+#pragma unroll
+      for (int i = 0; i < W::kNv; ++i) pv[i] = po[i] = Piece<T, VEC, NP>{};
+#pragma unroll
+      for (int i = 0; i < W::kNs; ++i) st[i] = gr[i] = zero4();
     }
     // dg of this value head
     sumc += __shfl_xor(sumc, 16);

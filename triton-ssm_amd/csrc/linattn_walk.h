@@ -92,16 +92,12 @@ template <int C>
 struct LinUnit {
   int64_t bh, b, h, hk, v0;
   int seg, n0, n1, nv;
-  // Workgroups of one head's segment, which share Q and K, are on one XCD, and so are
-  // neighbouring heads: together they read whole rows (with every eighth head on an XCD
-  // one of them took 80 us where the others took 67).
+  // workgroups of one head's segment, which share Q and K, are on one XCD
   __device__ inline bool init(const LinWalkArgs& g, uint32_t id) {
-    const uint32_t vb = (id >> 3) % g.nvb, each = (g.units + 7) / 8;
-    const uint32_t u = (id & 7) * each + (id >> 3) / g.nvb, heads = g.units / (uint32_t)g.walked;
-    if (u >= g.units || (id >> 3) / g.nvb >= each) return false;
-    const uint32_t s = u / heads;
-    bh = u - s * heads;
-    seg = g.first + (int)s;
+    const uint32_t vb = (id >> 3) % g.nvb, u = (id >> 3) / g.nvb * 8 + (id & 7);
+    if (u >= g.units) return false;
+    bh = u / (uint32_t)g.walked;
+    seg = g.first + (int)(u - (uint32_t)bh * (uint32_t)g.walked);
     n0 = seg * g.per;
     n1 = n0 + g.per < g.nch ? n0 + g.per : g.nch;
     const LinHead x = lin_head(g.a, (uint32_t)bh);
