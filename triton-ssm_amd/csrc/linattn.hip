@@ -13,13 +13,21 @@ bool takes(int64_t K, int64_t V) { return K <= 128 && V <= (INT64_C(1) << 21); }
 // Sequences up to here go step by step.
 bool by_steps(int64_t heads, int64_t L) { return L <= 16; }
 
-// Segments of a sequence: as many as fill the chip with two workgroups for each CU.
-int64_t segments(int64_t heads, int64_t L, int64_t V) {
-  const int64_t wgs = heads * cdiv64(V, 32);
-  if (wgs >= 256) return 1;
-  const int64_t most = cdiv64(L, 512);
-  const int64_t want = cdiv64(512, wgs);
-  return want < most ? want : most;
+// Segments of a sequence, which are walked side by side once a shorter pass (the states
+// alone) has the state that each starts from: as many as give every CU a workgroup, of
+// 256 steps at least, or 512 with gradients.  Us a call, whole against segments (B=1
+// 64 x 64 bf16): 8 heads L=8192 107 against 28, L=2048 30 against 20, 16 heads L=4096 56
+// against 27; with gradients 117 against 66, 36 against 38, 75 against 63.  Segments of
+// 2048 steps and more are halved, as the shorter pass has several workgroups on a CU: 8
+// heads L=65536 124 against 139, with gradients 365 against 388 (but L=8192 35 against
+// 28).  Two segments cost what they save (B=4 L=4096 H=16 64 x 64: 64 against 61;
+// gradients 194 against 170) but for K > 64, where the outputs are the larger part of a
+// walk: B=2 L=4096 H=16 128 x 128 92 against 104; gradients 408 against 373.
+int64_t segments(int64_t heads, int64_t L, int64_t K, int64_t V, bool grads) {
+  const int64_t wgs = heads * cdiv64(V, 32), most = L / (grads ? 512 : 256);
+  const int64_t fill = wgs > 0 ? 256 / wgs : 1, n = fill < most ? fill : most;
+  if (n < 3) return n == 2 && K > 64 && !grads ? 2 : 1;
+  return n < fill || L < n * 2048 ? n : 512 / wgs;
 }
 
 // The chunked form's plan over a workspace at base (which may be null: sizes).  chunk:
@@ -34,7 +42,7 @@ LinPlan lin_plan(char* base, int64_t B, int64_t L, int64_t Hv, int64_t K, int64_
     at += cdiv64(bytes, 256) * 256;
     return q;
   };
-  const int64_t nseg = segments(heads, L, V);
+  const int64_t nseg = segments(heads, L, K, V, chunk > 0);
   p.steps = cdiv64(cdiv64(L, nseg), 128) * 128;
   p.nseg = cdiv64(L, p.steps);
   if (p.nseg > 1) {
