@@ -72,8 +72,11 @@ struct LinWalk {
   static constexpr int TEAMS = MODE == kOutputs ? lin_teams(NP, KP) : 1, RING = TEAMS + 1;
   static constexpr int NW = MODE == kOutputs ? TEAMS * C / 32 : 0;  // output waves
   static constexpr int NT = 128;                            // threads of the loaders
-  static constexpr int kThreads = 64 * (NW + 2) + NT;
+  static constexpr bool CLOCK = NW == 0 || NW % 4 != 0;      // a wave for the decays
+  static constexpr int kThreads = 64 * (NW + 2 + CLOCK) + NT;
   static constexpr int kNk = (C * KP / 8 + NT - 1) / NT, kNv = (C * 4 + NT - 1) / NT;
+  // chunks on their way from memory
+  static constexpr int AHEAD = 2;
   typedef Swizzled<KP> KR;                   // rows of K and of the state's planes
   typedef Swizzled<32> VR;                   // of V
   struct Operands {  // of one chunk
@@ -125,7 +128,8 @@ __device__ inline void lin_bring(const LinWalkArgs& g, const LinUnit<C>& u,
   constexpr int NP = W::NP, NT = W::NT, kE = (int)sizeof(T), U = KP / 8;
   const LinArgs& a = g.a;
   const int lane = id & 63, cnt = u.n1 - u.n0, K = (int)a.K;
-  const bool first = __builtin_amdgcn_readfirstlane(id >> 6) == 0;
+  const int wave = __builtin_amdgcn_readfirstlane(id >> 6);
+  const bool clock = wave == (W::CLOCK ? NT / 64 : 0), rows = wave < NT / 64;
   RowsOf<C> rk, rv;
   rk.init(reinterpret_cast<const T*>(a.k) + u.b * a.k_b + u.hk * a.k_h, a.k_l, K, a.L);
   rv.init(reinterpret_cast<const T*>(a.v) + u.b * a.v_b + u.h * a.v_h + u.v0, a.v_l, u.nv, a.L);
@@ -133,65 +137,70 @@ __device__ inline void lin_bring(const LinWalkArgs& g, const LinUnit<C>& u,
   struct Regs {
     Piece<T, VEC, NP> k[W::kNk], v[W::kNv];
     Gaps<C> g;
-  } in0, in1;
+  } in[W::AHEAD];
   const auto fetch = [&](Regs& in, int m) {
     const int n = lin_chunk<C, REV>(u, m);
-    const auto dk = rk.at(n), dv = rv.at(n);
+    if (rows) {
+      const auto dk = rk.at(n), dv = rv.at(n);
 #pragma unroll
-    for (int i = 0; i < W::kNk; ++i) {
-      const int at = id + NT * i, r = at / U, x = at % U * 8;
-      in.k[i].load(dk, r < C && x < K ? r * rk.row + x * kE : kPast);
-    }
+      for (int i = 0; i < W::kNk; ++i) {
+        const int at = id + NT * i, r = at / U, x = at % U * 8;
+        in.k[i].load(dk, r < C && x < K ? r * rk.row + x * kE : kPast);
+      }
 #pragma unroll
-    for (int i = 0; i < W::kNv; ++i) {
-      const int at = id + NT * i, r = at >> 2, x = (at & 3) * 8;
-      in.v[i].load(dv, r < C && x < u.nv ? r * rv.row + x * kE : kPast);
+      for (int i = 0; i < W::kNv; ++i) {
+        const int at = id + NT * i, r = at >> 2, x = (at & 3) * 8;
+        in.v[i].load(dv, r < C && x < u.nv ? r * rv.row + x * kE : kPast);
+      }
     }
-    if (first) {
+    if (clock) {
       const int64_t t0 = (int64_t)n * C, rest = a.L - t0;
       in.g.load(gp + t0 * a.g_l, a.g_l, lane, rest < C ? (int)rest : C);
     }
   };
   const auto leave = [&](const Regs& in, typename W::Operands& o) {
+    if (rows) {
 #pragma unroll
-    for (int i = 0; i < W::kNk; ++i) {
-      const int at = id + NT * i, r = at / U, x = at % U;
-      u32x4 p[NP];
-      planes_apart(in.k[i], K - 8 * x, p);
-      if (C * U % NT == 0 || r < C) {
+      for (int i = 0; i < W::kNk; ++i) {
+        const int at = id + NT * i, r = at / U, x = at % U;
+        u32x4 p[NP];
+        planes_apart(in.k[i], K - 8 * x, p);
+        if (C * U % NT == 0 || r < C) {
 #pragma unroll
-        for (int y = 0; y < NP; ++y)
-          *reinterpret_cast<u32x4*>(&o.K[y][W::KR::at(r, x)]) = p[y];
+          for (int y = 0; y < NP; ++y)
+            *reinterpret_cast<u32x4*>(&o.K[y][W::KR::at(r, x)]) = p[y];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < W::kNv; ++i) {
+        const int at = id + NT * i, r = at >> 2, x = at & 3;
+        u32x4 p[NP];
+        planes_apart(in.v[i], u.nv - 8 * x, p);
+        if (C * 4 % NT == 0 || r < C) {
+#pragma unroll
+          for (int y = 0; y < NP; ++y)
+            *reinterpret_cast<u32x4*>(&o.V[y][W::VR::at(r, x)]) = p[y];
+        }
       }
     }
-#pragma unroll
-    for (int i = 0; i < W::kNv; ++i) {
-      const int at = id + NT * i, r = at >> 2, x = at & 3;
-      u32x4 p[NP];
-      planes_apart(in.v[i], u.nv - 8 * x, p);
-      if (C * 4 % NT == 0 || r < C) {
-#pragma unroll
-        for (int y = 0; y < NP; ++y)
-          *reinterpret_cast<u32x4*>(&o.V[y][W::VR::at(r, x)]) = p[y];
-      }
-    }
-    if (first) in.g.template decays<REV>(o.d, lane, a.scale);
+    if (clock) in.g.template decays<REV>(o.d, lane, a.scale);
   };
-  fetch(in0, 0);
-  fetch(in1, 1);
-  leave(in0, lds.op[0]);
-  fetch(in0, 2);
+#pragma unroll
+  for (int i = 0; i < W::AHEAD; ++i) fetch(in[i], i);
+  leave(in[0], lds.op[0]);
+  fetch(in[0], W::AHEAD);
   lds_barrier();
   int slot = 1;
-  const auto turn = [&](int m, Regs& in) {  // in holds chunk m + 1
-    leave(in, lds.op[slot]);
+  const auto turn = [&](int m, Regs& x) {  // x holds chunk m + 1
+    leave(x, lds.op[slot]);
     slot = slot + 1 < W::RING ? slot + 1 : 0;
-    fetch(in, m + 3);
+    fetch(x, m + 1 + W::AHEAD);
     lds_barrier();
   };
-  for (int m = 0; m < cnt; m += 2) {
-    turn(m, in1);
-    if (m + 1 < cnt) turn(m + 1, in0);
+  for (int m = 0; m < cnt; m += W::AHEAD) {
+#pragma unroll
+    for (int i = 0; i < W::AHEAD; ++i)
+      if (m + i < cnt) turn(m + i, in[(i + 1) % W::AHEAD]);
   }
   if constexpr (W::TEAMS == 2) lds_barrier();
 }
