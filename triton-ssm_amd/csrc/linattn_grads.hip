@@ -17,6 +17,13 @@
 // R^T) for dQ, so that every product's result is the next one's operand in place
 // (planes.h); R is formed in both places.  The states' planes take one buffer after
 // the other: S for dQ, then dS for dK and dV.
+//
+// What bounds it: memory.  B=4 L=4096 H=16 64 x 64 bf16 takes 86 us for 134 MB of inputs,
+// 134 MB of states and 100 MB of gradients, 4.3 TB/s where a copy reaches 5.1: two
+// workgroups are on a CU (one, with 266 registers, took 160 us), and what one waits for
+// is hidden by the other's work alone.  The states are read once, past the caches
+// (through them 92 us).  Chunks of 128 steps would halve the states and leave LDS for
+// one workgroup; chunks of 32 in fp32 took 380 us for 344 (the same sizes, all kernels).
 #include "linattn_dev.h"
 
 namespace tssm {
@@ -47,7 +54,9 @@ struct Grad {
 };
 
 template <typename T, int KP, bool VEC, int C>
-__global__ __launch_bounds__(4 * C, kPlanes<T> * KP <= 64 ? 2 : 1) void lin_grads_kernel(LinGradArgs g) {
+// two workgroups on a CU but where their registers would spill
+__global__ __launch_bounds__(4 * C, kPlanes<T> * KP <= 64 ? 2 : 1) void
+    lin_grads_kernel(LinGradArgs g) {
   typedef Grad<T, KP, C> W;
   typedef typename W::KR KR;
   typedef typename W::VR VR;
@@ -96,8 +105,8 @@ __global__ __launch_bounds__(4 * C, kPlanes<T> * KP <= 64 ? 2 : 1) void lin_grad
       const int tile = w + NW * i, vt = vb * VT + tile / KT;
       const int64_t at = (bh * g.nch + n) * elems +
                          ((int64_t)(vt < tiles ? vt : 0) * KT + tile % KT) * 256 + lane * 4;
-      st[i] = *reinterpret_cast<const f32x4*>(g.states + at);
-      gr[i] = *reinterpret_cast<const f32x4*>(g.grads + at);
+      st[i] = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(g.states + at));
+      gr[i] = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(g.grads + at));
     }
     gaps.load(a.g + b * a.g_b + h * a.g_h + t0 * a.g_l, a.g_l, lane, rows);
   };

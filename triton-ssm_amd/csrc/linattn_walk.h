@@ -12,16 +12,23 @@
 //     two chunks' time for it,
 //   2 state waves: 16 columns each.  K^T V of the whole chunk on top of the decayed
 //     state, whose planes go to LDS for the next chunk's outputs,
-//   loaders: the chunk after this one to LDS, from loads that are two chunks ahead.
+//   2 loaders: the chunk after this one to LDS, from loads that are two chunks ahead,
+//     and a wave for the decays where it is no fourth one on a SIMD (it would take a
+//     quarter of the others' registers: 32 x 64 fp32 steps 46 -> 88 us).
 // Everything is formed transposed (planes.h): P^T = K Q^T is the next product's operand
 // in place, queries come to their wave straight from memory, and a lane ends up with 8
 // neighbouring columns of one step's output.
 //
-// LDS sets the time: a 16-byte read takes it 16 cycles, so an operand that is read
-// should serve as many products as it can.  The two tiles of an output wave share K, V
-// and the state's planes (B=8 L=4096 H=16 64 x 64 bf16: WALKTIME us; 84 with a wave for
-// each tile), and a state wave that has all steps of its columns needs no exchange.
-// Tiles a and C / 16 - 1 - a are together, five blocks of K in all whatever a is.
+// What bounds it: one wave's chain and LDS.  B=8 L=4096 H=16 64 x 64 bf16 takes 84 us
+// for 270 MB (3.2 TB/s; 256 workgroups, one on a CU), a chunk of 128 steps 3800 cycles,
+// of which the state waves work 3200, the outputs 2400 to 3100 and the loader with the
+// decays 3000.  fp32 (3 planes) is bound by LDS: 3700 of a chunk's 5000 cycles (64
+// steps, K = 64).  LDS takes 16 cycles for a 16-byte read, so an operand that is read
+// should serve as many products as it can: the two tiles of an output wave share K, V
+// and the state's planes (with a wave for each tile 90 us), and a state wave that has
+// all steps of its columns needs no exchange.  In a chunk of 128 the tiles are dealt so
+// that an output wave beside a state wave on its SIMD has 2 blocks of K and one beside a
+// loader 4, for what is left of the SIMD's time.
 //
 // D of the 32 steps before a tile's own is a product of two factors with the decay from
 // that block's end between them: one exponential for a lane and block and a table of
