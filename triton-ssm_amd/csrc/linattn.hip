@@ -10,8 +10,15 @@ bool sizes_ok(int64_t B, int64_t L, int64_t Hk, int64_t Hv, int64_t K, int64_t V
 // A head's state takes 31 bits.
 bool takes(int64_t K, int64_t V) { return K <= 128 && V <= (INT64_C(1) << 21); }
 
-// Sequences up to here go step by step.
-bool by_steps(int64_t heads, int64_t L) { return L <= 16; }
+// Few steps go one by one: a step takes 0.4 us, a chunk 7.5 whatever it holds, once for
+// every 256 workgroups.  Us a call, one by one against a chunk, bf16 with a state in and
+// out: 8 heads of 64 x 64, 12 steps 7.1 against 7.5, 16 steps 8.7 against 7.5; 256 heads,
+// 24 steps 12.7 against 14.9, 32 steps 16.0 against 14.8; 512 heads, 48 steps 28 against
+// 28; 1024 heads, 48 steps 42 against 62, 96 steps 76 against 64.
+bool by_steps(int64_t heads, int64_t L, int64_t V) {
+  const int64_t most = heads * cdiv64(V, 32) / 20;
+  return L <= (most < 12 ? 12 : (most < 64 ? most : 64));
+}
 
 // Segments of a sequence, which are walked side by side once a shorter pass (the states
 // alone) has the state that each starts from: as many as give every CU a workgroup, of
@@ -91,7 +98,7 @@ extern "C" int64_t tssm_linear_attention_workspace_bytes(int64_t nbatch, int64_t
                                                          int64_t Hv, int64_t K, int64_t V) {
   if (!sizes_ok(nbatch, L, Hk, Hv, K, V)) return TSSM_ERR_SHAPE;
   if (!takes(K, V)) return TSSM_ERR_UNSUPPORTED;
-  if (nbatch == 0 || by_steps(nbatch * Hv, L)) return 0;
+  if (nbatch == 0 || by_steps(nbatch * Hv, L, V)) return 0;
   return lin_plan(nullptr, nbatch, L, Hv, K, V, 0).bytes;
 }
 
@@ -111,7 +118,7 @@ extern "C" int tssm_linear_attention_forward(
                      sq_b, sq_l, sq_h, sk_b, sk_l, sk_h, sv_b, sv_l, sv_h,
                      sg_b, sg_l, sg_h, so_b, so_l, so_h, scale};
   hipStream_t st = as_stream(stream);
-  if (by_steps(nbatch * Hv, L) || !chunk_rows(dtype, a)) return lin_seq_launch(dtype, a, st);
+  if (by_steps(nbatch * Hv, L, V) || !chunk_rows(dtype, a)) return lin_seq_launch(dtype, a, st);
   TSSM_CHECK(L < (INT64_C(1) << 31) && nbatch <= 0x7fffffff / Hv, TSSM_ERR_UNSUPPORTED);
   const LinPlan p = lin_plan(reinterpret_cast<char*>(workspace), nbatch, L, Hv, K, V, 0);
   TSSM_CHECK(p.bytes == 0 || (workspace && workspace_bytes >= p.bytes && aligned(workspace, 256)),
