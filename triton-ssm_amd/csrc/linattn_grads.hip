@@ -208,8 +208,7 @@ __global__ __launch_bounds__(4 * C, kPlanes<T> * KP <= 64 ? 2 : 1) void
 #pragma unroll
               for (int y = 0; y < NP; ++y)
                 fv[s][x][y] = VR::get(lds.V[y], 32 * ib + ar + 4 * x, 4 * s + j);
-          lds8(&lds.d.hi[32 * ib + 8 * j], h8);
-          lds8(&lds.d.lo[32 * ib + 8 * j], l8);
+          const float h1 = one_of8(&lds.d.hi[32 * ib], lane), l1 = one_of8(&lds.d.lo[32 * ib], lane);
 #pragma unroll
           for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
@@ -221,6 +220,8 @@ __global__ __launch_bounds__(4 * C, kPlanes<T> * KP <= 64 ? 2 : 1) void
           for (int s = 0; s < VS; ++s)
 #pragma unroll
             for (int x = 0; x < 2; ++x) q[x] = mfma_planes<NP, NP, NO>(fv[s][x], ob[s], q[x]);
+          eight(h1, h8);
+          eight(l1, l8);
 #pragma unroll
           for (int e = 0; e < 8; ++e) p8[e] = a.scale * diff2(ht, lt, h8[e], l8[e]);
 #pragma unroll
@@ -301,8 +302,7 @@ __global__ __launch_bounds__(4 * C, kPlanes<T> * KP <= 64 ? 2 : 1) void
             for (int s = 0; s < VS; ++s)
               fo[s][x][y] = VR::get(lds.O[y], 32 * tb + ar + 4 * x, 4 * s + j);
           }
-        lds8(&lds.d.hi[32 * tb + 8 * j], h8);
-        lds8(&lds.d.lo[32 * tb + 8 * j], l8);
+        const float h1 = one_of8(&lds.d.hi[32 * tb], lane), l1 = one_of8(&lds.d.lo[32 * tb], lane);
         if constexpr (NP == 1) __builtin_amdgcn_sched_barrier(0);
         f32x4 qk[2] = {zero4(), zero4()}, ov[2] = {zero4(), zero4()};  // rows t
 #pragma unroll
@@ -324,6 +324,8 @@ __global__ __launch_bounds__(4 * C, kPlanes<T> * KP <= 64 ? 2 : 1) void
             cq[kt][y] = KR::col(lds.Q[y], 32 * tb, 32 * (kt >> 1) + 4 * (kt & 1), lane);
         }
         float d8[8];
+        eight(h1, h8);
+        eight(l1, l8);
 #pragma unroll
         for (int e = 0; e < 8; ++e) d8[e] = a.scale * diff2(h8[e], l8[e], ht, lt);
 #pragma unroll

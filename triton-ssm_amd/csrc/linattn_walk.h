@@ -265,13 +265,13 @@ __device__ inline void lin_states(const LinWalkArgs& g, const LinUnit<C>& u,
 #pragma unroll
       for (int r = 0; r < 4; ++r) S[i][r] *= last;
     // operands asked for a block ahead: waited for, they would be a third of the time
-    float w8[2][8];
+    float w1[2];
     u32x4 fk[2][KT][NP], fv[2][NP];
     const auto ask = [&](int ib) {
 #pragma unroll
       for (int y = 0; y < NP; ++y)
         fv[ib & 1][y] = Swizzled<32>::col16(B.V[y], 32 * ib, 16 * vt, lane);
-      lds8(&B.d.w[32 * ib + 8 * j], w8[ib & 1]);
+      w1[ib & 1] = one_of8(&B.d.w[32 * ib], lane);
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
@@ -283,10 +283,11 @@ __device__ inline void lin_states(const LinWalkArgs& g, const LinUnit<C>& u,
     for (int ib = 0; ib < NB; ++ib) {
       if (ib + 1 < NB) ask(ib + 1);
       __builtin_amdgcn_sched_barrier(0);
-      float v8[8];
+      float v8[8], w8[8];
       operand_values<NP>(fv[ib & 1], v8);
+      eight(w1[ib & 1], w8);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v8[e] *= w8[ib & 1][e];
+      for (int e = 0; e < 8; ++e) v8[e] *= w8[e];
       u32x4 vp[3];
       split8<3>(v8, vp);
       // (tiles within planes: a tile's products wait for each other)
@@ -353,7 +354,7 @@ __device__ inline void lin_outputs(const LinWalkArgs& g, const LinUnit<C>& u,
     const auto& Sp = lds.S[slot];
     slot = slot + TEAMS < W::RING ? slot + TEAMS : slot + TEAMS - W::RING;
     u32x4 qb[NI][NS][NP], fk[2][NS][NP], fv[2][NP];
-    float u8[8], h8[8], l8[8], ht[NI], lt[NI];
+    float u1, h1, l1, ht[NI], lt[NI];
     const auto keys = [&](int ib) {
 #pragma unroll
       for (int s = 0; s < NS; ++s)
@@ -364,10 +365,10 @@ __device__ inline void lin_outputs(const LinWalkArgs& g, const LinUnit<C>& u,
             fk[x][s][y] = lds16(&B.K[y][KR::at(ar, 4 * s + j) + (32 * ib + 4 * x) * KP]);
     };
     const auto decays = [&](int ib) {
-      if (ib < LB) lds8(&B.d.u[32 * ib + 8 * j], u8);
+      if (ib < LB) u1 = one_of8(&B.d.u[32 * ib], lane);
       if (((ib == OWN) || ...)) {
-        lds8(&B.d.hi[32 * ib + 8 * j], h8);
-        lds8(&B.d.lo[32 * ib + 8 * j], l8);
+        h1 = one_of8(&B.d.hi[32 * ib], lane);
+        l1 = one_of8(&B.d.lo[32 * ib], lane);
       }
     };
     const auto values = [&](int ib) {
@@ -416,9 +417,14 @@ __device__ inline void lin_outputs(const LinWalkArgs& g, const LinUnit<C>& u,
         float w8[8];
         if (ib < kOwn[i]) {
           const float from = diff2(ht[i], lt[i], B.d.hi[32 * ib + 31], B.d.lo[32 * ib + 31]);
+          float u8[8];
+          eight(u1, u8);
 #pragma unroll
           for (int e = 0; e < 8; ++e) w8[e] = p[i][e >> 2][e & 3] * (u8[e] * from);
         } else {
+          float h8[8], l8[8];
+          eight(h1, h8);
+          eight(l1, l8);
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             float y = p[i][e >> 2][e & 3] * diff2(ht[i], lt[i], h8[e], l8[e]);
