@@ -22,18 +22,19 @@ bool by_steps(int64_t heads, int64_t L, int64_t V) {
 
 // Segments of a sequence, which are walked side by side once a shorter pass (the states
 // alone) has the state that each starts from: as many as give every CU a workgroup, of
-// 256 steps at least, or 512 with gradients.  Us a call, whole against segments (B=1
-// 64 x 64 bf16): 8 heads L=8192 107 against 28, L=2048 30 against 20, 16 heads L=4096 56
-// against 27; with gradients 117 against 66, 36 against 38, 75 against 63.  Segments of
+// 192 steps at least and 768 in all, or 512 and 1536 with gradients.  Us a call, whole
+// against segments (B=1 64 x 64 bf16): 8 heads L=8192 107 against 28, L=2048 30 against
+// 20, 16 heads L=4096 56 against 27; 48 workgroups, L=777, fp32 33 against 29, L=300 13
+// against 19; with gradients 117 against 66, 36 against 38, 75 against 63.  Segments of
 // 2048 steps and more are halved, as the shorter pass has several workgroups on a CU: 8
 // heads L=65536 124 against 139, with gradients 365 against 388 (but L=8192 35 against
 // 28).  Two segments cost what they save (B=4 L=4096 H=16 64 x 64: 64 against 61;
 // gradients 194 against 170) but for K > 64, where the outputs are the larger part of a
 // walk: B=2 L=4096 H=16 128 x 128 92 against 104; gradients 408 against 373.
 int64_t segments(int64_t heads, int64_t L, int64_t K, int64_t V, bool grads) {
-  const int64_t wgs = heads * cdiv64(V, 32), most = L / (grads ? 512 : 256);
+  const int64_t wgs = heads * cdiv64(V, 32), most = L / (grads ? 512 : 192);
   const int64_t fill = wgs > 0 ? 256 / wgs : 1, n = fill < most ? fill : most;
-  if (n < 3) return n == 2 && K > 64 && !grads ? 2 : 1;
+  if (n < 3 || L < 768) return n >= 2 && K > 64 && !grads ? 2 : 1;
   return n < fill || L < n * 2048 ? n : 512 / wgs;
 }
 
