@@ -139,6 +139,17 @@ def test_forms_of_the_gradients(dev, dtype, B, L, Hv, K, V):
     lin.check_gradients(dev, d, dtype, seed=L)
 
 
+@pytest.mark.parametrize("dtype,B,L,Hk,Hv,K,V", [
+    (BF16, 6, 2017, 1, 2, 16, 16), (F16, 3, 2100, 2, 6, 24, 40), (F32, 3, 1024, 4, 8, 32, 8),
+    (F32, 6, 1040, 1, 3, 100, 36),
+    (BF16, 2, 6080, 1, 2, 32, 32), (F32, 1, 6110, 2, 4, 16, 20),   # one chunk too few for it
+])
+def test_gradients_of_shared_heads(dev, dtype, B, L, Hk, Hv, K, V):
+    """Value heads one after the other in a workgroup, or in workgroups of their own."""
+    d = lin.inputs(dev, B, L, Hk, Hv, K, V, dtype, seed=L, h0=True, rate=0.1)
+    lin.check_gradients(dev, d, dtype, seed=L)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("K,V", [(64, 64), (128, 40), (24, 72)])
 def test_gradients_of_views(dev, dtype, K, V):

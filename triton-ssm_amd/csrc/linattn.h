@@ -40,6 +40,8 @@ struct LinPlan {
   float *ends, *back;        // nseg > 1
   double *sums, *back_sums;
   float *states, *grads;     // gradients only
+  int64_t split;             // workgroups that share the value heads of a chunk's key head
+  float* part;               // split > 1: [dQ, dK][split][B, L, Hk, K]
   int64_t bytes;
 };
 // vec: the rows of q, k, v and o are whole 16-byte accesses.

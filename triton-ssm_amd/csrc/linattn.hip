@@ -38,9 +38,17 @@ int64_t segments(int64_t heads, int64_t L, int64_t K, int64_t V, bool grads) {
   return n < fill || L < n * 2048 ? n : 512 / wgs;
 }
 
+// Workgroups that share the value heads of a key head in the gradients of the inputs,
+// by the workgroups that there are without: one for each head, and a sum of their dQ
+// and dK, while that fills CUs.  Us a call (64 x 64, 8 value heads, B=2), shared against
+// one after the other: 16 workgroups of 8 heads 34 against 94 (fp32), 64 of 4 31 against
+// 44 (bf16), 128 of 2 31 against 33, of 8 70 against 85; 256 of 2 46 against 43, of 8 111
+// against 103.
+int64_t shared(int64_t wgs, int64_t heads) { return wgs < 192 ? heads : 1; }
+
 // The chunked form's plan over a workspace at base (which may be null: sizes).  chunk:
 // steps between the states that the gradients keep, 0 for the forward.
-LinPlan lin_plan(char* base, int64_t B, int64_t L, int64_t Hv, int64_t K, int64_t V,
+LinPlan lin_plan(char* base, int64_t B, int64_t L, int64_t Hk, int64_t Hv, int64_t K, int64_t V,
                  int64_t chunk) {
   LinPlan p = {};
   const int64_t heads = B * Hv, elems = (K <= 32 ? 32 : (K <= 64 ? 64 : 128)) * cdiv64(V, 32) * 32;
@@ -64,6 +72,8 @@ LinPlan lin_plan(char* base, int64_t B, int64_t L, int64_t Hv, int64_t K, int64_
   if (chunk) {
     p.states = reinterpret_cast<float*>(take(heads * cdiv64(L, chunk) * elems * 4));
     p.grads = reinterpret_cast<float*>(take(heads * cdiv64(L, chunk) * elems * 4));
+    p.split = shared(B * Hk * cdiv64(L, chunk), Hv / Hk);
+    if (p.split > 1) p.part = reinterpret_cast<float*>(take(2 * p.split * B * L * Hk * K * 4));
   }
   p.bytes = at;
   return p;
@@ -100,7 +110,7 @@ extern "C" int64_t tssm_linear_attention_workspace_bytes(int64_t nbatch, int64_t
   if (!sizes_ok(nbatch, L, Hk, Hv, K, V)) return TSSM_ERR_SHAPE;
   if (!takes(K, V)) return TSSM_ERR_UNSUPPORTED;
   if (nbatch == 0 || by_steps(nbatch * Hv, L, V)) return 0;
-  return lin_plan(nullptr, nbatch, L, Hv, K, V, 0).bytes;
+  return lin_plan(nullptr, nbatch, L, Hk, Hv, K, V, 0).bytes;
 }
 
 extern "C" int tssm_linear_attention_forward(
@@ -121,7 +131,7 @@ extern "C" int tssm_linear_attention_forward(
   hipStream_t st = as_stream(stream);
   if (by_steps(nbatch * Hv, L, V) || !chunk_rows(dtype, a)) return lin_seq_launch(dtype, a, st);
   TSSM_CHECK(L < (INT64_C(1) << 31) && nbatch <= 0x7fffffff / Hv, TSSM_ERR_UNSUPPORTED);
-  const LinPlan p = lin_plan(reinterpret_cast<char*>(workspace), nbatch, L, Hv, K, V, 0);
+  const LinPlan p = lin_plan(reinterpret_cast<char*>(workspace), nbatch, L, Hk, Hv, K, V, 0);
   TSSM_CHECK(p.bytes == 0 || (workspace && workspace_bytes >= p.bytes && aligned(workspace, 256)),
              TSSM_ERR_WORKSPACE);
   const bool vec = vec_rows(dtype, a);
@@ -154,7 +164,7 @@ extern "C" int64_t tssm_linear_attention_backward_workspace_bytes(int dtype, int
   if (!sizes_ok(nbatch, L, Hk, Hv, K, V)) return TSSM_ERR_SHAPE;
   if (!takes(K, V)) return TSSM_ERR_UNSUPPORTED;
   if (L == 0 || nbatch == 0) return 256;
-  return lin_plan(nullptr, nbatch, L, Hv, K, V, lin_state_steps(dtype, K)).bytes;
+  return lin_plan(nullptr, nbatch, L, Hk, Hv, K, V, lin_state_steps(dtype, K)).bytes;
 }
 
 extern "C" int tssm_linear_attention_backward(
@@ -180,7 +190,7 @@ extern "C" int tssm_linear_attention_backward(
     a.v_l = sd_l = V;
   }
   TSSM_CHECK(chunk_rows(dtype, a) && fits(dtype, sd_l, V), TSSM_ERR_STRIDE);
-  const LinPlan p = lin_plan(reinterpret_cast<char*>(workspace), nbatch, L, Hv, K, V,
+  const LinPlan p = lin_plan(reinterpret_cast<char*>(workspace), nbatch, L, Hk, Hv, K, V,
                              lin_state_steps(dtype, K));
   TSSM_CHECK(workspace && workspace_bytes >= p.bytes && aligned(workspace, 256),
              TSSM_ERR_WORKSPACE);

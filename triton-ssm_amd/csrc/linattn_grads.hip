@@ -12,7 +12,8 @@
 // from the end) the differences of large sums would cost digits of small gradients.
 //
 // A workgroup of C / 16 waves has one chunk of one key head and goes through its
-// value heads and blocks of V, whose dQ and dK add up in registers, in order.  A wave
+// value heads and blocks of V, whose dQ and dK add up in registers, in order (where that
+// leaves CUs idle, a workgroup for each value head and a sum of theirs).  A wave
 // has 16 steps: as keys (columns of P and R) for dK and dV, as queries (columns of
 // R^T) for dQ, so that every product's result is the next one's operand in place
 // (planes.h); R is formed in both places.  The states' planes take one buffer after
@@ -33,7 +34,9 @@ struct LinGradArgs {
   LinArgs a;
   LinGrads d;
   const float *states, *grads;  // [bh][nch][state]
+  float* part;                  // split > 1: [dQ, dK][split][B, L, Hk, K]
   int nch, nvb;                 // chunks; blocks of VB columns
+  int split, heads;             // workgroups of a key head's value heads; heads of each
   uint32_t units;
 };
 
@@ -67,8 +70,9 @@ __global__ __launch_bounds__(4 * C, kPlanes<T> * KP <= 64 ? 2 : 1) void
   const LinArgs& a = g.a;
   const uint32_t id = block_of();
   if (id >= g.units) return;
-  const uint32_t bn = id / (uint32_t)a.Hk;
-  const int64_t hk = id - bn * (uint32_t)a.Hk, b = bn / (uint32_t)g.nch;
+  const uint32_t bnk = id / (uint32_t)g.split, bn = bnk / (uint32_t)a.Hk;
+  const int64_t hk = bnk - bn * (uint32_t)a.Hk, b = bn / (uint32_t)g.nch;
+  const int hs = (int)(id - bnk * (uint32_t)g.split), h0 = hs * g.heads, h1 = h0 + g.heads;
   const int n = (int)(bn - (uint32_t)b * (uint32_t)g.nch);
   const int per = (int)(a.Hv / a.Hk), K = (int)a.K;
   const int lane = threadIdx.x & 63, j = lane >> 4, c = lane & 15;
@@ -119,7 +123,7 @@ __global__ __launch_bounds__(4 * C, kPlanes<T> * KP <= 64 ? 2 : 1) void
       pq[i].load(dq, x < K ? r * rq.row + x * kE : kPast);
       pk[i].load(dk, x < K ? r * rk.row + x * kE : kPast);
     }
-    fetch(0, 0);
+    fetch(h0, 0);
 #pragma unroll
     for (int i = 0; i < W::kNk; ++i) {
       const int at = (int)threadIdx.x + NT * i, r = at / (KP / 8), x = at % (KP / 8);
@@ -136,13 +140,13 @@ __global__ __launch_bounds__(4 * C, kPlanes<T> * KP <= 64 ? 2 : 1) void
 #pragma unroll
   for (int i = 0; i < KT; ++i) dq[i] = dk[i] = zero4();
 
-  for (int hi = 0; hi < per; ++hi) {
+  for (int hi = h0; hi < h1; ++hi) {
     const int64_t h = hk * per + hi;
     float sumx = 0.0f, sumy = 0.0f, sumc = 0.0f, sumz = 0.0f;
     for (int vb = 0; vb < g.nvb; ++vb) {
       const int64_t v0 = (int64_t)vb * VB;
       const int nv = a.V - v0 < VB ? (int)(a.V - v0) : VB;
-      if (vb > 0 || hi > 0) fetch(hi, vb);
+      if (vb > 0 || hi > h0) fetch(hi, vb);
       lds_barrier();  // the one before is done with LDS
 #pragma unroll
       for (int i = 0; i < W::kNv; ++i) {
@@ -469,35 +473,53 @@ __global__ __launch_bounds__(4 * C, kPlanes<T> * KP <= 64 ? 2 : 1) void
   }
   // dQ and dK of the wave's 16 steps
   if (own < rows) {
-    const int64_t at = ((b * a.L + t0 + own) * a.Hk + hk) * a.K;
-    T* pq = reinterpret_cast<T*>(g.d.dq) + at;
-    T* pk = reinterpret_cast<T*>(g.d.dk) + at;
+    const int64_t at = ((b * a.L + t0 + own) * a.Hk + hk) * a.K, n = a.B * a.L * a.Hk * a.K;
+    const auto store = [&](auto* pq, auto* pk) {
+      typedef std::remove_reference_t<decltype(*pq)> O;
 #pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      const int x = 32 * s + 8 * j;
-      float q8[8], k8[8];
+      for (int s = 0; s < NS; ++s) {
+        const int x = 32 * s + 8 * j;
+        float q8[8], k8[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        q8[e] = dq[2 * s + (e >> 2)][e & 3];
-        k8[e] = dk[2 * s + (e >> 2)][e & 3];
-      }
-      if constexpr (VEC) {
-        if (x < K) {
-          st_lanes<T, 4>(pq + x, q8);
-          st_lanes<T, 4>(pq + x + 4, q8 + 4);
-          st_lanes<T, 4>(pk + x, k8);
-          st_lanes<T, 4>(pk + x + 4, k8 + 4);
+        for (int e = 0; e < 8; ++e) {
+          q8[e] = dq[2 * s + (e >> 2)][e & 3];
+          k8[e] = dk[2 * s + (e >> 2)][e & 3];
         }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (x + e < K) {
-            stf(pq + x + e, q8[e]);
-            stf(pk + x + e, k8[e]);
+        if constexpr (VEC) {
+          if (x < K) {
+            st_lanes<O, 4>(pq + x, q8);
+            st_lanes<O, 4>(pq + x + 4, q8 + 4);
+            st_lanes<O, 4>(pk + x, k8);
+            st_lanes<O, 4>(pk + x + 4, k8 + 4);
           }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (x + e < K) {
+              stf(pq + x + e, q8[e]);
+              stf(pk + x + e, k8[e]);
+            }
+        }
       }
-    }
+    };
+    if (g.part) store(g.part + hs * n + at, g.part + (g.split + hs) * n + at);
+    else store(reinterpret_cast<T*>(g.d.dq) + at, reinterpret_cast<T*>(g.d.dk) + at);
   }
+}
+
+// dQ and dK of value heads that had workgroups of their own, added up in order (4 us for
+// what 104 workgroups left: a launch).
+template <typename T>
+__global__ __launch_bounds__(256) void lin_parts_kernel(const float* part, T* dq, T* dk, int64_t n,
+                                                        int split) {
+  const int64_t i = (int64_t)block_of() * 256 + threadIdx.x;
+  if (i >= 2 * n) return;
+  const bool isk = i >= n;
+  const int64_t at = isk ? i - n : i;
+  const float* p = part + (isk ? split * n : 0) + at;
+  float s = p[0];
+  for (int h = 1; h < split; ++h) s += p[h * n];
+  stf((isk ? dk : dq) + at, s);
 }
 
 template <typename T, int KP, bool VEC>
@@ -507,7 +529,8 @@ int launch(LinGradArgs g, hipStream_t s) {
   static_assert(sizeof(typename W::Lds) <= 160 * 1024, "LDS of a CU");
   g.nch = (int)cdiv64(g.a.L, C);
   g.nvb = (int)cdiv64(g.a.V, W::VB);
-  const int64_t units = g.a.B * g.a.Hk * g.nch;
+  g.heads = (int)(g.a.Hv / g.a.Hk) / g.split;
+  const int64_t units = g.a.B * g.a.Hk * g.nch * g.split;
   if (units > 0x7fffffff) return TSSM_ERR_UNSUPPORTED;
   g.units = (uint32_t)units;
   const auto kernel = lin_grads_kernel<T, KP, VEC, C>;
@@ -518,6 +541,11 @@ int launch(LinGradArgs g, hipStream_t s) {
     if (e != hipSuccess) return (int)e;
   }
   kernel<<<grid_of(units), W::NT, sizeof(typename W::Lds), s>>>(g);
+  const int rc = launch_status();
+  if (rc || !g.part) return rc;
+  const int64_t n = g.a.B * g.a.L * g.a.Hk * g.a.K;
+  lin_parts_kernel<T><<<grid_of(cdiv64(2 * n, 256)), 256, 0, s>>>(
+      g.part, reinterpret_cast<T*>(g.d.dq), reinterpret_cast<T*>(g.d.dk), n, g.split);
   return launch_status();
 }
 
@@ -539,6 +567,8 @@ int lin_grads_launch(int dtype, const LinArgs& a, const LinGrads& d, bool vec, c
   g.d = d;
   g.states = p.states;
   g.grads = p.grads;
+  g.part = p.part;
+  g.split = (int)p.split;
   switch (dtype) {
     case TSSM_F32: return by_keys<float>(g, vec, s);
     case TSSM_BF16: return by_keys<bf16_t>(g, vec, s);
