@@ -7,14 +7,14 @@
 //
 // A workgroup walks 32 columns of V of one head's segment.  Its waves have roles, one
 // barrier a chunk:
-//   two teams of C / 32 output waves (one where LDS does not hold three chunks): 32
-//     steps of a chunk each, as two tiles of 16.  A team has every other chunk, and
-//     two chunks' time for it,
+//   two teams of C / 32 output waves: 32 steps of a chunk each, as two tiles of 16.  A
+//     team has every other chunk, and two chunks' time for it.  (Where LDS does not hold
+//     three chunks, one team, with a wave for each tile,)
 //   2 state waves: 16 columns each.  K^T V of the whole chunk on top of the decayed
 //     state, whose planes go to LDS for the next chunk's outputs,
-//   2 loaders: the chunk after this one to LDS, from loads that are two chunks ahead,
-//     and a wave for the decays where it is no fourth one on a SIMD (it would take a
-//     quarter of the others' registers: 32 x 64 fp32 steps 46 -> 88 us).
+//   2 loaders (4 beside one team): the chunk after this one to LDS, from loads that are
+//     two chunks ahead; and a wave for the decays where it is no third one on a SIMD (it
+//     would take a third of the others' registers: 64 steps of fp32 46 -> 88 us).
 // Everything is formed transposed (planes.h): P^T = K Q^T is the next product's operand
 // in place, queries come to their wave straight from memory, and a lane ends up with 8
 // neighbouring columns of one step's output.
@@ -77,9 +77,10 @@ struct LinWalk {
   static constexpr int NP = kPlanes<T>, NO = kOutPlanes<T>;
   static constexpr int NS = KP / 32, KT = KP / 16, NB = C / 32;
   static constexpr int TEAMS = MODE == kOutputs ? lin_teams(NP, KP) : 1, RING = TEAMS + 1;
-  static constexpr int NW = MODE == kOutputs ? TEAMS * C / 32 : 0;  // output waves
-  static constexpr int NT = 128;                            // threads of the loaders
-  static constexpr bool CLOCK = NW == 0 || NW % 4 != 0;      // a wave for the decays
+  // output waves: of two tiles of 16 steps, or one where there is one team
+  static constexpr int NW = MODE == kOutputs ? (TEAMS == 1 ? C / 16 : TEAMS * C / 32) : 0;
+  static constexpr int NT = NW == 2 && TEAMS == 1 ? 256 : 128;  // threads of the loaders
+  static constexpr bool CLOCK = NW <= 2 && NT == 128;       // a wave for the decays
   static constexpr int kThreads = 64 * (NW + 2 + CLOCK) + NT;
   static constexpr int kNk = (C * KP / 8 + NT - 1) / NT, kNv = (C * 4 + NT - 1) / NT;
   // chunks on their way from memory
@@ -345,7 +346,20 @@ __device__ inline void lin_outputs(const LinWalkArgs& g, const LinUnit<C>& u,
         in[i][s].load(d, y < K ? t[i] * rq.row + y * kE : kPast);
       }
   };
+  // Queries become operands as a chunk's work begins, or, where its first half has the
+  // one block of K, at the end of the second (halves of 3970 and 1590 cycles otherwise,
+  // 128 x 128 fp16: 54 against 50 us).
+  constexpr bool kLate = TEAMS == 2 && LB == 0;
+  u32x4 qb[NI][NS][NP];
+  const auto queries = [&](int m) {  // in place of chunk m's: the one that is fetched
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int s = 0; s < NS; ++s) planes_apart(in[i][s], K - 32 * s - 8 * j, qb[i][s]);
+    fetch(m + TEAMS);
+  };
   fetch(team);
+  if (kLate) queries(team);
   lds_barrier();
   if (team) lds_barrier();
   int slot = team;
@@ -353,7 +367,7 @@ __device__ inline void lin_outputs(const LinWalkArgs& g, const LinUnit<C>& u,
     const typename W::Operands& B = lds.op[slot];
     const auto& Sp = lds.S[slot];
     slot = slot + TEAMS < W::RING ? slot + TEAMS : slot + TEAMS - W::RING;
-    u32x4 qb[NI][NS][NP], fk[2][NS][NP], fv[2][NP];
+    u32x4 fk[2][NS][NP], fv[2][NP];
     float u1, h1, l1, ht[NI], lt[NI];
     const auto keys = [&](int ib) {
 #pragma unroll
@@ -387,11 +401,7 @@ __device__ inline void lin_outputs(const LinWalkArgs& g, const LinUnit<C>& u,
     }
     decays(0);
     values(0);
-#pragma unroll
-    for (int i = 0; i < NI; ++i)
-#pragma unroll
-      for (int s = 0; s < NS; ++s) planes_apart(in[i][s], K - 32 * s - 8 * j, qb[i][s]);
-    fetch(m + TEAMS);
+    if (!kLate) queries(m);
     __builtin_amdgcn_sched_barrier(0);
     f32x4 acc[NI][2], own[2];
 #pragma unroll
@@ -514,6 +524,7 @@ __device__ inline void lin_outputs(const LinWalkArgs& g, const LinUnit<C>& u,
           buf_put<T>(dst, 8 * j + e < u.nv ? off + e * kE : kPast, o8[e]);
       }
     }
+    if (kLate) queries(m + TEAMS);
     lds_barrier();
   }
   // the barriers that are left of cnt + 1: this team's chunks have had two each
@@ -538,7 +549,10 @@ __global__ __launch_bounds__((LinWalk<T, KP, kWalkSteps<T, KP>, kOutputs>::kThre
   } else {
     constexpr int kTeam = C / 32;  // waves of a team
     const int team = w / kTeam, n = w % kTeam;
-    if constexpr (C == 128) {
+    if constexpr (W::TEAMS == 1) {
+      static_assert(W::TEAMS == 2 || C == 32, "one block of K");
+      lin_outputs<T, KP, VEC, C, 0>(g, u, lds, lane, {w}, 0);
+    } else if constexpr (C == 128) {
       if (n < 2) lin_outputs<T, KP, VEC, C, 0, 1>(g, u, lds, lane, {n, 3 - n}, team);
       else lin_outputs<T, KP, VEC, C, 2, 3>(g, u, lds, lane, {n + 2, 9 - n}, team);
     } else {
