@@ -63,11 +63,13 @@ struct LinWalkArgs {
   double* sums;        // kEnds: [bh][nseg], of g / log 2
 };
 
-// Teams of output waves, and steps of a chunk: as many as LDS holds (a chunk more of K's
-// and the state's planes than there are teams).
-constexpr int lin_teams(int NP, int KP) { return NP * KP <= 256 ? 2 : 1; }
+// Teams of output waves, and steps of a chunk, by what LDS holds (a chunk more of K's and
+// the state's planes than there are teams).  128 x 128 fp16 would fit two teams of 32
+// steps: 51 against 47 us (B=2 L=2000 16 heads); 128 x 128 bf16 a chunk of 128 for one: 89
+// against 51 a call (B=2 L=2048 H=16).
+constexpr int lin_teams(int NP, int KP) { return NP * KP <= 192 ? 2 : 1; }
 template <typename T, int KP>
-constexpr int kWalkSteps = kPlanes<T> * KP <= 64 ? 128 : (kPlanes<T> * KP <= 192 ? 64 : 32);
+constexpr int kWalkSteps = kPlanes<T> * KP <= 64 ? 128 : (kPlanes<T> * KP <= 256 ? 64 : 32);
 // The gradients' kernel asks for chunks of its own.
 template <typename T, int KP>
 constexpr int kStateSteps = kPlanes<T> == 3 && KP == 128 ? 32 : 64;
@@ -346,12 +348,8 @@ __device__ inline void lin_outputs(const LinWalkArgs& g, const LinUnit<C>& u,
         in[i][s].load(d, y < K ? t[i] * rq.row + y * kE : kPast);
       }
   };
-  // Queries become operands as a chunk's work begins, or, where its first half has the
-  // one block of K, at the end of the second (halves of 3970 and 1590 cycles otherwise,
-  // 128 x 128 fp16: 54 against 50 us).
-  constexpr bool kLate = TEAMS == 2 && LB == 0;
   u32x4 qb[NI][NS][NP];
-  const auto queries = [&](int m) {  // in place of chunk m's: the one that is fetched
+  const auto queries = [&](int m) {
 #pragma unroll
     for (int i = 0; i < NI; ++i)
 #pragma unroll
@@ -359,7 +357,6 @@ __device__ inline void lin_outputs(const LinWalkArgs& g, const LinUnit<C>& u,
     fetch(m + TEAMS);
   };
   fetch(team);
-  if (kLate) queries(team);
   lds_barrier();
   if (team) lds_barrier();
   int slot = team;
@@ -401,7 +398,7 @@ __device__ inline void lin_outputs(const LinWalkArgs& g, const LinUnit<C>& u,
     }
     decays(0);
     values(0);
-    if (!kLate) queries(m);
+    queries(m);
     __builtin_amdgcn_sched_barrier(0);
     f32x4 acc[NI][2], own[2];
 #pragma unroll
@@ -524,7 +521,6 @@ __device__ inline void lin_outputs(const LinWalkArgs& g, const LinUnit<C>& u,
           buf_put<T>(dst, 8 * j + e < u.nv ? off + e * kE : kPast, o8[e]);
       }
     }
-    if (kLate) queries(m + TEAMS);
     lds_barrier();
   }
   // the barriers that are left of cnt + 1: this team's chunks have had two each
@@ -550,8 +546,8 @@ __global__ __launch_bounds__((LinWalk<T, KP, kWalkSteps<T, KP>, kOutputs>::kThre
     constexpr int kTeam = C / 32;  // waves of a team
     const int team = w / kTeam, n = w % kTeam;
     if constexpr (W::TEAMS == 1) {
-      static_assert(W::TEAMS == 2 || C == 32, "one block of K");
-      lin_outputs<T, KP, VEC, C, 0>(g, u, lds, lane, {w}, 0);
+      if (w < 2) lin_outputs<T, KP, VEC, C, 0>(g, u, lds, lane, {w}, 0);
+      else if constexpr (C == 64) lin_outputs<T, KP, VEC, C, 1>(g, u, lds, lane, {w}, 0);
     } else if constexpr (C == 128) {
       if (n < 2) lin_outputs<T, KP, VEC, C, 0, 1>(g, u, lds, lane, {n, 3 - n}, team);
       else lin_outputs<T, KP, VEC, C, 2, 3>(g, u, lds, lane, {n + 2, 9 - n}, team);
