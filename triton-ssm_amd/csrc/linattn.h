@@ -52,7 +52,7 @@ int lin_entry_launch(int dtype, const LinArgs& a, bool vec, const LinPlan& p, hi
 // for v, dh_last for h0, dh0 for h_last), segments included.
 int lin_states_launch(int dtype, const LinArgs& a, const LinArgs& way, bool vec, const LinPlan& p,
                       hipStream_t s);
-int64_t lin_state_steps(int dtype, int64_t K);  // steps of such a chunk
+constexpr int kLinChunk = 64;  // steps of such a chunk
 // Gradients of the inputs; outputs contiguous, dO with strides.
 struct LinGrads {
   const void* dout;

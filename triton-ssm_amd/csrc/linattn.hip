@@ -164,7 +164,7 @@ extern "C" int64_t tssm_linear_attention_backward_workspace_bytes(int dtype, int
   if (!sizes_ok(nbatch, L, Hk, Hv, K, V)) return TSSM_ERR_SHAPE;
   if (!takes(K, V)) return TSSM_ERR_UNSUPPORTED;
   if (L == 0 || nbatch == 0) return 256;
-  return lin_plan(nullptr, nbatch, L, Hk, Hv, K, V, lin_state_steps(dtype, K)).bytes;
+  return lin_plan(nullptr, nbatch, L, Hk, Hv, K, V, kLinChunk).bytes;
 }
 
 extern "C" int tssm_linear_attention_backward(
@@ -190,8 +190,7 @@ extern "C" int tssm_linear_attention_backward(
     a.v_l = sd_l = V;
   }
   TSSM_CHECK(chunk_rows(dtype, a) && fits(dtype, sd_l, V), TSSM_ERR_STRIDE);
-  const LinPlan p = lin_plan(reinterpret_cast<char*>(workspace), nbatch, L, Hk, Hv, K, V,
-                             lin_state_steps(dtype, K));
+  const LinPlan p = lin_plan(reinterpret_cast<char*>(workspace), nbatch, L, Hk, Hv, K, V, kLinChunk);
   TSSM_CHECK(workspace && workspace_bytes >= p.bytes && aligned(workspace, 256),
              TSSM_ERR_WORKSPACE);
   LinArgs way = a;  // the way back reads queries for keys and dO for v

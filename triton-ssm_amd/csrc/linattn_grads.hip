@@ -24,7 +24,8 @@
 // workgroups are on a CU (one, with 266 registers, took 160 us), and what one waits for
 // is hidden by the other's work alone.  The states are read once, past the caches
 // (through them 92 us).  Chunks of 128 steps would halve the states and leave LDS for
-// one workgroup; chunks of 32 in fp32 took 380 us for 344 (the same sizes, all kernels).
+// one workgroup; chunks of 32 in fp32 took 380 us for 344 (the same sizes, all kernels),
+// and 483 for 278 at B=2 L=2048 H=16 128 x 128: two waves on a CU.
 #include "linattn_dev.h"
 
 namespace tssm {
@@ -524,7 +525,7 @@ __global__ __launch_bounds__(256) void lin_parts_kernel(const float* part, T* dq
 
 template <typename T, int KP, bool VEC>
 int launch(LinGradArgs g, hipStream_t s) {
-  constexpr int C = kPlanes<T> == 3 && KP == 128 ? 32 : 64;
+  constexpr int C = kLinChunk;
   typedef Grad<T, KP, C> W;
   static_assert(sizeof(typename W::Lds) <= 160 * 1024, "LDS of a CU");
   g.nch = (int)cdiv64(g.a.L, C);

@@ -119,6 +119,4 @@ int lin_states_launch(int dtype, const LinArgs& a, const LinArgs& way, bool vec,
   return walk<kStates>(dtype, f, b, vec, s);
 }
 
-int64_t lin_state_steps(int dtype, int64_t K) { return dtype == TSSM_F32 && K > 64 ? 32 : 64; }
-
 }  // namespace tssm

@@ -70,9 +70,6 @@ struct LinWalkArgs {
 constexpr int lin_teams(int NP, int KP) { return NP * KP <= 192 ? 2 : 1; }
 template <typename T, int KP>
 constexpr int kWalkSteps = kPlanes<T> * KP <= 64 ? 128 : (kPlanes<T> * KP <= 256 ? 64 : 32);
-// The gradients' kernel asks for chunks of its own.
-template <typename T, int KP>
-constexpr int kStateSteps = kPlanes<T> == 3 && KP == 128 ? 32 : 64;
 
 template <typename T, int KP, int C, int MODE>
 struct LinWalk {
@@ -559,9 +556,9 @@ __global__ __launch_bounds__((LinWalk<T, KP, kWalkSteps<T, KP>, kOutputs>::kThre
 
 // The states' walk and its way back, side by side: the first nf workgroups go forward.
 template <typename T, int KP, bool VEC, int MODE>
-__global__ __launch_bounds__((LinWalk<T, KP, kStateSteps<T, KP>, MODE>::kThreads)) void
+__global__ __launch_bounds__((LinWalk<T, KP, kLinChunk, MODE>::kThreads)) void
     lin_states_kernel(LinWalkArgs f, LinWalkArgs back, uint32_t nf) {
-  constexpr int C = kStateSteps<T, KP>;
+  constexpr int C = kLinChunk;
   typedef LinWalk<T, KP, C, MODE> W;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   typename W::Lds& lds = *reinterpret_cast<typename W::Lds*>(smem);
@@ -615,10 +612,10 @@ int lin_walk_run(LinWalkArgs g, hipStream_t s) {
 // back.walked = 0: forward alone.
 template <typename T, int KP, bool VEC, int MODE>
 int lin_states_run(LinWalkArgs f, LinWalkArgs back, hipStream_t s) {
-  typedef LinWalk<T, KP, kStateSteps<T, KP>, MODE> W;
+  typedef LinWalk<T, KP, kLinChunk, MODE> W;
   static_assert(sizeof(typename W::Lds) <= 160 * 1024, "LDS of a CU");
-  const int64_t nf = lin_walk_sizes(f, kStateSteps<T, KP>);
-  const int64_t nb = lin_walk_sizes(back, kStateSteps<T, KP>);
+  const int64_t nf = lin_walk_sizes(f, kLinChunk);
+  const int64_t nb = lin_walk_sizes(back, kLinChunk);
   if (nf < 0 || nb < 0) return TSSM_ERR_UNSUPPORTED;
   const auto kernel = lin_states_kernel<T, KP, VEC, MODE>;
   const int rc = lin_lds(kernel, (int)sizeof(typename W::Lds));
