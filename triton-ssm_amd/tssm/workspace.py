@@ -117,9 +117,8 @@ def call(name: str, t: torch.Tensor, stream: int, nbytes: int, *args) -> None:
     if lock is None:
         lock = _call_locks.setdefault(key, threading.Lock())
     with lock:
-        buf = _cache.get(key)
-        if buf is None or buf.numel() < nbytes:
-            buf = get(t.device, stream, nbytes, SSD)
+        # (inside the lock: another thread may have replaced the buffer meanwhile)
+        buf = get(t.device, stream, nbytes, SSD)
         _lib.call(name, *args, buf.data_ptr(), buf.numel(), stream)
 
 
