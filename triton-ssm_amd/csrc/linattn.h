@@ -44,13 +44,14 @@ struct LinPlan {
   float* part;               // split > 1: [dQ, dK][split][B, L, Hk, K]
   int64_t bytes;
 };
-// vec: the rows of q, k, v and o are whole 16-byte accesses.
-int lin_walk_launch(int dtype, const LinArgs& a, bool vec, const LinPlan& p, hipStream_t s);
+// rows: what whole 16-byte accesses make up.
+enum LinRows { kNoRows, kKeyRows, kAllRows };  // none, the rows of q and k, those of v and o too
+int lin_walk_launch(int dtype, const LinArgs& a, LinRows rows, const LinPlan& p, hipStream_t s);
 // The segments' entry states, forward.
-int lin_entry_launch(int dtype, const LinArgs& a, bool vec, const LinPlan& p, hipStream_t s);
+int lin_entry_launch(int dtype, const LinArgs& a, LinRows rows, const LinPlan& p, hipStream_t s);
 // The states before the chunks and the gradients of those after them (way: q for k, dO
 // for v, dh_last for h0, dh0 for h_last), segments included.
-int lin_states_launch(int dtype, const LinArgs& a, const LinArgs& way, bool vec, const LinPlan& p,
+int lin_states_launch(int dtype, const LinArgs& a, const LinArgs& way, LinRows rows, const LinPlan& p,
                       hipStream_t s);
 constexpr int kLinChunk = 64;  // steps of such a chunk
 // Gradients of the inputs; outputs contiguous, dO with strides.
@@ -60,7 +61,7 @@ struct LinGrads {
   void *dq, *dk, *dv;
   float* dg;
 };
-int lin_grads_launch(int dtype, const LinArgs& a, const LinGrads& d, bool vec, const LinPlan& p,
+int lin_grads_launch(int dtype, const LinArgs& a, const LinGrads& d, LinRows rows, const LinPlan& p,
                      hipStream_t s);
 
 }  // namespace tssm

@@ -59,7 +59,7 @@ struct Grad {
   };
 };
 
-template <typename T, int KP, bool VEC, int C>
+template <typename T, int KP, LinRows ROWS, int C>
 // two workgroups on a CU but where their registers would spill
 __global__ __launch_bounds__(4 * C, kPlanes<T> < 3 && KP <= 64 ? 2 : 1) void
     lin_grads_kernel(LinGradArgs g) {
@@ -90,7 +90,7 @@ __global__ __launch_bounds__(4 * C, kPlanes<T> < 3 && KP <= 64 ? 2 : 1) void
   rk.init(reinterpret_cast<const T*>(a.k) + b * a.k_b + hk * a.k_h, a.k_l, K, a.L);
   // A value head's block of V, dO and the states, on their way from memory: the first
   // with Q and K, the next ones behind the last use of the registers before them.
-  Piece<T, VEC, NP> pv[W::kNv], po[W::kNv];
+  Piece<T, ROWS == kAllRows, NP> pv[W::kNv], po[W::kNv];
   f32x4 st[W::kNs], gr[W::kNs];
   Gaps<C> gaps;
   const auto fetch = [&](int hi, int vb) {
@@ -119,7 +119,7 @@ __global__ __launch_bounds__(4 * C, kPlanes<T> < 3 && KP <= 64 ? 2 : 1) void
   };
   {
     const auto dq = rq.at(n), dk = rk.at(n);
-    Piece<T, VEC, NP> pq[W::kNk], pk[W::kNk];
+    Piece<T, ROWS != kNoRows, NP> pq[W::kNk], pk[W::kNk];
 #pragma unroll
     for (int i = 0; i < W::kNk; ++i) {
       const int at = (int)threadIdx.x + NT * i, r = at / (KP / 8), x = at % (KP / 8) * 8;
@@ -423,7 +423,7 @@ __global__ __launch_bounds__(4 * C, kPlanes<T> < 3 && KP <= 64 ? 2 : 1) void
           const float o8[8] = {dvt[2 * i][0], dvt[2 * i][1], dvt[2 * i][2], dvt[2 * i][3],
                                dvt[2 * i + 1][0], dvt[2 * i + 1][1], dvt[2 * i + 1][2],
                                dvt[2 * i + 1][3]};
-          if constexpr (VEC) {
+          if constexpr (ROWS == kAllRows) {
             if (x < nv) {
               st_lanes<T, 4>(p + x, o8);
               st_lanes<T, 4>(p + x + 4, o8 + 4);
@@ -437,7 +437,7 @@ __global__ __launch_bounds__(4 * C, kPlanes<T> < 3 && KP <= 64 ? 2 : 1) void
       }
       // (that these are loaded again is more than the compiler sees)
 #pragma unroll
-      for (int i = 0; i < W::kNv; ++i) pv[i] = po[i] = Piece<T, VEC, NP>{};
+      for (int i = 0; i < W::kNv; ++i) pv[i] = po[i] = {};
 #pragma unroll
       for (int i = 0; i < W::kNs; ++i) st[i] = gr[i] = zero4();
     }
@@ -488,7 +488,7 @@ __global__ __launch_bounds__(4 * C, kPlanes<T> < 3 && KP <= 64 ? 2 : 1) void
           q8[e] = dq[2 * s + (e >> 2)][e & 3];
           k8[e] = dk[2 * s + (e >> 2)][e & 3];
         }
-        if constexpr (VEC) {
+        if constexpr (ROWS != kNoRows) {
           if (x < K) {
             st_lanes<O, 4>(pq + x, q8);
             st_lanes<O, 4>(pq + x + 4, q8 + 4);
@@ -525,7 +525,7 @@ __global__ __launch_bounds__(256) void lin_parts_kernel(const float* part, T* dq
   stf((isk ? dk : dq) + at, s);
 }
 
-template <typename T, int KP, bool VEC>
+template <typename T, int KP, LinRows ROWS>
 int launch(LinGradArgs g, hipStream_t s) {
   constexpr int C = kLinChunk;
   typedef Grad<T, KP, C> W;
@@ -536,7 +536,7 @@ int launch(LinGradArgs g, hipStream_t s) {
   const int64_t units = g.a.B * g.a.Hk * g.nch * g.split;
   if (units > 0x7fffffff) return TSSM_ERR_UNSUPPORTED;
   g.units = (uint32_t)units;
-  const auto kernel = lin_grads_kernel<T, KP, VEC, C>;
+  const auto kernel = lin_grads_kernel<T, KP, ROWS, C>;
   if (sizeof(typename W::Lds) > 65536) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                              hipFuncAttributeMaxDynamicSharedMemorySize,
@@ -553,8 +553,11 @@ int launch(LinGradArgs g, hipStream_t s) {
 }
 
 template <typename T>
-int by_keys(const LinGradArgs& g, bool vec, hipStream_t s) {
-#define TSSM_GRADS(KP) (vec ? launch<T, KP, true>(g, s) : launch<T, KP, false>(g, s))
+int by_keys(const LinGradArgs& g, LinRows rows, hipStream_t s) {
+#define TSSM_GRADS(KP)                                   \
+  (rows == kAllRows   ? launch<T, KP, kAllRows>(g, s)    \
+   : rows == kKeyRows ? launch<T, KP, kKeyRows>(g, s)    \
+                      : launch<T, KP, kNoRows>(g, s))
   if (g.a.K <= 32) return TSSM_GRADS(32);
   if (g.a.K <= 64) return TSSM_GRADS(64);
   return TSSM_GRADS(128);
@@ -563,7 +566,7 @@ int by_keys(const LinGradArgs& g, bool vec, hipStream_t s) {
 
 }  // namespace
 
-int lin_grads_launch(int dtype, const LinArgs& a, const LinGrads& d, bool vec, const LinPlan& p,
+int lin_grads_launch(int dtype, const LinArgs& a, const LinGrads& d, LinRows rows, const LinPlan& p,
                      hipStream_t s) {
   LinGradArgs g = {};
   g.a = a;
@@ -573,9 +576,9 @@ int lin_grads_launch(int dtype, const LinArgs& a, const LinGrads& d, bool vec, c
   g.part = p.part;
   g.split = (int)p.split;
   switch (dtype) {
-    case TSSM_F32: return by_keys<float>(g, vec, s);
-    case TSSM_BF16: return by_keys<bf16_t>(g, vec, s);
-    default: return by_keys<f16_t>(g, vec, s);
+    case TSSM_F32: return by_keys<float>(g, rows, s);
+    case TSSM_BF16: return by_keys<bf16_t>(g, rows, s);
+    default: return by_keys<f16_t>(g, rows, s);
   }
 }
 

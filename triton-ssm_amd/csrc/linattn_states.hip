@@ -61,9 +61,11 @@ int fold(const LinArgs& a, float* ends, const double* sums, int nseg, int rev, h
 }
 
 template <typename T, int MODE>
-int by_keys(const LinWalkArgs& f, const LinWalkArgs& b, bool vec, hipStream_t s) {
+int by_keys(const LinWalkArgs& f, const LinWalkArgs& b, LinRows rows, hipStream_t s) {
 #define TSSM_WALK(KP) \
-  (vec ? lin_states_run<T, KP, true, MODE>(f, b, s) : lin_states_run<T, KP, false, MODE>(f, b, s))
+  (rows == kAllRows   ? lin_states_run<T, KP, kAllRows, MODE>(f, b, s) \
+   : rows == kKeyRows ? lin_states_run<T, KP, kKeyRows, MODE>(f, b, s) \
+                      : lin_states_run<T, KP, kNoRows, MODE>(f, b, s))
   if (f.a.K <= 32) return TSSM_WALK(32);
   if (f.a.K <= 64) return TSSM_WALK(64);
   return TSSM_WALK(128);
@@ -71,11 +73,11 @@ int by_keys(const LinWalkArgs& f, const LinWalkArgs& b, bool vec, hipStream_t s)
 }
 
 template <int MODE>
-int walk(int dtype, const LinWalkArgs& f, const LinWalkArgs& b, bool vec, hipStream_t s) {
+int walk(int dtype, const LinWalkArgs& f, const LinWalkArgs& b, LinRows rows, hipStream_t s) {
   switch (dtype) {
-    case TSSM_F32: return by_keys<float, MODE>(f, b, vec, s);
-    case TSSM_BF16: return by_keys<bf16_t, MODE>(f, b, vec, s);
-    default: return by_keys<f16_t, MODE>(f, b, vec, s);
+    case TSSM_F32: return by_keys<float, MODE>(f, b, rows, s);
+    case TSSM_BF16: return by_keys<bf16_t, MODE>(f, b, rows, s);
+    default: return by_keys<f16_t, MODE>(f, b, rows, s);
   }
 }
 
@@ -94,18 +96,18 @@ LinWalkArgs ends_of(const LinArgs& a, const LinPlan& p, bool rev) {
 
 }  // namespace
 
-int lin_entry_launch(int dtype, const LinArgs& a, bool vec, const LinPlan& p, hipStream_t s) {
+int lin_entry_launch(int dtype, const LinArgs& a, LinRows rows, const LinPlan& p, hipStream_t s) {
   LinWalkArgs none = ends_of(a, p, false);
   none.walked = 0;
-  const int rc = walk<kEnds>(dtype, ends_of(a, p, false), none, vec, s);
+  const int rc = walk<kEnds>(dtype, ends_of(a, p, false), none, rows, s);
   return rc ? rc : fold(a, p.ends, p.sums, (int)p.nseg, 0, s);
 }
 
-int lin_states_launch(int dtype, const LinArgs& a, const LinArgs& way, bool vec, const LinPlan& p,
+int lin_states_launch(int dtype, const LinArgs& a, const LinArgs& way, LinRows rows, const LinPlan& p,
                       hipStream_t s) {
   LinWalkArgs f = ends_of(a, p, false), b = ends_of(way, p, true);
   if (p.nseg > 1) {
-    int rc = walk<kEnds>(dtype, f, b, vec, s);
+    int rc = walk<kEnds>(dtype, f, b, rows, s);
     if (!rc) rc = fold(a, p.ends, p.sums, (int)p.nseg, 0, s);
     if (!rc) rc = fold(way, p.back, p.back_sums, (int)p.nseg, 1, s);
     if (rc) return rc;
@@ -116,7 +118,7 @@ int lin_states_launch(int dtype, const LinArgs& a, const LinArgs& way, bool vec,
   b.entry = p.back;
   f.states = p.states;
   b.states = p.grads;
-  return walk<kStates>(dtype, f, b, vec, s);
+  return walk<kStates>(dtype, f, b, rows, s);
 }
 
 }  // namespace tssm

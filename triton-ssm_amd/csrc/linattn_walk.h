@@ -128,7 +128,7 @@ __device__ inline int lin_chunk(const LinUnit<C>& u, int m) {
 }
 
 // K's, V's and the decays' way to LDS.
-template <typename T, int KP, bool VEC, int C, int MODE, bool REV>
+template <typename T, int KP, LinRows ROWS, int C, int MODE, bool REV>
 __device__ inline void lin_bring(const LinWalkArgs& g, const LinUnit<C>& u,
                                  typename LinWalk<T, KP, C, MODE>::Lds& lds, int id) {
   typedef LinWalk<T, KP, C, MODE> W;
@@ -142,7 +142,8 @@ __device__ inline void lin_bring(const LinWalkArgs& g, const LinUnit<C>& u,
   rv.init(reinterpret_cast<const T*>(a.v) + u.b * a.v_b + u.h * a.v_h + u.v0, a.v_l, u.nv, a.L);
   const float* gp = a.g + u.b * a.g_b + u.h * a.g_h;
   struct Regs {
-    Piece<T, VEC, NP> k[W::kNk], v[W::kNv];
+    Piece<T, ROWS != kNoRows, NP> k[W::kNk];
+    Piece<T, ROWS == kAllRows, NP> v[W::kNv];
     Gaps<C> g;
   } in[W::AHEAD];
   const auto fetch = [&](Regs& in, int m) {
@@ -316,7 +317,7 @@ __device__ inline void lin_states(const LinWalkArgs& g, const LinUnit<C>& u,
 }
 
 // The outputs' waves: tiles of 16 steps, at 16 tile[i], whose own blocks of 32 steps are OWN.
-template <typename T, int KP, bool VEC, int C, int... OWN>
+template <typename T, int KP, LinRows ROWS, int C, int... OWN>
 __device__ inline void lin_outputs(const LinWalkArgs& g, const LinUnit<C>& u,
                                    typename LinWalk<T, KP, C, kOutputs>::Lds& lds, int lane,
                                    const int (&tile)[sizeof...(OWN)], int team) {
@@ -334,7 +335,7 @@ __device__ inline void lin_outputs(const LinWalkArgs& g, const LinUnit<C>& u,
   RowsOf<C> rq, ro;
   rq.init(reinterpret_cast<const T*>(a.q) + u.b * a.q_b + u.hk * a.q_h, a.q_l, K, a.L);
   ro.init(reinterpret_cast<const T*>(a.o) + u.b * a.o_b + u.h * a.o_h + u.v0, a.o_l, u.nv, a.L);
-  Piece<T, VEC, NP> in[NI][NS];
+  Piece<T, ROWS != kNoRows, NP> in[NI][NS];
   const auto fetch = [&](int m) {
     const auto d = rq.at(lin_chunk<C, false>(u, m));
 #pragma unroll
@@ -501,7 +502,7 @@ __device__ inline void lin_outputs(const LinWalkArgs& g, const LinUnit<C>& u,
 #pragma unroll
       for (int e = 0; e < 8; ++e)
         o8[e] = a.scale * __builtin_fmaf(y[e >> 2][e & 3], eg, acc[i][e >> 2][e & 3]);
-      if constexpr (VEC) {
+      if constexpr (ROWS == kAllRows) {
         const uint32_t to = 8 * j < u.nv ? off : kPast;
         union {
           T e[8];
@@ -524,7 +525,7 @@ __device__ inline void lin_outputs(const LinWalkArgs& g, const LinUnit<C>& u,
   if (TEAMS == 2 && ((cnt - team) & 1) == 0) lds_barrier();
 }
 
-template <typename T, int KP, bool VEC>
+template <typename T, int KP, LinRows ROWS>
 __global__ __launch_bounds__((LinWalk<T, KP, kWalkSteps<T, KP>, kOutputs>::kThreads)) void
     lin_walk_kernel(LinWalkArgs g) {
   constexpr int C = kWalkSteps<T, KP>;
@@ -536,26 +537,26 @@ __global__ __launch_bounds__((LinWalk<T, KP, kWalkSteps<T, KP>, kOutputs>::kThre
   const int id = (int)threadIdx.x, lane = id & 63;
   const int w = __builtin_amdgcn_readfirstlane(id >> 6);
   if (w >= W::NW + 2) {
-    lin_bring<T, KP, VEC, C, kOutputs, false>(g, u, lds, id - 64 * (W::NW + 2));
+    lin_bring<T, KP, ROWS, C, kOutputs, false>(g, u, lds, id - 64 * (W::NW + 2));
   } else if (w >= W::NW) {
     lin_states<T, KP, C, kOutputs, false>(g, u, lds, lane, w - W::NW);
   } else {
     constexpr int kTeam = C / 32;  // waves of a team
     const int team = w / kTeam, n = w % kTeam;
     if constexpr (W::TEAMS == 1) {
-      if (w < 2) lin_outputs<T, KP, VEC, C, 0>(g, u, lds, lane, {w}, 0);
-      else if constexpr (C == 64) lin_outputs<T, KP, VEC, C, 1>(g, u, lds, lane, {w}, 0);
+      if (w < 2) lin_outputs<T, KP, ROWS, C, 0>(g, u, lds, lane, {w}, 0);
+      else if constexpr (C == 64) lin_outputs<T, KP, ROWS, C, 1>(g, u, lds, lane, {w}, 0);
     } else if constexpr (C == 128) {
-      if (n < 2) lin_outputs<T, KP, VEC, C, 0, 1>(g, u, lds, lane, {n, 3 - n}, team);
-      else lin_outputs<T, KP, VEC, C, 2, 3>(g, u, lds, lane, {n + 2, 9 - n}, team);
+      if (n < 2) lin_outputs<T, KP, ROWS, C, 0, 1>(g, u, lds, lane, {n, 3 - n}, team);
+      else lin_outputs<T, KP, ROWS, C, 2, 3>(g, u, lds, lane, {n + 2, 9 - n}, team);
     } else {
-      lin_outputs<T, KP, VEC, C, 0, C / 32 - 1>(g, u, lds, lane, {n, C / 16 - 1 - n}, team);
+      lin_outputs<T, KP, ROWS, C, 0, C / 32 - 1>(g, u, lds, lane, {n, C / 16 - 1 - n}, team);
     }
   }
 }
 
 // The states' walk and its way back, side by side: the first nf workgroups go forward.
-template <typename T, int KP, bool VEC, int MODE>
+template <typename T, int KP, LinRows ROWS, int MODE>
 __global__ __launch_bounds__((LinWalk<T, KP, kLinChunk, MODE>::kThreads)) void
     lin_states_kernel(LinWalkArgs f, LinWalkArgs back, uint32_t nf) {
   constexpr int C = kLinChunk;
@@ -569,11 +570,11 @@ __global__ __launch_bounds__((LinWalk<T, KP, kLinChunk, MODE>::kThreads)) void
   if (block < nf) {
     if (!u.init(f, block)) return;
     if (w < 2) lin_states<T, KP, C, MODE, false>(f, u, lds, lane, w);
-    else lin_bring<T, KP, VEC, C, MODE, false>(f, u, lds, id - 128);
+    else lin_bring<T, KP, ROWS, C, MODE, false>(f, u, lds, id - 128);
   } else {
     if (!u.init(back, block - nf)) return;
     if (w < 2) lin_states<T, KP, C, MODE, true>(back, u, lds, lane, w);
-    else lin_bring<T, KP, VEC, C, MODE, true>(back, u, lds, id - 128);
+    else lin_bring<T, KP, ROWS, C, MODE, true>(back, u, lds, id - 128);
   }
 }
 
@@ -596,13 +597,13 @@ int lin_lds(K kernel, int bytes) {
                                                    bytes);
 }
 
-template <typename T, int KP, bool VEC>
+template <typename T, int KP, LinRows ROWS>
 int lin_walk_run(LinWalkArgs g, hipStream_t s) {
   typedef LinWalk<T, KP, kWalkSteps<T, KP>, kOutputs> W;
   static_assert(sizeof(typename W::Lds) <= 160 * 1024, "LDS of a CU");
   const int64_t wgs = lin_walk_sizes(g, kWalkSteps<T, KP>);
   if (wgs < 0) return TSSM_ERR_UNSUPPORTED;
-  const auto kernel = lin_walk_kernel<T, KP, VEC>;
+  const auto kernel = lin_walk_kernel<T, KP, ROWS>;
   const int rc = lin_lds(kernel, (int)sizeof(typename W::Lds));
   if (rc) return rc;
   kernel<<<grid_of(wgs), W::kThreads, sizeof(typename W::Lds), s>>>(g);
@@ -610,14 +611,14 @@ int lin_walk_run(LinWalkArgs g, hipStream_t s) {
 }
 
 // back.walked = 0: forward alone.
-template <typename T, int KP, bool VEC, int MODE>
+template <typename T, int KP, LinRows ROWS, int MODE>
 int lin_states_run(LinWalkArgs f, LinWalkArgs back, hipStream_t s) {
   typedef LinWalk<T, KP, kLinChunk, MODE> W;
   static_assert(sizeof(typename W::Lds) <= 160 * 1024, "LDS of a CU");
   const int64_t nf = lin_walk_sizes(f, kLinChunk);
   const int64_t nb = lin_walk_sizes(back, kLinChunk);
   if (nf < 0 || nb < 0) return TSSM_ERR_UNSUPPORTED;
-  const auto kernel = lin_states_kernel<T, KP, VEC, MODE>;
+  const auto kernel = lin_states_kernel<T, KP, ROWS, MODE>;
   const int rc = lin_lds(kernel, (int)sizeof(typename W::Lds));
   if (rc) return rc;
   kernel<<<grid_of(nf + nb), W::kThreads, sizeof(typename W::Lds), s>>>(f, back, (uint32_t)nf);

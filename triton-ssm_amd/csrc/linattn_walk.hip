@@ -5,8 +5,11 @@ namespace tssm {
 namespace {
 
 template <typename T>
-int by_keys(const LinWalkArgs& g, bool vec, hipStream_t s) {
-#define TSSM_WALK(KP) (vec ? lin_walk_run<T, KP, true>(g, s) : lin_walk_run<T, KP, false>(g, s))
+int by_keys(const LinWalkArgs& g, LinRows rows, hipStream_t s) {
+#define TSSM_WALK(KP)                                                \
+  (rows == kAllRows   ? lin_walk_run<T, KP, kAllRows>(g, s)          \
+   : rows == kKeyRows ? lin_walk_run<T, KP, kKeyRows>(g, s)          \
+                      : lin_walk_run<T, KP, kNoRows>(g, s))
   if (g.a.K <= 32) return TSSM_WALK(32);
   if (g.a.K <= 64) return TSSM_WALK(64);
   return TSSM_WALK(128);
@@ -15,16 +18,16 @@ int by_keys(const LinWalkArgs& g, bool vec, hipStream_t s) {
 
 }  // namespace
 
-int lin_walk_launch(int dtype, const LinArgs& a, bool vec, const LinPlan& p, hipStream_t s) {
+int lin_walk_launch(int dtype, const LinArgs& a, LinRows rows, const LinPlan& p, hipStream_t s) {
   LinWalkArgs g = {};
   g.a = a;
   g.steps = p.steps;
   g.nseg = g.walked = (int)p.nseg;
   g.entry = p.ends;
   switch (dtype) {
-    case TSSM_F32: return by_keys<float>(g, vec, s);
-    case TSSM_BF16: return by_keys<bf16_t>(g, vec, s);
-    default: return by_keys<f16_t>(g, vec, s);
+    case TSSM_F32: return by_keys<float>(g, rows, s);
+    case TSSM_BF16: return by_keys<bf16_t>(g, rows, s);
+    default: return by_keys<f16_t>(g, rows, s);
   }
 }
 
