@@ -180,6 +180,36 @@ def test_the_same_tensor_twice(dev):
     lin.compare_gradients(d, o, None, BF16)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("K,V", [(100, 117), (40, 30), (64, 65), (128, 5), (17, 4), (8, 3),
+                                 (33, 47), (64, 64), (16, 18)])
+@pytest.mark.parametrize("at", [0, 3])
+def test_states_of_odd_places(dev, dtype, K, V, at):
+    """States whose rows are no whole pieces, at any 4-byte address: what lies before and
+    behind stays, in a step, in few tokens and where a chunk reads it."""
+    from tssm import linear_attention_forward, linear_attention_step
+    S, H = 3, 2
+    d = lin.inputs(dev, S, 70, H, H, K, V, dtype, seed=K + V, h0=True)
+    n = S * H * K * V
+    for L in (1, 6, 70):
+        room = torch.full((n + 8,), 5.0, device=dev)
+        h = room[at:at + n].view(S, H, K, V)
+        h.copy_(d["h0"])
+        c = {x: t if x == "h0" else t[:, :L] for x, t in d.items()}
+        o_ref, S_ref = lin.oracle(c)
+        o, last = linear_attention_forward(*(c[x] for x in ("q", "k", "v", "g")), h0=h,
+                                           return_state=True)
+        assert_close(o, o_ref, lin.TOL[dtype], "o")
+        assert_close(last, S_ref, lin.TOL[F32], "state")
+        if L == 1:
+            o = linear_attention_step(*(c[x][:, 0] for x in ("q", "k", "v", "g")), h)
+            assert_close(o[:, None], o_ref, lin.TOL[dtype], "o")
+            assert_close(h, S_ref, lin.TOL[F32], "state")
+        else:
+            assert torch.equal(h, d["h0"])
+        assert (room[:at] == 5.0).all() and (room[at + n:] == 5.0).all()
+
+
 # ------------------------------------------------------------------ together
 # The longest sums have 140 terms (a weight's gradient over the tokens): 12 x 6e-8, 1e-6
 # of their size, behind four stages of which each adds 1e-5 of its largest value at
