@@ -320,3 +320,18 @@ def test_prompt_turns_and_steps(dev):
         parts.append(norm(o, c["z"][:, i])[:, None])
     assert_close(torch.cat(parts, 1), want.numpy(), TOL, "y")
     assert_close(S, last.numpy(), TOL, "state")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("K,R,pad", [(40, 40, 0), (40, 20, 0), (72, 72, 4), (24, 8, 2), (56, 28, 0),
+                                     (128, 64, 4), (128, 64, 2), (36, 36, 0), (68, 4, 0)])
+def test_norm_of_narrow_pieces(dev, dtype, interleaved, K, R, pad):
+    """Rows that are made of 8- or 4-byte pieces, by their sizes or by where they begin."""
+    d = qk.inputs(dev, 2, 37, 3, 2, K, R, dtype, seed=K + R)
+    for n in ("q", "k", "dq", "dk"):
+        t = d[n]
+        wide = torch.zeros(*t.shape[:3], K + pad, device=dev, dtype=dtype)
+        d[n] = wide[..., pad:]
+        d[n].copy_(t)
+    qk.check(d, interleaved=interleaved)

@@ -22,8 +22,8 @@
 // A workgroup has TB tokens; a group of LG lanes holds one row, TB groups beside
 // each other take tokens, the others heads, so a lane keeps its token's cosines in
 // registers over the heads it goes through.  A lane holds both members of its
-// pairs: two 16-byte vectors R/2 apart (or next to each other), or, where sizes or
-// alignment do not fit those, single elements.
+// pairs: two vectors of 16 (8, 4) bytes R/2 apart (or next to each other), or, where sizes
+// or alignment do not fit those, single elements.
 #include "planes.h"
 
 namespace tssm {
@@ -58,10 +58,12 @@ __device__ inline double position(const QkArgs& a, int64_t at) {
   }
 }
 
-// Lanes, pairs of a lane and the elements' places for one form.
+// Lanes, pairs of a lane (NS) and the elements' places for one form.
 template <typename T, int FORM, int LG_, int NS>
 struct Form {
-  static constexpr int LG = LG_, VE = 16 / (int)sizeof(T), NP = FORM == kSingle ? NS : VE;
+  // (single elements: that a Part has 32 bytes keeps 16-bit ones from being packed by two
+  // in registers, 142 against 112 us for 190 MB of rows of 100)
+  static constexpr int LG = LG_, VE = FORM == kSingle ? 16 / (int)sizeof(T) : NS, NP = NS;
   // first and second element of a lane's pair i; the second may be past K
   static __device__ inline void places(const QkArgs& a, int l, int i, int& ea, int& eb) {
     const int half = a.R / 2;
@@ -85,8 +87,10 @@ struct Form {
 template <typename T, int FORM, int LG, int NS>
 struct Part {
   typedef Form<T, FORM, LG, NS> F;
+  typedef std::conditional_t<F::VE * sizeof(T) == 16, u32x4,
+                             std::conditional_t<F::VE * sizeof(T) == 8, u32x2v, uint32_t>> word;
   union {
-    u32x4 v[2];
+    word v[2];
     T e[FORM == kSingle ? 2 * NS : 2 * F::VE];
   };
   __device__ inline void load(const QkArgs& a, const T* p, int l, bool on) {
@@ -103,8 +107,8 @@ struct Part {
       F::places(a, l, 0, ea, x);
       if constexpr (FORM == kHalf) eb = x;
       else eb = ea + F::VE;
-      v[0] = *reinterpret_cast<const u32x4*>(p + (on ? ea : 0));
-      v[1] = *reinterpret_cast<const u32x4*>(p + (on ? eb : 0));
+      v[0] = *reinterpret_cast<const word*>(p + (on ? ea : 0));
+      v[1] = *reinterpret_cast<const word*>(p + (on ? eb : 0));
     }
   }
   // pairs as floats, zero past K
@@ -143,8 +147,8 @@ struct Part {
       F::places(a, l, 0, ea, x0);
       if constexpr (FORM == kHalf) eb = x0;
       else eb = ea + F::VE;
-      *reinterpret_cast<u32x4*>(p + ea) = v[0];
-      *reinterpret_cast<u32x4*>(p + eb) = v[1];
+      *reinterpret_cast<word*>(p + ea) = v[0];
+      *reinterpret_cast<word*>(p + eb) = v[1];
     }
   }
 };
@@ -356,18 +360,25 @@ int sum_parts(const QkArgs& a, int rows, hipStream_t st) {
   return launch_status();
 }
 
-// Whether every row is whole vectors whose pairs lie within lanes.
+// The widest pieces, of 16, 8 or 4 bytes, that rows and their pairs are made of (0:
+// single elements), in elements.  Narrow ones for up to 16 lanes a row: 190 MB of rows
+// of 40 channels in bf16 98 against 153 us (all turned, 8 bytes), 162 against 176 (half of
+// them, 4 bytes); of 72, which take 18 lanes, 179 against 158.
 template <typename T>
-bool vectors(const QkArgs& a, bool back) {
-  const int VE = 16 / (int)sizeof(T), E = (int)sizeof(T);
+int pieces(const QkArgs& a, bool back) {
+  const int E = (int)sizeof(T);
   int64_t s = a.q_b | a.q_l | a.q_h | a.k_b | a.k_l | a.k_h | a.yq_b | a.yq_l | a.yq_h | a.yk_b |
               a.yk_l | a.yk_h;
-  bool at = aligned(a.q, 16) && aligned(a.k, 16) && aligned(a.yq, 16) && aligned(a.yk, 16);
-  if (back) {
-    s |= a.dq_b | a.dq_l | a.dq_h | a.dk_b | a.dk_l | a.dk_h;
-    at = at && aligned(a.dq, 16) && aligned(a.dk, 16);
+  if (back) s |= a.dq_b | a.dq_l | a.dq_h | a.dk_b | a.dk_l | a.dk_h;
+  for (int VE = 16 / E; VE > 1; VE /= 2) {
+    const int64_t n = VE * E;
+    if (a.K % (2 * VE) || a.R % (2 * VE) || s * E % n || a.K / (2 * VE) > (n == 16 ? 32 : 16))
+      continue;
+    if (aligned(a.q, n) && aligned(a.k, n) && aligned(a.yq, n) && aligned(a.yk, n) &&
+        (!back || (aligned(a.dq, n) && aligned(a.dk, n))))
+      return VE;
   }
-  return a.K % (2 * VE) == 0 && a.R % (2 * VE) == 0 && s * E % 16 == 0 && at;
+  return 0;
 }
 
 template <typename T, int FORM, int LG, int NS, bool BACK>
@@ -389,21 +400,34 @@ int launch(QkArgs a, hipStream_t st) {
   return launch_status();
 }
 
-template <typename T, int FORM, bool BACK>
+template <typename T, int FORM, int VE, bool BACK>
 int by_lanes(const QkArgs& a, hipStream_t st) {
-  const int64_t lanes = a.K / (2 * (16 / (int)sizeof(T)));
-  if (lanes <= 1) return launch<T, FORM, 1, 1, BACK>(a, st);
-  if (lanes <= 2) return launch<T, FORM, 2, 1, BACK>(a, st);
-  if (lanes <= 4) return launch<T, FORM, 4, 1, BACK>(a, st);
-  if (lanes <= 8) return launch<T, FORM, 8, 1, BACK>(a, st);
-  if (lanes <= 16) return launch<T, FORM, 16, 1, BACK>(a, st);
-  return launch<T, FORM, 32, 1, BACK>(a, st);
+  const int64_t lanes = a.K / (2 * VE);
+  if constexpr (VE * sizeof(T) == 16) {
+    if (lanes <= 1) return launch<T, FORM, 1, VE, BACK>(a, st);
+    if (lanes <= 2) return launch<T, FORM, 2, VE, BACK>(a, st);
+    if (lanes <= 4) return launch<T, FORM, 4, VE, BACK>(a, st);
+  }
+  if (lanes <= 8) return launch<T, FORM, 8, VE, BACK>(a, st);
+  if constexpr (VE * sizeof(T) == 16)
+    if (lanes > 16) return launch<T, FORM, 32, VE, BACK>(a, st);
+  return launch<T, FORM, 16, VE, BACK>(a, st);
+}
+
+template <typename T, int VE, bool BACK>
+int by_order(const QkArgs& a, hipStream_t st) {
+  return a.interleaved ? by_lanes<T, kNeighbours, VE, BACK>(a, st)
+                       : by_lanes<T, kHalf, VE, BACK>(a, st);
 }
 
 template <typename T, bool BACK>
 int by_form(const QkArgs& a, hipStream_t st) {
-  if (vectors<T>(a, BACK))
-    return a.interleaved ? by_lanes<T, kNeighbours, BACK>(a, st) : by_lanes<T, kHalf, BACK>(a, st);
+  constexpr int W = 16 / (int)sizeof(T);
+  const int VE = pieces<T>(a, BACK);
+  if (VE == W) return by_order<T, W, BACK>(a, st);
+  if (VE == W / 2) return by_order<T, W / 2, BACK>(a, st);
+  if constexpr (W == 8)
+    if (VE == 2) return by_order<T, 2, BACK>(a, st);
   const int slots = a.R / 2 + (a.K - a.R + 1) / 2;
   if (slots <= 16) return launch<T, kSingle, 16, 1, BACK>(a, st);
   if (slots <= 32) return launch<T, kSingle, 16, 2, BACK>(a, st);
