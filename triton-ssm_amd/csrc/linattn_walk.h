@@ -9,12 +9,14 @@
 // barrier a chunk:
 //   two teams of C / 32 output waves: 32 steps of a chunk each, as two tiles of 16.  A
 //     team has every other chunk, and two chunks' time for it.  (Where LDS does not hold
-//     three chunks, one team, with a wave for each tile,)
+//     three chunks, one team with a wave for each tile: 128 x 128 fp32, B=2 L=2048 H=16,
+//     114 us a call; 237 with one wave for both tiles of 32 steps.)
 //   2 state waves: 16 columns each.  K^T V of the whole chunk on top of the decayed
 //     state, whose planes go to LDS for the next chunk's outputs,
-//   2 loaders (4 beside one team): the chunk after this one to LDS, from loads that are
-//     two chunks ahead; and a wave for the decays where it is no third one on a SIMD (it
-//     would take a third of the others' registers: 64 steps of fp32 46 -> 88 us).
+//   2 loaders (4 beside two output waves): the chunk after this one to LDS, from loads
+//     that are two chunks ahead; where there are no outputs also a wave for the decays
+//     (which beside four output waves would be a third wave on a SIMD and take a third of
+//     the others' registers: B=3 L=1111 12 heads 40 x 72 fp32 46 -> 88 us).
 // Everything is formed transposed (planes.h): P^T = K Q^T is the next product's operand
 // in place, queries come to their wave straight from memory, and a lane ends up with 8
 // neighbouring columns of one step's output.
@@ -79,11 +81,10 @@ struct LinWalk {
   // output waves: of two tiles of 16 steps, or one where there is one team
   static constexpr int NW = MODE == kOutputs ? (TEAMS == 1 ? C / 16 : TEAMS * C / 32) : 0;
   static constexpr int NT = NW == 2 && TEAMS == 1 ? 256 : 128;  // threads of the loaders
-  static constexpr bool CLOCK = NW <= 2 && NT == 128;       // a wave for the decays
+  static constexpr bool CLOCK = NW == 0;                    // a wave for the decays
   static constexpr int kThreads = 64 * (NW + 2 + CLOCK) + NT;
   static constexpr int kNk = (C * KP / 8 + NT - 1) / NT, kNv = (C * 4 + NT - 1) / NT;
-  // chunks on their way from memory
-  static constexpr int AHEAD = 2;
+  static constexpr int AHEAD = 2;            // chunks on their way from memory
   typedef Swizzled<KP> KR;                   // rows of K and of the state's planes
   typedef Swizzled<32> VR;                   // of V
   struct Operands {  // of one chunk

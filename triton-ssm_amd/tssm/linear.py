@@ -132,7 +132,7 @@ def linear_attention_forward(q, k, v, g, *, scale=None, h0=None, return_state=Fa
     scale  of q; None: K ** -0.5
     h0     [B, Hv, K, V] float32 or None (zero initial state)
 
-    Returns o [B, L, Hv, V] (dtype of v; ``out`` if given) and, with
+    Returns o [B, L, Hv, V] (dtype of v; ``out`` if given, memory of its own) and, with
     ``return_state``, the final state [B, Hv, K, V] float32, which continues
     the sequence as the next call's ``h0`` or in ``linear_attention_step``.  An
     input that is not finite at some step changes no earlier output, and no
