@@ -1,0 +1,21 @@
+"""Gradients that are expanded along their rows, as those of sums are: the bits of
+contiguous ones."""
+import pytest
+import torch
+
+import test_gpu_linear as lin
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", [lin.F32, lin.BF16])
+@pytest.mark.parametrize("L", [1, 2, 150])
+def test_linear_attention(dev, dtype, L):
+    d = lin.inputs(dev, 2, L, 2, 8, 32, 4, dtype, seed=L, h0=True)
+    r = torch.Generator().manual_seed(1)
+    weights = torch.randn(2, L, 8, generator=r).to(dev, dtype)
+    for do in (torch.ones((), device=dev, dtype=dtype).expand(2, L, 8, 4),
+               weights[..., None].expand(2, L, 8, 4)):
+        want = lin.gradients(d, do.contiguous())
+        assert all(torch.equal(x, y) for x, y in zip(lin.gradients(d, do), want))
+        lin.compare_gradients(d, do, None, dtype)
