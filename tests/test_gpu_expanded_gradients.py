@@ -3,6 +3,7 @@ contiguous ones."""
 import pytest
 import torch
 
+import test_gpu_delta as delta
 import test_gpu_linear as lin
 
 pytestmark = pytest.mark.gpu
@@ -19,3 +20,14 @@ def test_linear_attention(dev, dtype, L):
         want = lin.gradients(d, do.contiguous())
         assert all(torch.equal(x, y) for x, y in zip(lin.gradients(d, do), want))
         lin.compare_gradients(d, do, None, dtype)
+
+
+@pytest.mark.parametrize("dtype", [lin.F32, lin.BF16])
+@pytest.mark.parametrize("L", [1, 2, 70])
+def test_delta_rule(dev, dtype, L):
+    d = delta.inputs(dev, 2, L, 2, 8, 32, 4, dtype, seed=L, h0=True)
+    weights = torch.randn(2, L, 8, generator=torch.Generator().manual_seed(1)).to(dev, dtype)
+    for do in (torch.ones((), device=dev, dtype=dtype).expand(2, L, 8, 4),
+               weights[..., None].expand(2, L, 8, 4)):
+        want = delta.gradients(d, do.contiguous())
+        assert all(torch.equal(x, y) for x, y in zip(delta.gradients(d, do), want))

@@ -96,12 +96,13 @@ def _explain(q, k, v, g, beta, lead):
 
 
 def _steps(t, chunks=False):
-    """t [B, L, H, N], copied where its steps overlap in memory (as expanded
-    ones do): the chunked kernels take steps that lie one after the other.  With
-    ``chunks`` (nothing but chunked kernels) also where a chunk of 32 steps and
-    one more would pass 31 bits."""
-    if t.shape[1] > 1 and (t.stride(1) < t.shape[3] or chunks and
-                           t.stride(1) >= (1 << 31) // (33 * t.element_size())):
+    """t [B, L, H, N], copied where its rows repeat one element (the gradient of a
+    sum) or its steps overlap in memory (as expanded ones do): the chunked kernels
+    take steps that lie one after the other.  With ``chunks`` (nothing but chunked
+    kernels) also where a chunk of 32 steps and one more would pass 31 bits."""
+    _, step, _, element = t.stride()
+    if element == 0 and t.shape[3] > 1 or t.shape[1] > 1 and (
+            step < t.shape[3] or chunks and step >= (1 << 31) // (33 * t.element_size())):
         return t.contiguous()
     return t
 
