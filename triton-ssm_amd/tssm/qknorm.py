@@ -87,6 +87,15 @@ def _like(t, what, x):
     return _rows(t, what)
 
 
+def _gradient(t, what, x):
+    """t checked, and its strides; copied where its rows repeat one element (the gradient
+    of a sum)."""
+    need_gpu(t, what)
+    if t.dim() and t.stride(-1) == 0 and t.shape[-1] > 1:
+        t = t.contiguous()
+    return t, _like(t, what, x)
+
+
 def _out(t, what, x):
     if t is None:
         return torch.empty_like(x, memory_format=torch.contiguous_format)
@@ -232,7 +241,8 @@ def qk_norm_rotary_backward(dq_out, dk_out, q, k, positions=None, freqs=None, we
     """
     code, norm_, sizes, pos, freqs, wq, wk = _operands(q, k, positions, freqs, weight_q,
                                                        weight_k, norm)
-    sdq, sdk = _like(dq_out, "dq_out", q), _like(dk_out, "dk_out", k)
+    dq_out, sdq = _gradient(dq_out, "dq_out", q)
+    dk_out, sdk = _gradient(dk_out, "dk_out", k)
     dq, dk = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k))
     dwq, dwk = (None if w is None else torch.empty(sizes[4], device=q.device, dtype=torch.float32)
                 for w in (wq, wk))
