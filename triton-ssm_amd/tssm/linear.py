@@ -96,11 +96,17 @@ def _steps(t, chunks=False):
     """t [B, L, H, N], copied where its rows repeat one element (the gradient of a sum) or
     its steps overlap in memory (as expanded ones do): the chunked kernels take steps that
     lie one after the other.  With ``chunks`` (nothing but chunked kernels) also where a
-    chunk of 128 steps and one more would pass 31 bits."""
+    chunk of 128 steps and one more would pass 31 bits, heads first if one step is so long
+    that it does not help to close the gaps."""
     _, step, _, element = t.stride()
-    if element == 0 and t.shape[3] > 1 or t.shape[1] > 1 and (
-            step < t.shape[3] or chunks and step >= (1 << 31) // (129 * t.element_size())):
-        return t.contiguous()
+    if element == 0 and t.shape[3] > 1 or t.shape[1] > 1 and step < t.shape[3]:
+        t = t.contiguous()
+    if chunks and t.shape[1] > 1:
+        most = (1 << 31) // (129 * t.element_size())
+        if t.stride(1) >= most:
+            t = t.contiguous()
+        if t.stride(1) >= most:
+            t = t.transpose(1, 2).contiguous().transpose(1, 2)
     return t
 
 
