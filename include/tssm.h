@@ -636,7 +636,8 @@ int tssm_gated_delta_step(int dtype, const void* q, const void* k, const void* v
  * strides (b, l, h) free; g f32 [B,L,Hv], three strides.  h0, h_last f32
  * contiguous [B,Hv,K,V] or NULL (zero, not returned); they may be one buffer.
  * K <= 128, V <= 2^21.  No reference counterpart.  The state and the sums that
- * reach it are fp32 whatever the dtype.  Workspace:
+ * reach it are fp32 whatever the dtype.  g = -inf drops what came before if it is
+ * finite (0 times a NaN or infinity is NaN).  Workspace:
  * tssm_linear_attention_workspace_bytes() bytes (0: may be NULL), 256-byte
  * aligned, raw fp32 (not look-back words), no clearing. */
 int64_t tssm_linear_attention_workspace_bytes(int64_t nbatch, int64_t L, int64_t Hk, int64_t Hv,

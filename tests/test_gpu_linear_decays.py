@@ -89,3 +89,22 @@ def test_nothing_before_the_first_step(dev, dtype):
     do = d["v"].flip(1).contiguous()
     dg = check(dev, d, do, None)
     assert not dg[:, 0].any()
+
+
+@pytest.mark.parametrize("dtype,L,t0", [(F32, 40, 17), (BF16, 300, 70), (F16, 300, 64),
+                                        (F32, 2000, 700), (BF16, 9, 4)])
+def test_a_reset_drops_what_is_finite(dev, dtype, L, t0):
+    """However large: the state before g = -inf is at 2^100, values there at 2^60 (2^15 in
+    fp16), and what comes after has the bits of its own sequence."""
+    from tssm import linear_attention_forward, linear_attention_step
+    d = inputs(dev, 1, L, 1, 2, 64, 40, dtype, seed=L, h0=True, rate=0.1)
+    d["g"][:, t0] = -float("inf")
+    ops = [d[n] for n in ("q", "k", "v", "g")]
+    want = linear_attention_forward(*ops, h0=d["h0"], return_state=True)
+    d["v"][:, :t0] *= 2.0 ** 15 / d["v"].abs().max() if dtype == F16 else 2.0 ** 60
+    d["k"][:, :t0] *= 2.0 ** 8
+    got = linear_attention_forward(*ops, h0=d["h0"] * 2.0 ** 100, return_state=True)
+    assert torch.equal(got[0][:, t0:], want[0][:, t0:]) and torch.equal(got[1], want[1])
+    at, state = [t[:, t0] for t in ops], d["h0"] * 2.0 ** 100
+    o, zero = linear_attention_step(*at, state), torch.zeros_like(state)
+    assert torch.equal(o, linear_attention_step(*at, zero)) and torch.equal(state, zero)

@@ -12,8 +12,11 @@ reference counterpart).
 q and k have Hk heads, v and g Hv, a multiple of Hk: value head h reads key head
 h // (Hv // Hk).  The state and every sum that reaches it are fp32.  ``g`` (log
 decay, at most 0) is read as float32; one rate for each head is ``rate.expand(B,
-L, Hv)``, and -inf at a step drops everything before it (several sequences in one
-row).  ``qk_norm_rotary_forward`` prepares q and k.
+L, Hv)``.  -inf at a step multiplies what came before by 0 and so drops it (several
+sequences in one row, a stream that begins anew), as long as it is finite: 0 times a
+NaN or infinity is NaN.  A state that holds one has to be zeroed instead, and a
+sequence with one belongs in a row of its own.  ``qk_norm_rotary_forward`` prepares q
+and k.
 """
 from __future__ import annotations
 
