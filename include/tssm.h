@@ -696,7 +696,8 @@ int tssm_linear_attention_step(int dtype, const void* q, const void* k, const vo
  * TSSM_POS_* type, freq f64 [R/2]; the angle is formed in 64 bits.  R = 0: no
  * rotation, pos and freq may be NULL.  K <= 256 (and
  * K > 1 with a norm: one channel's norm is its sign), B L < 2^31.  The outputs (of
- * `dtype`, strides like the inputs') may be the inputs.  The backward takes the
+ * `dtype`, strides like the inputs') may be their own inputs: yq q, yk k, with the
+ * same strides.  The backward takes the
  * outputs' gradients and writes dq, dk of `dtype` and dwq, dwk f32 [K] (NULL
  * where not wanted), summed in a fixed order through a workspace of
  * tssm_qk_norm_rotary_workspace_bytes() bytes (16-byte aligned, no clearing;

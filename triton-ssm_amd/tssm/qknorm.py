@@ -105,6 +105,16 @@ def _out(t, what, x):
     return t
 
 
+def _apart(q, k, yq, yk):
+    """Refuses an output that starts where the other input or output does, or where its own
+    input does with other strides: rows would be written before they are read."""
+    at, back = (q.data_ptr(), k.data_ptr()), (yq.data_ptr(), yk.data_ptr())
+    other = [a == b and any(n > 1 and s != z for n, s, z in zip(x.shape, x.stride(), y.stride()))
+             for a, b, x, y in zip(at, back, (q, k), (yq, yk))]
+    if at[0] == back[1] or at[1] == back[0] or back[0] == back[1] or any(other):
+        raise ValueError("out_q may be q and out_k may be k; outputs must not overlap otherwise")
+
+
 def _weight(t, what, K, device):
     if t is None:
         return None
@@ -215,13 +225,15 @@ def qk_norm_rotary_forward(q, k, positions=None, freqs=None, weight_q=None, weig
                None, with positions: no rotation
     weight_q, weight_k  [K] (read as float32) or None
 
-    Returns (q', k') of q's dtype, new or in ``out_q`` and ``out_k``, which may be
-    q and k.
+    Returns (q', k') of q's dtype, new or in ``out_q``, which may be q, and ``out_k``, which
+    may be k; neither overlaps anything else.
     """
     code, norm_, sizes, pos, freqs, wq, wk = _operands(q, k, positions, freqs, weight_q,
                                                        weight_k, norm)
     yq, yk = _out(out_q, "out_q", q), _out(out_k, "out_k", k)
     if q.numel():
+        if out_q is not None or out_k is not None:
+            _apart(q, k, yq, yk)
         on_device(q.get_device(), _lib.call, "tssm_qk_norm_rotary_fwd", code, norm_,
                   int(bool(interleaved)), q.data_ptr(), k.data_ptr(), pos[0], pos[1], ptr(freqs),
                   ptr(wq), ptr(wk), yq.data_ptr(), yk.data_ptr(), *sizes, *_rows(q, "q"),
