@@ -149,13 +149,6 @@ struct RowsOf {
 constexpr uint32_t kPast = 0x7ffffff0u;  // an offset past every descriptor's end
 
 template <typename T>
-__device__ inline T buf_elem(__amdgpu_buffer_rsrc_t r, uint32_t off) {
-  if constexpr (sizeof(T) == 4)
-    return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0));
-  else
-    return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b16(r, off, 0, 0));
-}
-template <typename T>
 __device__ inline void buf_put(__amdgpu_buffer_rsrc_t r, uint32_t off, float x) {
   T y;
   stf(&y, x);

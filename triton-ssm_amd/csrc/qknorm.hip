@@ -13,8 +13,8 @@
 // rate of 1 leaves 20 bits of an fp32 angle before the point), are formed once
 // for a token by the workgroup and shared by its heads through LDS.
 //
-// The forward reaches 4.4 to 5.0 TB/s (B=8 L=4096, 16 + 16 heads of 64, bf16: 54 us;
-// B=4 L=4096, 16 + 8 of 128: 45), a copy 5.15.  It is waves in flight that decide: rows
+// The forward reaches 4.3 to 4.8 TB/s (B=8 L=4096, 16 + 16 heads of 64, bf16: 56 us;
+// B=4 L=4096, 16 + 8 of 128: 47), a copy 5.15.  It is waves in flight that decide: rows
 // are asked for before the angles are formed, and the weights, which both would hold 32
 // registers, are in LDS (with them in registers and the next rows ahead, 200 registers
 // and two waves a SIMD, 65 us each).
@@ -164,7 +164,6 @@ __global__ __launch_bounds__(kThreads, BACK ? 3 : 1) void qk_kernel(QkArgs a) {
   typedef Part<T, FORM, LG, NS> P;
   typedef Form<T, FORM, LG, NS> F;
   constexpr int NP = F::NP, NI = BACK ? 1 : 4;  // rows that a lane has in flight
-  constexpr int kGroups = kThreads / LG;
   __shared__ float2 table[kTable];
   __shared__ __attribute__((aligned(16))) float weights[2 * LG * 2 * NP];
   __shared__ float sums[BACK ? 2 * LG * 2 * NP * 4 : 1];
