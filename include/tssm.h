@@ -660,8 +660,9 @@ int tssm_linear_attention_forward(int dtype, const void* q, const void* k, const
  * (TSSM_ERR_STRIDE).  The states are formed again from the inputs and kept in the
  * workspace (tssm_linear_attention_backward_workspace_bytes() bytes, else as
  * the forward's): 8 K' V' bytes for every 64 steps of a value head, K' being K
- * rounded up to 32, 64 or 128 and V' V to a multiple of 32, for few heads and long sequences as much for each segment of a head, and for
- * small calls with shared key heads 8 K bytes for each step of a value head.
+ * rounded up to 32, 64 or 128 and V' V to a multiple of 32, for few heads and long
+ * sequences as much for each segment of a head, and for small calls with shared key
+ * heads 8 K bytes for each step of a value head.
  * With L = 0 nothing is written (dh0 would be dh_last). */
 int64_t tssm_linear_attention_backward_workspace_bytes(int dtype, int64_t nbatch, int64_t L,
                                                        int64_t Hk, int64_t Hv, int64_t K,

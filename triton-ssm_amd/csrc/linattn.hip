@@ -28,9 +28,9 @@ bool by_steps(int64_t heads, int64_t L, int64_t V) {
 // against 19; with gradients 117 against 66, 36 against 38, 75 against 63.  Segments of
 // 2048 steps and more are halved, as the shorter pass has several workgroups on a CU: 8
 // heads L=65536 124 against 139, with gradients 365 against 388 (but L=8192 35 against
-// 28).  Two segments cost what they save (B=4 L=4096 H=16 64 x 64: 64 against 61;
-// gradients 194 against 170) but for K > 64, where the outputs are the larger part of a
-// walk: B=2 L=4096 H=16 128 x 128 92 against 104; gradients 408 against 373.
+// 28).  Two segments cost what they save (B=4 L=4096 H=16 64 x 64: whole 63, in two 67;
+// with gradients 170 and 199) but for K > 64, where the outputs are the larger part of a
+// walk: B=2 L=4096 H=16 128 x 128 whole 104, in two 97; with gradients 345 and 396.
 int64_t segments(int64_t heads, int64_t L, int64_t K, int64_t V, bool grads) {
   const int64_t wgs = heads * cdiv64(V, 32), most = L / (grads ? 512 : 192);
   const int64_t fill = wgs > 0 ? 256 / wgs : 1, n = fill < most ? fill : most;

@@ -8,9 +8,10 @@ namespace tssm {
 namespace {
 
 // Planes of an input (fp32 three, fp16 two, bf16 one: exactly), and of what is
-// formed on the way to the outputs alone (two, 2^-17 of a value that is rounded to
-// 2^-9 or 2^-12; three where nothing is rounded).  What reaches the state always
-// has three.
+// formed on the way to the outputs alone (two, each 2^-17 of a term of sums that are
+// rounded to 2^-8 or 2^-11 at the end: with the planes' products left out 2^-16, which
+// counts where terms cancel by more than 2^8 or 2^5; three where nothing is rounded).
+// What reaches the state always has three.
 template <typename T>
 constexpr int kPlanes = sizeof(T) == 4 ? 3 : (std::is_same<T, bf16_t>::value ? 1 : 2);
 template <typename T>

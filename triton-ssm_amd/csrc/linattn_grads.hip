@@ -22,11 +22,11 @@
 // (planes.h); R is formed in both places.  The states' planes take one buffer after
 // the other: S for dQ, then dS for dK and dV.
 //
-// What bounds it: memory.  B=4 L=4096 H=16 64 x 64 bf16 takes 86 us for 134 MB of inputs,
-// 134 MB of states and 100 MB of gradients, 4.3 TB/s where a copy reaches 5.1: two
+// What bounds it: memory.  B=4 L=4096 H=16 64 x 64 bf16 takes 87 us for 134 MB of inputs,
+// 134 MB of states and 100 MB of gradients, 4.2 TB/s where a copy reaches 5.1: two
 // workgroups are on a CU (one, with 266 registers, took 160 us), and what one waits for
 // is hidden by the other's work alone.  The states are read once, past the caches
-// (through them 92 us).  Chunks of 128 steps would halve the states and leave LDS for
+// (through them 6 us more).  Chunks of 128 steps would halve the states and leave LDS for
 // one workgroup; chunks of 32 in fp32 took 380 us for 344 (the same sizes, all kernels),
 // and 483 for 278 at B=2 L=2048 H=16 128 x 128: two waves on a CU.
 #include "linattn_dev.h"

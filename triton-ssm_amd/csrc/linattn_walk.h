@@ -21,7 +21,7 @@
 // in place, queries come to their wave straight from memory, and a lane ends up with 8
 // neighbouring columns of one step's output.
 //
-// What bounds it: one wave's chain and LDS.  B=8 L=4096 H=16 64 x 64 bf16 takes 84 us
+// What bounds it: one wave's chain and LDS.  B=8 L=4096 H=16 64 x 64 bf16 takes 85 us
 // for 270 MB (3.2 TB/s; 256 workgroups, one on a CU), a chunk of 128 steps 3800 cycles,
 // of which the state waves work 3200, the outputs 2400 to 3100 and the loader with the
 // decays 3000.  fp32 (3 planes) is bound by LDS: 3700 of a chunk's 5000 cycles (64

@@ -27,7 +27,7 @@ from .workspace import check  # noqa: F401
 __all__ = ["multihead_ssm_forward", "selective_scan_forward", "ssd_scan_forward",
            "ssd_stream_step", "fused_interp_ssm_forward", "time_aware_interp_corrected",
            "streaming_interp_step_corrected", "gated_delta_forward", "gated_delta_backward",
-           "gated_delta_step", "linear_attention_forward",
-           "linear_attention_backward", "linear_attention_step", "qk_norm_rotary_forward", "qk_norm_rotary_backward", "rotary_frequencies",
-           "rotary_amplitude", "group_norm_act_forward", "group_norm_act_backward", "check",
-           "TssmError"]
+           "gated_delta_step", "linear_attention_forward", "linear_attention_backward",
+           "linear_attention_step", "qk_norm_rotary_forward", "qk_norm_rotary_backward",
+           "rotary_frequencies", "rotary_amplitude", "group_norm_act_forward",
+           "group_norm_act_backward", "check", "TssmError"]

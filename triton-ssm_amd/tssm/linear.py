@@ -10,7 +10,10 @@ reference counterpart).
 ``linear_attention_step``      one step of many streams, the state in place (decode)
 
 q and k have Hk heads, v and g Hv, a multiple of Hk: value head h reads key head
-h // (Hv // Hk).  The state and every sum that reaches it are fp32.  ``g`` (log
+h // (Hv // Hk).  The state and every sum that reaches it are fp32.  With 16-bit
+operands the weights between steps, and the state on its way to o and dv, count with 16
+bits in products that fp32 sums add up: below the rounding of o, dq, dk and dv but where
+their terms cancel by more than 2^8 (bfloat16) or 2^5 (float16).  ``g`` (log
 decay, at most 0) is read as float32; one rate for each head is ``rate.expand(B,
 L, Hv)``.  -inf at a step multiplies what came before by 0 and so drops it (several
 sequences in one row, a stream that begins anew), as long as it is finite: 0 times a
@@ -208,7 +211,7 @@ def linear_attention_step(q, k, v, g, state, *, scale=None, out=None):
 
     q, k [S, Hk, K], v [S, Hv, V] of one dtype (float32 / bfloat16 / float16),
     g [S, Hv], state [S, Hv, K, V] float32 contiguous.  Returns o [S, Hv, V]
-    (dtype of v; ``out`` if given).  The same step as
+    (dtype of v; ``out`` if given, memory of its own).  The same step as
     ``linear_attention_forward`` with L = 1.
     """
     (S, Hk, Hv, K, V), code, g = _operands(q, k, v, g, 1)

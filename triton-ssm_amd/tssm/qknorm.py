@@ -9,7 +9,9 @@ for the R/2 pairs of the first R channels, (j, j + R/2) or, interleaved, (2 j, 2
 1), by the angle position * freqs[j]; the other channels stay n.  Positions are
 token numbers or the times of irregular samples; angles are formed in 64 bits.
 ``rotary_frequencies`` gives the rates, scaled for long contexts if asked to.
-What comes out is what ``linear_attention_*`` and ``gated_delta_*`` read as q and k.
+What comes out is what ``linear_attention_*`` and ``gated_delta_*`` read as q and k, if
+both have the same number of heads: those share key heads among value heads, not among
+queries.
 """
 from __future__ import annotations
 
