@@ -10,10 +10,12 @@
 //   dQ = e^G X1 + M K,
 //   dK = M^T Q + (E + E^T) K + e^(G_last - G) X2 - beta e^G X3,
 //   dbeta = sum_v dR Y + sum_i dA D kk,
-//   dG_t = e^G sum_v (scale dO (Q S) - beta dR (K S)) - b_t
-//          + sum_i F[t][i] - sum_i F[i][t],
-//     F = dP P + dA A,  b_t = e^(G_last - G_t) sum_v U (K G'),
-//   dG_last += sum_t b_t + e^(G_last) <S, G'>,   dg_t = sum of dG from t on.
+//   dg_t = sum over s >= t of e^(G_s) sum_v (scale dO (Q S) - beta dR (K S))
+//          + sum over s >= t > i of F[s][i] + sum over i < t of b_i + e^(G_last) <S, G'>,
+//     F = dP P + dA A,  b_i = e^(G_last - G_i) sum_v U (K G').
+// (Nothing but terms that hold e^(g_t): sums of F's rows less those of its columns, rounded
+// to fp32, leave 1e-6 of the chunk's largest dg where a strong decay among slow ones makes
+// it 1e-13.)
 // A workgroup of four waves takes one chunk of one key head and goes through
 // its value heads (whose gradients of q and k add up in registers, in order),
 // and through V in slices of 64 columns: first column by column as the walks
@@ -67,7 +69,7 @@ struct Grad {
     // a wave's sums for each step: F, dA D kk, dR Y, e^G (scale dO (Q S) - beta dR (K S)),
     // e^(G_last - G) U (K G')
     float row[4][5][kC];
-    float col[4][kC];     // and of F over t
+    float col[8][kC];     // and of F's columns, over four rows each
     float dot[4];
   };
 };
@@ -466,21 +468,23 @@ __global__ __launch_bounds__(256, (Grad<T, KP, VEC>::kWaves)) void delta_grads_k
     // the 32 x 32 tiles: M, E and the sums of F
     {
       f32x4 M, E;
-      float fcol = 0.0f, frow[4], kb[4];
+      float frow[4], kb[4];
       const float4 b4 = *reinterpret_cast<const float4*>(&lds.fac[kBeta][8 * j + 4 * tx]);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const float bt = (&b4.x)[r], p = a.scale * dP[r], q = -dA[r];
         M[r] = p * dd[r];
         E[r] = ti < 8 * j + 4 * tx + r ? q * dd[r] * bt : 0.0f;
-        const float f = __builtin_fmaf(p, pp[r], q * bt * dkk[r]);
-        fcol += f;
-        frow[r] = group_sum<16>(f);
+        frow[r] = __builtin_fmaf(p, pp[r], q * bt * dkk[r]);
         kb[r] = group_sum<16>(q * dkk[r]);
       }
-      fcol += __shfl_xor(fcol, 16);
-      fcol += __shfl_xor(fcol, 32);
-      if (j == 0) lds.col[w][ti] = fcol;
+      // F's columns before each row, from it on: in four rows here, the later ones below
+#pragma unroll
+      for (int r = 2; r >= 0; --r) frow[r] += frow[r + 1];
+      lds.col[2 * j + tx][ti] = frow[0];
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        frow[r] = group_sum<16>(ti < 8 * j + 4 * tx + r ? frow[r] : 0.0f);
       if (c == 0) {
         *reinterpret_cast<float4*>(&lds.row[w][0][8 * j + 4 * tx]) =
             make_float4(frow[0], frow[1], frow[2], frow[3]);
@@ -498,21 +502,25 @@ __global__ __launch_bounds__(256, (Grad<T, KP, VEC>::kWaves)) void delta_grads_k
       const auto sum4 = [&](int i) {
         return (lds.row[0][i][t] + lds.row[1][i][t]) + (lds.row[2][i][t] + lds.row[3][i][t]);
       };
-      const float f = lds.row[2 * x][0][t] + lds.row[2 * x + 1][0][t];
       const float kb = lds.row[2 * x][1][t] + lds.row[2 * x + 1][1][t];
-      const float fc = lds.col[x][t] + lds.col[2 + x][t];  // column t: waves x and 2 + x
-      const float bt = sum4(4);
-      double G_ = (double)(f - fc) + (double)(sum4(3) - bt), B = bt;
+      float f = lds.row[2 * x][0][t] + lds.row[2 * x + 1][0][t], later = 0.0f;
 #pragma unroll
-      for (int s = 1; s < 32; s *= 2) B += __shfl_xor(B, s, 32);
-      if (t == 31)
-        G_ += B + (double)lds.fac[kEg][31] *
-                      (double)((lds.dot[0] + lds.dot[1]) + (lds.dot[2] + lds.dot[3]));
+      for (int i = 6; i >= 0; --i) {  // what crosses the rows of group i in the groups past it
+        const float y = lds.col[i + 1][t ? t - 1 : 0];
+        later += t ? y : 0.0f;
+        const float before = scan_incl<32>(later);
+        f += t >> 2 == i ? before : 0.0f;
+      }
+      const float prev = __shfl_up(sum4(4), 1, 32);
+      f += scan_incl<32>(t ? prev : 0.0f);
+      double G_ = (double)sum4(3);
 #pragma unroll
       for (int s = 1; s < 32; s *= 2) {
         const double y = __shfl_down(G_, s, 32);
         if (t + s < 32) G_ += y;
       }
+      G_ += (double)f + (double)lds.fac[kEg][31] *
+                            (double)((lds.dot[0] + lds.dot[1]) + (lds.dot[2] + lds.dot[3]));
       if (lane < rows) {
         const int64_t at = (b * a.L + t0 + t) * a.Hv + h;
         g.dg[at] = (float)G_;
